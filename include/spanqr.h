@@ -284,6 +284,74 @@ int spanqr_chol64(spanqr_chol64_plan* plan, const double* G, long ldg, const dou
                   float* Lf, float* Lif, void* stream);
 int spanqr_chol64_status(spanqr_chol64_plan* plan, void* stream);
 
+/* ---- training operators beside orth: the loss over the vocabulary, root-mean-square norm, clipping ----
+ * No counterpart in the reference, whose caller's training step forms the gradients that its optimizer turns into X
+ * (README.md:19-30). Conventions: matrices are row-major in device memory with row strides in elements and neighbouring
+ * elements in a row; element alignment is enough. Types are SPANQR_BF16, SPANQR_FP16 and SPANQR_FP32. Calls enqueue on
+ * the stream and neither allocate nor synchronise; a workspace belongs to the caller, is needed until the call's work
+ * is done and needs 256-byte alignment; calls with workspaces of their own can overlap. All sums are fp32 or fp64 in a
+ * fixed order, so a call repeats its bits. */
+enum {
+    SPANQR_FP32 = 0,
+    SPANQR_BF16 = 1,
+    SPANQR_FP16 = 2,
+};
+enum {
+    SPANQR_QUANT_NONE = 0,
+    SPANQR_QUANT_FP8 = 1,        /* e4m3 (OCP), largest 448 */
+    SPANQR_QUANT_INT8 = 2,       /* -127 to 127 */
+};
+enum {
+    SPANQR_REDUCE_NONE = 0,
+    SPANQR_REDUCE_SUM = 1,
+    SPANQR_REDUCE_MEAN = 2,      /* over the tokens that are not ignored (0 if there are none) */
+};
+
+/* y = norm(h) weight for each of `rows` rows of D elements (1 to 2^24): h = x, or with `residual` h = x + residual,
+ * rounded to the type, written to h [rows, D] and normed as rounded; norm(h) = h / sqrt(mean(h^2) + eps). weight [D] of
+ * type wtype, or null for 1. quant none: y [rows, D] of x's type, scale null. Else y [rows, D] of 8 bits and scale
+ * [rows] fp32 with y scale ~ norm(h) weight: scale = max|norm(h) weight| / 448 or / 127, to nearest even; a row of
+ * zeros has scale 0, a row with a NaN has scale NaN. h and y are contiguous. */
+int spanqr_rms_norm(int type, int wtype, int quant, long rows, long D, const void* x, long ldx, const void* residual,
+                    long ldr, const void* weight, float eps, void* h, void* y, float* scale, void* stream);
+
+/* Gradient of it (of the unrounded y, also where y was taken in 8 bits): from dy and h (x where there was no residual),
+ * dx [rows, D], the gradient of x and of the residual alike, with dh (or null), the gradient that reaches h otherwise,
+ * added; and dw [D] of type wtype, or null. dw is also written for rows = 0 (zeros). workspace:
+ * spanqr_rms_norm_backward_workspace(rows, D) bytes, needed where dw is wanted. */
+long spanqr_rms_norm_backward_workspace(long rows, long D);
+int spanqr_rms_norm_backward(int type, int wtype, long rows, long D, const void* dy, long lddy, const void* h, long ldh,
+                             const void* weight, const void* dh, long lddh, float eps, void* dx, void* dw,
+                             void* workspace, long workspace_bytes, void* stream);
+
+/* norm = sqrt(sum of g^2 over all n tensors) in fp32 (squares and sums in fp64), on the device. grads, numel and type
+ * are host arrays of device addresses, element counts (0 allowed) and types; they are read at the call. workspace:
+ * spanqr_grad_norm_workspace(n) bytes. */
+long spanqr_grad_norm_workspace(int n);
+int spanqr_grad_norm(int n, const void* const* grads, const long* numel, const int* type, float* norm, void* workspace,
+                     long workspace_bytes, void* stream);
+
+/* The same, and out[i] = grads[i] min(1, max_norm / norm), of type out_type[i], element for element in memory order;
+ * out[i] may be grads[i] itself (in place, and then nothing is written where the norm is within max_norm), but not
+ * overlap it otherwise. A NaN norm makes every element NaN; an infinite one makes finite elements 0. */
+int spanqr_clip_grad_norm(int n, const void* const* grads, const long* numel, const int* type, void* const* out,
+                          const int* out_type, float max_norm, float* norm, void* workspace, long workspace_bytes,
+                          void* stream);
+
+/* Softmax cross entropy of the logits x w^T, which are not kept, for N tokens: x [N, H] and w [V, H] of `type` (bf16 or
+ * fp16), target [N] int64. loss_i = row_weight_i (log sum_j exp z_ij - z_i,target_i); a token whose target is
+ * ignore_index has loss 0 and no gradient, one whose target is no column otherwise has loss NaN (and makes the
+ * gradients NaN). row_weight [N] fp32, or null for 1. loss: [N] fp32 (none), or one fp32: the sum, or the sum over the
+ * number of tokens not ignored (mean). lse [N] fp32 (log sum exp) or null. dx [N, H] and dw [V, H], contiguous, of
+ * `type`, each or null: the gradients of the sum (none, sum) or of the mean, times *grad_scale (device, or null for 1).
+ * workspace: what spanqr_linear_cross_entropy_workspace gives for `grads` (1: dx, 2: dw, 3: both, 0: neither) and
+ * most_bytes, which bounds it: the tokens go through in pieces whose 16-bit exponentials fit (256 tokens at least). */
+long spanqr_linear_cross_entropy_workspace(int type, long N, long H, long V, int grads, long most_bytes);
+int spanqr_linear_cross_entropy(int type, int reduction, long N, long H, long V, const void* x, long ldx, const void* w,
+                                long ldw, const long* target, long ignore_index, const float* row_weight,
+                                const float* grad_scale, float* loss, float* lse, void* dx, void* dw, void* workspace,
+                                long workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,15 +6,17 @@ point raises: there is no CPU or PyTorch fallback for the hot path.
 import ctypes
 import os
 import subprocess
+import tempfile
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libspanqr.so")
-SRC = os.path.join(_HERE, "csrc", "spanqr.hip")
+# orth's path, and the training operators beside it
+SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("spanqr.hip", "loss.hip", "norm.hip", "clip.hip")]
 INCLUDE = os.path.join(os.path.dirname(_HERE), "include", "spanqr.h")
 
 # hipcc flags: gfx950 only; packed fp32 VALU ops disabled (the kernels never rely on them); no fast-math so every
 # fp32 operation keeps IEEE rounding and subnormals.
-HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 # plan queries (include/spanqr.h)
@@ -25,6 +27,11 @@ MAX_R = 4096     # SPANQR_MAX_R
 # kernels for spanqr_profile_kernel
 (K_AMAX, K_GRAM_PASS1, K_GRAM, K_REDUCE, K_CHOL, K_TRSM_PASS1, K_TRSM, K_NS_APPLY, K_CHOL_SOLVE_PASS1,
  K_CHOL_SOLVE) = range(10)
+
+# types, 8-bit forms and reductions of the training operators
+FP32, BF16, FP16 = range(3)
+QUANT_NONE, QUANT_FP8, QUANT_INT8 = range(3)
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = range(3)
 
 # every exported symbol of include/spanqr.h: (restype, argtypes)
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
@@ -60,6 +67,15 @@ SIGNATURES = {
     "spanqr_chol64_plan_destroy": (None, [_P]),
     "spanqr_chol64": (_I, [_P, _P, _L, _P, _P, _P, _P, _P, _P]),
     "spanqr_chol64_status": (_I, [_P, _P]),
+    "spanqr_rms_norm": (_I, [_I, _I, _I, _L, _L, _P, _L, _P, _L, _P, _F, _P, _P, _P, _P]),
+    "spanqr_rms_norm_backward_workspace": (_L, [_L, _L]),
+    "spanqr_rms_norm_backward": (_I, [_I, _I, _L, _L, _P, _L, _P, _L, _P, _P, _L, _F, _P, _P, _P, _L, _P]),
+    "spanqr_grad_norm_workspace": (_L, [_I]),
+    "spanqr_grad_norm": (_I, [_I, _P, _P, _P, _P, _P, _L, _P]),
+    "spanqr_clip_grad_norm": (_I, [_I, _P, _P, _P, _P, _P, _F, _P, _P, _L, _P]),
+    "spanqr_linear_cross_entropy_workspace": (_L, [_I, _L, _L, _L, _I, _L]),
+    "spanqr_linear_cross_entropy": (_I, [_I, _I, _L, _L, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _L,
+                                         _P]),
 }
 
 _lib = None
@@ -71,11 +87,20 @@ class SpanqrError(RuntimeError):
 
 def build(verbose=False):
     """compile libspanqr.so in place (hipcc cross-compiles gfx950 without a GPU)"""
-    cmd = ["hipcc", *HIPCC_FLAGS, "-o", LIB_PATH, SRC]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    out = "\n".join(l for l in (res.stdout + res.stderr).splitlines() if "packed-fp32-ops" not in l)
-    if res.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({res.returncode}):\n{out}")
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, os.path.basename(src) + ".o") for src in SOURCES]
+        compiles = [subprocess.Popen(["hipcc", *HIPCC_FLAGS, "-c", "-o", obj, src], stdout=subprocess.PIPE,
+                                     stderr=subprocess.STDOUT, text=True) for src, obj in zip(SOURCES, objects)]
+        said = [p.communicate()[0] for p in compiles]
+        failed = [p.returncode for p in compiles if p.returncode != 0]
+        if not failed:
+            link = subprocess.run(["hipcc", "--offload-arch=gfx950", "-shared", "-o", LIB_PATH, *objects],
+                                  capture_output=True, text=True)
+            said.append(link.stdout + link.stderr)
+            failed = [link.returncode] if link.returncode != 0 else []
+    out = "\n".join(l for text in said for l in text.splitlines() if "packed-fp32-ops" not in l)
+    if failed:
+        raise RuntimeError(f"hipcc failed ({failed[0]}):\n{out}")
     if verbose and out.strip():
         print(out)
     return LIB_PATH

@@ -1,0 +1,545 @@
+// norm.hip -- root-mean-square norm with the residual's addition, in the model's type or in 8 bits, and its gradient.
+//
+//   h = round(x + r),  s = (sum_j h_j^2 / D + eps)^(-1/2),  y_j = h_j s w_j
+//   8 bits: q_j = round8(y_j M / a), scale = a / M, a = max_j |y_j|, M = 448 (fp8 e4m3) or 127 (int8); y in fp32
+//   gradient: n = h s, u = dy w, dx = s (u - n sum_j(u_j n_j) / D) + dh, dw = sum over rows of dy n
+//
+// Both are bound by memory: one read of every input and one write of every output, with the row in registers between
+// the sums and the output. A row belongs to GROUP threads with NCH pieces of eight elements each, so the same kernel
+// serves 16 lanes a row (128 elements) to 1024 threads a row (32768); longer rows are read again for each step
+// (k_rms_long, k_rms_grad_long). All sums are fp32 per thread over at most 32 elements, then a tree in a fixed order.
+#include "elements.h"
+#include "host.h"
+
+using namespace spanqr_dev;
+using spanqr_host::error;
+using spanqr_host::launched;
+
+namespace {
+
+struct NormArgs {
+    long rows, D, ldx, ldr;
+    const void *x, *residual, *weight;   // residual, weight may be null
+    int wtype;                           // weight's type (SPANQR_BF16 ...)
+    int quant;
+    float eps;
+    void *h, *y;
+    float* scale;
+};
+
+struct GradArgs {
+    long rows, D, lddy, ldh, lddh;
+    const void *dy, *h, *weight, *dh;    // weight, dh may be null
+    int wtype;
+    float eps;
+    void* dx;
+    float* part;                         // [gridDim.x, D] sums of dy n over the block's rows, or null
+};
+
+// eight weights as fp32; 1 without weights
+__device__ __forceinline__ void load_weight(const void* w, int type, long at, int n, float (&f)[8]) {
+    if (w == nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = 1.0f;
+    } else if (type == SPANQR_BF16) {
+        load8((const bf16*)w + at, n, f);
+    } else if (type == SPANQR_FP16) {
+        load8((const fp16*)w + at, n, f);
+    } else {
+        load8((const float*)w + at, n, f);
+    }
+}
+
+// elements of the piece at `at` that are inside the row (0 to 8)
+__device__ __forceinline__ int inside(long D, long at) { return D - at >= 8 ? 8 : D > at ? (int)(D - at) : 0; }
+
+__device__ __forceinline__ float quant_max(int quant) { return quant == SPANQR_QUANT_FP8 ? 448.0f : 127.0f; }
+
+// what y is multiplied by. A row of zeros gives zeros; where M / a would overflow the largest finite factor is used.
+// A NaN (of the row or of a weight) stays NaN in the scale.
+__device__ __forceinline__ float quant_factor(float a, float M) {
+    if (a == 0.0f) return 0.0f;
+    const float f = M / a;
+    return f > 3.402823466e38f ? 3.402823466e38f : f;
+}
+
+// |v| <= M by construction of the factor (up to one rounding, which round8 takes back to M)
+__device__ __forceinline__ void store_quant(int quant, uint8_t* q, int n, const float (&v)[8]) {
+    uint32_t lo, hi;
+    if (quant == SPANQR_QUANT_FP8) {
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+        lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+        hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
+    } else {
+        int k[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[i] = (int)rintf(v[i]);
+        lo = (k[0] & 255) | (k[1] & 255) << 8 | (k[2] & 255) << 16 | (uint32_t)k[3] << 24;
+        hi = (k[4] & 255) | (k[5] & 255) << 8 | (k[6] & 255) << 16 | (uint32_t)k[7] << 24;
+    }
+    if (n >= 8) {
+        struct __attribute__((packed, aligned(1))) Two { uint32_t a, b; };
+        *reinterpret_cast<Two*>(q) = Two{lo, hi};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) q[i] = (uint8_t)((i < 4 ? lo : hi) >> 8 * (i & 3));
+    }
+}
+
+template <int GROUP, typename OP, typename A>
+__device__ __forceinline__ A reduce_group(A v, A* slot) {
+    if constexpr (GROUP <= 64)
+        return reduce_lanes<GROUP, OP>(v);
+    else
+        return reduce_threads<GROUP, OP>(v, slot);
+}
+
+template <typename T, int GROUP, int NCH>
+__global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void k_rms(const NormArgs p) {
+    constexpr int BLOCK = GROUP > 256 ? GROUP : 256, ROWS = BLOCK / GROUP;
+    __shared__ float slot[BLOCK / 64];
+    const int lane = threadIdx.x % GROUP;
+    float w[NCH][8];
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        const long at = 8l * (lane + c * GROUP);
+        load_weight(p.weight, p.wtype, at, inside(p.D, at), w[c]);
+    }
+    for (long base = (long)blockIdx.x * ROWS; base < p.rows; base += (long)gridDim.x * ROWS) {
+        const long row = base + threadIdx.x / GROUP;
+        const bool on = row < p.rows;   // the group's lanes all take part in the reductions
+        float v[NCH][8];
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const long at = 8l * (lane + c * GROUP);
+            load8((const T*)p.x + row * p.ldx + at, on ? inside(p.D, at) : 0, v[c]);
+        }
+        if (p.residual != nullptr) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const long at = 8l * (lane + c * GROUP);
+                const int n = on ? inside(p.D, at) : 0;
+                float r[8];
+                load8((const T*)p.residual + row * p.ldr + at, n, r);
+                // the stream is rounded as it is kept; the norm is of the rounded values
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[c][i] = (float)(T)(v[c][i] + r[i]);
+                store8((T*)p.h + row * p.D + at, n, v[c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = fmaf(v[c][i], v[c][i], sum);
+        sum = reduce_group<GROUP, Sum>(sum, slot);
+        const float s = rsqrtf(sum / (float)p.D + p.eps);
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] = v[c][i] * s * w[c][i];
+        if (p.quant == SPANQR_QUANT_NONE) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const long at = 8l * (lane + c * GROUP);
+                store8((T*)p.y + row * p.D + at, on ? inside(p.D, at) : 0, v[c]);
+            }
+        } else {
+            // (elements past the row's end are 0, or NaN where s is: then the row is NaN anyway)
+            float a = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a = nan_max(a, fabsf(v[c][i]));
+            a = reduce_group<GROUP, NanMax>(a, slot);
+            const float M = quant_max(p.quant), f = quant_factor(a, M);
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const long at = 8l * (lane + c * GROUP);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[c][i] *= f;
+                store_quant(p.quant, (uint8_t*)p.y + row * p.D + at, on ? inside(p.D, at) : 0, v[c]);
+            }
+            if (on && lane == 0) p.scale[row] = a / M;
+        }
+    }
+}
+
+// rows longer than 32768: one workgroup a row, the row read again for each step (from the cache where it fits)
+template <typename T>
+__global__ __launch_bounds__(1024) void k_rms_long(const NormArgs p) {
+    __shared__ float slot[16];
+    for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T* src = p.residual != nullptr ? (const T*)p.h + row * p.D : (const T*)p.x + row * p.ldx;
+        float sum = 0.0f, v[8], w[8];
+        for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
+            const int n = inside(p.D, at);
+            load8((const T*)p.x + row * p.ldx + at, n, v);
+            if (p.residual != nullptr) {
+                load8((const T*)p.residual + row * p.ldr + at, n, w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = (float)(T)(v[i] + w[i]);
+                store8((T*)p.h + row * p.D + at, n, v);
+            }
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) part = fmaf(v[i], v[i], part);
+            sum += part;
+        }
+        sum = reduce_threads<1024, Sum>(sum, slot);
+        const float s = rsqrtf(sum / (float)p.D + p.eps);
+        float a = 0.0f, f = 1.0f;
+        const float M = quant_max(p.quant);
+        for (int step = p.quant == SPANQR_QUANT_NONE ? 1 : 0; step < 2; ++step) {
+            // a thread reads back only what it wrote itself
+            for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
+                const int n = inside(p.D, at);
+                load8(src + at, n, v);
+                load_weight(p.weight, p.wtype, at, n, w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = v[i] * s * w[i];
+                if (step == 0) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) a = nan_max(a, fabsf(v[i]));
+                } else if (p.quant == SPANQR_QUANT_NONE) {
+                    store8((T*)p.y + row * p.D + at, n, v);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] *= f;
+                    store_quant(p.quant, (uint8_t*)p.y + row * p.D + at, n, v);
+                }
+            }
+            if (step == 0) {
+                a = reduce_threads<1024, NanMax>(a, slot);
+                f = quant_factor(a, M);
+                if (threadIdx.x == 0) p.scale[row] = a / M;
+            }
+        }
+    }
+}
+
+// The weight's gradient is a sum over rows: a workgroup keeps its rows' part in registers (each thread always holds the
+// same columns), adds its ROWS groups through LDS and writes one row of partial sums; k_rms_dw adds those.
+template <typename T, int GROUP, int NCH>
+__global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void k_rms_grad(const GradArgs p) {
+    constexpr int BLOCK = GROUP > 256 ? GROUP : 256, ROWS = BLOCK / GROUP;
+    struct Two {
+        float a, b;
+        __device__ __forceinline__ Two operator+(const Two& o) const { return Two{a + o.a, b + o.b}; }
+    };
+    __shared__ float slot[2 * (BLOCK / 64)];
+    __shared__ float add[ROWS > 1 ? (ROWS - 1) * GROUP * NCH * 8 : 1];
+    const int lane = threadIdx.x % GROUP, group = threadIdx.x / GROUP;
+    float w[NCH][8], dw[NCH][8];
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        const long at = 8l * (lane + c * GROUP);
+        load_weight(p.weight, p.wtype, at, inside(p.D, at), w[c]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dw[c][i] = 0.0f;
+    }
+    for (long base = (long)blockIdx.x * ROWS; base < p.rows; base += (long)gridDim.x * ROWS) {
+        const long row = base + group;
+        const bool on = row < p.rows;
+        float h[NCH][8], u[NCH][8];
+        float hh = 0.0f, uh = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const long at = 8l * (lane + c * GROUP);
+            const int n = on ? inside(p.D, at) : 0;
+            load8((const T*)p.h + row * p.ldh + at, n, h[c]);
+            load8((const T*)p.dy + row * p.lddy + at, n, u[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                hh = fmaf(h[c][i], h[c][i], hh);
+                uh = fmaf(u[c][i] * w[c][i], h[c][i], uh);
+            }
+        if constexpr (GROUP <= 64) {
+            hh = reduce_lanes<GROUP, Sum>(hh);
+            uh = reduce_lanes<GROUP, Sum>(uh);
+        } else {
+            hh = reduce_lanes<64, Sum>(hh);
+            uh = reduce_lanes<64, Sum>(uh);
+            if ((threadIdx.x & 63) == 0) {
+                slot[threadIdx.x >> 6] = hh;
+                slot[(BLOCK / 64) + (threadIdx.x >> 6)] = uh;
+            }
+            __syncthreads();
+            hh = slot[0];
+            uh = slot[BLOCK / 64];
+#pragma unroll
+            for (int i = 1; i < BLOCK / 64; ++i) {
+                hh += slot[i];
+                uh += slot[BLOCK / 64 + i];
+            }
+            __syncthreads();
+        }
+        // a group without a row adds zeros, also where eps is 0
+        const float s = on ? rsqrtf(hh / (float)p.D + p.eps) : 0.0f;
+        const float m = s * uh / (float)p.D;   // the mean of u n
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const long at = 8l * (lane + c * GROUP);
+            const int n = on ? inside(p.D, at) : 0;
+            float d[8];
+            if (p.dh != nullptr) {
+                load8((const T*)p.dh + row * p.lddh + at, n, d);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float nrm = h[c][i] * s;
+                dw[c][i] = fmaf(u[c][i], nrm, dw[c][i]);
+                d[i] = fmaf(s, u[c][i] * w[c][i] - nrm * m, d[i]);
+            }
+            store8((T*)p.dx + row * p.D + at, n, d);
+        }
+    }
+    if (p.part == nullptr) return;
+    if constexpr (ROWS > 1) {
+        if (group > 0) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) add[((group - 1) * NCH * 8 + c * 8 + i) * GROUP + lane] = dw[c][i];
+        }
+        __syncthreads();
+        if (group > 0) return;
+        for (int g = 0; g < ROWS - 1; ++g)
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dw[c][i] += add[(g * NCH * 8 + c * 8 + i) * GROUP + lane];
+    }
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+        const long at = 8l * (lane + c * GROUP);
+        store8(p.part + blockIdx.x * p.D + at, inside(p.D, at), dw[c]);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void k_rms_grad_long(const GradArgs p) {
+    __shared__ float slot[16];
+    for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const T* hr = (const T*)p.h + row * p.ldh;
+        const T* ur = (const T*)p.dy + row * p.lddy;
+        float h[8], u[8], w[8], d[8];
+        float hh = 0.0f, uh = 0.0f;
+        for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
+            const int n = inside(p.D, at);
+            load8(hr + at, n, h);
+            load8(ur + at, n, u);
+            load_weight(p.weight, p.wtype, at, n, w);
+            float a = 0.0f, b = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                a = fmaf(h[i], h[i], a);
+                // (weights past the end are not read as 0 without a weight tensor; u is 0 there)
+                b = fmaf(u[i] * w[i], h[i], b);
+            }
+            hh += a;
+            uh += b;
+        }
+        hh = reduce_threads<1024, Sum>(hh, slot);
+        uh = reduce_threads<1024, Sum>(uh, slot);
+        const float s = rsqrtf(hh / (float)p.D + p.eps);
+        const float m = s * uh / (float)p.D;
+        for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
+            const int n = inside(p.D, at);
+            load8(hr + at, n, h);
+            load8(ur + at, n, u);
+            load_weight(p.weight, p.wtype, at, n, w);
+            if (p.dh != nullptr) {
+                load8((const T*)p.dh + row * p.lddh + at, n, d);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] = 0.0f;
+            }
+            float dw[8];
+            float* part = p.part == nullptr ? nullptr : p.part + blockIdx.x * p.D + at;
+            if (part != nullptr && row != blockIdx.x) {
+                load8(part, n, dw);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dw[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float nrm = h[i] * s;
+                dw[i] = fmaf(u[i], nrm, dw[i]);
+                d[i] = fmaf(s, u[i] * w[i] - nrm * m, d[i]);
+            }
+            store8((T*)p.dx + row * p.D + at, n, d);
+            if (part != nullptr) store8(part, n, dw);
+        }
+    }
+}
+
+// dw[d] = sum of part[0..parts)[d]: 64 columns a workgroup, 16 threads a column, added in a fixed order
+__global__ __launch_bounds__(1024) void k_rms_dw(const float* part, int parts, long D, void* dw, int wtype) {
+    __shared__ float add[16][64];
+    const int col = threadIdx.x & 63, at = threadIdx.x >> 6;
+    const long d = 64l * blockIdx.x + col;
+    float sum = 0.0f;
+    if (d < D) {
+#pragma unroll 8
+        for (int i = at; i < parts; i += 16) sum += part[i * D + d];
+    }
+    add[at][col] = sum;
+    __syncthreads();
+    if (at > 0 || d >= D) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) sum += add[i][col];
+    if (wtype == SPANQR_BF16)
+        ((bf16*)dw)[d] = (bf16)sum;
+    else if (wtype == SPANQR_FP16)
+        ((fp16*)dw)[d] = (fp16)sum;
+    else
+        ((float*)dw)[d] = sum;
+}
+
+constexpr long LONG_ROW = 32768;    // longest row that stays in registers
+constexpr long MAX_D = 1l << 24;
+constexpr int GRAD_PARTS = 1024;    // most workgroups of the gradient, and so rows of partial sums
+
+// threads a row (GROUP) and pieces a thread (NCH) for rows of D elements
+struct Split {
+    int group, nch;
+};
+Split split_of(long D) {
+    if (D <= 128) return {16, 1};
+    if (D <= 512) return {64, 1};
+    if (D <= 1024) return {64, 2};
+    if (D <= 2048) return {64, 4};
+    if (D <= 4096) return {256, 2};
+    if (D <= 8192) return {256, 4};
+    if (D <= 16384) return {512, 4};
+    return {1024, 4};
+}
+
+int grid_of(long rows, int group, int most) {
+    const int per = group >= 256 ? 1 : 256 / group;
+    const long need = (rows + per - 1) / per;
+    return (int)(need < most ? need : most);
+}
+
+int grad_parts(long rows, long D) {
+    if (D > LONG_ROW) return (int)(rows < 256 ? rows : 256);
+    return grid_of(rows, split_of(D).group, GRAD_PARTS);
+}
+
+#define SPANQR_SPLITS(LAUNCH)                     \
+    switch (s.group * 8 + s.nch) {                \
+        case 16 * 8 + 1: LAUNCH(16, 1); break;    \
+        case 64 * 8 + 1: LAUNCH(64, 1); break;    \
+        case 64 * 8 + 2: LAUNCH(64, 2); break;    \
+        case 64 * 8 + 4: LAUNCH(64, 4); break;    \
+        case 256 * 8 + 2: LAUNCH(256, 2); break;  \
+        case 256 * 8 + 4: LAUNCH(256, 4); break;  \
+        case 512 * 8 + 4: LAUNCH(512, 4); break;  \
+        default: LAUNCH(1024, 4); break;          \
+    }
+
+template <typename T>
+void launch_norm(const NormArgs& p, hipStream_t st) {
+    if (p.D > LONG_ROW) {
+        k_rms_long<T><<<(int)(p.rows < 1024 ? p.rows : 1024), 1024, 0, st>>>(p);
+        return;
+    }
+    const Split s = split_of(p.D);
+    const int grid = grid_of(p.rows, s.group, 2048);
+#define LAUNCH(G, C) k_rms<T, G, C><<<grid, G > 256 ? G : 256, 0, st>>>(p)
+    SPANQR_SPLITS(LAUNCH)
+#undef LAUNCH
+}
+
+template <typename T>
+void launch_grad(const GradArgs& p, int grid, hipStream_t st) {
+    if (p.D > LONG_ROW) {
+        k_rms_grad_long<T><<<grid, 1024, 0, st>>>(p);
+        return;
+    }
+    const Split s = split_of(p.D);
+#define LAUNCH(G, C) k_rms_grad<T, G, C><<<grid, G > 256 ? G : 256, 0, st>>>(p)
+    SPANQR_SPLITS(LAUNCH)
+#undef LAUNCH
+}
+
+bool known(int type) { return type == SPANQR_BF16 || type == SPANQR_FP16 || type == SPANQR_FP32; }
+
+int check_sizes(const char* what, int type, int wtype, long rows, long D) {
+    if (!known(type) || !known(wtype)) return error(SPANQR_EINVAL, "%s: unknown type", what);
+    if (rows < 0 || D < 1 || D > MAX_D || rows > (1l << 40) / D)
+        return error(SPANQR_EINVAL, "%s: rows = %ld, D = %ld (D from 1 to %ld)", what, rows, D, MAX_D);
+    return SPANQR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int spanqr_rms_norm(int type, int wtype, int quant, long rows, long D, const void* x, long ldx, const void* residual,
+                    long ldr, const void* weight, float eps, void* h, void* y, float* scale, void* stream) {
+    const int rc = check_sizes("rms_norm", type, wtype, rows, D);
+    if (rc != SPANQR_OK) return rc;
+    if (quant != SPANQR_QUANT_NONE && quant != SPANQR_QUANT_FP8 && quant != SPANQR_QUANT_INT8)
+        return error(SPANQR_EINVAL, "rms_norm: unknown quant %d", quant);
+    if (rows == 0) return SPANQR_OK;
+    if (x == nullptr || y == nullptr || (residual != nullptr) != (h != nullptr) ||
+        (quant != SPANQR_QUANT_NONE) != (scale != nullptr))
+        return error(SPANQR_EINVAL, "rms_norm: a missing or needless pointer");
+    if (rows > 1 && (ldx < D || (residual != nullptr && ldr < D)))
+        return error(SPANQR_EINVAL, "rms_norm: a row stride below D");
+    const NormArgs p = {rows, D, ldx, ldr, x, residual, weight, wtype, quant, eps, h, y, scale};
+    hipStream_t st = (hipStream_t)stream;
+    if (type == SPANQR_BF16)
+        launch_norm<bf16>(p, st);
+    else if (type == SPANQR_FP16)
+        launch_norm<fp16>(p, st);
+    else
+        launch_norm<float>(p, st);
+    return launched("rms_norm");
+}
+
+long spanqr_rms_norm_backward_workspace(long rows, long D) {
+    if (rows < 0 || D < 1 || D > MAX_D) return error(SPANQR_EINVAL, "rms_norm_backward: rows = %ld, D = %ld", rows, D);
+    return 4l * grad_parts(rows, D) * D;
+}
+
+int spanqr_rms_norm_backward(int type, int wtype, long rows, long D, const void* dy, long lddy, const void* h, long ldh,
+                             const void* weight, const void* dh, long lddh, float eps, void* dx, void* dw,
+                             void* workspace, long workspace_bytes, void* stream) {
+    const int rc = check_sizes("rms_norm_backward", type, wtype, rows, D);
+    if (rc != SPANQR_OK) return rc;
+    const int parts = grad_parts(rows, D);
+    if (dw != nullptr && parts > 0 && (workspace == nullptr || workspace_bytes < 4l * parts * D))
+        return error(SPANQR_EINVAL, "rms_norm_backward: the workspace needs %ld bytes", 4l * parts * D);
+    hipStream_t st = (hipStream_t)stream;
+    if (rows > 0) {
+        if (dy == nullptr || h == nullptr || dx == nullptr)
+            return error(SPANQR_EINVAL, "rms_norm_backward: a missing pointer");
+        if (rows > 1 && (lddy < D || ldh < D || (dh != nullptr && lddh < D)))
+            return error(SPANQR_EINVAL, "rms_norm_backward: a row stride below D");
+        const GradArgs p = {rows, D, lddy, ldh, lddh, dy, h, weight, dh, wtype, eps, dx,
+                            dw == nullptr ? nullptr : (float*)workspace};
+        if (type == SPANQR_BF16)
+            launch_grad<bf16>(p, parts, st);
+        else if (type == SPANQR_FP16)
+            launch_grad<fp16>(p, parts, st);
+        else
+            launch_grad<float>(p, parts, st);
+    }
+    if (dw != nullptr)
+        k_rms_dw<<<(int)((D + 63) / 64), 1024, 0, st>>>((const float*)workspace, parts, D, dw, wtype);
+    return launched("rms_norm_backward");
+}
+
+}  // extern "C"

@@ -36,6 +36,7 @@
 #include <tuple>
 
 #include "../../include/spanqr.h"
+#include "host.h"
 
 #pragma clang fp contract(off)
 
@@ -3507,6 +3508,18 @@ int enqueue_orth(spanqr_plan* p, int n, const MatsIn& X, long ldx, const MatsOut
 }
 
 }  // namespace
+
+// the error text of the library's other source files (host.h)
+namespace spanqr_host {
+int set_error(int code, const char* text) noexcept {
+    try {
+        g_err = text;
+    } catch (...) {
+        g_err.clear();
+    }
+    return code;
+}
+}  // namespace spanqr_host
 
 extern "C" {
 

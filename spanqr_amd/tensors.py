@@ -1,0 +1,70 @@
+"""What the training operators (loss.py, norm.py, clip.py) share: types of the C ABI, checks of tensors, and the device
+and stream a call runs on."""
+import contextlib
+
+import torch
+
+from . import _lib
+from .plan import stream_handle
+
+TYPES = {torch.float32: _lib.FP32, torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
+
+
+def check_tensor(what, name, t, dtypes=tuple(TYPES)):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what}: {name} must be a tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{what}: {name} must be {' or '.join(str(d)[6:] for d in dtypes)}, got {t.dtype}")
+    if t.device.type != "cuda":
+        raise TypeError(f"{what}: {name} must be on a GPU (ROCm device); there is no CPU implementation")
+
+
+def check_same(what, name, t, device, shape=None, dtype=None):
+    if t.device != device:
+        raise ValueError(f"{what}: {name} is on {t.device}, not on {device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} must be {list(shape)}, got {list(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{what}: {name} must be {str(dtype)[6:]}, got {t.dtype}")
+
+
+def rows_of(t, D):
+    """t [..., D] as [rows, D] with neighbouring elements in a row; copied only where no such view exists (or rows
+    overlap)"""
+    if t.dim() != 2:
+        t = t.reshape(-1, D)
+    if (t.stride(1) != 1 and D > 1) or (t.stride(0) < D and t.shape[0] > 1):
+        t = t.contiguous()
+    return t
+
+
+@contextlib.contextmanager
+def _other_device(device):
+    with torch.cuda.device(device):
+        yield stream_handle(device)
+
+
+class _Here:
+    """`with` on the current device: the stream alone"""
+    __slots__ = ("stream",)
+
+    def __init__(self, stream):
+        self.stream = stream
+
+    def __enter__(self):
+        return self.stream
+
+    def __exit__(self, *exc):
+        return False
+
+
+def on(device):
+    """`with on(device) as stream`: the call's current stream on `device`, with that device current"""
+    if device.index == torch.cuda.current_device():
+        return _Here(stream_handle(device))
+    return _other_device(device)
+
+
+def workspace(nbytes, device):
+    """from torch's caching allocator: it may be freed while the call's work is pending on the current stream"""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
