@@ -109,6 +109,17 @@ def test_loss_and_gradients(cuda, N, H, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,H,V", [(2100, 136, 9001), (4111, 264, 20000), (700, 1032, 33000), (2304, 2048, 8192)])
+def test_large(cuda, N, H, V, dtype):
+    """the largest tiles, dx over several parts of the vocabulary, pieces of the tokens"""
+    print(f"linear_cross_entropy {N}x{H}x{V} {dtype}", flush=True)
+    x, W, t = make(N, H, V, dtype, 21)
+    check_call(x, W, t, "none", (sp.linear_cross_entropy(x, W, t, reduction="none"), None, None))
+    check_call(x, W, t, "mean", sp.linear_cross_entropy_grad(x, W, t))
+    check_call(x, W, t, "mean", sp.linear_cross_entropy_grad(x, W, t, max_workspace=100 << 20))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("N,H,V", [(7, 65, 33), (300, 128, 520), (64, 200, 1000)])
 def test_weights_and_scale(cuda, N, H, V, dtype):
     x, W, t = make(N, H, V, dtype, 2)
