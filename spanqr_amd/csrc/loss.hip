@@ -9,6 +9,8 @@
 // the exponentials p = exp(z - m) themselves, rounded to the 16-bit type once. One pass over p turns them into G
 // (times exp(m - lse), the target's element from its fp32 logit), and G goes into the other two products. So nothing
 // is multiplied twice, and what is held is 16 bits an element for as many tokens at a time as the workspace takes.
+#include <type_traits>
+
 #include "elements.h"
 #include "host.h"
 
@@ -91,55 +93,54 @@ __device__ __forceinline__ void load_lds_any(const void* at, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "memory");
 }
 
-// One operand's tile of R rows (m or n) by 64 k in LDS, and its way there and into registers.
-// ROWS (k neighbours in memory): R rows of 128 bytes; the 16-byte chunk c of a row lies at c ^ swizzle(row), so that
+constexpr int BK = 32, STAGES = 4;   // k of a step, and steps in LDS
+
+// One operand's tiles of R rows (m or n) by 32 k in LDS, and the way there and into registers.
+// ROWS (k neighbours in memory): R rows of 64 bytes; the 16-byte chunk c of a row lies at c ^ swizzle(row), so that
 // the 16 rows a matrix instruction reads spread over the banks.
-// Otherwise (m or n neighbours): 64 k-rows of 2 R bytes, read by the transposing LDS read (16 lanes fetch 4 k-rows of
+// Otherwise (m or n neighbours): 32 k-rows of 2 R bytes, read by the transposing LDS read (16 lanes fetch 4 k-rows of
 // 16 columns and each gets one column's 4 k); the 32-byte block b of a row lies at b ^ swizzle(k).
 // SPREAD (ROWS, logits): row r of subtile i of a group of 64 is row 16 (r / 4) + 4 i + r % 4, so that a lane's results
 // of four subtiles are 16 neighbouring columns of C.
 template <typename T, bool ROWS, bool SPREAD, int R, int WAVES, int SUB>
 struct Tile {
     typedef typename Vec<T>::x8 x8;
-    static constexpr int BYTES = R * 128;
-    static constexpr int LOADS = BYTES / 1024 / WAVES;   // instructions of 64 x 16 bytes per wavefront
+    static constexpr int BYTES = R * 2 * BK;
+    static constexpr int LOADS = BYTES / 1024 / WAVES;   // instructions of 64 x 16 bytes per wavefront and step
     static constexpr int RB = 2 * R, PER = 1024 / RB, LPR = RB / 16;
 
     const char* base;            // of this tile's rows at k = 0
-    long step;                   // bytes for 64 k
+    long step;                   // bytes for 32 k
     uint32_t off[LOADS];
     uint32_t dst;                // LDS of the wavefront's first instruction
-    uint32_t at[ROWS ? 2 : SUB]; // LDS of the lane's fragments
-    long ld;
+    uint32_t at[ROWS ? 1 : SUB]; // LDS of the lane's fragments
 
     __device__ __forceinline__ static int swizzle(int i) {   // of a row, or of a k
         if constexpr (ROWS)
-            return SPREAD ? (i & 3) | (i >> 4 & 1) << 2 : i & 7;
+            return SPREAD ? i >> 4 & 3 : i >> 2 & 3;
         else
             return R >= 256 ? (i & 3) | (i >> 3 & 3) << 2 : R == 128 ? (i & 3) | (i >> 3 & 1) << 2 : (i >> 1 & 1) | (i >> 3 & 1) << 1;
     }
 
-    __device__ __forceinline__ void init(const void* src, long ld_, long rows, long r0, long k0, lds_char* lds, int wave,
-                                         int lane, int first) {
-        ld = ld_;
+    __device__ __forceinline__ void init(const void* src, long ld, long rows, long r0, long k0, lds_char* lds, int wave, int lane,
+                                         int first) {
         const int lo = lane & 15, hi = lane >> 4;
         const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
         dst = __builtin_amdgcn_readfirstlane(lds0 + wave * LOADS * 1024);
         if constexpr (ROWS) {
             base = (const char*)src + 2 * (r0 * ld + k0);
-            step = 128;
+            step = 2 * BK;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const int row = 8 * (wave * LOADS + i) + (lane >> 3);
+                const int row = 16 * (wave * LOADS + i) + (lane >> 2);
                 const long r = r0 + row < rows ? row : rows - 1 - r0;   // rows past the end: any, not used
-                off[i] = (uint32_t)(2 * r * ld + 16 * ((lane & 7) ^ swizzle(row)));
+                off[i] = (uint32_t)(2 * r * ld + 16 * ((lane & 3) ^ swizzle(row)));
             }
             const int row = SPREAD ? 16 * (lo >> 2) + (lo & 3) : lo;
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) at[ks] = lds0 + (first + row) * 128 + 16 * ((4 * ks + hi) ^ (lo & 7));
+            at[0] = lds0 + (first + row) * 64 + 16 * (hi ^ swizzle(row));
         } else {
             base = (const char*)src + 2 * (r0 + k0 * ld);
-            step = 128 * ld;
+            step = 2 * BK * ld;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int k = (wave * LOADS + i) * PER + lane / LPR, c = lane % LPR;
@@ -154,33 +155,40 @@ struct Tile {
         }
     }
 
-    // 64 k from k step `t` on into buffer `buf`; `left`: how many of them there are
-    __device__ __forceinline__ void load(int t, int buf, long left, const void* zeros, int wave, int lane) const {
+    // Stages 0 and 1 are those of this turn of the loop, 2 and 3 of the other. The bit is clear in every fragment's and
+    // every load's address: an operand's stages start on a multiple of all of them.
+    __device__ __forceinline__ void turn() {
+        dst ^= 2 * BYTES;
+#pragma unroll
+        for (int i = 0; i < (ROWS ? 1 : SUB); ++i) at[i] ^= 2 * BYTES;
+    }
+
+    // instruction i of the load of k 32 t on into stage `stage`
+    __device__ __forceinline__ void load(int t, int stage, int i) const {
+        load_lds(base + t * step, off[i], (dst ^ (stage & 2) * BYTES) + (stage & 1) * BYTES + i * 1024);
+    }
+    // the whole of it where only `left` k are left (none where left <= 0)
+    __device__ __forceinline__ void load_end(int t, int stage, int left, const void* zeros, int wave, int lane) const {
         const char* b = base + t * step;
-        if (left >= 64) {
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) load_lds(b, off[i], dst + buf * BYTES + i * 1024);
-        } else {
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                int k;
-                if constexpr (ROWS)
-                    k = 8 * ((lane & 7) ^ swizzle(8 * (wave * LOADS + i) + (lane >> 3)));
-                else
-                    k = (wave * LOADS + i) * PER + lane / LPR;
-                load_lds_any(k < left ? (const void*)(b + off[i]) : zeros, dst + buf * BYTES + i * 1024);
-            }
+        for (int i = 0; i < LOADS; ++i) {
+            int k;
+            if constexpr (ROWS)
+                k = 8 * ((lane & 3) ^ swizzle(16 * (wave * LOADS + i) + (lane >> 2)));
+            else
+                k = (wave * LOADS + i) * PER + lane / LPR;
+            load_lds_any(k < left ? (const void*)(b + off[i]) : zeros, (dst ^ (stage & 2) * BYTES) + (stage & 1) * BYTES + i * 1024);
         }
     }
 
-    // subtile i (16 rows) of k 32 ks to 32 ks + 31
-    __device__ __forceinline__ x8 read(int i, int ks, int buf) const {
+    // subtile i (16 rows)
+    __device__ __forceinline__ x8 read(int i, int stage) const {
         if constexpr (ROWS) {
             const int row = SPREAD ? 64 * (i >> 2) + 4 * (i & 3) : 16 * i;
-            return *(__attribute__((address_space(3))) const x8*)(uintptr_t)(at[ks] + buf * BYTES + row * 128);
+            return *(__attribute__((address_space(3))) const x8*)(uintptr_t)(at[0] + stage * BYTES + row * 64);
         } else {
             typedef __attribute__((address_space(3))) s16x4 lds_s4;
-            const uint32_t a = at[i] + buf * BYTES + ks * 32 * RB;
+            const uint32_t a = at[i] + stage * BYTES;
             const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)a);
             const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(a + 4 * RB));
             return __builtin_bit_cast(x8, __builtin_shufflevector(v, w, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -188,18 +196,19 @@ struct Tile {
     }
 };
 
-// A workgroup's tile is BM x BN, a wavefront's WM x WN in 16 x 16 subtiles, 64 k at a time through two LDS buffers. A k
-// step has four parts, each with half the wavefront's rows of A and 32 k: a part's matrix instructions run while the
-// next part's operands come from LDS. Before the last part every wavefront has read the whole step, so there is the one
-// barrier: behind it the next step's first operands are read and the step after that is loaded into the buffer that
-// became free, while the last part's instructions run.
+// A workgroup's tile is BM x BN, a wavefront's WM x WN in 16 x 16 subtiles, with four steps of 32 k in LDS. A step has two
+// parts, each with half the wavefront's rows of A: a part's matrix instructions run while the next part's operands come
+// from LDS. Between the parts every wavefront has read the whole step, so there is the one barrier: behind it the
+// next step's first operands are read and the step four on is loaded into the stage that became free. A load has two and a half
+// steps to arrive.
 template <typename T, bool A_ROWS, bool B_ROWS, int EPILOGUE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const ProductArgs q) {
     typedef typename Vec<T>::x8 x8;
     constexpr int WAVES = (BM / WM) * (BN / WN), IM = WM / 16, IN = WN / 16, HALF = IM / 2;
     typedef Tile<T, A_ROWS, EPILOGUE == LOGITS, BM, WAVES, IM> TA;
     typedef Tile<T, B_ROWS, false, BN, WAVES, IN> TB;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * (TA::BYTES + TB::BYTES)];
+    constexpr int LOADS = TA::LOADS + TB::LOADS;
+    __shared__ __attribute__((aligned(1024))) char smem[STAGES * (TA::BYTES + TB::BYTES)];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
     const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
 
@@ -216,92 +225,138 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const
 
     const long k0 = split * q.split_k, k1 = k0 + q.split_k < q.K ? k0 + q.split_k : q.K;
     const long K = k1 > k0 ? k1 - k0 : 0;
-    const int steps = (int)((K + 63) / 64);
+    const int steps = 2 * (int)((K + 2 * BK - 1) / (2 * BK));
     TA a;
     TB b;
     a.init(q.A, q.lda, q.M, m0, k0, (lds_char*)smem, wave, lane, wm);
-    b.init(q.B, q.ldb, q.N, n0, k0, (lds_char*)smem + 2 * TA::BYTES, wave, lane, wn);
+    b.init(q.B, q.ldb, q.N, n0, k0, (lds_char*)smem + STAGES * TA::BYTES, wave, lane, wn);
 
     f32x4 c[IM][IN] = {};
     x8 fa0[HALF], fa1[HALF], fb0[IN], fb1[IN];
-    auto load = [&](int t, int buf) {
-        a.load(t, buf, K - 64l * t, q.zeros, wave, lane);
-        b.load(t, buf, K - 64l * t, q.zeros, wave, lane);
-    };
-    auto read_a = [&](x8(&f)[HALF], int half, int ks, int buf) {
+    // The last 64 k, the only ones that may be fewer, are steps 0 and 1, and k 32 (t - 2) on are step t: so the loop loads
+    // whole steps only, and there is an even number of them.
+    auto load_first = [&](int t) {
+        const int k = steps - 2 + t;
+        const long left = K - (long)BK * k;
+        if (left >= BK) {
 #pragma unroll
-        for (int i = 0; i < HALF; ++i) f[i] = a.read(half * HALF + i, ks, buf);
-    };
-    auto read_b = [&](x8(&f)[IN], int ks, int buf) {
+            for (int i = 0; i < TA::LOADS; ++i) a.load(k, t, i);
 #pragma unroll
-        for (int j = 0; j < IN; ++j) f[j] = b.read(j, ks, buf);
-    };
-    auto multiply = [&](const x8(&f)[HALF], const x8(&g)[IN], int half) {
-#pragma unroll
-        for (int i = 0; i < HALF; ++i)
-#pragma unroll
-            for (int j = 0; j < IN; ++j) c[half * HALF + i][j] = Vec<T>::mfma(f[i], g[j], c[half * HALF + i][j]);
-    };
-    auto arrived = [&] {   // this wavefront's LDS reads and loads are done, and then everybody's
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    };
-    auto step = [&](int t, int buf) {
-        read_a(fa1, 1, 0, buf);
-        multiply(fa0, fb0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        read_a(fa0, 0, 1, buf);
-        read_b(fb1, 1, buf);
-        multiply(fa1, fb0, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        read_a(fa1, 1, 1, buf);
-        multiply(fa0, fb1, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        if (t + 1 < steps) {
-            arrived();
-            if (t + 2 < steps) load(t + 2, buf);
-            read_a(fa0, 0, 0, buf ^ 1);
-            read_b(fb0, 0, buf ^ 1);
+            for (int i = 0; i < TB::LOADS; ++i) b.load(k, t, i);
+        } else {
+            a.load_end(k, t, (int)left, q.zeros, wave, lane);
+            b.load_end(k, t, (int)left, q.zeros, wave, lane);
         }
-        multiply(fa1, fb1, 1);
-        __builtin_amdgcn_sched_barrier(0);
+    };
+    // Step t in stage ODD (0 or 1) of this turn; f: this step's part of B, g: where the next one's goes. Reads and loads
+    // are spread over the subtile rows' instructions, and the fences keep that order. Behind the last step an old stage
+    // is read once more, for nothing.
+    auto step = [&](int t, auto odd, x8(&f)[IN], x8(&g)[IN]) {
+        constexpr int ODD = decltype(odd)::value;
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) {
+            if (2 * i < HALF) {
+                fa1[2 * i] = a.read(HALF + 2 * i, ODD);
+                fa1[2 * i + 1] = a.read(HALF + 2 * i + 1, ODD);
+            }
+#pragma unroll
+            for (int j = 0; j < IN; ++j) c[i][j] = Vec<T>::mfma(fa0[i], f[j], c[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // This wavefront has read the step and its loads of the next one have arrived (those of the two after it may be
+        // under way); then everybody's.
+        if (t + 3 < steps)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");
+        if constexpr (ODD) {
+            a.turn();
+            b.turn();
+        }
+        constexpr int NEXT = ODD ? 0 : 1, FREE = ODD ? 3 : 0;
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) {
+#pragma unroll
+            for (int j = 2 * i * IN / HALF; j < 2 * (i + 1) * IN / HALF && j < IN; ++j) g[j] = b.read(j, NEXT);
+            if (2 * i >= HALF) {
+                fa0[2 * i - HALF] = a.read(2 * i - HALF, NEXT);
+                fa0[2 * i - HALF + 1] = a.read(2 * i - HALF + 1, NEXT);
+            }
+            if (t + STAGES < steps) {
+#pragma unroll
+                for (int j = i * LOADS / HALF; j < (i + 1) * LOADS / HALF; ++j) {
+                    if (j < TA::LOADS)
+                        a.load(t + STAGES - 2, FREE, j);
+                    else
+                        b.load(t + STAGES - 2, FREE, j - TA::LOADS);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < IN; ++j) c[HALF + i][j] = Vec<T>::mfma(fa1[i], f[j], c[HALF + i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     if (steps > 0) {
-        load(0, 0);
-        arrived();
-        if (steps > 1) load(1, 1);
-        read_a(fa0, 0, 0, 0);
-        read_b(fb0, 0, 0);
-        for (int t = 0; t < steps; t += 2) {
-            step(t, 0);
-            if (t + 1 < steps) step(t + 1, 1);
+        load_first(0);
+        load_first(1);
+        if (steps > 2) {
+#pragma unroll
+            for (int t = 2; t < STAGES; ++t) {
+#pragma unroll
+                for (int i = 0; i < TA::LOADS; ++i) a.load(t - 2, t, i);
+#pragma unroll
+                for (int i = 0; i < TB::LOADS; ++i) b.load(t - 2, t, i);
+            }
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
+        asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < IN; ++j) fb0[j] = b.read(j, 0);
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) fa0[i] = a.read(i, 0);
+        int t = 0;
+        do {
+            step(t, std::integral_constant<int, 0>{}, fb0, fb1);
+            step(t + 1, std::integral_constant<int, 1>{}, fb1, fb0);
+            t += 2;
+        } while (t < steps);
     }
 
     // lane: row n = lo of C, elements m = 4 hi + 0..3 of each subtile (16 hi + 0..15 of four subtiles where SPREAD)
-#pragma unroll
-    for (int j = 0; j < IN; ++j) {
-        const long n = n0 + wn + 16 * j + lo;
-        if constexpr (EPILOGUE == LOGITS) {
-            const long first = m0 + wm + 16 * hi;   // of the lane's columns; each group of four subtiles is 64 on
-            float m = -INFINITY;
+    if constexpr (EPILOGUE == LOGITS) {
+        const long first = m0 + wm + 16 * hi;   // of the lane's columns; each group of four subtiles is 64 on
+        if (m0 + wm + WM > q.M) {               // columns past the vocabulary
 #pragma unroll
             for (int i = 0; i < IM; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if (first + 64 * (i >> 2) + 4 * (i & 3) + r >= q.M) c[i][j][r] = -INFINITY;
-                    m = nan_max(m, c[i][j][r]);
+                    const bool out = first + 64 * (i >> 2) + 4 * (i & 3) + r >= q.M;
+#pragma unroll
+                    for (int j = 0; j < IN; ++j) c[i][j][r] = out ? -INFINITY : c[i][j][r];
                 }
+        }
+#pragma unroll
+        for (int j = 0; j < IN; ++j) {
+            const long n = n0 + wn + 16 * j + lo;
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < IM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m = nan_max(m, c[i][j][r]);
             m = nan_max(m, __shfl_xor(m, 16));
             m = nan_max(m, __shfl_xor(m, 32));
             const float top = m == -INFINITY ? 0.0f : m;
             const long tgt = n < q.N ? q.target[n] - first : -1;
             if (tgt >= 0 && tgt < 64 * (IM / 4) && (tgt & 63) < 16 && first + tgt < q.M) {
+                const int k = (int)tgt;
                 float z = 0.0f;
 #pragma unroll
                 for (int i = 0; i < IM; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (tgt == 64 * (i >> 2) + 4 * (i & 3) + r) z = c[i][j][r];
+                    for (int r = 0; r < 4; ++r) z = k == 64 * (i >> 2) + 4 * (i & 3) + r ? c[i][j][r] : z;
                 q.zt[n] = z;
             }
             float sum = 0.0f;
@@ -324,8 +379,12 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
             if (hi == 0 && n < q.N && m0 + wm < q.M) q.stat[n * q.segs + (m0 + wm) / WM] = make_float2(m, sum);
-        } else {
-            const float alpha = q.acc == nullptr ? *q.alpha : 1.0f;
+        }
+    } else {
+        const float alpha = q.acc == nullptr ? *q.alpha : 1.0f;
+#pragma unroll
+        for (int j = 0; j < IN; ++j) {
+            const long n = n0 + wn + 16 * j + lo;
 #pragma unroll
             for (int i = 0; i < IM; ++i) {
                 const long m = m0 + wm + 16 * i + 4 * hi;
