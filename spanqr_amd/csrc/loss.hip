@@ -97,7 +97,8 @@ constexpr int BK = 32, STAGES = 4;   // k of a step, and steps in LDS
 
 // One operand's tiles of R rows (m or n) by 32 k in LDS, and the way there and into registers.
 // ROWS (k neighbours in memory): R rows of 64 bytes; the 16-byte chunk c of a row lies at c ^ swizzle(row), so that
-// the 16 rows a matrix instruction reads spread over the banks.
+// the 16 rows a matrix instruction reads spread over the banks (a 16-byte read takes lanes 0-3, 12-15, 20-27 of each 32
+// together, and then the others: 4 clocks this way, 8 with row / 4 itself in the place of its negative).
 // Otherwise (m or n neighbours): 32 k-rows of 2 R bytes, read by the transposing LDS read (16 lanes fetch 4 k-rows of
 // 16 columns and each gets one column's 4 k); the 32-byte block b of a row lies at b ^ swizzle(k).
 // SPREAD (ROWS, logits): row r of subtile i of a group of 64 is row 16 (r / 4) + 4 i + r % 4, so that a lane's results
@@ -117,7 +118,7 @@ struct Tile {
 
     __device__ __forceinline__ static int swizzle(int i) {   // of a row, or of a k
         if constexpr (ROWS)
-            return SPREAD ? i >> 4 & 3 : i >> 2 & 3;
+            return -(SPREAD ? i >> 4 : i >> 2) & 3;
         else
             return R >= 256 ? (i & 3) | (i >> 3 & 3) << 2 : R == 128 ? (i & 3) | (i >> 3 & 1) << 2 : (i >> 1 & 1) | (i >> 3 & 1) << 1;
     }
@@ -251,8 +252,9 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const
     // Step t in stage ODD (0 or 1) of this turn; f: this step's part of B, g: where the next one's goes. Reads and loads
     // are spread over the subtile rows' instructions, and the fences keep that order. Behind the last step an old stage
     // is read once more, for nothing.
-    auto step = [&](int t, auto odd, x8(&f)[IN], x8(&g)[IN]) {
+    auto step = [&](int t, auto odd, auto more, x8(&f)[IN], x8(&g)[IN]) {
         constexpr int ODD = decltype(odd)::value;
+        constexpr bool LOAD = decltype(more)::value;   // step t + 4 is loaded
 #pragma unroll
         for (int i = 0; i < HALF; ++i) {
             if (2 * i < HALF) {
@@ -265,7 +267,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const
         }
         // This wavefront has read the step and its loads of the next one have arrived (those of the two after it may be
         // under way); then everybody's.
-        if (t + 3 < steps)
+        if constexpr (LOAD)
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");
         else
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -283,7 +285,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const
                 fa0[2 * i - HALF] = a.read(2 * i - HALF, NEXT);
                 fa0[2 * i - HALF + 1] = a.read(2 * i - HALF + 1, NEXT);
             }
-            if (t + STAGES < steps) {
+            if constexpr (LOAD) {
 #pragma unroll
                 for (int j = i * LOADS / HALF; j < (i + 1) * LOADS / HALF; ++j) {
                     if (j < TA::LOADS)
@@ -313,16 +315,21 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         asm volatile("s_barrier" ::: "memory");
+        // (scalar loads that are still under way would make the compiler wait for all LDS reads in every turn)
+        __builtin_amdgcn_s_waitcnt(0xc07f);
 #pragma unroll
         for (int j = 0; j < IN; ++j) fb0[j] = b.read(j, 0);
 #pragma unroll
         for (int i = 0; i < HALF; ++i) fa0[i] = a.read(i, 0);
         int t = 0;
-        do {
-            step(t, std::integral_constant<int, 0>{}, fb0, fb1);
-            step(t + 1, std::integral_constant<int, 1>{}, fb1, fb0);
-            t += 2;
-        } while (t < steps);
+        for (; t + STAGES < steps; t += 2) {
+            step(t, std::integral_constant<int, 0>{}, std::true_type{}, fb0, fb1);
+            step(t + 1, std::integral_constant<int, 1>{}, std::true_type{}, fb1, fb0);
+        }
+        for (; t < steps; t += 2) {
+            step(t, std::integral_constant<int, 0>{}, std::false_type{}, fb0, fb1);
+            step(t + 1, std::integral_constant<int, 1>{}, std::false_type{}, fb1, fb0);
+        }
     }
 
     // lane: row n = lo of C, elements m = 4 hi + 0..3 of each subtile (16 hi + 0..15 of four subtiles where SPREAD)
