@@ -10,6 +10,7 @@
 // (times exp(m - lse), the target's element from its fp32 logit), and G goes into the other two products. So nothing
 // is multiplied twice, and what is held is 16 bits an element for as many tokens at a time as the workspace takes.
 #include <type_traits>
+#include <utility>
 
 #include "elements.h"
 #include "host.h"
@@ -24,26 +25,62 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 fp16x8 __attribute__((ext_vector_type(8)));
 
-constexpr float LOG2E = 1.44269504088896340736f;
-
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 template <typename T>
 struct Vec;
 template <>
 struct Vec<bf16> {
     typedef bf16x8 x8;
-    __device__ __forceinline__ static f32x4 mfma(x8 a, x8 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
 };
 template <>
 struct Vec<fp16> {
     typedef fp16x8 x8;
-    __device__ __forceinline__ static f32x4 mfma(x8 a, x8 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-    }
 };
+
+// c += a b, 16 x 16 x 32. In inline asm, because c has to stay where it is: the compiler moves accumulators about
+// between registers when they fill half the file. ACC: c in accumulation registers. It does not know that these are
+// matrix instructions, so the products' kernel waits itself before it reads c.
+#define SPANQR_MFMA(OP, AT)                                                                     \
+    asm volatile("v_mfma_f32_16x16x32_" OP " %0, %1, %2, %0" : "+" AT(c) : "v"(a), "v"(b))
+// The same, and behind it 16 bytes a lane from base + off to LDS at `lds` + IMM + 16 lane, asynchronously (counted by
+// vmcnt). The load too is in inline asm because the compiler would wait for it before any later LDS read; it has no
+// register output. The matrix instruction fills the wait between m0 and its use.
+#define SPANQR_MFMA_LOAD(OP, AT)                                                                 \
+    asm volatile("s_add_u32 m0, %5, %6\n\tv_mfma_f32_16x16x32_" OP " %0, %1, %2, %0\n\t"         \
+                 "global_load_lds_dwordx4 %3, %4"                                                \
+                 : "+" AT(c)                                                                     \
+                 : "v"(a), "v"(b), "v"(off), "s"(base), "s"(lds), "n"(IMM)                       \
+                 : "memory", "scc")
+template <typename T, bool ACC>
+__device__ __forceinline__ void mfma(typename Vec<T>::x8 a, typename Vec<T>::x8 b, f32x4& c) {
+    if constexpr (std::is_same<T, bf16>::value) {
+        if constexpr (ACC)
+            SPANQR_MFMA("bf16", "a");
+        else
+            SPANQR_MFMA("bf16", "v");
+    } else {
+        if constexpr (ACC)
+            SPANQR_MFMA("f16", "a");
+        else
+            SPANQR_MFMA("f16", "v");
+    }
+}
+template <typename T, bool ACC, int IMM>
+__device__ __forceinline__ void mfma_load(typename Vec<T>::x8 a, typename Vec<T>::x8 b, f32x4& c, const void* base, uint32_t off,
+                                          uint32_t lds) {
+    if constexpr (std::is_same<T, bf16>::value) {
+        if constexpr (ACC)
+            SPANQR_MFMA_LOAD("bf16", "a");
+        else
+            SPANQR_MFMA_LOAD("bf16", "v");
+    } else {
+        if constexpr (ACC)
+            SPANQR_MFMA_LOAD("f16", "a");
+        else
+            SPANQR_MFMA_LOAD("f16", "v");
+    }
+}
 
 // G is held in 16 bits; half precision has it times 2^10, so that probabilities down to 2^-34 stay normal or at least
 // count (bf16 has fp32's exponents)
@@ -65,14 +102,14 @@ struct ProductArgs {
     // logits
     const long* target;          // of token 0 of this piece
     float* zt;                   // the target's logit
-    float2* stat;                // [token][segs]: maximum, sum
+    float2* stat;                // [token][segs]: maximum (of z log2 e), sum
     long segs;
     void* p;                     // exponentials [token][ldp], or null
     long ldp;
     // dx, dW
     void* C;
     long ldc;
-    int vector;                  // C takes 8-byte stores
+    int vector;                  // C takes 16-byte stores
     float* acc;                  // fp32 sums [split][N][ldacc], or null: C directly
     long ldacc;
     int add;                     // add to what acc holds
@@ -84,8 +121,7 @@ enum { LOGITS, OUT };
 typedef __attribute__((address_space(3))) char lds_char;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// 16 bytes a lane from base + off to LDS at `lds` + 16 lane, asynchronously (counted by vmcnt). In inline asm because the
-// compiler would wait for it before any later LDS read; it has no register output.
+// 16 bytes a lane from base + off to LDS at `lds` + 16 lane, asynchronously
 __device__ __forceinline__ void load_lds(const void* base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
@@ -93,13 +129,14 @@ __device__ __forceinline__ void load_lds_any(const void* at, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "memory");
 }
 
-constexpr int BK = 32, STAGES = 4;   // k of a step, and steps in LDS
+constexpr int BK = 64;               // k of a step; two steps are in LDS
 
-// One operand's tiles of R rows (m or n) by 32 k in LDS, and the way there and into registers.
-// ROWS (k neighbours in memory): R rows of 64 bytes; the 16-byte chunk c of a row lies at c ^ swizzle(row), so that
-// the 16 rows a matrix instruction reads spread over the banks (a 16-byte read takes lanes 0-3, 12-15, 20-27 of each 32
-// together, and then the others: 4 clocks this way, 8 with row / 4 itself in the place of its negative).
-// Otherwise (m or n neighbours): 32 k-rows of 2 R bytes, read by the transposing LDS read (16 lanes fetch 4 k-rows of
+// One operand's tiles of R rows (m or n) by 64 k in LDS, and the way there and into registers.
+// ROWS (k neighbours in memory): R rows of 128 bytes; the 16-byte chunk c of a row lies at c ^ swizzle(row), so that the
+// 16 rows a matrix instruction reads spread over the banks. LDS serves lanes 0-3, 12-15, 20-27 of each 32 together and
+// then the others: the swizzle gives each of those sixteen a slot of its own among 256 bytes (a read then takes 4
+// clocks; 8 with swizzle(row) = row % 8).
+// Otherwise (m or n neighbours): 64 k-rows of 2 R bytes, read by the transposing LDS read (16 lanes fetch 4 k-rows of
 // 16 columns and each gets one column's 4 k); the 32-byte block b of a row lies at b ^ swizzle(k).
 // SPREAD (ROWS, logits): row r of subtile i of a group of 64 is row 16 (r / 4) + 4 i + r % 4, so that a lane's results
 // of four subtiles are 16 neighbouring columns of C.
@@ -111,16 +148,18 @@ struct Tile {
     static constexpr int RB = 2 * R, PER = 1024 / RB, LPR = RB / 16;
 
     const char* base;            // of this tile's rows at k = 0
-    long step;                   // bytes for 32 k
+    long step;                   // bytes for 64 k
     uint32_t off[LOADS];
-    uint32_t dst;                // LDS of the wavefront's first instruction
-    uint32_t at[ROWS ? 1 : SUB]; // LDS of the lane's fragments
+    uint32_t dst;                // LDS of the wavefront's first load into this step's buffer
+    uint32_t at[ROWS ? 2 : SUB]; // LDS of the lane's fragments in this step's buffer
 
     __device__ __forceinline__ static int swizzle(int i) {   // of a row, or of a k
-        if constexpr (ROWS)
-            return -(SPREAD ? i >> 4 : i >> 2) & 3;
-        else
+        if constexpr (ROWS) {
+            const int u = SPREAD ? (i >> 4 & 3) << 1 | (i >> 1 & 1) : i >> 1 & 7;
+            return ((u >> 2 ^ u >> 1) & 1) << 2 | (u >> 2) << 1 | (u & 1);
+        } else {
             return R >= 256 ? (i & 3) | (i >> 3 & 3) << 2 : R == 128 ? (i & 3) | (i >> 3 & 1) << 2 : (i >> 1 & 1) | (i >> 3 & 1) << 1;
+        }
     }
 
     __device__ __forceinline__ void init(const void* src, long ld, long rows, long r0, long k0, lds_char* lds, int wave, int lane,
@@ -133,12 +172,13 @@ struct Tile {
             step = 2 * BK;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const int row = 16 * (wave * LOADS + i) + (lane >> 2);
-                const long r = r0 + row < rows ? row : rows - 1 - r0;   // rows past the end: any, not used
-                off[i] = (uint32_t)(2 * r * ld + 16 * ((lane & 3) ^ swizzle(row)));
+                const int row = 8 * (wave * LOADS + i) + (lane >> 3);
+                const int r = (int)(r0 + row < rows ? row : rows - 1 - r0);   // rows past the end: any, not used
+                off[i] = (uint32_t)(2 * r) * (uint32_t)ld + 16 * ((lane & 7) ^ swizzle(row));
             }
             const int row = SPREAD ? 16 * (lo >> 2) + (lo & 3) : lo;
-            at[0] = lds0 + (first + row) * 64 + 16 * (hi ^ swizzle(row));
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) at[ks] = lds0 + (first + row) * 128 + 16 * ((4 * ks + hi) ^ swizzle(row));
         } else {
             base = (const char*)src + 2 * (r0 + k0 * ld);
             step = 2 * BK * ld;
@@ -147,7 +187,7 @@ struct Tile {
                 const int k = (wave * LOADS + i) * PER + lane / LPR, c = lane % LPR;
                 int col = 16 * ((c >> 1) ^ swizzle(k)) + 8 * (c & 1);
                 if (r0 + col >= rows) col = 0;
-                off[i] = (uint32_t)(2 * (k * ld + col));
+                off[i] = (uint32_t)(2 * k) * (uint32_t)ld + 2 * col;
             }
             const int k = 8 * hi + (lo >> 2);
 #pragma unroll
@@ -156,40 +196,38 @@ struct Tile {
         }
     }
 
-    // Stages 0 and 1 are those of this turn of the loop, 2 and 3 of the other. The bit is clear in every fragment's and
-    // every load's address: an operand's stages start on a multiple of all of them.
+    // to the other buffer (the bit is clear in every address: each operand's buffers start on a multiple of both)
     __device__ __forceinline__ void turn() {
-        dst ^= 2 * BYTES;
+        dst ^= BYTES;
 #pragma unroll
-        for (int i = 0; i < (ROWS ? 1 : SUB); ++i) at[i] ^= 2 * BYTES;
+        for (int i = 0; i < (ROWS ? 2 : SUB); ++i) at[i] ^= BYTES;
     }
 
-    // instruction i of the load of k 32 t on into stage `stage`
-    __device__ __forceinline__ void load(int t, int stage, int i) const {
-        load_lds(base + t * step, off[i], (dst ^ (stage & 2) * BYTES) + (stage & 1) * BYTES + i * 1024);
-    }
-    // the whole of it where only `left` k are left (none where left <= 0)
-    __device__ __forceinline__ void load_end(int t, int stage, int left, const void* zeros, int wave, int lane) const {
+    // instruction i of the load of k 64 t on into this step's buffer (other = 0) or the other one (BYTES)
+    __device__ __forceinline__ void load(int t, int other, int i) const { load_lds(base + t * step, off[i], (dst ^ other) + i * 1024); }
+
+    // all of the load of k 64 t on into this step's buffer where only `left` k are left
+    __device__ __forceinline__ void load_end(int t, int left, const void* zeros, int wave, int lane) const {
         const char* b = base + t * step;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             int k;
             if constexpr (ROWS)
-                k = 8 * ((lane & 3) ^ swizzle(16 * (wave * LOADS + i) + (lane >> 2)));
+                k = 8 * ((lane & 7) ^ swizzle(8 * (wave * LOADS + i) + (lane >> 3)));
             else
                 k = (wave * LOADS + i) * PER + lane / LPR;
-            load_lds_any(k < left ? (const void*)(b + off[i]) : zeros, (dst ^ (stage & 2) * BYTES) + (stage & 1) * BYTES + i * 1024);
+            load_lds_any(k < left ? (const void*)(b + off[i]) : zeros, dst + i * 1024);
         }
     }
 
-    // subtile i (16 rows)
-    __device__ __forceinline__ x8 read(int i, int stage) const {
+    // subtile i (16 rows), k 32 ks to 32 ks + 31 of this step
+    __device__ __forceinline__ x8 read(int i, int ks) const {
         if constexpr (ROWS) {
             const int row = SPREAD ? 64 * (i >> 2) + 4 * (i & 3) : 16 * i;
-            return *(__attribute__((address_space(3))) const x8*)(uintptr_t)(at[0] + stage * BYTES + row * 64);
+            return *(__attribute__((address_space(3))) const x8*)(uintptr_t)(at[ks] + row * 128);
         } else {
             typedef __attribute__((address_space(3))) s16x4 lds_s4;
-            const uint32_t a = at[i] + stage * BYTES;
+            const uint32_t a = at[i] + ks * 32 * RB;
             const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)a);
             const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(a + 4 * RB));
             return __builtin_bit_cast(x8, __builtin_shufflevector(v, w, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -197,19 +235,32 @@ struct Tile {
     }
 };
 
-// A workgroup's tile is BM x BN, a wavefront's WM x WN in 16 x 16 subtiles, with four steps of 32 k in LDS. A step has two
-// parts, each with half the wavefront's rows of A: a part's matrix instructions run while the next part's operands come
-// from LDS. Between the parts every wavefront has read the whole step, so there is the one barrier: behind it the
-// next step's first operands are read and the step four on is loaded into the stage that became free. A load has two and a half
-// steps to arrive.
+template <int... I, typename F>
+__device__ __forceinline__ void each(std::integer_sequence<int, I...>, F f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// A workgroup's tile is BM x BN, each of its four wavefronts' WM x WN in 16 x 16 subtiles. A step of 64 k has two
+// halves: while one half's matrix instructions run, the other half's operands come from LDS, in its first rows. Between the halves every
+// wavefront has read the whole step, so there is the one barrier: behind it the next step's first half is read and the step
+// after that is loaded into the buffer that became free.
+// A 128 x 128 part for each wavefront (one per SIMD) reads LDS least: 64 KB for 64 matrix instructions a SIMD and 32 k, where
+// eight wavefronts of 128 x 64 read 96.
 template <typename T, bool A_ROWS, bool B_ROWS, int EPILOGUE, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const ProductArgs q) {
+__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const ProductArgs q) {
     typedef typename Vec<T>::x8 x8;
-    constexpr int WAVES = (BM / WM) * (BN / WN), IM = WM / 16, IN = WN / 16, HALF = IM / 2;
+    constexpr int WAVES = (BM / WM) * (BN / WN), IM = WM / 16, IN = WN / 16;
+    static_assert(WAVES == 4, "");
     typedef Tile<T, A_ROWS, EPILOGUE == LOGITS, BM, WAVES, IM> TA;
     typedef Tile<T, B_ROWS, false, BN, WAVES, IN> TB;
     constexpr int LOADS = TA::LOADS + TB::LOADS;
-    __shared__ __attribute__((aligned(1024))) char smem[STAGES * (TA::BYTES + TB::BYTES)];
+    __shared__ __attribute__((aligned(1024))) char smem[2 * (TA::BYTES + TB::BYTES)];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
     const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
 
@@ -226,91 +277,76 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const
 
     const long k0 = split * q.split_k, k1 = k0 + q.split_k < q.K ? k0 + q.split_k : q.K;
     const long K = k1 > k0 ? k1 - k0 : 0;
-    const int steps = 2 * (int)((K + 2 * BK - 1) / (2 * BK));
+    const int steps = (int)((K + BK - 1) / BK);
     TA a;
     TB b;
     a.init(q.A, q.lda, q.M, m0, k0, (lds_char*)smem, wave, lane, wm);
-    b.init(q.B, q.ldb, q.N, n0, k0, (lds_char*)smem + STAGES * TA::BYTES, wave, lane, wn);
+    b.init(q.B, q.ldb, q.N, n0, k0, (lds_char*)smem + 2 * TA::BYTES, wave, lane, wn);
 
     f32x4 c[IM][IN] = {};
-    x8 fa0[HALF], fa1[HALF], fb0[IN], fb1[IN];
-    // The last 64 k, the only ones that may be fewer, are steps 0 and 1, and k 32 (t - 2) on are step t: so the loop loads
-    // whole steps only, and there is an even number of them.
-    auto load_first = [&](int t) {
-        const int k = steps - 2 + t;
-        const long left = K - (long)BK * k;
-        if (left >= BK) {
+    x8 fa[2][IM], fb[2][IN];
+    // The last 64 k, the only ones that may be fewer, are step 0, and k 64 (t - 1) on are step t: so the loop loads whole
+    // steps only.
+    auto load_first = [&] {
+        const int t = steps - 1, left = (int)(K - (long)BK * t);
+        if (left == BK) {
 #pragma unroll
-            for (int i = 0; i < TA::LOADS; ++i) a.load(k, t, i);
+            for (int i = 0; i < TA::LOADS; ++i) a.load(t, 0, i);
 #pragma unroll
-            for (int i = 0; i < TB::LOADS; ++i) b.load(k, t, i);
+            for (int i = 0; i < TB::LOADS; ++i) b.load(t, 0, i);
         } else {
-            a.load_end(k, t, (int)left, q.zeros, wave, lane);
-            b.load_end(k, t, (int)left, q.zeros, wave, lane);
+            a.load_end(t, left, q.zeros, wave, lane);
+            b.load_end(t, left, q.zeros, wave, lane);
         }
     };
-    // Step t in stage ODD (0 or 1) of this turn; f: this step's part of B, g: where the next one's goes. Reads and loads
-    // are spread over the subtile rows' instructions, and the fences keep that order. Behind the last step an old stage
-    // is read once more, for nothing.
-    auto step = [&](int t, auto odd, auto more, x8(&f)[IN], x8(&g)[IN]) {
-        constexpr int ODD = decltype(odd)::value;
-        constexpr bool LOAD = decltype(more)::value;   // step t + 4 is loaded
-#pragma unroll
-        for (int i = 0; i < HALF; ++i) {
-            if (2 * i < HALF) {
-                fa1[2 * i] = a.read(HALF + 2 * i, ODD);
-                fa1[2 * i + 1] = a.read(HALF + 2 * i + 1, ODD);
+    // Half KS of a step: its matrix instructions, one after the other, and between them, where the matrix pipe is busy
+    // anyway, the reads of the other half (of this step, or of the next one behind `turn`) in the first half of them, and in half 1 the
+    // loads at pa and pb into the other buffer. The fences keep that order.
+    auto half = [&](auto ks, const char* pa, const char* pb) {
+        constexpr int KS = decltype(ks)::value, SLOTS = IM * IN, READS = IM + IN;
+        const uint32_t da = a.dst ^ TA::BYTES, db = b.dst ^ TB::BYTES;
+        auto slot = [&](auto at) {
+            constexpr int S = decltype(at)::value, i = S / IN, j = S % IN;
+            constexpr int l = (S * LOADS + SLOTS - 1) / SLOTS;   // the load whose slot this is, if any
+            if constexpr (KS == 1 && l < LOADS && l * SLOTS / LOADS == S) {
+                if constexpr (l < TA::LOADS)
+                    mfma_load<T, BM == 256, l * 1024>(fa[KS][i], fb[KS][j], c[i][j], pa, a.off[l], da);
+                else
+                    mfma_load<T, BM == 256, (l - TA::LOADS) * 1024>(fa[KS][i], fb[KS][j], c[i][j], pb, b.off[l - TA::LOADS], db);
+            } else {
+                mfma<T, BM == 256>(fa[KS][i], fb[KS][j], c[i][j]);
             }
 #pragma unroll
-            for (int j = 0; j < IN; ++j) c[i][j] = Vec<T>::mfma(fa0[i], f[j], c[i][j]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        // This wavefront has read the step and its loads of the next one have arrived (those of the two after it may be
-        // under way); then everybody's.
-        if constexpr (LOAD)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * LOADS) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        asm volatile("s_barrier" ::: "memory");
-        if constexpr (ODD) {
-            a.turn();
-            b.turn();
-        }
-        constexpr int NEXT = ODD ? 0 : 1, FREE = ODD ? 3 : 0;
-#pragma unroll
-        for (int i = 0; i < HALF; ++i) {
-#pragma unroll
-            for (int j = 2 * i * IN / HALF; j < 2 * (i + 1) * IN / HALF && j < IN; ++j) g[j] = b.read(j, NEXT);
-            if (2 * i >= HALF) {
-                fa0[2 * i - HALF] = a.read(2 * i - HALF, NEXT);
-                fa0[2 * i - HALF + 1] = a.read(2 * i - HALF + 1, NEXT);
-            }
-            if constexpr (LOAD) {
-#pragma unroll
-                for (int j = i * LOADS / HALF; j < (i + 1) * LOADS / HALF; ++j) {
-                    if (j < TA::LOADS)
-                        a.load(t + STAGES - 2, FREE, j);
+            for (int r = 0; r < READS; ++r)
+                if (r * SLOTS / (2 * READS) == S) {
+                    if (r < IN)
+                        fb[1 - KS][r] = b.read(r, 1 - KS);
                     else
-                        b.load(t + STAGES - 2, FREE, j - TA::LOADS);
+                        fa[1 - KS][r - IN] = a.read(r - IN, 1 - KS);
                 }
-            }
-#pragma unroll
-            for (int j = 0; j < IN; ++j) c[HALF + i][j] = Vec<T>::mfma(fa1[i], f[j], c[HALF + i][j]);
             __builtin_amdgcn_sched_barrier(0);
-        }
+        };
+        each(std::make_integer_sequence<int, SLOTS>{}, slot);
+    };
+    // Step t. Behind the last step an old buffer is read once more, for nothing, and behind the last two step 1 is loaded
+    // again, so that the loop has no branches.
+    auto step = [&](int t) {
+        half(std::integral_constant<int, 0>{}, nullptr, nullptr);
+        // this wavefront has read the step and its loads of the next one have arrived; then everybody's
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        a.turn();
+        b.turn();
+        const int k = t + 2 < steps ? t + 1 : 0;
+        half(std::integral_constant<int, 1>{}, a.base + k * a.step, b.base + k * b.step);
     };
     if (steps > 0) {
-        load_first(0);
-        load_first(1);
-        if (steps > 2) {
+        load_first();
+        if (steps > 1) {
 #pragma unroll
-            for (int t = 2; t < STAGES; ++t) {
+            for (int i = 0; i < TA::LOADS; ++i) a.load(0, TA::BYTES, i);
 #pragma unroll
-                for (int i = 0; i < TA::LOADS; ++i) a.load(t - 2, t, i);
-#pragma unroll
-                for (int i = 0; i < TB::LOADS; ++i) b.load(t - 2, t, i);
-            }
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS) : "memory");
+            for (int i = 0; i < TB::LOADS; ++i) b.load(0, TB::BYTES, i);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
@@ -318,19 +354,24 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const
         // (scalar loads that are still under way would make the compiler wait for all LDS reads in every turn)
         __builtin_amdgcn_s_waitcnt(0xc07f);
 #pragma unroll
-        for (int j = 0; j < IN; ++j) fb0[j] = b.read(j, 0);
+        for (int j = 0; j < IN; ++j) fb[0][j] = b.read(j, 0);
 #pragma unroll
-        for (int i = 0; i < HALF; ++i) fa0[i] = a.read(i, 0);
-        int t = 0;
-        for (; t + STAGES < steps; t += 2) {
-            step(t, std::integral_constant<int, 0>{}, std::true_type{}, fb0, fb1);
-            step(t + 1, std::integral_constant<int, 1>{}, std::true_type{}, fb1, fb0);
-        }
-        for (; t < steps; t += 2) {
-            step(t, std::integral_constant<int, 0>{}, std::false_type{}, fb0, fb1);
-            step(t + 1, std::integral_constant<int, 1>{}, std::false_type{}, fb1, fb0);
-        }
+        for (int i = 0; i < IM; ++i) fa[0][i] = a.read(i, 0);
+        for (int t = 0; t < steps; ++t) step(t);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
     }
+
+    // the last matrix instructions' results are there after 18 clocks at most, and nothing reads c before that
+    asm volatile("s_nop 15\n\ts_nop 3");
+#pragma unroll
+    for (int i = 0; i < IM; ++i)
+#pragma unroll
+        for (int j = 0; j < IN; ++j) {
+            if constexpr (BM == 256)
+                asm volatile("" : "+a"(c[i][j]));
+            else
+                asm volatile("" : "+v"(c[i][j]));
+        }
 
     // lane: row n = lo of C, elements m = 4 hi + 0..3 of each subtile (16 hi + 0..15 of four subtiles where SPREAD)
     if constexpr (EPILOGUE == LOGITS) {
@@ -345,18 +386,21 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const
                     for (int j = 0; j < IN; ++j) c[i][j][r] = out ? -INFINITY : c[i][j][r];
                 }
         }
+        T* to = q.p == nullptr ? nullptr : (T*)q.p + (n0 + wn + lo) * q.ldp + first;
 #pragma unroll
         for (int j = 0; j < IN; ++j) {
             const long n = n0 + wn + 16 * j + lo;
+            const bool on = n < q.N;
+            // (a maximum that passes NaN by: the sum has it)
             float m = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < IM; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) m = nan_max(m, c[i][j][r]);
-            m = nan_max(m, __shfl_xor(m, 16));
-            m = nan_max(m, __shfl_xor(m, 32));
-            const float top = m == -INFINITY ? 0.0f : m;
-            const long tgt = n < q.N ? q.target[n] - first : -1;
+            for (int i = 0; i < IM; ++i) m = max3(max3(m, c[i][j][0], c[i][j][1]), c[i][j][2], c[i][j][3]);
+            m = max3(m, m, __shfl_xor(m, 16));
+            m = max3(m, m, __shfl_xor(m, 32));
+            // exponentials are 2^(z log2 e - top): top is kept rounded as it is used here, so that its rounding
+            // cancels where the parts are put together
+            const float top = m == -INFINITY ? 0.0f : m * LOG2E;
+            const long tgt = on ? q.target[n] - first : -1;
             if (tgt >= 0 && tgt < 64 * (IM / 4) && (tgt & 63) < 16 && first + tgt < q.M) {
                 const int k = (int)tgt;
                 float z = 0.0f;
@@ -369,48 +413,64 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), 2) void k_product(const
             float sum = 0.0f;
 #pragma unroll
             for (int g = 0; g < IM / 4; ++g) {
-                T e[16];
+                x8 e[2];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float v = exp_of(c[4 * g + i / 4][j][i & 3] - top);
+                    const float v = __builtin_amdgcn_exp2f(fmaf(c[4 * g + i / 4][j][i & 3], LOG2E, -top));
                     sum += v;
-                    e[i] = (T)v;
+                    e[i >> 3][i & 7] = (T)v;
                 }
-                const long v = first + 64 * g;
-                if (q.p != nullptr && n < q.N && v < q.ldp) {
-                    T* to = (T*)q.p + n * q.ldp + v;
-                    *(x8*)to = *(const x8*)e;
-                    *(x8*)(to + 8) = *(const x8*)(e + 8);
+                if (to != nullptr && on && first + 64 * g < q.ldp) {
+                    *(x8*)(to + 64 * g) = e[0];
+                    *(x8*)(to + 64 * g + 8) = e[1];
                 }
             }
+            to = to == nullptr ? nullptr : to + 16 * q.ldp;
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
-            if (hi == 0 && n < q.N && m0 + wm < q.M) q.stat[n * q.segs + (m0 + wm) / WM] = make_float2(m, sum);
+            if (hi == 0 && on && m0 + wm < q.M) q.stat[n * q.segs + (m0 + wm) / WM] = make_float2(top, sum);
         }
-    } else {
-        const float alpha = q.acc == nullptr ? *q.alpha : 1.0f;
+    } else if (q.acc != nullptr) {
+        float* to = q.acc + (split * q.N + n0 + wn + lo) * q.ldacc + m0 + wm + 4 * hi;
 #pragma unroll
-        for (int j = 0; j < IN; ++j) {
-            const long n = n0 + wn + 16 * j + lo;
+        for (int j = 0; j < IN; ++j, to += 16 * q.ldacc)
 #pragma unroll
             for (int i = 0; i < IM; ++i) {
-                const long m = m0 + wm + 16 * i + 4 * hi;
-                if (n >= q.N || m >= q.M) continue;
+                if (n0 + wn + 16 * j + lo >= q.N || m0 + wm + 16 * i + 4 * hi >= q.M) continue;
                 f32x4 v = c[i][j];
-                if (q.acc != nullptr) {
-                    f32x4* to = (f32x4*)(q.acc + (split * q.N + n) * q.ldacc + m);
-                    if (q.add) v += *to;
-                    *to = v;
-                    continue;
-                }
-                T* to = (T*)q.C + n * q.ldc + m;
-                T e[4] = {(T)(v[0] * alpha), (T)(v[1] * alpha), (T)(v[2] * alpha), (T)(v[3] * alpha)};
-                if (q.vector) {
-                    *(uint2*)to = *(const uint2*)e;
-                } else {
+                if (q.add) v += *(f32x4*)(to + 16 * i);
+                *(f32x4*)(to + 16 * i) = v;
+            }
+    } else {
+        const float alpha = *q.alpha;
+        const bool whole = q.vector && m0 + BM <= q.M;
+        // Two subtiles side by side: the lanes of odd hi get the second one's elements of the lane below and give
+        // theirs of the first, so that a lane has 8 neighbouring elements and four lanes 64 bytes of a row.
+        const int col = 16 * (hi & 1) + 8 * (hi >> 1);
+        T* to = (T*)q.C + (n0 + wn + lo) * q.ldc + m0 + wm;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (m + r < q.M) to[r] = e[r];
+        for (int j = 0; j < IN; ++j, to += 16 * q.ldc) {
+            const bool on = n0 + wn + 16 * j + lo < q.N;
+#pragma unroll
+            for (int i = 0; i < IM; i += 2) {
+                typedef T x4 __attribute__((ext_vector_type(4)));
+                x4 e[2];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    e[0][r] = (T)(c[i][j][r] * alpha);
+                    e[1][r] = (T)(c[i + 1][j][r] * alpha);
+                }
+                if (whole) {
+                    const uint2 u = __builtin_bit_cast(uint2, e[0]), v = __builtin_bit_cast(uint2, e[1]);
+                    const auto x = __builtin_amdgcn_permlane16_swap(u.x, v.x, false, false);
+                    const auto y = __builtin_amdgcn_permlane16_swap(u.y, v.y, false, false);
+                    if (on) *(uint4*)(to + 16 * i + col) = make_uint4(x[0], y[0], x[1], y[1]);
+                } else if (on) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (m0 + wm + 16 * (i + h) + 4 * hi + r < q.M) to[16 * (i + h) + 4 * hi + r] = e[h][r];
                 }
             }
         }
@@ -496,9 +556,9 @@ __global__ __launch_bounds__(256) void k_finish(const FinishArgs q) {
     for (long s = threadIdx.x; s < q.segs; s += 256) m = nan_max(m, stat[s].x);
     m = reduce_threads<256, NanMax>(m, slot);
     float sum = 0.0f;
-    for (long s = threadIdx.x; s < q.segs; s += 256) sum += stat[s].y * exp_of(stat[s].x - m);
+    for (long s = threadIdx.x; s < q.segs; s += 256) sum += stat[s].y * __builtin_amdgcn_exp2f(stat[s].x - m);
     sum = reduce_threads<256, Sum>(sum, slot);
-    const float lse = m + logf(sum);
+    const float lse2 = m + log2f(sum), lse = lse2 * LN2;
     const long t = q.target[i];
     const float w = weight_of(t, q.ignore, q.V, q.row_weight, i);
     const bool in = t >= 0 && t < q.V && t != q.ignore;
@@ -517,7 +577,7 @@ __global__ __launch_bounds__(256) void k_finish(const FinishArgs q) {
             for (int k = 0; k < 8; ++k) e[k] = 0.0f;
         } else {
             load8(p + v, 8, e);
-            const float s = v < q.V ? f * exp_of(stat[v >> q.seg].x - lse) : 0.0f;
+            const float s = v < q.V ? f * __builtin_amdgcn_exp2f(stat[v >> q.seg].x - lse2) : 0.0f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) e[k] = v + k < q.V ? e[k] * s : 0.0f;
             if (in && t >= v && t < v + 8) {
@@ -556,7 +616,7 @@ constexpr long MAX_N = 1l << 31, MAX_HV = 1l << 22;   // 256 rows stay within 32
 long up(long v, long to) { return (v + to - 1) / to * to; }
 long over(long v, long by) { return (v + by - 1) / by; }
 
-// the workgroup tiles: 256 x 256 for eight wavefronts, 128 x 128 and 128 (m) x 64 (n) for four
+// the workgroup tiles: 256 x 256, 128 x 128 and 128 (m) x 64 (n)
 enum { BIG, MID, NARROW };
 constexpr int TILE_M[] = {256, 128, 128}, TILE_N[] = {256, 128, 64};
 constexpr int SLOTS[] = {256, 512, 768};        // workgroups the device holds at once
@@ -678,7 +738,7 @@ void product(const Shape& s, ProductArgs q, hipStream_t st) {
     q.m_tiles = (int)s.m_tiles, q.n_tiles = (int)s.n_tiles, q.splits = s.splits, q.split_k = s.split_k;
     const unsigned grid = (unsigned)(s.m_tiles * s.n_tiles * s.splits);
     if (s.kind == BIG)
-        k_product<T, A_ROWS, B_ROWS, EPILOGUE, 256, 256, 128, 64><<<grid, 512, 0, st>>>(q);
+        k_product<T, A_ROWS, B_ROWS, EPILOGUE, 256, 256, 128, 128><<<grid, 256, 0, st>>>(q);
     else if (s.kind == MID)
         k_product<T, A_ROWS, B_ROWS, EPILOGUE, 128, 128, 64, 64><<<grid, 256, 0, st>>>(q);
     else
@@ -734,7 +794,7 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
             d.B = ws + l.p, d.ldb = l.ldp;
             T* C = (T*)c.dx + at * c.H;
             d.C = C;
-            d.vector = c.H % 4 == 0 && (uintptr_t)C % 8 == 0;
+            d.vector = c.H % 8 == 0 && (uintptr_t)C % 16 == 0;
             d.acc = l.dx.splits > 1 ? (float*)(ws + l.dx_acc) : nullptr;
             Shape s = l.dx;
             s.n_tiles = over(n, TILE_N[s.kind]);
@@ -748,7 +808,7 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
             d.A = x + at * ldx, d.lda = ldx;
             d.B = ws + l.p, d.ldb = l.ldp;
             d.C = c.dw;
-            d.vector = c.H % 4 == 0 && (uintptr_t)c.dw % 8 == 0;
+            d.vector = c.H % 8 == 0 && (uintptr_t)c.dw % 16 == 0;
             d.acc = tokens < c.N ? (float*)(ws + l.dw_acc) : nullptr;
             d.add = at > 0;
             product<T, false, false, OUT>(shape_of(c.H, c.V, n, 1), d, st);
