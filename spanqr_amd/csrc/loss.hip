@@ -9,6 +9,8 @@
 // the exponentials p = exp(z - m) themselves, rounded to the 16-bit type once. One pass over p turns them into G
 // (times exp(m - lse), the target's element from its fp32 logit), and G goes into the other two products. So nothing
 // is multiplied twice, and what is held is 16 bits an element for as many tokens at a time as the workspace takes.
+#include <math.h>
+
 #include <type_traits>
 #include <utility>
 
@@ -620,7 +622,8 @@ long over(long v, long by) { return (v + by - 1) / by; }
 enum { BIG, MID, NARROW };
 constexpr int TILE_M[] = {256, 128, 128}, TILE_N[] = {256, 128, 64};
 constexpr int SLOTS[] = {256, 512, 768};        // workgroups the device holds at once
-constexpr double STEP_US[] = {1.8, 1.1, 0.8};   // 64 k of a full device
+constexpr double STEP_US[] = {1.6, 0.95, 0.8};  // 64 k of a full device, at the clock that it keeps under this load
+constexpr double ENDS_US[] = {13.0, 9.0, 7.0};  // a workgroup's first loads and its epilogue
 
 struct Shape {
     int kind;
@@ -629,11 +632,18 @@ struct Shape {
     long split_k;
 };
 
-// microseconds of C [N][M] over K in tiles of `kind`, in `splits` parts of K
+// Microseconds of C [N][M] over K in tiles of `kind`, in `splits` parts of K. Measured, in us, for 256 / 128 / 64-wide tiles:
+// logits of 512 x 768 x 32000 40 / 35 / 41, of 4000 x 1024 x 50257 475 / 493 / 544, of 64 x 2048 x 50000 75 / 57 / 55; dW
+// of the same 43 / 35 / 42, 398 / 413 / 521 and 84 / 58 / 63; dx of 512 x 768 x 32000 (and the sum of its parts) 50 + 7 / 32 +
+// 7 / 35 + 7 in 16 parts, 78 + 5 / 43 + 5 / 40 + 5 in 8.
 double time_of(int kind, long M, long N, long K, long splits) {
-    const double rounds = (double)over(over(M, TILE_M[kind]) * over(N, TILE_N[kind]) * splits, SLOTS[kind]);
+    const double tiles = (double)(over(M, TILE_M[kind]) * over(N, TILE_N[kind]) * splits);
+    double rounds = tiles / SLOTS[kind], step = STEP_US[kind];
+    if (tiles <= 256) step = kind == BIG ? step : kind == MID ? 0.6 : 0.5;   // one a compute unit
+    // tiles that share a compute unit fill each other's gaps, and the last round's
+    rounds = rounds <= 1.0 ? 1.0 : kind == BIG ? ceil(rounds) : rounds + 0.3;
     const double join = splits > 1 ? 4.0 + 8.0 * (double)(M * N * splits) / 4e6 : 0.0;
-    return rounds * (STEP_US[kind] * (double)over(over(K, 64), splits) + 2.0) + join;
+    return rounds * (step * (double)over(over(K, 64), splits) + ENDS_US[kind]) + join;
 }
 
 // rows of fp32 sums that dx over several parts of K may take. Like all of the workspace it does not shrink with more
