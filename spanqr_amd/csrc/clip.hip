@@ -6,8 +6,8 @@
 // where they fit its 256 MB; the second pass runs backwards, so that it begins with what was read last). Two launches
 // for each TABLE tensors: the tensors' addresses travel in the kernel's arguments, so there is no table to upload and a
 // captured graph keeps them. Work is cut into CHUNK elements, whatever tensor they are of; a workgroup takes every
-// gridDim-th chunk and leaves one partial sum, and every workgroup of the second pass adds all partial sums itself, in
-// the same order, instead of waiting for a third launch. Squares are added in fp64: no order of additions matters to
+// gridDim-th chunk and leaves one partial sum, and with one table every workgroup of the second pass adds all partial sums
+// itself, in the same order, instead of waiting for a third launch. Squares are added in fp64: no order of additions matters to
 // the fp32 result's rounding, and gradients whose squares leave fp32's range keep their norm.
 #include "elements.h"
 #include "host.h"
@@ -21,7 +21,7 @@ namespace {
 constexpr int TABLE = 112;          // tensors a launch (its arguments stay below 4 KB)
 constexpr int THREADS = 256;
 constexpr int CHUNK = THREADS * 32; // elements
-constexpr int MAX_PARTS = 2048;     // partial sums of a call with one table
+constexpr int MAX_PARTS = 2048;     // partial sums of a table
 
 struct Table {
     const void* src[TABLE];
@@ -84,9 +84,13 @@ __device__ __forceinline__ double norm_of(const double* part, int parts) {
     return sqrt(reduce_threads<THREADS, Sum>(sum, slot));
 }
 
-__global__ __launch_bounds__(THREADS) void k_norm(const double* part, int parts, float* norm) {
+// square (or null): the squared norm, as the one partial sum of the second pass
+__global__ __launch_bounds__(THREADS) void k_norm(const double* part, int parts, float* norm, double* square) {
     const double v = norm_of(part, parts);
-    if (threadIdx.x == 0) *norm = (float)v;
+    if (threadIdx.x == 0) {
+        *norm = (float)v;
+        if (square != nullptr) *square = v * v;
+    }
 }
 
 template <typename T, typename O>
@@ -134,11 +138,7 @@ __global__ __launch_bounds__(THREADS) void k_clip(const Table t, const double* p
     }
 }
 
-// partial sums a table of `chunks` chunks leaves, where the call has `tables` of them
-int parts_of(uint32_t chunks, int tables) {
-    const int most = MAX_PARTS / tables > 256 ? MAX_PARTS / tables : 256;
-    return chunks < (uint32_t)most ? (int)chunks : most;
-}
+int grid_of(uint32_t chunks) { return chunks < (uint32_t)MAX_PARTS ? (int)chunks : MAX_PARTS; }
 
 unsigned long chunks_of(unsigned long n) { return (n + CHUNK - 1) / CHUNK; }
 
@@ -171,11 +171,8 @@ int check(const char* what, int n, const long* numel) {
 
 bool known(int type) { return type == SPANQR_BF16 || type == SPANQR_FP16 || type == SPANQR_FP32; }
 
-// one bound for any tables that fill() makes: each has at most TABLE tensors
-long workspace_of(int n) {
-    const long tables = n / TABLE + 1;
-    return 8l * (MAX_PARTS + 256l * tables);
-}
+// for any tables that fill() makes of n tensors
+long workspace_of(int n) { return 8l * MAX_PARTS * (n / TABLE + 1) + 8; }
 
 int enqueue(const char* what, int n, const void* const* src, const long* numel, const int* type, void* const* dst,
             const int* out, float max_norm, float* norm, void* workspace, long workspace_bytes, hipStream_t st) {
@@ -184,35 +181,33 @@ int enqueue(const char* what, int n, const void* const* src, const long* numel, 
     if (norm == nullptr || workspace == nullptr || (n > 0 && (src == nullptr || type == nullptr)))
         return error(SPANQR_EINVAL, "%s: a missing pointer", what);
     if (workspace_bytes < workspace_of(n)) return error(SPANQR_EINVAL, "%s: the workspace needs %ld bytes", what, workspace_of(n));
-    int filled = 0;
     for (int i = 0; i < n; ++i) {
         if (!known(type[i]) || (out != nullptr && !known(out[i]))) return error(SPANQR_EINVAL, "%s: tensor %d: unknown type", what, i);
         if (numel[i] > 0 && (src[i] == nullptr || (dst != nullptr && dst[i] == nullptr)))
             return error(SPANQR_EINVAL, "%s: tensor %d: a missing pointer", what, i);
-        filled += numel[i] > 0;
     }
-    const int tables = filled / TABLE + 1;
-    double* part = (double*)workspace;
-    int parts = 0;
+    double *square = (double*)workspace, *part = square + 1;
+    int parts = 0, tables = 0;
     Table t;
     for (int i = 0; i < n;) {
         i = fill(t, i, n, src, dst, numel, type, out);
         if (t.count == 0) break;
-        const int grid = parts_of(t.first[t.count], tables);
+        const int grid = grid_of(t.first[t.count]);
         k_squares<<<grid, THREADS, 0, st>>>(t, part + parts);
         parts += grid;
+        ++tables;
     }
-    if (dst == nullptr || parts == 0) {
-        k_norm<<<1, THREADS, 0, st>>>(part, parts, norm);
-        return launched(what);
+    if (dst == nullptr || tables != 1) {
+        k_norm<<<1, THREADS, 0, st>>>(part, parts, norm, square);
+        if (dst == nullptr || parts == 0) return launched(what);
+        part = square, parts = 1, norm = nullptr;
     }
     for (int i = 0; i < n;) {
         const bool first = i == 0;
         i = fill(t, i, n, src, dst, numel, type, out);
         if (t.count == 0) break;
         const uint32_t chunks = t.first[t.count];
-        k_clip<<<(int)(chunks < MAX_PARTS ? chunks : MAX_PARTS), THREADS, 0, st>>>(t, part, parts, max_norm,
-                                                                                  first ? norm : nullptr);
+        k_clip<<<grid_of(chunks), THREADS, 0, st>>>(t, part, parts, max_norm, first ? norm : nullptr);
     }
     return launched(what);
 }

@@ -5,9 +5,10 @@
 //   gradient: n = h s, u = dy w, dx = s (u - n sum_j(u_j n_j) / D) + dh, dw = sum over rows of dy n
 //
 // Both are bound by memory: one read of every input and one write of every output, with the row in registers between
-// the sums and the output. A row belongs to GROUP threads with NCH pieces of eight elements each, so the same kernel
-// serves 16 lanes a row (128 elements) to 1024 threads a row (32768); longer rows are read again for each step
-// (k_rms_long, k_rms_grad_long). All sums are fp32 per thread over at most 32 elements, then a tree in a fixed order.
+// the sums and the output. A row belongs to `group` threads with NCH pieces of eight elements each: 16 lanes for up to
+// 128 elements, a wavefront for up to 2048 (no barriers), and then one workgroup of as many wavefronts as the row
+// fills, to 1024 threads and 32768 elements; longer rows are read again for each step (k_rms_long, k_rms_grad_long).
+// All sums are fp32 per thread over at most 32 elements, then a tree in a fixed order.
 #include "elements.h"
 #include "host.h"
 
@@ -88,39 +89,62 @@ __device__ __forceinline__ void store_quant(int quant, uint8_t* q, int n, const 
     }
 }
 
-template <int GROUP, typename OP, typename A>
-__device__ __forceinline__ A reduce_group(A v, A* slot) {
-    if constexpr (GROUP <= 64)
-        return reduce_lanes<GROUP, OP>(v);
-    else
-        return reduce_threads<GROUP, OP>(v, slot);
-}
+// Threads of a row: GROUP lanes of a wavefront (16 or 64; then a workgroup of 256 threads has several rows), or with GROUP
+// 0 the whole workgroup, of any number of wavefronts.
+template <int GROUP>
+struct Group {
+    static constexpr int MOST = GROUP ? 256 : 1024;
+    __device__ __forceinline__ static int size() { return GROUP ? GROUP : (int)blockDim.x; }
+    __device__ __forceinline__ static int rows() { return GROUP ? 256 / GROUP : 1; }
+    __device__ __forceinline__ static int lane() { return GROUP ? threadIdx.x % GROUP : threadIdx.x; }
+    __device__ __forceinline__ static int index() { return GROUP ? threadIdx.x / GROUP : 0; }
+    // N values over the group's threads. One barrier: `slot` ([N][16]) may be used again only behind another one.
+    template <typename OP, int N>
+    __device__ __forceinline__ static void reduce(float (&v)[N], float (*slot)[16]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = reduce_lanes<GROUP ? GROUP : 64, OP>(v[i]);
+        if constexpr (GROUP == 0) {
+            const int waves = blockDim.x >> 6;
+            if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) slot[i][threadIdx.x >> 6] = v[i];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = slot[i][0];
+            for (int w = 1; w < waves; ++w) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = OP::of(v[i], slot[i][w]);
+            }
+        }
+    }
+};
 
 template <typename T, int GROUP, int NCH>
-__global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void k_rms(const NormArgs p) {
-    constexpr int BLOCK = GROUP > 256 ? GROUP : 256, ROWS = BLOCK / GROUP;
-    __shared__ float slot[BLOCK / 64];
-    const int lane = threadIdx.x % GROUP;
+__global__ __launch_bounds__(Group<GROUP>::MOST) void k_rms(const NormArgs p) {
+    typedef Group<GROUP> G;
+    __shared__ float slot[3][1][16];   // the sums' by turns, and the maximum's
+    const int lane = G::lane(), size = G::size();
     float w[NCH][8];
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const long at = 8l * (lane + c * GROUP);
+        const long at = 8l * (lane + c * size);
         load_weight(p.weight, p.wtype, at, inside(p.D, at), w[c]);
     }
-    for (long base = (long)blockIdx.x * ROWS; base < p.rows; base += (long)gridDim.x * ROWS) {
-        const long row = base + threadIdx.x / GROUP;
+    int turn = 0;
+    for (long base = (long)blockIdx.x * G::rows(); base < p.rows; base += (long)gridDim.x * G::rows(), turn ^= 1) {
+        const long row = base + G::index();
         const bool on = row < p.rows;   // the group's lanes all take part in the reductions
         float v[NCH][8];
-        float sum = 0.0f;
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const long at = 8l * (lane + c * GROUP);
+            const long at = 8l * (lane + c * size);
             load8((const T*)p.x + row * p.ldx + at, on ? inside(p.D, at) : 0, v[c]);
         }
         if (p.residual != nullptr) {
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
-                const long at = 8l * (lane + c * GROUP);
+                const long at = 8l * (lane + c * size);
                 const int n = on ? inside(p.D, at) : 0;
                 float r[8];
                 load8((const T*)p.residual + row * p.ldr + at, n, r);
@@ -130,12 +154,13 @@ __global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void k_rms(const NormArg
                 store8((T*)p.h + row * p.D + at, n, v[c]);
             }
         }
+        float sum[1] = {0.0f};
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(v[c][i], v[c][i], sum);
-        sum = reduce_group<GROUP, Sum>(sum, slot);
-        const float s = rsqrtf(sum / (float)p.D + p.eps);
+            for (int i = 0; i < 8; ++i) sum[0] = fmaf(v[c][i], v[c][i], sum[0]);
+        G::template reduce<Sum>(sum, slot[turn]);
+        const float s = rsqrtf(sum[0] / (float)p.D + p.eps);
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
 #pragma unroll
@@ -143,26 +168,26 @@ __global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void k_rms(const NormArg
         if (p.quant == SPANQR_QUANT_NONE) {
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
-                const long at = 8l * (lane + c * GROUP);
+                const long at = 8l * (lane + c * size);
                 store8((T*)p.y + row * p.D + at, on ? inside(p.D, at) : 0, v[c]);
             }
         } else {
             // (elements past the row's end are 0, or NaN where s is: then the row is NaN anyway)
-            float a = 0.0f;
+            float a[1] = {0.0f};
 #pragma unroll
             for (int c = 0; c < NCH; ++c)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) a = nan_max(a, fabsf(v[c][i]));
-            a = reduce_group<GROUP, NanMax>(a, slot);
-            const float M = quant_max(p.quant), f = quant_factor(a, M);
+                for (int i = 0; i < 8; ++i) a[0] = nan_max(a[0], fabsf(v[c][i]));
+            G::template reduce<NanMax>(a, slot[2]);
+            const float M = quant_max(p.quant), f = quant_factor(a[0], M);
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
-                const long at = 8l * (lane + c * GROUP);
+                const long at = 8l * (lane + c * size);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[c][i] *= f;
                 store_quant(p.quant, (uint8_t*)p.y + row * p.D + at, on ? inside(p.D, at) : 0, v[c]);
             }
-            if (on && lane == 0) p.scale[row] = a / M;
+            if (on && lane == 0) p.scale[row] = a[0] / M;
         }
     }
 }
@@ -221,85 +246,62 @@ __global__ __launch_bounds__(1024) void k_rms_long(const NormArgs p) {
 }
 
 // The weight's gradient is a sum over rows: a workgroup keeps its rows' part in registers (each thread always holds the
-// same columns), adds its ROWS groups through LDS and writes one row of partial sums; k_rms_dw adds those.
+// same columns), adds its groups through LDS and writes one row of partial sums; k_rms_dw adds those.
 template <typename T, int GROUP, int NCH>
-__global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void k_rms_grad(const GradArgs p) {
-    constexpr int BLOCK = GROUP > 256 ? GROUP : 256, ROWS = BLOCK / GROUP;
-    struct Two {
-        float a, b;
-        __device__ __forceinline__ Two operator+(const Two& o) const { return Two{a + o.a, b + o.b}; }
-    };
-    __shared__ float slot[2 * (BLOCK / 64)];
+__global__ __launch_bounds__(Group<GROUP>::MOST) void k_rms_grad(const GradArgs p) {
+    typedef Group<GROUP> G;
+    __shared__ float slot[2][2][16];
+    constexpr int ROWS = GROUP ? 256 / GROUP : 1;
     __shared__ float add[ROWS > 1 ? (ROWS - 1) * GROUP * NCH * 8 : 1];
-    const int lane = threadIdx.x % GROUP, group = threadIdx.x / GROUP;
+    const int lane = G::lane(), group = G::index(), size = G::size();
     float w[NCH][8], dw[NCH][8];
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const long at = 8l * (lane + c * GROUP);
+        const long at = 8l * (lane + c * size);
         load_weight(p.weight, p.wtype, at, inside(p.D, at), w[c]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dw[c][i] = 0.0f;
     }
-    for (long base = (long)blockIdx.x * ROWS; base < p.rows; base += (long)gridDim.x * ROWS) {
+    int turn = 0;
+    for (long base = (long)blockIdx.x * ROWS; base < p.rows; base += (long)gridDim.x * ROWS, turn ^= 1) {
         const long row = base + group;
         const bool on = row < p.rows;
-        float h[NCH][8], u[NCH][8];
-        float hh = 0.0f, uh = 0.0f;
+        float h[NCH][8], u[NCH][8], d[NCH][8];
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const long at = 8l * (lane + c * GROUP);
+            const long at = 8l * (lane + c * size);
             const int n = on ? inside(p.D, at) : 0;
             load8((const T*)p.h + row * p.ldh + at, n, h[c]);
             load8((const T*)p.dy + row * p.lddy + at, n, u[c]);
+            if (p.dh != nullptr) {
+                load8((const T*)p.dh + row * p.lddh + at, n, d[c]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[c][i] = 0.0f;
+            }
         }
+        float sum[2] = {0.0f, 0.0f};   // of h^2, and of u h
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                hh = fmaf(h[c][i], h[c][i], hh);
-                uh = fmaf(u[c][i] * w[c][i], h[c][i], uh);
+                sum[0] = fmaf(h[c][i], h[c][i], sum[0]);
+                sum[1] = fmaf(u[c][i] * w[c][i], h[c][i], sum[1]);
             }
-        if constexpr (GROUP <= 64) {
-            hh = reduce_lanes<GROUP, Sum>(hh);
-            uh = reduce_lanes<GROUP, Sum>(uh);
-        } else {
-            hh = reduce_lanes<64, Sum>(hh);
-            uh = reduce_lanes<64, Sum>(uh);
-            if ((threadIdx.x & 63) == 0) {
-                slot[threadIdx.x >> 6] = hh;
-                slot[(BLOCK / 64) + (threadIdx.x >> 6)] = uh;
-            }
-            __syncthreads();
-            hh = slot[0];
-            uh = slot[BLOCK / 64];
-#pragma unroll
-            for (int i = 1; i < BLOCK / 64; ++i) {
-                hh += slot[i];
-                uh += slot[BLOCK / 64 + i];
-            }
-            __syncthreads();
-        }
+        G::template reduce<Sum>(sum, slot[turn]);
         // a group without a row adds zeros, also where eps is 0
-        const float s = on ? rsqrtf(hh / (float)p.D + p.eps) : 0.0f;
-        const float m = s * uh / (float)p.D;   // the mean of u n
+        const float s = on ? rsqrtf(sum[0] / (float)p.D + p.eps) : 0.0f;
+        const float m = s * sum[1] / (float)p.D;   // the mean of u n
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            const long at = 8l * (lane + c * GROUP);
-            const int n = on ? inside(p.D, at) : 0;
-            float d[8];
-            if (p.dh != nullptr) {
-                load8((const T*)p.dh + row * p.lddh + at, n, d);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = 0.0f;
-            }
+            const long at = 8l * (lane + c * size);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float nrm = h[c][i] * s;
                 dw[c][i] = fmaf(u[c][i], nrm, dw[c][i]);
-                d[i] = fmaf(s, u[c][i] * w[c][i] - nrm * m, d[i]);
+                d[c][i] = fmaf(s, u[c][i] * w[c][i] - nrm * m, d[c][i]);
             }
-            store8((T*)p.dx + row * p.D + at, n, d);
+            store8((T*)p.dx + row * p.D + at, on ? inside(p.D, at) : 0, d[c]);
         }
     }
     if (p.part == nullptr) return;
@@ -320,7 +322,7 @@ __global__ __launch_bounds__(GROUP > 256 ? GROUP : 256) void k_rms_grad(const Gr
     }
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-        const long at = 8l * (lane + c * GROUP);
+        const long at = 8l * (lane + c * size);
         store8(p.part + blockIdx.x * p.D + at, inside(p.D, at), dw[c]);
     }
 }
@@ -410,42 +412,45 @@ constexpr long LONG_ROW = 32768;    // longest row that stays in registers
 constexpr long MAX_D = 1l << 24;
 constexpr int GRAD_PARTS = 1024;    // most workgroups of the gradient, and so rows of partial sums
 
-// threads a row (GROUP) and pieces a thread (NCH) for rows of D elements
+// threads of a row and pieces a thread
 struct Split {
-    int group, nch;
+    int group, nch;   // group 16 or 64: lanes of a wavefront; else (64 and `block`) a workgroup
+    bool block;
 };
-Split split_of(long D) {
-    if (D <= 128) return {16, 1};
-    if (D <= 512) return {64, 1};
-    if (D <= 1024) return {64, 2};
-    if (D <= 2048) return {64, 4};
-    if (D <= 4096) return {256, 2};
-    if (D <= 8192) return {256, 4};
-    if (D <= 16384) return {512, 4};
-    return {1024, 4};
+Split split_of(long rows, long D) {
+    const long pieces = (D + 7) / 8;
+    // with few rows a row takes as many threads as it can
+    if (rows <= 512 && D > 512 && D <= 8192) return {(int)((pieces + 63) / 64 * 64), 1, true};
+    if (D <= 128) return {16, 1, false};
+    if (D <= 512) return {64, 1, false};
+    if (D <= 1024) return {64, 2, false};
+    if (D <= 2048) return {64, 4, false};
+    const int nch = D <= 16384 ? 2 : 4;
+    return {(int)(((pieces + nch - 1) / nch + 63) / 64 * 64), nch, true};
 }
 
-int grid_of(long rows, int group, int most) {
-    const int per = group >= 256 ? 1 : 256 / group;
+int grid_of(long rows, const Split& s, int most) {
+    const int per = s.block ? 1 : 256 / s.group;
     const long need = (rows + per - 1) / per;
     return (int)(need < most ? need : most);
 }
 
 int grad_parts(long rows, long D) {
     if (D > LONG_ROW) return (int)(rows < 256 ? rows : 256);
-    return grid_of(rows, split_of(D).group, GRAD_PARTS);
+    return grid_of(rows, split_of(rows, D), GRAD_PARTS);
 }
 
-#define SPANQR_SPLITS(LAUNCH)                     \
-    switch (s.group * 8 + s.nch) {                \
-        case 16 * 8 + 1: LAUNCH(16, 1); break;    \
-        case 64 * 8 + 1: LAUNCH(64, 1); break;    \
-        case 64 * 8 + 2: LAUNCH(64, 2); break;    \
-        case 64 * 8 + 4: LAUNCH(64, 4); break;    \
-        case 256 * 8 + 2: LAUNCH(256, 2); break;  \
-        case 256 * 8 + 4: LAUNCH(256, 4); break;  \
-        case 512 * 8 + 4: LAUNCH(512, 4); break;  \
-        default: LAUNCH(1024, 4); break;          \
+#define SPANQR_SPLITS(LAUNCH)                                       \
+    if (s.block) {                                                  \
+        if (s.nch == 1) LAUNCH(0, 1, s.group);                      \
+        else if (s.nch == 2) LAUNCH(0, 2, s.group);                 \
+        else LAUNCH(0, 4, s.group);                                 \
+    } else if (s.group == 16) {                                     \
+        LAUNCH(16, 1, 256);                                         \
+    } else {                                                        \
+        if (s.nch == 1) LAUNCH(64, 1, 256);                         \
+        else if (s.nch == 2) LAUNCH(64, 2, 256);                    \
+        else LAUNCH(64, 4, 256);                                    \
     }
 
 template <typename T>
@@ -454,9 +459,9 @@ void launch_norm(const NormArgs& p, hipStream_t st) {
         k_rms_long<T><<<(int)(p.rows < 1024 ? p.rows : 1024), 1024, 0, st>>>(p);
         return;
     }
-    const Split s = split_of(p.D);
-    const int grid = grid_of(p.rows, s.group, 2048);
-#define LAUNCH(G, C) k_rms<T, G, C><<<grid, G > 256 ? G : 256, 0, st>>>(p)
+    const Split s = split_of(p.rows, p.D);
+    const int grid = grid_of(p.rows, s, 4096);
+#define LAUNCH(G, C, N) k_rms<T, G, C><<<grid, N, 0, st>>>(p)
     SPANQR_SPLITS(LAUNCH)
 #undef LAUNCH
 }
@@ -467,8 +472,8 @@ void launch_grad(const GradArgs& p, int grid, hipStream_t st) {
         k_rms_grad_long<T><<<grid, 1024, 0, st>>>(p);
         return;
     }
-    const Split s = split_of(p.D);
-#define LAUNCH(G, C) k_rms_grad<T, G, C><<<grid, G > 256 ? G : 256, 0, st>>>(p)
+    const Split s = split_of(p.rows, p.D);
+#define LAUNCH(G, C, N) k_rms_grad<T, G, C><<<grid, N, 0, st>>>(p)
     SPANQR_SPLITS(LAUNCH)
 #undef LAUNCH
 }
