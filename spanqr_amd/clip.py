@@ -1,7 +1,7 @@
 """The norm over many tensors and clipping by it, through the native library (csrc/clip.hip): what a training step does
 with its gradients before the optimizer forms the X that orth takes. No counterpart in the reference.
 """
-import ctypes
+from array import array
 
 import torch
 
@@ -21,42 +21,78 @@ def _dense(t):
     return True
 
 
-def _check(what, grads):
-    if isinstance(grads, torch.Tensor):
-        grads = [grads]
-    grads = list(grads)
-    for g in grads:
-        check_tensor(what, "every gradient", g)
-        check_same(what, "a gradient", g, grads[0].device)
-    return grads
+def _tensors(what, name, ts, device=None):
+    """ts as a list of tensors of the three types on one GPU, and that device"""
+    ts = [ts] if isinstance(ts, torch.Tensor) else list(ts)
+    if not ts:
+        return ts, device or torch.device("cuda", torch.cuda.current_device())
+    first = ts[0]
+    try:   # hundreds of tensors: what is right is seen in one go, and only what is wrong is looked for
+        dev = first.device if device is None else device
+        if (dev.type == "cuda" and {t.get_device() for t in ts} == {dev.index} and
+                all([t.dtype in TYPES for t in ts])):
+            return ts, dev
+    except AttributeError:
+        pass
+    for t in ts:
+        check_tensor(what, name, t)
+        check_same(what, name, t, device or first.device)
+    return ts, first.device
 
 
-def _table(ts):
-    """host arrays of the tensors' addresses and of their types"""
-    n = len(ts)
-    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]), (ctypes.c_int * n)(*[TYPES[t.dtype] for t in ts]))
+def _pointers(ts):
+    return array("Q", [t.data_ptr() for t in ts])
 
 
-def _norm_device(grads):
-    return grads[0].device if grads else torch.device("cuda", torch.cuda.current_device())
+def _types(ts):
+    return array("i", [TYPES[t.dtype] for t in ts])
+
+
+def _sizes(ts):
+    return array("q", [t.numel() for t in ts])
+
+
+def _at(values):
+    return values.buffer_info()[0]
 
 
 def grad_norm(grads):
     """sqrt of the sum of squares over all tensors of a list (or of one tensor): float32, bfloat16 and float16 mixed, of
     any shapes and strides, on one ROCm device. A float32 tensor without axes on that device, no host synchronisation;
     squares and sums in float64. An empty list gives 0."""
-    grads = _check("grad_norm", grads)
-    dev = _norm_device(grads)
-    ts = [g if _dense(g) else g.contiguous() for g in grads]
+    ts, dev = _tensors("grad_norm", "every gradient", grads)
+    if not all([t.is_contiguous() for t in ts]):
+        ts = [t if _dense(t) else t.contiguous() for t in ts]
     n = len(ts)
-    at, types = _table(ts)
-    numel = (ctypes.c_long * n)(*[t.numel() for t in ts])
+    at, numel, types = _pointers(ts), _sizes(ts), _types(ts)
     norm = torch.empty((), dtype=torch.float32, device=dev)
+    lib = _lib.lib()
     with on(dev) as stream:
-        nbytes = _lib.lib().spanqr_grad_norm_workspace(n)
+        nbytes = lib.spanqr_grad_norm_workspace(n)
         ws = workspace(nbytes, dev)
-        _lib.check(_lib.lib().spanqr_grad_norm(n, at, numel, types, norm.data_ptr(), ws.data_ptr(), nbytes, stream))
+        _lib.check(lib.spanqr_grad_norm(n, _at(at), _at(numel), _at(types), norm.data_ptr(), ws.data_ptr(), nbytes, stream))
     return norm
+
+
+def _in_rows(grads, out, dev):
+    """(src, dst, back) where some tensor is strided: pairs that lie in one order, and what is copied back into out
+    afterwards"""
+    src, dst, back = [], [], []
+    for g, o in zip(grads, out):
+        if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
+            raise ValueError("clip_grad_norm: a tensor to write to has elements that share memory (an expanded tensor)")
+        if g.stride() == o.stride() and _dense(g):
+            src.append(g)
+            dst.append(o)
+            continue
+        src.append(g.contiguous())
+        if o.is_contiguous():
+            dst.append(o)
+        else:
+            dst.append(src[-1] if o.dtype == g.dtype and src[-1] is not g else
+                       torch.empty(o.shape, dtype=o.dtype, device=dev))
+            back.append((o, dst[-1]))
+    return src, dst, back
 
 
 def clip_grad_norm(grads, max_norm, out=None):
@@ -67,47 +103,33 @@ def clip_grad_norm(grads, max_norm, out=None):
 
     A NaN norm makes every result NaN, an infinite norm makes finite gradients 0: look at the norm before the step. out
     may share no memory with the gradients, other than out[i] being grads[i]."""
-    grads = _check("clip_grad_norm", grads)
+    grads, dev = _tensors("clip_grad_norm", "every gradient", grads)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm: max_norm must not be negative, got {max_norm}")
-    dev = _norm_device(grads)
     if out is None:
         out = grads
     else:
-        out = [out] if isinstance(out, torch.Tensor) else list(out)
-        if len(out) != len(grads):
-            raise ValueError(f"clip_grad_norm: {len(grads)} gradients but {len(out)} tensors in out")
-        for g, o in zip(grads, out):
-            check_tensor("clip_grad_norm", "every tensor of out", o)
-            check_same("clip_grad_norm", "a tensor of out", o, dev, g.shape)
-    src, dst, back = [], [], []
-    for g, o in zip(grads, out):
-        if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
-            raise ValueError("clip_grad_norm: a tensor to write to has elements that share memory (an expanded tensor)")
-        same = g.stride() == o.stride()
-        if same and _dense(g):
-            src.append(g)
-            dst.append(o)
-            continue
-        # strided views, or two different orders: through a copy that lies in rows
-        src.append(g.contiguous())
-        if o.is_contiguous():
-            dst.append(o)
-        else:
-            dst.append(src[-1] if o.dtype == g.dtype and src[-1] is not g else
-                       torch.empty(o.shape, dtype=o.dtype, device=dev))
-            back.append((o, dst[-1]))
+        out, _ = _tensors("clip_grad_norm", "every tensor of out", out, dev)
+        if [g.shape for g in grads] != [o.shape for o in out]:
+            if len(out) != len(grads):
+                raise ValueError(f"clip_grad_norm: {len(grads)} gradients but {len(out)} tensors in out")
+            for g, o in zip(grads, out):
+                check_same("clip_grad_norm", "a tensor of out", o, dev, g.shape)
+    back = ()
+    src, dst = grads, out
+    if not (all([g.is_contiguous() for g in grads]) and (out is grads or all([o.is_contiguous() for o in out]))):
+        src, dst, back = _in_rows(grads, out, dev)
     n = len(src)
-    at, types = _table(src)
-    to, out_types = _table(dst)
-    numel = (ctypes.c_long * n)(*[t.numel() for t in src])
+    at, numel, types = _pointers(src), _sizes(src), _types(src)
+    to, out_types = (at, types) if dst is src else (_pointers(dst), _types(dst))
     norm = torch.empty((), dtype=torch.float32, device=dev)
+    lib = _lib.lib()
     with on(dev) as stream:
-        nbytes = _lib.lib().spanqr_grad_norm_workspace(n)
+        nbytes = lib.spanqr_grad_norm_workspace(n)
         ws = workspace(nbytes, dev)
-        _lib.check(_lib.lib().spanqr_clip_grad_norm(n, at, numel, types, to, out_types, max_norm, norm.data_ptr(),
-                                                    ws.data_ptr(), nbytes, stream))
+        _lib.check(lib.spanqr_clip_grad_norm(n, _at(at), _at(numel), _at(types), _at(to), _at(out_types), max_norm,
+                                             norm.data_ptr(), ws.data_ptr(), nbytes, stream))
     for o, copy in back:
         o.copy_(copy)
     return norm

@@ -20,7 +20,8 @@ namespace {
 
 constexpr int TABLE = 112;          // tensors a launch (its arguments stay below 4 KB)
 constexpr int THREADS = 256;
-constexpr int CHUNK = THREADS * 32; // elements
+constexpr int PIECES = 4;           // of 8 elements a thread and chunk
+constexpr int CHUNK = THREADS * 8 * PIECES;
 constexpr int MAX_PARTS = 2048;     // partial sums of a table
 
 struct Table {
@@ -48,11 +49,19 @@ __device__ __forceinline__ int tensor_of(const Table& t, uint32_t chunk) {
 template <typename T>
 __device__ __forceinline__ double squares(const T* p, unsigned long n, unsigned long at) {
     double sum = 0.0;
+    if (n - at >= CHUNK) {   // all loads at once
+        Pack8<T> k[PIECES];
 #pragma unroll
-    for (int c = 0; c < CHUNK / (8 * THREADS); ++c) {
-        const unsigned long i = at + 8ul * (threadIdx.x + c * THREADS);
+        for (int c = 0; c < PIECES; ++c) k[c] = *(const Pack8<T>*)(p + at + 8ul * (threadIdx.x + c * THREADS));
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = fma((double)(float)k[c].v[i], (double)(float)k[c].v[i], sum);
+        return sum;
+    }
+    for (unsigned long i = at + 8ul * threadIdx.x; i < n; i += 8ul * THREADS) {
         float f[8];
-        load8(p + i, i >= n ? 0 : n - i >= 8 ? 8 : (int)(n - i), f);
+        load8(p + i, n - i >= 8 ? 8 : (int)(n - i), f);
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum = fma((double)f[k], (double)f[k], sum);
     }
@@ -95,11 +104,21 @@ __global__ __launch_bounds__(THREADS) void k_norm(const double* part, int parts,
 
 template <typename T, typename O>
 __device__ __forceinline__ void scaled(const T* p, O* out, unsigned long n, unsigned long at, float f) {
+    float v[8];
+    if (n - at >= CHUNK) {
+        Pack8<T> k[PIECES];
 #pragma unroll
-    for (int c = 0; c < CHUNK / (8 * THREADS); ++c) {
-        const unsigned long i = at + 8ul * (threadIdx.x + c * THREADS);
-        const int k = i >= n ? 0 : n - i >= 8 ? 8 : (int)(n - i);
-        float v[8];
+        for (int c = 0; c < PIECES; ++c) k[c] = *(const Pack8<T>*)(p + at + 8ul * (threadIdx.x + c * THREADS));
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (float)k[c].v[i] * f;
+            store8(out + at + 8ul * (threadIdx.x + c * THREADS), 8, v);
+        }
+        return;
+    }
+    for (unsigned long i = at + 8ul * threadIdx.x; i < n; i += 8ul * THREADS) {
+        const int k = n - i >= 8 ? 8 : (int)(n - i);
         load8(p + i, k, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= f;

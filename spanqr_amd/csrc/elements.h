@@ -46,6 +46,40 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&f)[8]) {
     }
 }
 
+// Eight elements of a row of D >= 8 from `at` on, in two steps, so that many loads can be under way at once: fetch8 reads
+// the last eight where fewer are left (no branch, nothing past the row), and settle8 moves those to their place and
+// puts 0 behind them. n: how many are left, 0 to 8.
+template <typename T>
+__device__ __forceinline__ Pack8<T> fetch8(const T* row, long D, long at) {
+    return *reinterpret_cast<const Pack8<T>*>(row + (at < D - 8 ? at : D - 8));
+}
+template <typename T>
+__device__ __forceinline__ void settle8(const Pack8<T>& k, int n, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)k.v[i];
+    if (n < 8) {
+#pragma unroll
+        for (int b = 4; b > 0; b >>= 1) {   // by 8 - n places
+            const bool move = (8 - n) & b;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = move ? (i + b < 8 ? f[i + b] : 0.0f) : f[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < n ? f[i] : 0.0f;
+    }
+}
+
+// makes the compiler unpack k again behind this point instead of keeping what it unpacked before
+template <typename T>
+__device__ __forceinline__ void again(Pack8<T>& k) {
+    constexpr int N = sizeof(T) * 8 / 4;
+    struct Words { uint32_t w[N]; };
+    Words b = __builtin_bit_cast(Words, k);
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(b.w[i]));
+    k = __builtin_bit_cast(Pack8<T>, b);
+}
+
 // the larger of two magnitudes; NaN if either is
 __device__ __forceinline__ float nan_max(float a, float b) { return (b > a || b != b) ? b : a; }
 

@@ -694,7 +694,7 @@ Layout layout_of(long N, long H, long V, int grads, bool pad, long tokens) {
     l.p = take(grads ? 2 * tokens * l.ldp : 0);
     l.dx_acc = take((grads & 1) ? 4 * split_rows(tokens) * l.Hp : 0);
     l.dw_acc = take((grads & 2) && tokens < N ? 4 * l.Hp * V : 0);
-    l.x = take(pad ? 2 * N * l.Hp : 0);
+    l.x = take(pad ? 2 * tokens * l.Hp : 0);
     l.w = take(pad ? 2 * V * l.Hp : 0);
     l.bytes = at;
     return l;
@@ -762,14 +762,16 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
     Scalars* scal = (Scalars*)(ws + l.scal);
     float* loss = c.reduced ? (float*)(ws + l.loss) : c.loss;
     const T *x = (const T*)c.x, *w = (const T*)c.w;
-    long ldx = c.ldx, ldw = c.ldw;
-    k_prepare<<<1, 1024, 0, st>>>(c.target, c.N, c.ignore, c.mean, c.row_weight, c.grad_scale, g_scale<T>(), scal);
+    const long ldx = c.ldx;
+    long ldw = c.ldw;
+    // (each token's loss alone needs no scale, and zeros only where the hidden size is no multiple of a step)
+    if (grads || c.reduced || l.Hp % BK != 0)
+        k_prepare<<<1, 1024, 0, st>>>(c.target, c.N, c.ignore, c.mean, c.row_weight, c.grad_scale, g_scale<T>(), scal);
+    auto pad_grid = [&](long rows) { return (unsigned)(over(rows * l.Hp / 8, 256) < 4096 ? over(rows * l.Hp / 8, 256) : 4096); };
     if (c.pad) {
-        auto grid = [&](long rows) { return (unsigned)(over(rows * l.Hp / 8, 256) < 4096 ? over(rows * l.Hp / 8, 256) : 4096); };
-        if (c.N > 0) k_pad<T><<<grid(c.N), 256, 0, st>>>(x, ldx, c.N, c.H, l.Hp, (T*)(ws + l.x));
-        k_pad<T><<<grid(c.V), 256, 0, st>>>(w, ldw, c.V, c.H, l.Hp, (T*)(ws + l.w));
-        x = (const T*)(ws + l.x), w = (const T*)(ws + l.w);
-        ldx = ldw = l.Hp;
+        k_pad<T><<<pad_grid(c.V), 256, 0, st>>>(w, ldw, c.V, c.H, l.Hp, (T*)(ws + l.w));
+        w = (const T*)(ws + l.w);
+        ldw = l.Hp;
     }
     ProductArgs base = {};
     base.zeros = scal->zeros;
@@ -779,11 +781,18 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
     // no tokens: dW is a product over nothing
     for (long at = 0; at < c.N || (at == 0 && c.dw != nullptr); at += tokens > 0 ? tokens : 1) {
         const long n = c.N - at < tokens ? c.N - at : tokens;
+        const T* xs = x + at * ldx;   // this piece's tokens
+        long ldxs = ldx;
+        if (c.pad && n > 0) {
+            k_pad<T><<<pad_grid(n), 256, 0, st>>>(xs, ldx, n, c.H, l.Hp, (T*)(ws + l.x));
+            xs = (const T*)(ws + l.x);
+            ldxs = l.Hp;
+        }
         if (n > 0) {
             ProductArgs q = base;
             q.M = c.V, q.N = n, q.K = l.Hp;
             q.A = w, q.lda = ldw;
-            q.B = x + at * ldx, q.ldb = ldx;
+            q.B = xs, q.ldb = ldxs;
             q.target = c.target + at;
             q.zt = (float*)(ws + l.zt);
             q.stat = (float2*)(ws + l.stat);
@@ -815,7 +824,7 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
         if (c.dw != nullptr) {
             ProductArgs d = base;
             d.M = c.H, d.N = c.V, d.K = n;
-            d.A = x + at * ldx, d.lda = ldx;
+            d.A = xs, d.lda = ldxs;
             d.B = ws + l.p, d.ldb = l.ldp;
             d.C = c.dw;
             d.vector = c.H % 8 == 0 && (uintptr_t)c.dw % 16 == 0;
@@ -837,8 +846,8 @@ extern "C" {
 long spanqr_linear_cross_entropy_workspace(int type, long N, long H, long V, int grads, long most_bytes) {
     const int rc = check_sizes(type, N, H, V);
     if (rc != SPANQR_OK) return rc;
-    // (with room for the copies that unaligned operands need)
-    return layout_of(N, H, V, grads, true, tokens_of(N, H, V, grads, true, most_bytes)).bytes;
+    const bool pad = (grads & 4) || H % 8 != 0;
+    return layout_of(N, H, V, grads & 3, pad, tokens_of(N, H, V, grads & 3, pad, most_bytes)).bytes;
 }
 
 int spanqr_linear_cross_entropy(int type, int reduction, long N, long H, long V, const void* x, long ldx, const void* w,

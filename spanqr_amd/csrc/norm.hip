@@ -6,7 +6,7 @@
 //
 // Both are bound by memory: one read of every input and one write of every output, with the row in registers between
 // the sums and the output. A row belongs to `group` threads with NCH pieces of eight elements each: 16 lanes for up to
-// 128 elements, a wavefront for up to 2048 (no barriers), and then one workgroup of as many wavefronts as the row
+// 128 elements, a wavefront for up to 512 (no barriers), and then one workgroup of as many wavefronts as the row
 // fills, to 1024 threads and 32768 elements; longer rows are read again for each step (k_rms_long, k_rms_grad_long).
 // All sums are fp32 per thread over at most 32 elements, then a tree in a fixed order.
 #include "elements.h"
@@ -120,7 +120,26 @@ struct Group {
     }
 };
 
-template <typename T, int GROUP, int NCH>
+// piece `at` of a row; WHOLE: the row has 8 elements at least (shorter ones are read one by one)
+template <bool WHOLE, typename T>
+__device__ __forceinline__ Pack8<T> piece(const T* row, long D, long at, int n) {
+    if constexpr (WHOLE) return fetch8(row, D, at);
+    Pack8<T> k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k.v[i] = i < n ? row[at + i] : (T)0.0f;
+    return k;
+}
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void settle(const Pack8<T>& k, int n, float (&f)[8]) {
+    if constexpr (WHOLE) {
+        settle8(k, n, f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (float)k.v[i];
+    }
+}
+
+template <typename T, int GROUP, int NCH, bool WHOLE>
 __global__ __launch_bounds__(Group<GROUP>::MOST) void k_rms(const NormArgs p) {
     typedef Group<GROUP> G;
     __shared__ float slot[3][1][16];   // the sums' by turns, and the maximum's
@@ -135,24 +154,37 @@ __global__ __launch_bounds__(Group<GROUP>::MOST) void k_rms(const NormArgs p) {
     for (long base = (long)blockIdx.x * G::rows(); base < p.rows; base += (long)gridDim.x * G::rows(), turn ^= 1) {
         const long row = base + G::index();
         const bool on = row < p.rows;   // the group's lanes all take part in the reductions
+        const T* x = (const T*)p.x + (on ? row : base) * p.ldx;
         float v[NCH][8];
+        Pack8<T> kx[NCH];
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
             const long at = 8l * (lane + c * size);
-            load8((const T*)p.x + row * p.ldx + at, on ? inside(p.D, at) : 0, v[c]);
+            kx[c] = piece<WHOLE>(x, p.D, at, inside(p.D, at));
         }
         if (p.residual != nullptr) {
+            const T* r = (const T*)p.residual + (on ? row : base) * p.ldr;
+            Pack8<T> kr[NCH];
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const long at = 8l * (lane + c * size);
+                kr[c] = piece<WHOLE>(r, p.D, at, inside(p.D, at));
+            }
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
                 const long at = 8l * (lane + c * size);
                 const int n = on ? inside(p.D, at) : 0;
-                float r[8];
-                load8((const T*)p.residual + row * p.ldr + at, n, r);
+                float u[8];
+                settle<WHOLE>(kx[c], n, v[c]);
+                settle<WHOLE>(kr[c], n, u);
                 // the stream is rounded as it is kept; the norm is of the rounded values
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[c][i] = (float)(T)(v[c][i] + r[i]);
+                for (int i = 0; i < 8; ++i) v[c][i] = (float)(T)(v[c][i] + u[i]);
                 store8((T*)p.h + row * p.D + at, n, v[c]);
             }
+        } else {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) settle<WHOLE>(kx[c], on ? inside(p.D, 8l * (lane + c * size)) : 0, v[c]);
         }
         float sum[1] = {0.0f};
 #pragma unroll
@@ -247,7 +279,7 @@ __global__ __launch_bounds__(1024) void k_rms_long(const NormArgs p) {
 
 // The weight's gradient is a sum over rows: a workgroup keeps its rows' part in registers (each thread always holds the
 // same columns), adds its groups through LDS and writes one row of partial sums; k_rms_dw adds those.
-template <typename T, int GROUP, int NCH>
+template <typename T, int GROUP, int NCH, bool WHOLE>
 __global__ __launch_bounds__(Group<GROUP>::MOST) void k_rms_grad(const GradArgs p) {
     typedef Group<GROUP> G;
     __shared__ float slot[2][2][16];
@@ -266,42 +298,61 @@ __global__ __launch_bounds__(Group<GROUP>::MOST) void k_rms_grad(const GradArgs 
     for (long base = (long)blockIdx.x * ROWS; base < p.rows; base += (long)gridDim.x * ROWS, turn ^= 1) {
         const long row = base + group;
         const bool on = row < p.rows;
-        float h[NCH][8], u[NCH][8], d[NCH][8];
+        const long from = on ? row : base;
+        Pack8<T> kh[NCH], ku[NCH], kd[NCH];
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
             const long at = 8l * (lane + c * size);
-            const int n = on ? inside(p.D, at) : 0;
-            load8((const T*)p.h + row * p.ldh + at, n, h[c]);
-            load8((const T*)p.dy + row * p.lddy + at, n, u[c]);
-            if (p.dh != nullptr) {
-                load8((const T*)p.dh + row * p.lddh + at, n, d[c]);
-            } else {
+            const int n = inside(p.D, at);
+            kh[c] = piece<WHOLE>((const T*)p.h + from * p.ldh, p.D, at, n);
+            ku[c] = piece<WHOLE>((const T*)p.dy + from * p.lddy, p.D, at, n);
+        }
+        if (p.dh != nullptr) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[c][i] = 0.0f;
+            for (int c = 0; c < NCH; ++c) {
+                const long at = 8l * (lane + c * size);
+                kd[c] = piece<WHOLE>((const T*)p.dh + from * p.lddh, p.D, at, inside(p.D, at));
             }
+        } else {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) kd[c].v[i] = (T)0.0f;
         }
         float sum[2] = {0.0f, 0.0f};   // of h^2, and of u h
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
+        for (int c = 0; c < NCH; ++c) {
+            float h[8], u[8];
+            const int n = on ? inside(p.D, 8l * (lane + c * size)) : 0;
+            settle<WHOLE>(kh[c], n, h);
+            settle<WHOLE>(ku[c], n, u);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                sum[0] = fmaf(h[c][i], h[c][i], sum[0]);
-                sum[1] = fmaf(u[c][i] * w[c][i], h[c][i], sum[1]);
+                sum[0] = fmaf(h[i], h[i], sum[0]);
+                sum[1] = fmaf(u[i] * w[c][i], h[i], sum[1]);
             }
+        }
         G::template reduce<Sum>(sum, slot[turn]);
         // a group without a row adds zeros, also where eps is 0
         const float s = on ? rsqrtf(sum[0] / (float)p.D + p.eps) : 0.0f;
         const float m = s * sum[1] / (float)p.D;   // the mean of u n
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
+            again(kh[c]);   // (packed they take half the registers until here)
+            again(ku[c]);
             const long at = 8l * (lane + c * size);
+            const int n = on ? inside(p.D, at) : 0;
+            float h[8], u[8], d[8];
+            settle<WHOLE>(kh[c], n, h);
+            settle<WHOLE>(ku[c], n, u);
+            settle<WHOLE>(kd[c], n, d);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float nrm = h[c][i] * s;
-                dw[c][i] = fmaf(u[c][i], nrm, dw[c][i]);
-                d[c][i] = fmaf(s, u[c][i] * w[c][i] - nrm * m, d[c][i]);
+                const float nrm = h[i] * s;
+                dw[c][i] = fmaf(u[i], nrm, dw[c][i]);
+                d[i] = fmaf(s, u[i] * w[c][i] - nrm * m, d[i]);
             }
-            store8((T*)p.dx + row * p.D + at, on ? inside(p.D, at) : 0, d[c]);
+            store8((T*)p.dx + row * p.D + at, n, d);
         }
     }
     if (p.part == nullptr) return;
@@ -327,51 +378,63 @@ __global__ __launch_bounds__(Group<GROUP>::MOST) void k_rms_grad(const GradArgs 
     }
 }
 
-template <typename T>
+// The gradient of rows longer than 16384, whose sums for dw would not stay in registers beside the row: the row is
+// read twice (from L2 the second time), and the sums are in LDS (up to 32768 columns), or in the partial sums' own memory.
+template <typename T, bool IN_LDS>
 __global__ __launch_bounds__(1024) void k_rms_grad_long(const GradArgs p) {
-    __shared__ float slot[16];
-    for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    __shared__ float slot[2][2][16];
+    __shared__ float add[IN_LDS ? 32768 : 1];
+    typedef Group<0> G;
+    const int t = threadIdx.x;
+    if constexpr (IN_LDS) {
+        for (int i = t; i < 32768; i += 1024) add[i] = 0.0f;   // (a thread's own words)
+    }
+    int turn = 0;
+    for (long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const T* hr = (const T*)p.h + row * p.ldh;
         const T* ur = (const T*)p.dy + row * p.lddy;
         float h[8], u[8], w[8], d[8];
-        float hh = 0.0f, uh = 0.0f;
-        for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll 2
+        for (long at = 8l * t; at < p.D; at += 8192) {
             const int n = inside(p.D, at);
-            load8(hr + at, n, h);
-            load8(ur + at, n, u);
+            const Pack8<T> kh = fetch8(hr, p.D, at), ku = fetch8(ur, p.D, at);
             load_weight(p.weight, p.wtype, at, n, w);
+            settle8(kh, n, h);
+            settle8(ku, n, u);
             float a = 0.0f, b = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 a = fmaf(h[i], h[i], a);
-                // (weights past the end are not read as 0 without a weight tensor; u is 0 there)
                 b = fmaf(u[i] * w[i], h[i], b);
             }
-            hh += a;
-            uh += b;
+            sum[0] += a;
+            sum[1] += b;
         }
-        hh = reduce_threads<1024, Sum>(hh, slot);
-        uh = reduce_threads<1024, Sum>(uh, slot);
-        const float s = rsqrtf(hh / (float)p.D + p.eps);
-        const float m = s * uh / (float)p.D;
-        for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
+        G::template reduce<Sum>(sum, slot[turn]);
+        const float s = rsqrtf(sum[0] / (float)p.D + p.eps);
+        const float m = s * sum[1] / (float)p.D;
+        float* mine = add + t;
+#pragma unroll 2
+        for (long at = 8l * t; at < p.D; at += 8192, mine += 8192) {
             const int n = inside(p.D, at);
-            load8(hr + at, n, h);
-            load8(ur + at, n, u);
-            load_weight(p.weight, p.wtype, at, n, w);
+            const Pack8<T> kh = fetch8(hr, p.D, at), ku = fetch8(ur, p.D, at);
             if (p.dh != nullptr) {
-                load8((const T*)p.dh + row * p.lddh + at, n, d);
+                settle8(fetch8((const T*)p.dh + row * p.lddh, p.D, at), n, d);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) d[i] = 0.0f;
             }
+            load_weight(p.weight, p.wtype, at, n, w);
+            settle8(kh, n, h);
+            settle8(ku, n, u);
             float dw[8];
             float* part = p.part == nullptr ? nullptr : p.part + blockIdx.x * p.D + at;
-            if (part != nullptr && row != blockIdx.x) {
+            if (!IN_LDS && part != nullptr && row != blockIdx.x) {
                 load8(part, n, dw);
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dw[i] = 0.0f;
+                for (int i = 0; i < 8; ++i) dw[i] = IN_LDS ? mine[1024 * i] : 0.0f;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -380,26 +443,41 @@ __global__ __launch_bounds__(1024) void k_rms_grad_long(const GradArgs p) {
                 d[i] = fmaf(s, u[i] * w[i] - nrm * m, d[i]);
             }
             store8((T*)p.dx + row * p.D + at, n, d);
-            if (part != nullptr) store8(part, n, dw);
+            if constexpr (IN_LDS) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mine[1024 * i] = dw[i];
+            } else if (part != nullptr) {
+                store8(part, n, dw);
+            }
+        }
+    }
+    if (IN_LDS && p.part != nullptr) {
+        const float* mine = add + t;
+        for (long at = 8l * t; at < p.D; at += 8192, mine += 8192) {
+            float dw[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dw[i] = mine[1024 * i];
+            store8(p.part + blockIdx.x * p.D + at, inside(p.D, at), dw);
         }
     }
 }
 
-// dw[d] = sum of part[0..parts)[d]: 64 columns a workgroup, 16 threads a column, added in a fixed order
+// dw[d] = sum of part[0..parts)[d]: 16 columns a workgroup, 64 threads a column, added in a fixed order
 __global__ __launch_bounds__(1024) void k_rms_dw(const float* part, int parts, long D, void* dw, int wtype) {
-    __shared__ float add[16][64];
-    const int col = threadIdx.x & 63, at = threadIdx.x >> 6;
-    const long d = 64l * blockIdx.x + col;
+    __shared__ float add[64][17];
+    const int col = threadIdx.x & 15, at = threadIdx.x >> 4;
+    long d = 16l * blockIdx.x + col;
     float sum = 0.0f;
     if (d < D) {
 #pragma unroll 8
-        for (int i = at; i < parts; i += 16) sum += part[i * D + d];
+        for (int i = at; i < parts; i += 64) sum += part[i * D + d];
     }
     add[at][col] = sum;
     __syncthreads();
-    if (at > 0 || d >= D) return;
-#pragma unroll
-    for (int i = 1; i < 16; ++i) sum += add[i][col];
+    // a wavefront a column
+    d = 16l * blockIdx.x + (threadIdx.x >> 6);
+    sum = reduce_lanes<64, Sum>(add[threadIdx.x & 63][threadIdx.x >> 6]);
+    if ((threadIdx.x & 63) != 0 || d >= D) return;
     if (wtype == SPANQR_BF16)
         ((bf16*)dw)[d] = (bf16)sum;
     else if (wtype == SPANQR_FP16)
@@ -409,48 +487,47 @@ __global__ __launch_bounds__(1024) void k_rms_dw(const float* part, int parts, l
 }
 
 constexpr long LONG_ROW = 32768;    // longest row that stays in registers
+constexpr long LONG_GRAD = 16384;   // and in the gradient
 constexpr long MAX_D = 1l << 24;
 constexpr int GRAD_PARTS = 1024;    // most workgroups of the gradient, and so rows of partial sums
 
-// threads of a row and pieces a thread
+// Threads of a row and pieces a thread. Measured, forward / backward in us: 16384 x 2048 bf16 as 256 threads of one piece
+// 51 / 50, as 128 of two 53 / 53, as a wavefront of four 60 / 55; 4096 x 5120 with 8 bits as 640 of one 40, as 320 of two 31,
+// as 192 of four 35. One token of 5120 as 640 of one 3.8, as 256 of four 6.7.
 struct Split {
     int group, nch;   // group 16 or 64: lanes of a wavefront; else (64 and `block`) a workgroup
     bool block;
 };
 Split split_of(long rows, long D) {
     const long pieces = (D + 7) / 8;
-    // with few rows a row takes as many threads as it can
-    if (rows <= 512 && D > 512 && D <= 8192) return {(int)((pieces + 63) / 64 * 64), 1, true};
     if (D <= 128) return {16, 1, false};
     if (D <= 512) return {64, 1, false};
-    if (D <= 1024) return {64, 2, false};
-    if (D <= 2048) return {64, 4, false};
-    const int nch = D <= 16384 ? 2 : 4;
+    const int nch = D <= 2048 || (rows <= 512 && D <= 8192) ? 1 : D <= 16384 ? 2 : 4;
     return {(int)(((pieces + nch - 1) / nch + 63) / 64 * 64), nch, true};
 }
 
+// workgroups for `rows` rows, each of about as many rows as the others, `most` at most
 int grid_of(long rows, const Split& s, int most) {
     const int per = s.block ? 1 : 256 / s.group;
-    const long need = (rows + per - 1) / per;
-    return (int)(need < most ? need : most);
+    const long need = (rows + per - 1) / per, turns = (need + most - 1) / most;
+    return turns < 1 ? 0 : (int)((need + turns - 1) / turns);
 }
 
 int grad_parts(long rows, long D) {
-    if (D > LONG_ROW) return (int)(rows < 256 ? rows : 256);
+    if (D > LONG_GRAD) return (int)(rows < 256 ? rows : 256);
     return grid_of(rows, split_of(rows, D), GRAD_PARTS);
 }
 
 #define SPANQR_SPLITS(LAUNCH)                                       \
     if (s.block) {                                                  \
-        if (s.nch == 1) LAUNCH(0, 1, s.group);                      \
-        else if (s.nch == 2) LAUNCH(0, 2, s.group);                 \
-        else LAUNCH(0, 4, s.group);                                 \
+        if (s.nch == 1) LAUNCH(0, 1, true, s.group);                \
+        else if (s.nch == 2) LAUNCH(0, 2, true, s.group);           \
+        else LAUNCH(0, 4, true, s.group);                           \
     } else if (s.group == 16) {                                     \
-        LAUNCH(16, 1, 256);                                         \
+        if (p.D >= 8) LAUNCH(16, 1, true, 256);                     \
+        else LAUNCH(16, 1, false, 256);                             \
     } else {                                                        \
-        if (s.nch == 1) LAUNCH(64, 1, 256);                         \
-        else if (s.nch == 2) LAUNCH(64, 2, 256);                    \
-        else LAUNCH(64, 4, 256);                                    \
+        LAUNCH(64, 1, true, 256);                                   \
     }
 
 template <typename T>
@@ -460,20 +537,23 @@ void launch_norm(const NormArgs& p, hipStream_t st) {
         return;
     }
     const Split s = split_of(p.rows, p.D);
-    const int grid = grid_of(p.rows, s, 4096);
-#define LAUNCH(G, C, N) k_rms<T, G, C><<<grid, N, 0, st>>>(p)
+    const int grid = grid_of(p.rows, s, s.block ? 1024 : 2048);
+#define LAUNCH(G, C, W, N) k_rms<T, G, C, W><<<grid, N, 0, st>>>(p)
     SPANQR_SPLITS(LAUNCH)
 #undef LAUNCH
 }
 
 template <typename T>
 void launch_grad(const GradArgs& p, int grid, hipStream_t st) {
-    if (p.D > LONG_ROW) {
-        k_rms_grad_long<T><<<grid, 1024, 0, st>>>(p);
+    if (p.D > LONG_GRAD) {
+        if (p.D <= 32768)
+            k_rms_grad_long<T, true><<<grid, 1024, 0, st>>>(p);
+        else
+            k_rms_grad_long<T, false><<<grid, 1024, 0, st>>>(p);
         return;
     }
     const Split s = split_of(p.rows, p.D);
-#define LAUNCH(G, C, N) k_rms_grad<T, G, C><<<grid, N, 0, st>>>(p)
+#define LAUNCH(G, C, W, N) k_rms_grad<T, G, C == 4 ? 2 : C, W><<<grid, N, 0, st>>>(p)   // (four pieces: rows above 16384)
     SPANQR_SPLITS(LAUNCH)
 #undef LAUNCH
 }
@@ -543,7 +623,7 @@ int spanqr_rms_norm_backward(int type, int wtype, long rows, long D, const void*
             launch_grad<float>(p, parts, st);
     }
     if (dw != nullptr)
-        k_rms_dw<<<(int)((D + 63) / 64), 1024, 0, st>>>((const float*)workspace, parts, D, dw, wtype);
+        k_rms_dw<<<(int)((D + 15) / 16), 1024, 0, st>>>((const float*)workspace, parts, D, dw, wtype);
     return launched("rms_norm_backward");
 }
 

@@ -9,12 +9,13 @@ from .tensors import TYPES, check_same, check_tensor, on, workspace
 
 IGNORE_INDEX = -100
 MAX_WORKSPACE = 4 << 30   # bytes: 16-bit exponentials of 16384 tokens over 128000 columns
+MAX_STRIDE = 1 << 22
 REDUCTIONS = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
 
 
 def _rows(t):
-    """rows of neighbouring elements, apart from each other"""
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+    """rows of neighbouring elements, apart from each other but not further than the library's offsets reach"""
+    if (t.stride(1) != 1 and t.shape[1] > 1) or (not t.shape[1] <= t.stride(0) <= MAX_STRIDE and t.shape[0] > 1):
         t = t.contiguous()
     return t
 
@@ -50,6 +51,8 @@ def _run(x, weight, target, reduction, ignore_index, row_weight, grad_scale, nee
     dx = torch.empty(N, H, dtype=x.dtype, device=dev) if need_dx else None
     dw = torch.empty(V, H, dtype=x.dtype, device=dev) if need_dw else None
     t, grads = TYPES[x.dtype], int(need_dx) + 2 * int(need_dw)
+    if (x.data_ptr() | weight.data_ptr() | 2 * (x.stride(0) if N > 1 else 0) | 2 * (weight.stride(0) if V > 1 else 0)) % 16:
+        grads += 4   # rows that do not start on 16 bytes are copied once
     with on(dev) as stream:
         nbytes = _lib.lib().spanqr_linear_cross_entropy_workspace(t, N, H, V, grads, int(max_workspace))
         if nbytes < 0:

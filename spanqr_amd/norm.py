@@ -25,12 +25,12 @@ def _forward(x, weight, residual, eps, quant):
     D = x.shape[-1]
     x2 = rows_of(x, D)
     dev = x.device
-    code, qtype = QUANT[quant]
+    code, qtype = QUANT[quant]   # (no type of its own: x's)
     r2 = h = scale = None
     if residual is not None:
         r2 = rows_of(residual, D)
-        h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    y = torch.empty(x.shape, dtype=qtype or x.dtype, device=dev)
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
+    y = torch.empty_like(x, dtype=qtype, memory_format=torch.contiguous_format)
     if code:
         scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     if weight is not None:
@@ -103,7 +103,7 @@ def rms_norm_backward(dy, h, weight=None, eps=1e-6, dh=None, need_dw=True):
         check_same("rms_norm_backward", "dh", dh, dev, h.shape, h.dtype)
         dh = rows_of(dh, D)
     h2, dy = rows_of(h, D), rows_of(dy, D)
-    dx = torch.empty(h.shape, dtype=h.dtype, device=dev)
+    dx = torch.empty_like(h, memory_format=torch.contiguous_format)
     dw = ws = None
     nbytes = 0
     if weight is not None:

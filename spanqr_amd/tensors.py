@@ -5,7 +5,6 @@ import contextlib
 import torch
 
 from . import _lib
-from .plan import stream_handle
 
 TYPES = {torch.float32: _lib.FP32, torch.bfloat16: _lib.BF16, torch.float16: _lib.FP16}
 
@@ -38,10 +37,15 @@ def rows_of(t, D):
     return t
 
 
+# the current stream's handle by the device's index: what torch.cuda.current_stream(device).cuda_stream gives, without
+# the stream object around it (0.1 us instead of 1.9)
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
 @contextlib.contextmanager
 def _other_device(device):
     with torch.cuda.device(device):
-        yield stream_handle(device)
+        yield _stream(device.index)
 
 
 class _Here:
@@ -61,7 +65,7 @@ class _Here:
 def on(device):
     """`with on(device) as stream`: the call's current stream on `device`, with that device current"""
     if device.index == torch.cuda.current_device():
-        return _Here(stream_handle(device))
+        return _Here(_stream(device.index))
     return _other_device(device)
 
 
