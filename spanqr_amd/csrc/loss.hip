@@ -479,6 +479,118 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
     }
 }
 
+// The logits of few tokens (16 NB at most): bound by one read of W, which goes straight into registers, at any
+// alignment. A workgroup has FEW_ROWS columns of the vocabulary; its four wavefronts share the hidden size, 32 k of every
+// 128 each, and put their parts together in LDS, so that there are many loads under way (a wavefront's next four steps) and many wavefronts. Statistics
+// and exponentials as in the other kernel, for FEW_ROWS columns together.
+// 1 x 1024 x 32000: 13 us for 65 MB; the tiles above take 15, and unaligned rows would have to be copied for them.
+constexpr int FEW_ROWS = 32, FEW_TOKENS = 32;
+template <typename T, int NB>
+__global__ __launch_bounds__(256) void k_few(const ProductArgs q) {
+    typedef typename Vec<T>::x8 x8;
+    constexpr int MA = FEW_ROWS / 16, AHEAD = 4;
+    __shared__ float part[4][16 * NB][FEW_ROWS + 1];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
+    const long m0 = (long)FEW_ROWS * blockIdx.x;
+    const T *a[MA], *b[NB];
+#pragma unroll
+    for (int i = 0; i < MA; ++i) {
+        const long row = m0 + 16 * i + lo;
+        a[i] = (const T*)q.A + (row < q.M ? row : q.M - 1) * q.lda;
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const long row = 16 * j + lo;
+        b[j] = (const T*)q.B + (row < q.N ? row : q.N - 1) * q.ldb;
+    }
+    f32x4 c[MA][NB] = {};
+    auto step = [&](long k, x8(&fa)[MA], x8(&fb)[NB]) {
+#pragma unroll
+        for (int i = 0; i < MA; ++i) fa[i] = __builtin_bit_cast(x8, *(const Pack8<T>*)(a[i] + k));
+#pragma unroll
+        for (int j = 0; j < NB; ++j) fb[j] = __builtin_bit_cast(x8, *(const Pack8<T>*)(b[j] + k));
+    };
+    auto multiply = [&](const x8(&fa)[MA], const x8(&fb)[NB], f32x4(&d)[MA][NB]) {
+#pragma unroll
+        for (int i = 0; i < MA; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                if constexpr (std::is_same<T, bf16>::value)
+                    d[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], d[i][j], 0, 0, 0);
+                else
+                    d[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[i], fb[j], d[i][j], 0, 0, 0);
+            }
+    };
+    const long whole = q.K / 32;   // steps of 32 k without an end
+    long s = wave;
+    for (; s + 4 * (AHEAD - 1) < whole; s += 4 * AHEAD) {
+        x8 fa[AHEAD][MA], fb[AHEAD][NB];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) step(32 * (s + 4 * u) + 8 * hi, fa[u], fb[u]);
+        // a sum of its own for these 512 k: a long chain of additions would round at the whole sum's size
+        f32x4 d[MA][NB] = {};
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) multiply(fa[u], fb[u], d);
+#pragma unroll
+        for (int i = 0; i < MA; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) c[i][j] += d[i][j];
+    }
+    for (; 32 * s < q.K; s += 4) {
+        x8 fa[MA], fb[NB];
+        const long k = 32 * s + 8 * hi;
+        if (s < whole) {
+            step(k, fa, fb);
+        } else {
+            const int n = q.K - k >= 8 ? 8 : q.K > k ? (int)(q.K - k) : 0;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+#pragma unroll
+                for (int i = 0; i < MA; ++i) fa[i][r] = r < n ? a[i][k + r] : (T)0.0f;
+#pragma unroll
+                for (int j = 0; j < NB; ++j) fb[j][r] = r < n ? b[j][k + r] : (T)0.0f;
+            }
+        }
+        multiply(fa, fb, c);
+    }
+#pragma unroll
+    for (int i = 0; i < MA; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) part[wave][16 * j + lo][16 * i + 4 * hi + r] = c[i][j][r];
+    __syncthreads();
+    // a token's columns belong to 8 lanes, four each
+    for (int n = threadIdx.x >> 3; n < 16 * NB; n += 32) {
+        const int col = 4 * (threadIdx.x & 7);
+        const long v = m0 + col;
+        float z[4], m = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            z[r] = (part[0][n][col + r] + part[1][n][col + r]) + (part[2][n][col + r] + part[3][n][col + r]);
+            if (v + r >= q.M) z[r] = -INFINITY;
+            m = fmaxf(m, z[r]);
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        const float top = m == -INFINITY ? 0.0f : m * LOG2E;
+        const bool on = n < q.N;
+        const long tgt = on ? q.target[n] : -1;
+        T e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (v + r == tgt && v + r < q.M) q.zt[n] = z[r];
+            const float x = __builtin_amdgcn_exp2f(fmaf(z[r], LOG2E, -top));
+            sum += x;
+            e[r] = (T)x;
+        }
+        sum = reduce_lanes<8, Sum>(sum);
+        if (!on) continue;
+        if (q.p != nullptr && v < q.ldp) *(uint2*)((T*)q.p + n * q.ldp + v) = *(const uint2*)e;
+        if ((threadIdx.x & 7) == 0) q.stat[n * q.segs + blockIdx.x] = make_float2(top, sum);
+    }
+}
+
 // C = alpha times the sum of the splits' parts, in their order
 template <typename T>
 __global__ __launch_bounds__(256) void k_join(const float* acc, int splits, long rows, long M, long Mp, void* C, const float* alpha) {
@@ -672,13 +784,17 @@ Shape shape_of(long M, long N, long K, long most) {
 struct Layout {
     long scal, loss, zt, stat, p, dx_acc, dw_acc, x, w, bytes;
     long segs, ldp, Hp;
+    int seg;                     // columns that share a maximum, 2^seg
+    bool few;                    // the logits by k_few
     Shape logits, dx;            // of a full piece of the tokens
 };
 Layout layout_of(long N, long H, long V, int grads, bool pad, long tokens) {
     Layout l;
     l.logits = shape_of(V, tokens, H, 1);
     l.dx = shape_of(H, tokens, V, tokens > 0 ? split_rows(tokens) / tokens : 1);
-    l.segs = over(V, TILE_M[l.logits.kind] / 2);
+    l.few = tokens <= FEW_TOKENS;
+    l.seg = l.few ? 5 : l.logits.kind == BIG ? 7 : 6;
+    l.segs = over(V, 1l << l.seg);
     l.ldp = up(V, 64);
     l.Hp = up(H, 8);
     long at = 0;
@@ -690,7 +806,7 @@ Layout layout_of(long N, long H, long V, int grads, bool pad, long tokens) {
     l.scal = take(sizeof(Scalars));
     l.loss = take(4 * N);
     l.zt = take(4 * tokens);
-    l.stat = take(8 * tokens * over(V, 64));
+    l.stat = take(8 * (tokens <= FEW_TOKENS ? tokens * over(V, FEW_ROWS) : (tokens > 2 * FEW_TOKENS ? tokens : 2 * FEW_TOKENS) * over(V, 64)));
     l.p = take(grads ? 2 * tokens * l.ldp : 0);
     l.dx_acc = take((grads & 1) ? 4 * split_rows(tokens) * l.Hp : 0);
     l.dw_acc = take((grads & 2) && tokens < N ? 4 * l.Hp * V : 0);
@@ -765,7 +881,7 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
     const long ldx = c.ldx;
     long ldw = c.ldw;
     // (each token's loss alone needs no scale, and zeros only where the hidden size is no multiple of a step)
-    if (grads || c.reduced || l.Hp % BK != 0)
+    if (grads || c.reduced || (!l.few && l.Hp % BK != 0))
         k_prepare<<<1, 1024, 0, st>>>(c.target, c.N, c.ignore, c.mean, c.row_weight, c.grad_scale, g_scale<T>(), scal);
     auto pad_grid = [&](long rows) { return (unsigned)(over(rows * l.Hp / 8, 256) < 4096 ? over(rows * l.Hp / 8, 256) : 4096); };
     if (c.pad) {
@@ -790,7 +906,7 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
         }
         if (n > 0) {
             ProductArgs q = base;
-            q.M = c.V, q.N = n, q.K = l.Hp;
+            q.M = c.V, q.N = n, q.K = c.pad ? l.Hp : c.H;
             q.A = w, q.lda = ldw;
             q.B = xs, q.ldb = ldxs;
             q.target = c.target + at;
@@ -799,8 +915,13 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
             q.p = grads ? ws + l.p : nullptr;
             Shape s = l.logits;
             s.n_tiles = over(n, TILE_N[s.kind]);
-            product<T, true, true, LOGITS>(s, q, st);
-            FinishArgs f = {c.V, l.segs, l.ldp, c.ignore, s.kind == BIG ? 7 : 6, c.target + at,
+            if (!l.few)
+                product<T, true, true, LOGITS>(s, q, st);
+            else if (n <= 16)
+                k_few<T, 1><<<(unsigned)l.segs, 256, 0, st>>>(q);
+            else
+                k_few<T, 2><<<(unsigned)l.segs, 256, 0, st>>>(q);
+            FinishArgs f = {c.V, l.segs, l.ldp, c.ignore, l.seg, c.target + at,
                             c.row_weight == nullptr ? nullptr : c.row_weight + at, q.zt, q.stat, q.p, loss + at,
                             c.lse == nullptr ? nullptr : c.lse + at, scal};
             const long split = grads ? (n >= 2048 ? 1 : 2048 / n) : 1, most = over(l.ldp, 2048);
@@ -846,7 +967,7 @@ extern "C" {
 long spanqr_linear_cross_entropy_workspace(int type, long N, long H, long V, int grads, long most_bytes) {
     const int rc = check_sizes(type, N, H, V);
     if (rc != SPANQR_OK) return rc;
-    const bool pad = (grads & 4) || H % 8 != 0;
+    const bool pad = ((grads & 4) || H % 8 != 0) && ((grads & 3) || N > FEW_TOKENS);
     return layout_of(N, H, V, grads & 3, pad, tokens_of(N, H, V, grads & 3, pad, most_bytes)).bytes;
 }
 
@@ -865,7 +986,8 @@ int spanqr_linear_cross_entropy(int type, int reduction, long N, long H, long V,
     if ((N > 1 && ldx < H) || (V > 1 && ldw < H))
         return error(SPANQR_EINVAL, "linear_cross_entropy: a row stride below H");
     const int grads = (dx != nullptr ? 1 : 0) | (dw != nullptr ? 2 : 0);
-    const bool pad = needs_pad(x, N > 1 ? ldx : 0, w, V > 1 ? ldw : 0, H);
+    // (few tokens' losses take any alignment)
+    const bool pad = needs_pad(x, N > 1 ? ldx : 0, w, V > 1 ? ldw : 0, H) && (grads || N > FEW_TOKENS);
     const long tokens = tokens_of(N, H, V, grads, pad, workspace_bytes), need = layout_of(N, H, V, grads, pad, tokens).bytes;
     if (need > workspace_bytes) return error(SPANQR_EINVAL, "linear_cross_entropy: the workspace needs %ld bytes", need);
     const Call c = {reduction == SPANQR_REDUCE_MEAN, reduced, pad, N, H, V, x, w, ldx, ldw, target, ignore_index,
