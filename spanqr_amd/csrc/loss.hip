@@ -222,6 +222,13 @@ struct Tile {
         }
     }
 
+    // from here on every load reads the same 16 bytes
+    __device__ __forceinline__ void stay(const void* at16) {
+        base = (const char*)at16;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) off[i] = 0;
+    }
+
     // subtile i (16 rows), k 32 ks to 32 ks + 31 of this step
     __device__ __forceinline__ x8 read(int i, int ks) const {
         if constexpr (ROWS) {
@@ -331,7 +338,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
         each(std::make_integer_sequence<int, SLOTS>{}, slot);
     };
     // Step t. Behind the last step an old buffer is read once more, for nothing, and behind the last two step 1 is loaded
-    // again, so that the loop has no branches.
+    // again (the zeros, where there is only step 0), so that the loop has no branches.
     auto step = [&](int t) {
         half(std::integral_constant<int, 0>{}, nullptr, nullptr);
         // this wavefront has read the step and its loads of the next one have arrived; then everybody's
@@ -350,6 +357,9 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
             for (int i = 0; i < TB::LOADS; ++i) b.load(0, TB::BYTES, i);
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
         } else {
+            // there is no whole step that the loop could load again
+            a.stay(q.zeros);
+            b.stay(q.zeros);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         asm volatile("s_barrier" ::: "memory");
