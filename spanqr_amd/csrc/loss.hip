@@ -744,8 +744,8 @@ long over(long v, long by) { return (v + by - 1) / by; }
 enum { BIG, MID, NARROW };
 constexpr int TILE_M[] = {256, 128, 128}, TILE_N[] = {256, 128, 64};
 constexpr int SLOTS[] = {256, 512, 768};        // workgroups the device holds at once
-constexpr double STEP_US[] = {1.6, 0.95, 0.8};  // 64 k of a full device, at the clock that it keeps under this load
-constexpr double ENDS_US[] = {13.0, 9.0, 7.0};  // a workgroup's first loads and its epilogue
+constexpr double STEP_US[] = {1.65, 1.0, 0.95}; // 64 k of a full device, at the clock that it keeps under this load
+constexpr double ENDS_US[] = {11.0, 4.5, 3.5};  // a workgroup's first loads and its epilogue
 
 struct Shape {
     int kind;
@@ -755,17 +755,22 @@ struct Shape {
 };
 
 // Microseconds of C [N][M] over K in tiles of `kind`, in `splits` parts of K. Measured, in us, for 256 / 128 / 64-wide tiles:
-// logits of 512 x 768 x 32000 40 / 35 / 41, of 4000 x 1024 x 50257 475 / 493 / 544, of 64 x 2048 x 50000 75 / 57 / 55; dW
-// of the same 43 / 35 / 42, 398 / 413 / 521 and 84 / 58 / 63; dx of 512 x 768 x 32000 (and the sum of its parts) 50 + 7 / 32 +
-// 7 / 35 + 7 in 16 parts, 78 + 5 / 43 + 5 / 40 + 5 in 8.
+// logits of 512 x 768 x 32000 40 / 35 / 41, of 128 x 1024 x 32000 37 / 19 / 16, of 2000 x 2048 x 50257 435 / 462 / 538, of
+// 4000 x 1024 x 50257 475 / 493 / 544; dW of the same 43 / 35 / 42, 28 / 24 / 28, 384 / 428 / 525, 398 / 413 / 521; dx (and
+// the sum of its parts) of 512 x 768 x 32000 in 16 parts 50 + 7 / 32 + 7 / 35 + 7, in 8 78 + 5 / 43 + 5 / 40 + 5, of 2000 x
+// 2048 x 50257 in 4 parts 327 + 13 / 414 + 14 / 590 + 15, in 2 547 + 9 / 401 + 9 / 642 + 9.
 double time_of(int kind, long M, long N, long K, long splits) {
     const double tiles = (double)(over(M, TILE_M[kind]) * over(N, TILE_N[kind]) * splits);
-    double rounds = tiles / SLOTS[kind], step = STEP_US[kind];
-    if (tiles <= 256) step = kind == BIG ? step : kind == MID ? 0.6 : 0.5;   // one a compute unit
-    // tiles that share a compute unit fill each other's gaps, and the last round's
-    rounds = rounds <= 1.0 ? 1.0 : kind == BIG ? ceil(rounds) : rounds + 0.3;
-    const double join = splits > 1 ? 4.0 + 8.0 * (double)(M * N * splits) / 4e6 : 0.0;
-    return rounds * (step * (double)over(over(K, 64), splits) + ENDS_US[kind]) + join;
+    double rounds = tiles / SLOTS[kind], step = STEP_US[kind], ends = ENDS_US[kind];
+    if (tiles <= 256) {   // one a compute unit: nothing fills a gap, and small tiles have it to themselves
+        step = kind == BIG ? step : kind == MID ? 0.6 : 0.5;
+        ends += 3.0;
+    }
+    // the last round of the largest starts as workgroups end, one after the other; tiles that share a compute unit fill
+    // each other's gaps
+    rounds = rounds <= 1.0 ? 1.0 : kind == BIG ? 0.5 * (rounds + ceil(rounds)) : rounds;
+    const double join = splits > 1 ? 3.0 + 1e-6 * (double)(M * N * splits) : 0.0;
+    return rounds * (step * (double)over(over(K, 64), splits) + ends) + join;
 }
 
 // rows of fp32 sums that dx over several parts of K may take. Like all of the workspace it does not shrink with more
