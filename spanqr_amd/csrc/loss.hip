@@ -286,7 +286,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
 
     const long k0 = split * q.split_k, k1 = k0 + q.split_k < q.K ? k0 + q.split_k : q.K;
     const long K = k1 > k0 ? k1 - k0 : 0;
-    const int steps = (int)((K + BK - 1) / BK);
+    const int steps = K > 0 ? (int)((K + BK - 1) / BK) : 1;   // (without k one step of zeros)
     TA a;
     TB b;
     a.init(q.A, q.lda, q.M, m0, k0, (lds_char*)smem, wave, lane, wm);
@@ -348,30 +348,28 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
         const int k = t + 2 < steps ? t + 1 : 0;
         half(std::integral_constant<int, 1>{}, a.base + k * a.step, b.base + k * b.step);
     };
-    if (steps > 0) {
-        load_first();
-        if (steps > 1) {
+    load_first();
+    if (steps > 1) {
 #pragma unroll
-            for (int i = 0; i < TA::LOADS; ++i) a.load(0, TA::BYTES, i);
+        for (int i = 0; i < TA::LOADS; ++i) a.load(0, TA::BYTES, i);
 #pragma unroll
-            for (int i = 0; i < TB::LOADS; ++i) b.load(0, TB::BYTES, i);
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
-        } else {
-            // there is no whole step that the loop could load again
-            a.stay(q.zeros);
-            b.stay(q.zeros);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
-        asm volatile("s_barrier" ::: "memory");
-        // (scalar loads that are still under way would make the compiler wait for all LDS reads in every turn)
-        __builtin_amdgcn_s_waitcnt(0xc07f);
-#pragma unroll
-        for (int j = 0; j < IN; ++j) fb[0][j] = b.read(j, 0);
-#pragma unroll
-        for (int i = 0; i < IM; ++i) fa[0][i] = a.read(i, 0);
-        for (int t = 0; t < steps; ++t) step(t);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
+        for (int i = 0; i < TB::LOADS; ++i) b.load(0, TB::BYTES, i);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+    } else {
+        // there is no whole step that the loop could load again
+        a.stay(q.zeros);
+        b.stay(q.zeros);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
+    asm volatile("s_barrier" ::: "memory");
+    // (scalar loads that are still under way would make the compiler wait for all LDS reads in every turn)
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+#pragma unroll
+    for (int j = 0; j < IN; ++j) fb[0][j] = b.read(j, 0);
+#pragma unroll
+    for (int i = 0; i < IM; ++i) fa[0][i] = a.read(i, 0);
+    for (int t = 0; t < steps; ++t) step(t);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
 
     // the last matrix instructions' results are there after 18 clocks at most, and nothing reads c before that
     asm volatile("s_nop 15\n\ts_nop 3");
@@ -388,56 +386,55 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
     // lane: row n = lo of C, elements m = 4 hi + 0..3 of each subtile (16 hi + 0..15 of four subtiles where SPREAD)
     if constexpr (EPILOGUE == LOGITS) {
         const long first = m0 + wm + 16 * hi;   // of the lane's columns; each group of four subtiles is 64 on
-        if (m0 + wm + WM > q.M) {               // columns past the vocabulary
-#pragma unroll
-            for (int i = 0; i < IM; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool out = first + 64 * (i >> 2) + 4 * (i & 3) + r >= q.M;
-#pragma unroll
-                    for (int j = 0; j < IN; ++j) c[i][j][r] = out ? -INFINITY : c[i][j][r];
-                }
-        }
-        T* to = q.p == nullptr ? nullptr : (T*)q.p + (n0 + wn + lo) * q.ldp + first;
+        const int inside = (int)(q.M - first < 2 * WM ? q.M - first : 2 * WM);   // of them before the vocabulary's end
+        const bool whole = m0 + wm + WM <= q.M;
+        T* to = (T*)q.p + (n0 + wn + lo) * q.ldp + first;
 #pragma unroll
         for (int j = 0; j < IN; ++j) {
             const long n = n0 + wn + 16 * j + lo;
             const bool on = n < q.N;
+            float z[4 * IM];
+#pragma unroll
+            for (int i = 0; i < 4 * IM; ++i) z[i] = c[i / 4][j][i & 3];   // column 64 (i / 16) + i % 16
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 4 * IM; ++i) z[i] = 64 * (i >> 4) + (i & 15) < inside ? z[i] : -INFINITY;
+            }
             // (a maximum that passes NaN by: the sum has it)
             float m = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < IM; ++i) m = max3(max3(m, c[i][j][0], c[i][j][1]), c[i][j][2], c[i][j][3]);
+            for (int i = 0; i < 4 * IM; i += 2) m = max3(m, z[i], z[i + 1]);
             m = max3(m, m, __shfl_xor(m, 16));
             m = max3(m, m, __shfl_xor(m, 32));
             // exponentials are 2^(z log2 e - top): top is kept rounded as it is used here, so that its rounding
             // cancels where the parts are put together
             const float top = m == -INFINITY ? 0.0f : m * LOG2E;
-            const long tgt = on ? q.target[n] - first : -1;
-            if (tgt >= 0 && tgt < 64 * (IM / 4) && (tgt & 63) < 16 && first + tgt < q.M) {
-                const int k = (int)tgt;
-                float z = 0.0f;
+            const long target = on ? q.target[n] - first : -1;
+            const int at = target >= 0 && target < inside ? (int)target : -1;
+            if (at >= 0 && at < 64 * (IM / 4) && (at & 63) < 16) {
+                float zt = 0.0f;
 #pragma unroll
-                for (int i = 0; i < IM; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) z = k == 64 * (i >> 2) + 4 * (i & 3) + r ? c[i][j][r] : z;
-                q.zt[n] = z;
+                for (int i = 0; i < 4 * IM; ++i) zt = at == 64 * (i >> 4) + (i & 15) ? z[i] : zt;
+                q.zt[n] = zt;
             }
             float sum = 0.0f;
 #pragma unroll
-            for (int g = 0; g < IM / 4; ++g) {
-                x8 e[2];
+            for (int i = 0; i < 4 * IM; ++i) z[i] = __builtin_amdgcn_exp2f(fmaf(z[i], LOG2E, -top));
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float v = __builtin_amdgcn_exp2f(fmaf(c[4 * g + i / 4][j][i & 3], LOG2E, -top));
-                    sum += v;
-                    e[i >> 3][i & 7] = (T)v;
-                }
-                if (to != nullptr && on && first + 64 * g < q.ldp) {
-                    *(x8*)(to + 64 * g) = e[0];
-                    *(x8*)(to + 64 * g + 8) = e[1];
+            for (int i = 0; i < 4 * IM; ++i) sum += z[i];
+            if (q.p != nullptr && on) {
+#pragma unroll
+                for (int g = 0; g < IM / 4; ++g) {
+                    x8 e[2];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) e[i >> 3][i & 7] = (T)z[16 * g + i];
+                    if (whole || m0 + wm + 64 * g < q.ldp) {   // (rows of p are whole 64s)
+                        *(x8*)(to + 64 * g) = e[0];
+                        *(x8*)(to + 64 * g + 8) = e[1];
+                    }
                 }
             }
-            to = to == nullptr ? nullptr : to + 16 * q.ldp;
+            to += 16 * q.ldp;
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
             if (hi == 0 && on && m0 + wm < q.M) q.stat[n * q.segs + (m0 + wm) / WM] = make_float2(top, sum);
@@ -455,35 +452,40 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
             }
     } else {
         const float alpha = *q.alpha;
-        const bool whole = q.vector && m0 + BM <= q.M;
-        // Two subtiles side by side: the lanes of odd hi get the second one's elements of the lane below and give
-        // theirs of the first, so that a lane has 8 neighbouring elements and four lanes 64 bytes of a row.
-        const int col = 16 * (hi & 1) + 8 * (hi >> 1);
         T* to = (T*)q.C + (n0 + wn + lo) * q.ldc + m0 + wm;
+        if (q.vector && m0 + BM <= q.M) {
+            // Two subtiles side by side: the lanes of odd hi get the second one's elements of the lane below and give
+            // theirs of the first, so that a lane has 8 neighbouring elements and four lanes 64 bytes of a row.
+            to += 16 * (hi & 1) + 8 * (hi >> 1);
 #pragma unroll
-        for (int j = 0; j < IN; ++j, to += 16 * q.ldc) {
-            const bool on = n0 + wn + 16 * j + lo < q.N;
+            for (int j = 0; j < IN; ++j, to += 16 * q.ldc) {
+                const bool on = n0 + wn + 16 * j + lo < q.N;
 #pragma unroll
-            for (int i = 0; i < IM; i += 2) {
-                typedef T x4 __attribute__((ext_vector_type(4)));
-                x4 e[2];
+                for (int i = 0; i < IM; i += 2) {
+                    typedef T x4 __attribute__((ext_vector_type(4)));
+                    x4 e[2];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    e[0][r] = (T)(c[i][j][r] * alpha);
-                    e[1][r] = (T)(c[i + 1][j][r] * alpha);
-                }
-                if (whole) {
+                    for (int r = 0; r < 4; ++r) {
+                        e[0][r] = (T)(c[i][j][r] * alpha);
+                        e[1][r] = (T)(c[i + 1][j][r] * alpha);
+                    }
                     const uint2 u = __builtin_bit_cast(uint2, e[0]), v = __builtin_bit_cast(uint2, e[1]);
                     const auto x = __builtin_amdgcn_permlane16_swap(u.x, v.x, false, false);
                     const auto y = __builtin_amdgcn_permlane16_swap(u.y, v.y, false, false);
-                    if (on) *(uint4*)(to + 16 * i + col) = make_uint4(x[0], y[0], x[1], y[1]);
-                } else if (on) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (m0 + wm + 16 * (i + h) + 4 * hi + r < q.M) to[16 * (i + h) + 4 * hi + r] = e[h][r];
+                    if (on) *(uint4*)(to + 16 * i) = make_uint4(x[0], y[0], x[1], y[1]);
                 }
+            }
+        } else {
+            const int left = (int)(q.M - m0 - wm < 4 * BM ? q.M - m0 - wm : 4 * BM) - 4 * hi;   // elements of the row
+            to += 4 * hi;
+#pragma unroll
+            for (int j = 0; j < IN; ++j, to += 16 * q.ldc) {
+                if (n0 + wn + 16 * j + lo >= q.N) continue;
+#pragma unroll
+                for (int i = 0; i < IM; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (16 * i + r < left) to[16 * i + r] = (T)(c[i][j][r] * alpha);
             }
         }
     }
