@@ -42,9 +42,11 @@ struct Vec<fp16> {
 
 // c += a b, 16 x 16 x 32. In inline asm, because c has to stay where it is: the compiler moves accumulators about
 // between registers when they fill half the file. ACC: c in accumulation registers. It does not know that these are
-// matrix instructions, so the products' kernel waits itself before it reads c.
-#define SPANQR_MFMA(OP, AT)                                                                     \
-    asm volatile("v_mfma_f32_16x16x32_" OP " %0, %1, %2, %0" : "+" AT(c) : "v"(a), "v"(b))
+// matrix instructions, whose results may not be read for up to 18 clocks, and may copy c as soon as a loop ends: so the
+// loop's last one waits (LAST; the matrix pipe is busy with it for most of that time), in the same piece of asm.
+#define SPANQR_MFMA(OP, AT, WAIT)                                                               \
+    asm volatile("v_mfma_f32_16x16x32_" OP " %0, %1, %2, %0" WAIT : "+" AT(c) : "v"(a), "v"(b))
+#define SPANQR_MFMA_WAIT "\n\ts_nop 15\n\ts_nop 3"
 // The same, and behind it 16 bytes a lane from base + off to LDS at `lds` + IMM + 16 lane, asynchronously (counted by
 // vmcnt). The load too is in inline asm because the compiler would wait for it before any later LDS read; it has no
 // register output. The matrix instruction fills the wait between m0 and its use.
@@ -54,18 +56,26 @@ struct Vec<fp16> {
                  : "+" AT(c)                                                                     \
                  : "v"(a), "v"(b), "v"(off), "s"(base), "s"(lds), "n"(IMM)                       \
                  : "memory", "scc")
-template <typename T, bool ACC>
+template <typename T, bool ACC, bool LAST>
 __device__ __forceinline__ void mfma(typename Vec<T>::x8 a, typename Vec<T>::x8 b, f32x4& c) {
     if constexpr (std::is_same<T, bf16>::value) {
-        if constexpr (ACC)
-            SPANQR_MFMA("bf16", "a");
+        if constexpr (ACC && LAST)
+            SPANQR_MFMA("bf16", "a", SPANQR_MFMA_WAIT);
+        else if constexpr (ACC)
+            SPANQR_MFMA("bf16", "a", "");
+        else if constexpr (LAST)
+            SPANQR_MFMA("bf16", "v", SPANQR_MFMA_WAIT);
         else
-            SPANQR_MFMA("bf16", "v");
+            SPANQR_MFMA("bf16", "v", "");
     } else {
-        if constexpr (ACC)
-            SPANQR_MFMA("f16", "a");
+        if constexpr (ACC && LAST)
+            SPANQR_MFMA("f16", "a", SPANQR_MFMA_WAIT);
+        else if constexpr (ACC)
+            SPANQR_MFMA("f16", "a", "");
+        else if constexpr (LAST)
+            SPANQR_MFMA("f16", "v", SPANQR_MFMA_WAIT);
         else
-            SPANQR_MFMA("f16", "v");
+            SPANQR_MFMA("f16", "v", "");
     }
 }
 template <typename T, bool ACC, int IMM>
@@ -313,6 +323,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
     // loads at pa and pb into the other buffer. The fences keep that order.
     auto half = [&](auto ks, const char* pa, const char* pb) {
         constexpr int KS = decltype(ks)::value, SLOTS = IM * IN, READS = IM + IN;
+        static_assert(LOADS < SLOTS, "the last slot has no load");
         const uint32_t da = a.dst ^ TA::BYTES, db = b.dst ^ TB::BYTES;
         auto slot = [&](auto at) {
             constexpr int S = decltype(at)::value, i = S / IN, j = S % IN;
@@ -323,7 +334,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
                 else
                     mfma_load<T, BM == 256, (l - TA::LOADS) * 1024>(fa[KS][i], fb[KS][j], c[i][j], pb, b.off[l - TA::LOADS], db);
             } else {
-                mfma<T, BM == 256>(fa[KS][i], fb[KS][j], c[i][j]);
+                mfma<T, BM == 256, KS == 1 && S == SLOTS - 1>(fa[KS][i], fb[KS][j], c[i][j]);
             }
 #pragma unroll
             for (int r = 0; r < READS; ++r)
@@ -371,17 +382,16 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
     for (int t = 0; t < steps; ++t) step(t);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
 
-    // the last matrix instructions' results are there after 18 clocks at most, and nothing reads c before that
-    asm volatile("s_nop 15\n\ts_nop 3");
+    // (the compiler moves all of c about right here if it may)
+    auto pin = [&](int j) {
 #pragma unroll
-    for (int i = 0; i < IM; ++i)
-#pragma unroll
-        for (int j = 0; j < IN; ++j) {
+        for (int i = 0; i < IM; ++i) {
             if constexpr (BM == 256)
                 asm volatile("" : "+a"(c[i][j]));
             else
                 asm volatile("" : "+v"(c[i][j]));
         }
+    };
 
     // lane: row n = lo of C, elements m = 4 hi + 0..3 of each subtile (16 hi + 0..15 of four subtiles where SPREAD)
     if constexpr (EPILOGUE == LOGITS) {
@@ -393,6 +403,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
         for (int j = 0; j < IN; ++j) {
             const long n = n0 + wn + 16 * j + lo;
             const bool on = n < q.N;
+            pin(j);
             float z[4 * IM];
 #pragma unroll
             for (int i = 0; i < 4 * IM; ++i) z[i] = c[i / 4][j][i & 3];   // column 64 (i / 16) + i % 16
@@ -442,7 +453,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
     } else if (q.acc != nullptr) {
         float* to = q.acc + (split * q.N + n0 + wn + lo) * q.ldacc + m0 + wm + 4 * hi;
 #pragma unroll
-        for (int j = 0; j < IN; ++j, to += 16 * q.ldacc)
+        for (int j = 0; j < IN; ++j, to += 16 * q.ldacc) {
+            pin(j);
 #pragma unroll
             for (int i = 0; i < IM; ++i) {
                 if (n0 + wn + 16 * j + lo >= q.N || m0 + wm + 16 * i + 4 * hi >= q.M) continue;
@@ -450,6 +462,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
                 if (q.add) v += *(f32x4*)(to + 16 * i);
                 *(f32x4*)(to + 16 * i) = v;
             }
+        }
     } else {
         const float alpha = *q.alpha;
         T* to = (T*)q.C + (n0 + wn + lo) * q.ldc + m0 + wm;
@@ -460,6 +473,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
 #pragma unroll
             for (int j = 0; j < IN; ++j, to += 16 * q.ldc) {
                 const bool on = n0 + wn + 16 * j + lo < q.N;
+                pin(j);
 #pragma unroll
                 for (int i = 0; i < IM; i += 2) {
                     typedef T x4 __attribute__((ext_vector_type(4)));
@@ -480,6 +494,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
             to += 4 * hi;
 #pragma unroll
             for (int j = 0; j < IN; ++j, to += 16 * q.ldc) {
+                pin(j);
                 if (n0 + wn + 16 * j + lo >= q.N) continue;
 #pragma unroll
                 for (int i = 0; i < IM; ++i)

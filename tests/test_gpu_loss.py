@@ -120,6 +120,18 @@ def test_large(cuda, N, H, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,H,V", [(4096, 4096, 1024), (1024, 4096, 4096), (4096, 2048, 4096), (3999, 4001, 4099), (2001, 2049, 33003)])
+def test_largest_tiles(cuda, N, H, V, dtype):
+    """each product in 256 x 256 tiles, whole and cut ones, straight, in parts of the vocabulary and in pieces of the
+    tokens; the tokens that share a target column or a row's last 64 are many enough to reach every element of a tile"""
+    print(f"linear_cross_entropy {N}x{H}x{V} {dtype}", flush=True)
+    x, W, t = make(N, H, V, dtype, 22, ignored=0.02)
+    check_call(x, W, t, "none", (sp.linear_cross_entropy(x, W, t, reduction="none"), None, None))
+    check_call(x, W, t, "mean", sp.linear_cross_entropy_grad(x, W, t))
+    check_call(x, W, t, "sum", sp.linear_cross_entropy_grad(x, W, t, reduction="sum", max_workspace=N * V))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("N,H,V", [(7, 65, 33), (300, 128, 520), (64, 200, 1000)])
 def test_weights_and_scale(cuda, N, H, V, dtype):
     x, W, t = make(N, H, V, dtype, 2)
