@@ -21,6 +21,10 @@ def _dense(t):
     return True
 
 
+# (called through map: for hundreds of tensors a third less time than a method call each)
+_device_of, _dtype_of = torch.Tensor.get_device, torch.Tensor.dtype.__get__
+
+
 def _tensors(what, name, ts, device=None):
     """ts as a list of tensors of the three types on one GPU, and that device"""
     ts = [ts] if isinstance(ts, torch.Tensor) else list(ts)
@@ -29,10 +33,9 @@ def _tensors(what, name, ts, device=None):
     first = ts[0]
     try:   # hundreds of tensors: what is right is seen in one go, and only what is wrong is looked for
         dev = first.device if device is None else device
-        if (dev.type == "cuda" and {t.get_device() for t in ts} == {dev.index} and
-                all([t.dtype in TYPES for t in ts])):
+        if dev.type == "cuda" and set(map(_device_of, ts)) == {dev.index} and TYPES.keys() >= set(map(_dtype_of, ts)):
             return ts, dev
-    except AttributeError:
+    except (AttributeError, TypeError):   # not a tensor
         pass
     for t in ts:
         check_tensor(what, name, t)
@@ -40,11 +43,18 @@ def _tensors(what, name, ts, device=None):
     return ts, first.device
 
 
+def _contiguous(ts):
+    return all(map(torch.Tensor.is_contiguous, ts))
+
+
 def _pointers(ts):
     return array("Q", [t.data_ptr() for t in ts])
 
 
 def _types(ts):
+    kinds = set(map(_dtype_of, ts))
+    if len(kinds) == 1:   # as a rule
+        return array("i", [TYPES[kinds.pop()]]) * len(ts)
     return array("i", [TYPES[t.dtype] for t in ts])
 
 
@@ -61,7 +71,7 @@ def grad_norm(grads):
     any shapes and strides, on one ROCm device. A float32 tensor without axes on that device, no host synchronisation;
     squares and sums in float64. An empty list gives 0."""
     ts, dev = _tensors("grad_norm", "every gradient", grads)
-    if not all([t.is_contiguous() for t in ts]):
+    if not _contiguous(ts):
         ts = [t if _dense(t) else t.contiguous() for t in ts]
     n = len(ts)
     at, numel, types = _pointers(ts), _sizes(ts), _types(ts)
@@ -118,7 +128,7 @@ def clip_grad_norm(grads, max_norm, out=None):
                 check_same("clip_grad_norm", "a tensor of out", o, dev, g.shape)
     back = ()
     src, dst = grads, out
-    if not (all([g.is_contiguous() for g in grads]) and (out is grads or all([o.is_contiguous() for o in out]))):
+    if not (_contiguous(grads) and (out is grads or _contiguous(out))):
         src, dst, back = _in_rows(grads, out, dev)
     n = len(src)
     at, numel, types = _pointers(src), _sizes(src), _types(src)

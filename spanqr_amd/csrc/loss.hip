@@ -510,6 +510,9 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
 // alignment. A workgroup has FEW_ROWS columns of the vocabulary; its four wavefronts share the hidden size, 32 k of every
 // 128 each, and put their parts together in LDS, so that there are many loads under way (a wavefront's next four steps) and many wavefronts. Statistics
 // and exponentials as in the other kernel, for FEW_ROWS columns together.
+// With few tokens a single rounding of G shows in a whole gradient (no other tokens' average it away), and rows of the
+// products' tiles are free: so p and G have two rows a token, the rounded values and behind all of those what was
+// rounded off, and the gradients see 16 bits of them (bf16) or 21.
 // 1 x 1024 x 32000: 13 us for 65 MB; the tiles above take 15, and unaligned rows would have to be copied for them.
 constexpr int FEW_ROWS = 32, FEW_TOKENS = 32;
 template <typename T, int NB>
@@ -603,29 +606,45 @@ __global__ __launch_bounds__(256) void k_few(const ProductArgs q) {
         const float top = m == -INFINITY ? 0.0f : m * LOG2E;
         const bool on = n < q.N;
         const long tgt = on ? q.target[n] : -1;
-        T e[4];
+        typedef T x4 __attribute__((ext_vector_type(4)));
+        x4 e, rest;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             if (v + r == tgt && v + r < q.M) q.zt[n] = z[r];
             const float x = __builtin_amdgcn_exp2f(fmaf(z[r], LOG2E, -top));
             sum += x;
             e[r] = (T)x;
+            rest[r] = (T)(x - (float)e[r]);
         }
         sum = reduce_lanes<8, Sum>(sum);
         if (!on) continue;
-        if (q.p != nullptr && v < q.ldp) *(uint2*)((T*)q.p + n * q.ldp + v) = *(const uint2*)e;
+        if (q.p != nullptr && v < q.ldp) {
+            *(x4*)((T*)q.p + n * q.ldp + v) = e;
+            *(x4*)((T*)q.p + (q.N + n) * q.ldp + v) = rest;
+        }
         if ((threadIdx.x & 7) == 0) q.stat[n * q.segs + blockIdx.x] = make_float2(top, sum);
     }
 }
 
-// C = alpha times the sum of the splits' parts, in their order
+// C = alpha times the sum of the splits' parts, in their order, of `rows` rows each; two: of twice as many, the second
+// half added to the first
 template <typename T>
-__global__ __launch_bounds__(256) void k_join(const float* acc, int splits, long rows, long M, long Mp, void* C, const float* alpha) {
+__global__ __launch_bounds__(256) void k_join(const float* acc, int splits, bool two, long rows, long M, long Mp, void* C,
+                                              const float* alpha) {
     const long n = rows * Mp / 4;
+    const int parts = two ? 2 * splits : splits;
     const float a = *alpha;
     for (long i = blockIdx.x * 256l + threadIdx.x; i < n; i += 256l * gridDim.x) {
         f32x4 v = ((const f32x4*)acc)[i];
-        for (int s = 1; s < splits; ++s) v += ((const f32x4*)acc)[s * n + i];
+        int s = 1;
+        for (; s + 8 <= parts; s += 8) {   // (their loads together)
+            f32x4 u[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) u[k] = ((const f32x4*)acc)[(s + k) * n + i];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v += u[k];
+        }
+        for (; s < parts; ++s) v += ((const f32x4*)acc)[s * n + i];
         const long row = 4 * i / Mp, m = 4 * i - row * Mp;
         T* to = (T*)C + row * M + m;
 #pragma unroll
@@ -685,6 +704,7 @@ struct FinishArgs {
     void* p;                     // or null: the loss alone
     float *loss, *lse;
     const Scalars* scal;
+    long rest;                   // elements from a row of p to the one with what was rounded off, or 0
 };
 
 // one token a blockIdx.x: lse from the segments' statistics, the loss, and p -> G in the columns of blockIdx.y
@@ -718,6 +738,12 @@ __global__ __launch_bounds__(256) void k_finish(const FinishArgs q) {
             for (int k = 0; k < 8; ++k) e[k] = 0.0f;
         } else {
             load8(p + v, 8, e);
+            if (q.rest) {
+                float r[8];
+                load8(p + q.rest + v, 8, r);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) e[k] += r[k];
+            }
             const float s = v < q.V ? f * __builtin_amdgcn_exp2f(stat[v >> q.seg].x - lse2) : 0.0f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) e[k] = v + k < q.V ? e[k] * s : 0.0f;
@@ -728,6 +754,14 @@ __global__ __launch_bounds__(256) void k_finish(const FinishArgs q) {
             }
         }
         store8(p + v, 8, e);
+        if (q.rest) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float r = e[k] - (float)(T)e[k];
+                e[k] = r == r ? r : 0.0f;   // (infinite or NaN: the first row has it)
+            }
+            store8(p + q.rest + v, 8, e);
+        }
     }
 }
 
@@ -740,14 +774,15 @@ __global__ __launch_bounds__(1024) void k_total(const float* loss, long N, const
     if (threadIdx.x == 0) *out = (float)(sum * (double)scal->per);
 }
 
-// rows of H elements to rows of Hp (the next multiple of 8), the rest 0: operands whose rows do not start on 16 bytes
+// rows of H elements to rows of Hp (the next multiple of 8), the rest 0: operands whose rows do not start on 16 bytes.
+// `times` the same rows, one lot after the other.
 template <typename T>
-__global__ __launch_bounds__(256) void k_pad(const T* src, long ld, long rows, long H, long Hp, T* dst) {
+__global__ __launch_bounds__(256) void k_pad(const T* src, long ld, long rows, int times, long H, long Hp, T* dst) {
     const long pieces = Hp / 8;
-    for (long i = blockIdx.x * 256l + threadIdx.x; i < rows * pieces; i += 256l * gridDim.x) {
+    for (long i = blockIdx.x * 256l + threadIdx.x; i < times * rows * pieces; i += 256l * gridDim.x) {
         const long row = i / pieces, at = 8 * (i - row * pieces);
         float v[8];
-        load8(src + row * ld + at, H - at >= 8 ? 8 : (int)(H - at), v);
+        load8(src + row % rows * ld + at, H - at >= 8 ? 8 : (int)(H - at), v);
         store8(dst + row * Hp + at, 8, v);
     }
 }
@@ -794,7 +829,8 @@ double time_of(int kind, long M, long N, long K, long splits) {
 // tokens, so that what fits for some fits for fewer.
 long split_rows(long tokens) {
     const long most = 2 * tokens > 16384 ? 2 * tokens : 16384;
-    return 64 * tokens < most ? 64 * tokens : most;
+    const long rows = tokens <= FEW_TOKENS ? 128 * tokens : tokens <= 2 * FEW_TOKENS ? 128 * FEW_TOKENS : 64 * tokens;
+    return rows < most ? rows : most;
 }
 
 // the fastest by time_of, in at most `most` parts of K
@@ -817,14 +853,15 @@ struct Layout {
     long scal, loss, zt, stat, p, dx_acc, dw_acc, x, w, bytes;
     long segs, ldp, Hp;
     int seg;                     // columns that share a maximum, 2^seg
-    bool few;                    // the logits by k_few
+    bool few;                    // the logits by k_few, p and G in two rows a token
     Shape logits, dx;            // of a full piece of the tokens
 };
 Layout layout_of(long N, long H, long V, int grads, bool pad, long tokens) {
     Layout l;
     l.logits = shape_of(V, tokens, H, 1);
-    l.dx = shape_of(H, tokens, V, tokens > 0 ? split_rows(tokens) / tokens : 1);
     l.few = tokens <= FEW_TOKENS;
+    const long rows = l.few ? 2 * tokens : tokens;   // of p
+    l.dx = shape_of(H, rows, V, rows > 0 ? split_rows(tokens) / rows : 1);
     l.seg = l.few ? 5 : l.logits.kind == BIG ? 7 : 6;
     l.segs = over(V, 1l << l.seg);
     l.ldp = up(V, 64);
@@ -838,11 +875,12 @@ Layout layout_of(long N, long H, long V, int grads, bool pad, long tokens) {
     l.scal = take(sizeof(Scalars));
     l.loss = take(4 * N);
     l.zt = take(4 * tokens);
-    l.stat = take(8 * (tokens <= FEW_TOKENS ? tokens * over(V, FEW_ROWS) : (tokens > 2 * FEW_TOKENS ? tokens : 2 * FEW_TOKENS) * over(V, 64)));
-    l.p = take(grads ? 2 * tokens * l.ldp : 0);
+    const long most = l.few || tokens > 2 * FEW_TOKENS ? rows : 2 * FEW_TOKENS;   // (not below what fewer tokens need)
+    l.stat = take(8 * (l.few ? tokens * over(V, FEW_ROWS) : most * over(V, 64)));
+    l.p = take(grads ? 2 * most * l.ldp : 0);
     l.dx_acc = take((grads & 1) ? 4 * split_rows(tokens) * l.Hp : 0);
     l.dw_acc = take((grads & 2) && tokens < N ? 4 * l.Hp * V : 0);
-    l.x = take(pad ? 2 * tokens * l.Hp : 0);
+    l.x = take(pad ? 2 * most * l.Hp : (grads & 2) ? 2 * (l.few ? rows : 2 * FEW_TOKENS) * l.Hp : 0);
     l.w = take(pad ? 2 * V * l.Hp : 0);
     l.bytes = at;
     return l;
@@ -917,7 +955,7 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
         k_prepare<<<1, 1024, 0, st>>>(c.target, c.N, c.ignore, c.mean, c.row_weight, c.grad_scale, g_scale<T>(), scal);
     auto pad_grid = [&](long rows) { return (unsigned)(over(rows * l.Hp / 8, 256) < 4096 ? over(rows * l.Hp / 8, 256) : 4096); };
     if (c.pad) {
-        k_pad<T><<<pad_grid(c.V), 256, 0, st>>>(w, ldw, c.V, c.H, l.Hp, (T*)(ws + l.w));
+        k_pad<T><<<pad_grid(c.V), 256, 0, st>>>(w, ldw, c.V, 1, c.H, l.Hp, (T*)(ws + l.w));
         w = (const T*)(ws + l.w);
         ldw = l.Hp;
     }
@@ -931,8 +969,10 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
         const long n = c.N - at < tokens ? c.N - at : tokens;
         const T* xs = x + at * ldx;   // this piece's tokens
         long ldxs = ldx;
-        if (c.pad && n > 0) {
-            k_pad<T><<<pad_grid(n), 256, 0, st>>>(xs, ldx, n, c.H, l.Hp, (T*)(ws + l.x));
+        const bool two = l.few && n > 0;   // rows a token in p, and x twice for dW
+        if (n > 0 && (c.pad || (two && c.dw != nullptr))) {
+            const int times = two && c.dw != nullptr ? 2 : 1;
+            k_pad<T><<<pad_grid(times * n), 256, 0, st>>>(xs, ldx, n, times, c.H, l.Hp, (T*)(ws + l.x));
             xs = (const T*)(ws + l.x);
             ldxs = l.Hp;
         }
@@ -955,37 +995,37 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
                 k_few<T, 2><<<(unsigned)l.segs, 256, 0, st>>>(q);
             FinishArgs f = {c.V, l.segs, l.ldp, c.ignore, l.seg, c.target + at,
                             c.row_weight == nullptr ? nullptr : c.row_weight + at, q.zt, q.stat, q.p, loss + at,
-                            c.lse == nullptr ? nullptr : c.lse + at, scal};
+                            c.lse == nullptr ? nullptr : c.lse + at, scal, two ? n * l.ldp : 0};
             const long split = grads ? (n >= 2048 ? 1 : 2048 / n) : 1, most = over(l.ldp, 2048);
             k_finish<T><<<dim3((unsigned)n, (unsigned)(split < most ? split : most)), 256, 0, st>>>(f);
         }
         if (c.dx != nullptr && n > 0) {
             ProductArgs d = base;
-            d.M = c.H, d.N = n, d.K = c.V;
+            d.M = c.H, d.N = two ? 2 * n : n, d.K = c.V;
             d.A = w, d.lda = ldw;
             d.B = ws + l.p, d.ldb = l.ldp;
             T* C = (T*)c.dx + at * c.H;
             d.C = C;
             d.vector = c.H % 8 == 0 && (uintptr_t)C % 16 == 0;
-            d.acc = l.dx.splits > 1 ? (float*)(ws + l.dx_acc) : nullptr;
+            d.acc = two || l.dx.splits > 1 ? (float*)(ws + l.dx_acc) : nullptr;
             Shape s = l.dx;
-            s.n_tiles = over(n, TILE_N[s.kind]);
+            s.n_tiles = over(d.N, TILE_N[s.kind]);
             product<T, false, true, OUT>(s, d, st);
             if (d.acc != nullptr)
-                k_join<T><<<2048, 256, 0, st>>>(d.acc, s.splits, n, c.H, l.Hp, C, &scal->alpha);
+                k_join<T><<<2048, 256, 0, st>>>(d.acc, s.splits, two, n, c.H, l.Hp, C, &scal->alpha);
         }
         if (c.dw != nullptr) {
             ProductArgs d = base;
-            d.M = c.H, d.N = c.V, d.K = n;
+            d.M = c.H, d.N = c.V, d.K = two ? 2 * n : n;
             d.A = xs, d.lda = ldxs;
             d.B = ws + l.p, d.ldb = l.ldp;
             d.C = c.dw;
             d.vector = c.H % 8 == 0 && (uintptr_t)c.dw % 16 == 0;
             d.acc = tokens < c.N ? (float*)(ws + l.dw_acc) : nullptr;
             d.add = at > 0;
-            product<T, false, false, OUT>(shape_of(c.H, c.V, n, 1), d, st);
+            product<T, false, false, OUT>(shape_of(c.H, c.V, d.K, 1), d, st);
             if (d.acc != nullptr && at + n == c.N)
-                k_join<T><<<2048, 256, 0, st>>>(d.acc, 1, c.V, c.H, l.Hp, c.dw, &scal->alpha);
+                k_join<T><<<2048, 256, 0, st>>>(d.acc, 1, false, c.V, c.H, l.Hp, c.dw, &scal->alpha);
         }
     }
     if (c.reduced) k_total<<<1, 1024, 0, st>>>(loss, c.N, scal, c.loss);

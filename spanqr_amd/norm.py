@@ -5,7 +5,7 @@ whose gradients the optimizer that calls orth works on.
 import torch
 
 from . import _lib
-from .tensors import TYPES, check_same, check_tensor, on, rows_of, workspace
+from .tensors import TYPES, check_like, check_same, check_tensor, like, on, rows_of, workspace
 
 QUANT = {None: (_lib.QUANT_NONE, None), "fp8": (_lib.QUANT_FP8, torch.float8_e4m3fn), "int8": (_lib.QUANT_INT8, torch.int8)}
 
@@ -14,7 +14,7 @@ def _check(what, x, weight):
     check_tensor(what, "x", x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what}: x must be [..., D] with D >= 1, got {list(x.shape)}")
-    if weight is not None:
+    if weight is not None and not like(weight, x, x.shape[-1:]):
         check_tensor(what, "weight", weight)
         check_same(what, "weight", weight, x.device, (x.shape[-1],))
         if weight.dtype != x.dtype and weight.dtype != torch.float32:
@@ -78,8 +78,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, quant=None):
     if quant not in QUANT:
         raise ValueError(f"rms_norm: quant must be None, 'fp8' or 'int8', got {quant!r}")
     if residual is not None:
-        check_tensor("rms_norm", "residual", residual)
-        check_same("rms_norm", "residual", residual, x.device, x.shape, x.dtype)
+        check_like("rms_norm", "residual", residual, x, x.shape)
     if quant is None and torch.is_grad_enabled() and (
             x.requires_grad or (weight is not None and weight.requires_grad) or
             (residual is not None and residual.requires_grad)):
@@ -96,11 +95,9 @@ def rms_norm_backward(dy, h, weight=None, eps=1e-6, dh=None, need_dw=True):
     dx. dw is None without a weight or with need_dw=False; it has the weight's type."""
     _check("rms_norm_backward", h, weight)
     D, dev = h.shape[-1], h.device
-    check_tensor("rms_norm_backward", "dy", dy)
-    check_same("rms_norm_backward", "dy", dy, dev, h.shape, h.dtype)
+    check_like("rms_norm_backward", "dy", dy, h, h.shape)
     if dh is not None:
-        check_tensor("rms_norm_backward", "dh", dh)
-        check_same("rms_norm_backward", "dh", dh, dev, h.shape, h.dtype)
+        check_like("rms_norm_backward", "dh", dh, h, h.shape)
         dh = rows_of(dh, D)
     h2, dy = rows_of(h, D), rows_of(dy, D)
     dx = torch.empty_like(h, memory_format=torch.contiguous_format)

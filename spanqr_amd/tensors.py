@@ -27,6 +27,17 @@ def check_same(what, name, t, device, shape=None, dtype=None):
         raise TypeError(f"{what}: {name} must be {str(dtype)[6:]}, got {t.dtype}")
 
 
+def like(t, x, shape):
+    """whether t has this shape, and the type and device of x, which is checked: the usual case in one short look"""
+    return isinstance(t, torch.Tensor) and t.dtype is x.dtype and t.shape == shape and t.get_device() == x.get_device()
+
+
+def check_like(what, name, t, x, shape):
+    if not like(t, x, shape):
+        check_tensor(what, name, t)
+        check_same(what, name, t, x.device, shape, x.dtype)
+
+
 def rows_of(t, D):
     """t [..., D] as [rows, D] with neighbouring elements in a row; copied only where no such view exists (or rows
     overlap)"""
