@@ -20,9 +20,8 @@ namespace {
 
 constexpr int TABLE = 112;          // tensors a launch (its arguments stay below 4 KB)
 constexpr int THREADS = 256;
-constexpr int PIECES = 4;           // of 8 elements a thread and chunk
-constexpr int CHUNK = THREADS * 8 * PIECES;
-constexpr int MAX_PARTS = 2048;     // partial sums of a table
+constexpr int CHUNK = THREADS * 32; // elements
+constexpr int MAX_PARTS = 4096;     // partial sums of a table
 
 struct Table {
     const void* src[TABLE];
@@ -46,17 +45,26 @@ __device__ __forceinline__ int tensor_of(const Table& t, uint32_t chunk) {
     return lo;
 }
 
+// W neighbouring elements at the element's own alignment. A wavefront's access has no gaps if it is 16 bytes a lane at
+// most: 4 elements where fp32 is read or written, else 8.
+template <typename T, int W>
+struct Vector {
+    typedef T type __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+};
+
 template <typename T>
 __device__ __forceinline__ double squares(const T* p, unsigned long n, unsigned long at) {
     double sum = 0.0;
     if (n - at >= CHUNK) {   // all loads at once
-        Pack8<T> k[PIECES];
+        constexpr int W = 16 / sizeof(T), PIECES = CHUNK / THREADS / W;
+        typedef typename Vector<T, W>::type V;
+        V k[PIECES];
 #pragma unroll
-        for (int c = 0; c < PIECES; ++c) k[c] = *(const Pack8<T>*)(p + at + 8ul * (threadIdx.x + c * THREADS));
+        for (int c = 0; c < PIECES; ++c) k[c] = *(const V*)(p + at + (unsigned long)W * (threadIdx.x + c * THREADS));
 #pragma unroll
         for (int c = 0; c < PIECES; ++c)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fma((double)(float)k[c].v[i], (double)(float)k[c].v[i], sum);
+            for (int i = 0; i < W; ++i) sum = fma((double)(float)k[c][i], (double)(float)k[c][i], sum);
         return sum;
     }
     for (unsigned long i = at + 8ul * threadIdx.x; i < n; i += 8ul * THREADS) {
@@ -89,7 +97,15 @@ __global__ __launch_bounds__(THREADS) void k_squares(const Table t, double* part
 __device__ __forceinline__ double norm_of(const double* part, int parts) {
     __shared__ double slot[THREADS / 64];
     double sum = 0.0;
-    for (int i = threadIdx.x; i < parts; i += THREADS) sum += part[i];
+    int i = threadIdx.x;
+    for (; i + 7 * THREADS < parts; i += 8 * THREADS) {   // (eight loads together)
+        double v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = part[i + k * THREADS];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += v[k];
+    }
+    for (; i < parts; i += THREADS) sum += part[i];
     return sqrt(reduce_threads<THREADS, Sum>(sum, slot));
 }
 
@@ -102,21 +118,32 @@ __global__ __launch_bounds__(THREADS) void k_norm(const double* part, int parts,
     }
 }
 
-template <typename T, typename O>
+template <bool STREAM, typename T, typename O>
 __device__ __forceinline__ void scaled(const T* p, O* out, unsigned long n, unsigned long at, float f) {
-    float v[8];
     if (n - at >= CHUNK) {
-        Pack8<T> k[PIECES];
-#pragma unroll
-        for (int c = 0; c < PIECES; ++c) k[c] = *(const Pack8<T>*)(p + at + 8ul * (threadIdx.x + c * THREADS));
+        constexpr int W = sizeof(T) == 4 || sizeof(O) == 4 ? 4 : 8, PIECES = CHUNK / THREADS / W;
+        typedef typename Vector<T, W>::type V;
+        typedef typename Vector<O, W>::type X;
+        V k[PIECES];
 #pragma unroll
         for (int c = 0; c < PIECES; ++c) {
+            const V* from = (const V*)(p + at + (unsigned long)W * (threadIdx.x + c * THREADS));
+            k[c] = STREAM ? __builtin_nontemporal_load(from) : *from;
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = (float)k[c].v[i] * f;
-            store8(out + at + 8ul * (threadIdx.x + c * THREADS), 8, v);
+        for (int c = 0; c < PIECES; ++c) {
+            X v;
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = (O)((float)k[c][i] * f);
+            X* to = (X*)(out + at + (unsigned long)W * (threadIdx.x + c * THREADS));
+            if (STREAM)
+                __builtin_nontemporal_store(v, to);
+            else
+                *to = v;
         }
         return;
     }
+    float v[8];
     for (unsigned long i = at + 8ul * threadIdx.x; i < n; i += 8ul * THREADS) {
         const int k = n - i >= 8 ? 8 : (int)(n - i);
         load8(p + i, k, v);
@@ -126,16 +153,18 @@ __device__ __forceinline__ void scaled(const T* p, O* out, unsigned long n, unsi
     }
 }
 
-template <typename T>
+template <bool STREAM, typename T>
 __device__ __forceinline__ void scaled_to(const T* p, void* out, int type, unsigned long n, unsigned long at, float f) {
     if (type == SPANQR_BF16)
-        scaled(p, (bf16*)out, n, at, f);
+        scaled<STREAM>(p, (bf16*)out, n, at, f);
     else if (type == SPANQR_FP16)
-        scaled(p, (fp16*)out, n, at, f);
+        scaled<STREAM>(p, (fp16*)out, n, at, f);
     else
-        scaled(p, (float*)out, n, at, f);
+        scaled<STREAM>(p, (float*)out, n, at, f);
 }
 
+// STREAM: past the caches
+template <bool STREAM>
 __global__ __launch_bounds__(THREADS) void k_clip(const Table t, const double* part, int parts, float max_norm,
                                                   float* norm) {
     const double v = norm_of(part, parts);
@@ -149,15 +178,20 @@ __global__ __launch_bounds__(THREADS) void k_clip(const Table t, const double* p
         if (f == 1.0f && t.src[i] == t.dst[i]) continue;   // in place and within the bound: nothing changes
         const unsigned long at = (unsigned long)(chunk - t.first[i]) * CHUNK;
         if (t.type[i] == SPANQR_BF16)
-            scaled_to((const bf16*)t.src[i], t.dst[i], t.out[i], t.n[i], at, f);
+            scaled_to<STREAM>((const bf16*)t.src[i], t.dst[i], t.out[i], t.n[i], at, f);
         else if (t.type[i] == SPANQR_FP16)
-            scaled_to((const fp16*)t.src[i], t.dst[i], t.out[i], t.n[i], at, f);
+            scaled_to<STREAM>((const fp16*)t.src[i], t.dst[i], t.out[i], t.n[i], at, f);
         else
-            scaled_to((const float*)t.src[i], t.dst[i], t.out[i], t.n[i], at, f);
+            scaled_to<STREAM>((const float*)t.src[i], t.dst[i], t.out[i], t.n[i], at, f);
     }
 }
 
-int grid_of(uint32_t chunks) { return chunks < (uint32_t)MAX_PARTS ? (int)chunks : MAX_PARTS; }
+unsigned at_most(uint32_t chunks, unsigned most) { return chunks < most ? chunks : most; }
+
+// What passes through the memory-side cache (256 MB) finds nothing there afterwards: then the second pass leaves the
+// cache to the gradients it has still to read. Gradients of 715 MB and their fp32 copies (three tables), in us for both
+// passes: past the caches 637, otherwise 700 to 790; 47 MB with their copies 40 and 38.
+constexpr unsigned long CACHE = 256ul << 20;
 
 unsigned long chunks_of(unsigned long n) { return (n + CHUNK - 1) / CHUNK; }
 
@@ -207,13 +241,15 @@ int enqueue(const char* what, int n, const void* const* src, const long* numel, 
     }
     double *square = (double*)workspace, *part = square + 1;
     int parts = 0, tables = 0;
+    unsigned long bytes = 0;
     Table t;
     for (int i = 0; i < n;) {
         i = fill(t, i, n, src, dst, numel, type, out);
         if (t.count == 0) break;
-        const int grid = grid_of(t.first[t.count]);
+        for (int k = 0; k < t.count; ++k) bytes += t.n[k] * (t.type[k] == SPANQR_FP32 ? 4 : 2);
+        const unsigned grid = at_most(t.first[t.count], MAX_PARTS);
         k_squares<<<grid, THREADS, 0, st>>>(t, part + parts);
-        parts += grid;
+        parts += (int)grid;
         ++tables;
     }
     if (dst == nullptr || tables != 1) {
@@ -225,8 +261,12 @@ int enqueue(const char* what, int n, const void* const* src, const long* numel, 
         const bool first = i == 0;
         i = fill(t, i, n, src, dst, numel, type, out);
         if (t.count == 0) break;
-        const uint32_t chunks = t.first[t.count];
-        k_clip<<<grid_of(chunks), THREADS, 0, st>>>(t, part, parts, max_norm, first ? norm : nullptr);
+        // (with many partial sums to add in each, fewer workgroups)
+        const unsigned grid = at_most(t.first[t.count], parts > 1 ? 2048 : 8192);
+        if (bytes > CACHE)
+            k_clip<true><<<grid, THREADS, 0, st>>>(t, part, parts, max_norm, first ? norm : nullptr);
+        else
+            k_clip<false><<<grid, THREADS, 0, st>>>(t, part, parts, max_norm, first ? norm : nullptr);
     }
     return launched(what);
 }
