@@ -26,21 +26,24 @@ _device_of, _dtype_of = torch.Tensor.get_device, torch.Tensor.dtype.__get__
 
 
 def _tensors(what, name, ts, device=None):
-    """ts as a list of tensors of the three types on one GPU, and that device"""
+    """ts as a list of tensors of the three types on one GPU, that device, and the tensors' types for the C ABI"""
     ts = [ts] if isinstance(ts, torch.Tensor) else list(ts)
     if not ts:
-        return ts, device or torch.device("cuda", torch.cuda.current_device())
+        return ts, device or torch.device("cuda", torch.cuda.current_device()), array("i")
     first = ts[0]
     try:   # hundreds of tensors: what is right is seen in one go, and only what is wrong is looked for
         dev = first.device if device is None else device
-        if dev.type == "cuda" and set(map(_device_of, ts)) == {dev.index} and TYPES.keys() >= set(map(_dtype_of, ts)):
-            return ts, dev
-    except (AttributeError, TypeError):   # not a tensor
+        if dev.type == "cuda" and set(map(_device_of, ts)) == {dev.index}:
+            kinds = set(map(_dtype_of, ts))
+            if len(kinds) == 1:   # as a rule
+                return ts, dev, array("i", [TYPES[kinds.pop()]]) * len(ts)
+            return ts, dev, _types(ts)
+    except (AttributeError, KeyError, TypeError):   # not a tensor, or of another type
         pass
     for t in ts:
         check_tensor(what, name, t)
         check_same(what, name, t, device or first.device)
-    return ts, first.device
+    return ts, first.device, _types(ts)
 
 
 def _contiguous(ts):
@@ -52,9 +55,6 @@ def _pointers(ts):
 
 
 def _types(ts):
-    kinds = set(map(_dtype_of, ts))
-    if len(kinds) == 1:   # as a rule
-        return array("i", [TYPES[kinds.pop()]]) * len(ts)
     return array("i", [TYPES[t.dtype] for t in ts])
 
 
@@ -70,11 +70,11 @@ def grad_norm(grads):
     """sqrt of the sum of squares over all tensors of a list (or of one tensor): float32, bfloat16 and float16 mixed, of
     any shapes and strides, on one ROCm device. A float32 tensor without axes on that device, no host synchronisation;
     squares and sums in float64. An empty list gives 0."""
-    ts, dev = _tensors("grad_norm", "every gradient", grads)
+    ts, dev, types = _tensors("grad_norm", "every gradient", grads)
     if not _contiguous(ts):
         ts = [t if _dense(t) else t.contiguous() for t in ts]
     n = len(ts)
-    at, numel, types = _pointers(ts), _sizes(ts), _types(ts)
+    at, numel = _pointers(ts), _sizes(ts)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     lib = _lib.lib()
     with on(dev) as stream:
@@ -113,14 +113,14 @@ def clip_grad_norm(grads, max_norm, out=None):
 
     A NaN norm makes every result NaN, an infinite norm makes finite gradients 0: look at the norm before the step. out
     may share no memory with the gradients, other than out[i] being grads[i]."""
-    grads, dev = _tensors("clip_grad_norm", "every gradient", grads)
+    grads, dev, types = _tensors("clip_grad_norm", "every gradient", grads)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm: max_norm must not be negative, got {max_norm}")
     if out is None:
-        out = grads
+        out, out_types = grads, types
     else:
-        out, _ = _tensors("clip_grad_norm", "every tensor of out", out, dev)
+        out, _, out_types = _tensors("clip_grad_norm", "every tensor of out", out, dev)
         if [g.shape for g in grads] != [o.shape for o in out]:
             if len(out) != len(grads):
                 raise ValueError(f"clip_grad_norm: {len(grads)} gradients but {len(out)} tensors in out")
@@ -131,8 +131,8 @@ def clip_grad_norm(grads, max_norm, out=None):
     if not (_contiguous(grads) and (out is grads or _contiguous(out))):
         src, dst, back = _in_rows(grads, out, dev)
     n = len(src)
-    at, numel, types = _pointers(src), _sizes(src), _types(src)
-    to, out_types = (at, types) if dst is src else (_pointers(dst), _types(dst))
+    at, numel = _pointers(src), _sizes(src)
+    to = at if dst is src else _pointers(dst)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     lib = _lib.lib()
     with on(dev) as stream:
