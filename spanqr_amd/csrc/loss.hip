@@ -4,11 +4,13 @@
 //   z = x W^T [N, V],  lse_i = log sum_j exp z_ij,  loss_i = w_i (lse_i - z_i,t_i)      (w_i = 0 where t_i is ignored)
 //   G_ij = w_i (exp(z_ij - lse_i) - [j = t_i]),  dx = a G W,  dW = a G^T x      (a = 1, or 1 / tokens that count)
 //
-// Three products of 2 N H V operations each. The product of the logits ends in its own softmax statistics: for
-// 64 or 128 neighbouring columns of a token it leaves the maximum m and the sum of exp(z - m), and, where gradients are wanted,
+// Three products of 2 N H V operations each. The product of the logits ends in its own softmax statistics: for 64 or
+// 128 neighbouring columns of a token it leaves the maximum m and the sum of exp(z - m), and, where gradients are wanted,
 // the exponentials p = exp(z - m) themselves, rounded to the 16-bit type once. One pass over p turns them into G
 // (times exp(m - lse), the target's element from its fp32 logit), and G goes into the other two products. So nothing
-// is multiplied twice, and what is held is 16 bits an element for as many tokens at a time as the workspace takes.
+// is multiplied twice, and what is held is 16 bits an element for as many tokens at a time as the workspace takes. The
+// gradients' error is then that of G's elements, rounded twice, and of one rounding at the end: 1.3 times the error of
+// a result that is rounded at the end alone (1.0 times for up to 32 tokens, whose p and G keep what is rounded off).
 #include <math.h>
 
 #include <type_traits>
@@ -266,11 +268,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // A workgroup's tile is BM x BN, each of its four wavefronts' WM x WN in 16 x 16 subtiles. A step of 64 k has two
-// halves: while one half's matrix instructions run, the other half's operands come from LDS, in its first rows. Between the halves every
-// wavefront has read the whole step, so there is the one barrier: behind it the next step's first half is read and the step
-// after that is loaded into the buffer that became free.
-// A 128 x 128 part for each wavefront (one per SIMD) reads LDS least: 64 KB for 64 matrix instructions a SIMD and 32 k, where
-// eight wavefronts of 128 x 64 read 96.
+// halves: while one half's matrix instructions run, the other half's operands come from LDS, in its first rows. Between
+// the halves every wavefront has read the whole step, so there is the one barrier: behind it the next step's first half is
+// read and the step after that is loaded into the buffer that became free.
+// A 128 x 128 part for each wavefront (one per SIMD) reads LDS least: 64 KB for 64 matrix instructions a SIMD and 32 k,
+// where eight wavefronts of 128 x 64 read 96 (8.6 / 8.0 / 8.65 ms for the three products of the size below).
+// Bound by the matrix pipe and the clock that it leaves (1.7 to 1.85 GHz under this load): logits, dx and dW of
+// 8192 x 5120 x 128000 in 8.0, 8.1 and 8.3 ms, 1300 to 1350 TFLOP/s; with a short k by what surrounds the loop, the first
+// loads and the epilogue: 4000 x 1024 x 50257 in 490, 350 and 415 us, 1180 TFLOP/s at most.
 template <typename T, bool A_ROWS, bool B_ROWS, int EPILOGUE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const ProductArgs q) {
     typedef typename Vec<T>::x8 x8;
@@ -319,8 +324,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
         }
     };
     // Half KS of a step: its matrix instructions, one after the other, and between them, where the matrix pipe is busy
-    // anyway, the reads of the other half (of this step, or of the next one behind `turn`) in the first half of them, and in half 1 the
-    // loads at pa and pb into the other buffer. The fences keep that order.
+    // anyway, the reads of the other half (of this step, or of the next one behind `turn`) in the first half of them, and
+    // in half 1 the loads at pa and pb into the other buffer. The fences keep that order.
     auto half = [&](auto ks, const char* pa, const char* pb) {
         constexpr int KS = decltype(ks)::value, SLOTS = IM * IN, READS = IM + IN;
         static_assert(LOADS < SLOTS, "the last slot has no load");
@@ -508,8 +513,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
 
 // The logits of few tokens (16 NB at most): bound by one read of W, which goes straight into registers, at any
 // alignment. A workgroup has FEW_ROWS columns of the vocabulary; its four wavefronts share the hidden size, 32 k of every
-// 128 each, and put their parts together in LDS, so that there are many loads under way (a wavefront's next four steps) and many wavefronts. Statistics
-// and exponentials as in the other kernel, for FEW_ROWS columns together.
+// 128 each, and put their parts together in LDS, so that there are many loads under way (a wavefront's next four steps)
+// and many wavefronts. Statistics and exponentials as in the other kernel, for FEW_ROWS columns together.
 // With few tokens a single rounding of G shows in a whole gradient (no other tokens' average it away), and rows of the
 // products' tiles are free: so p and G have two rows a token, the rounded values and behind all of those what was
 // rounded off, and the gradients see 16 bits of them (bf16) or 21.
@@ -707,7 +712,8 @@ struct FinishArgs {
     long rest;                   // elements from a row of p to the one with what was rounded off, or 0
 };
 
-// one token a blockIdx.x: lse from the segments' statistics, the loss, and p -> G in the columns of blockIdx.y
+// one token a blockIdx.x: lse from the segments' statistics, the loss, and p -> G in the columns of blockIdx.y.
+// Bound by memory where there are gradients: 8192 x 128000, read and written, in 910 us (4.6 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void k_finish(const FinishArgs q) {
     __shared__ float slot[4];
@@ -806,8 +812,8 @@ struct Shape {
     long split_k;
 };
 
-// Microseconds of C [N][M] over K in tiles of `kind`, in `splits` parts of K. Measured, in us, for 256 / 128 / 64-wide tiles:
-// logits of 512 x 768 x 32000 40 / 35 / 41, of 128 x 1024 x 32000 37 / 19 / 16, of 2000 x 2048 x 50257 435 / 462 / 538, of
+// Microseconds of C [N][M] over K in tiles of `kind`, in `splits` parts of K. Measured, in us, for 256 / 128 / 64-wide
+// tiles: logits of 512 x 768 x 32000 40 / 35 / 41, of 128 x 1024 x 32000 37 / 19 / 16, of 2000 x 2048 x 50257 435 / 462 / 538, of
 // 4000 x 1024 x 50257 475 / 493 / 544; dW of the same 43 / 35 / 42, 28 / 24 / 28, 384 / 428 / 525, 398 / 413 / 521; dx (and
 // the sum of its parts) of 512 x 768 x 32000 in 16 parts 50 + 7 / 32 + 7 / 35 + 7, in 8 78 + 5 / 43 + 5 / 40 + 5, of 2000 x
 // 2048 x 50257 in 4 parts 327 + 13 / 414 + 14 / 590 + 15, in 2 547 + 9 / 401 + 9 / 642 + 9.
