@@ -267,6 +267,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
+// over the four rows of 16 lanes of a wavefront, lane for lane, without going through LDS
+template <typename OP>
+__device__ __forceinline__ float reduce_rows(float v, OP op) {
+    auto both = [&](auto swapped) {
+        const uint32_t a = swapped[0], b = swapped[1];   // (a bit_cast of a vector's element takes the first one)
+        return op(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+    };
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    u = __builtin_bit_cast(uint32_t, both(__builtin_amdgcn_permlane16_swap(u, u, false, false)));
+    return both(__builtin_amdgcn_permlane32_swap(u, u, false, false));
+}
+
 // A workgroup's tile is BM x BN, each of its four wavefronts' WM x WN in 16 x 16 subtiles. A step of 64 k has two
 // halves: while one half's matrix instructions run, the other half's operands come from LDS, in its first rows. Between
 // the halves every wavefront has read the whole step, so there is the one barrier: behind it the next step's first half is
@@ -321,6 +333,16 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
         } else {
             a.load_end(t, left, q.zeros, wave, lane);
             b.load_end(t, left, q.zeros, wave, lane);
+        }
+    };
+    // (behind the loop the compiler moves all of c about if it may)
+    auto pin = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < IM; ++i) {
+            if constexpr (BM == 256)
+                asm volatile("" : "+a"(c[i][j]));
+            else
+                asm volatile("" : "+v"(c[i][j]));
         }
     };
     // Half KS of a step: its matrix instructions, one after the other, and between them, where the matrix pipe is busy
@@ -378,6 +400,22 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     asm volatile("s_barrier" ::: "memory");
+    // what the epilogue needs, so that it is not fetched behind the loop
+    ProductArgs end;
+    auto keep = [](auto& to, auto from) {
+        to = from;
+        asm volatile("" : "+s"(to));
+    };
+    float alpha = 0.0f;
+    keep(end.M, q.M), keep(end.N, q.N);
+    if constexpr (EPILOGUE == LOGITS) {
+        keep(end.target, q.target), keep(end.zt, q.zt), keep(end.stat, q.stat);
+        keep(end.segs, q.segs), keep(end.p, q.p), keep(end.ldp, q.ldp);
+    } else {
+        keep(end.C, q.C), keep(end.ldc, q.ldc), keep(end.vector, q.vector);
+        keep(end.acc, q.acc), keep(end.ldacc, q.ldacc), keep(end.add, q.add);
+        keep(alpha, *(const __attribute__((address_space(4))) float*)q.alpha);   // (by a scalar load)
+    }
     // (scalar loads that are still under way would make the compiler wait for all LDS reads in every turn)
     __builtin_amdgcn_s_waitcnt(0xc07f);
 #pragma unroll
@@ -387,31 +425,29 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
     for (int t = 0; t < steps; ++t) step(t);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
 
-    // (the compiler moves all of c about right here if it may)
-    auto pin = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < IM; ++i) {
-            if constexpr (BM == 256)
-                asm volatile("" : "+a"(c[i][j]));
-            else
-                asm volatile("" : "+v"(c[i][j]));
-        }
-    };
-
     // lane: row n = lo of C, elements m = 4 hi + 0..3 of each subtile (16 hi + 0..15 of four subtiles where SPREAD)
     if constexpr (EPILOGUE == LOGITS) {
         const long first = m0 + wm + 16 * hi;   // of the lane's columns; each group of four subtiles is 64 on
-        const int inside = (int)(q.M - first < 2 * WM ? q.M - first : 2 * WM);   // of them before the vocabulary's end
-        const bool whole = m0 + wm + WM <= q.M;
-        T* to = (T*)q.p + (n0 + wn + lo) * q.ldp + first;
+        const int inside = (int)(end.M - first < 2 * WM ? end.M - first : 2 * WM);   // of them before the vocabulary's end
+        const bool whole = m0 + wm + WM <= end.M;
+        T* to = (T*)end.p + (n0 + wn + lo) * end.ldp + first;
+        long t[IN];   // (here, because loads between the stores would wait for those)
 #pragma unroll
         for (int j = 0; j < IN; ++j) {
             const long n = n0 + wn + 16 * j + lo;
-            const bool on = n < q.N;
+            t[j] = end.target[n < end.N ? n : end.N - 1];
+        }
+#pragma unroll
+        for (int j = 0; j < IN; ++j) {
+            const long n = n0 + wn + 16 * j + lo;
+            const bool on = n < end.N;
             pin(j);
             float z[4 * IM];
 #pragma unroll
-            for (int i = 0; i < 4 * IM; ++i) z[i] = c[i / 4][j][i & 3];   // column 64 (i / 16) + i % 16
+            for (int i = 0; i < 4 * IM; ++i) {   // column 64 (i / 16) + i % 16
+                z[i] = c[i / 4][j][i & 3];
+                asm volatile("" : "+v"(z[i]));   // (read once from the accumulation registers)
+            }
             if (!whole) {
 #pragma unroll
                 for (int i = 0; i < 4 * IM; ++i) z[i] = 64 * (i >> 4) + (i & 15) < inside ? z[i] : -INFINITY;
@@ -420,64 +456,63 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
             float m = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4 * IM; i += 2) m = max3(m, z[i], z[i + 1]);
-            m = max3(m, m, __shfl_xor(m, 16));
-            m = max3(m, m, __shfl_xor(m, 32));
+            // (fmaxf, not the asm of max3: the compiler has to see what a permlane reads, which needs a wait behind it)
+            m = reduce_rows(fmaxf(m, z[0]), [](float a, float b) { return fmaxf(a, b); });
             // exponentials are 2^(z log2 e - top): top is kept rounded as it is used here, so that its rounding
             // cancels where the parts are put together
             const float top = m == -INFINITY ? 0.0f : m * LOG2E;
-            const long target = on ? q.target[n] - first : -1;
+            const long target = on ? t[j] - first : -1;
             const int at = target >= 0 && target < inside ? (int)target : -1;
-            if (at >= 0 && at < 64 * (IM / 4) && (at & 63) < 16) {
+            const bool here = at >= 0 && at < 64 * (IM / 4) && (at & 63) < 16;
+            if (__builtin_expect(__ballot(here) != 0, 0)) {
                 float zt = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4 * IM; ++i) zt = at == 64 * (i >> 4) + (i & 15) ? z[i] : zt;
-                q.zt[n] = zt;
+                if (here) end.zt[n] = zt;
             }
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4 * IM; ++i) z[i] = __builtin_amdgcn_exp2f(fmaf(z[i], LOG2E, -top));
 #pragma unroll
             for (int i = 0; i < 4 * IM; ++i) sum += z[i];
-            if (q.p != nullptr && on) {
+            if (end.p != nullptr && on) {
 #pragma unroll
                 for (int g = 0; g < IM / 4; ++g) {
                     x8 e[2];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) e[i >> 3][i & 7] = (T)z[16 * g + i];
-                    if (whole || m0 + wm + 64 * g < q.ldp) {   // (rows of p are whole 64s)
+                    if (whole || m0 + wm + 64 * g < end.ldp) {   // (rows of p are whole 64s)
                         *(x8*)(to + 64 * g) = e[0];
                         *(x8*)(to + 64 * g + 8) = e[1];
                     }
                 }
             }
-            to += 16 * q.ldp;
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (hi == 0 && on && m0 + wm < q.M) q.stat[n * q.segs + (m0 + wm) / WM] = make_float2(top, sum);
+            to += 16 * end.ldp;
+            sum = reduce_rows(sum, [](float a, float b) { return a + b; });
+            if (hi == 0 && on && m0 + wm < end.M) end.stat[n * end.segs + (m0 + wm) / WM] = make_float2(top, sum);
         }
-    } else if (q.acc != nullptr) {
-        float* to = q.acc + (split * q.N + n0 + wn + lo) * q.ldacc + m0 + wm + 4 * hi;
+    } else if (end.acc != nullptr) {
+        float* to = end.acc + (split * end.N + n0 + wn + lo) * end.ldacc + m0 + wm + 4 * hi;
 #pragma unroll
-        for (int j = 0; j < IN; ++j, to += 16 * q.ldacc) {
+        for (int j = 0; j < IN; ++j, to += 16 * end.ldacc) {
             pin(j);
 #pragma unroll
             for (int i = 0; i < IM; ++i) {
-                if (n0 + wn + 16 * j + lo >= q.N || m0 + wm + 16 * i + 4 * hi >= q.M) continue;
+                if (n0 + wn + 16 * j + lo >= end.N || m0 + wm + 16 * i + 4 * hi >= end.M) continue;
                 f32x4 v = c[i][j];
-                if (q.add) v += *(f32x4*)(to + 16 * i);
+                if (end.add) v += *(f32x4*)(to + 16 * i);
                 *(f32x4*)(to + 16 * i) = v;
             }
         }
     } else {
-        const float alpha = *q.alpha;
-        T* to = (T*)q.C + (n0 + wn + lo) * q.ldc + m0 + wm;
-        if (q.vector && m0 + BM <= q.M) {
+        T* to = (T*)end.C + (n0 + wn + lo) * end.ldc + m0 + wm;
+        if (end.vector && m0 + BM <= end.M) {
             // Two subtiles side by side: the lanes of odd hi get the second one's elements of the lane below and give
             // theirs of the first, so that a lane has 8 neighbouring elements and four lanes 64 bytes of a row.
             to += 16 * (hi & 1) + 8 * (hi >> 1);
 #pragma unroll
-            for (int j = 0; j < IN; ++j, to += 16 * q.ldc) {
-                const bool on = n0 + wn + 16 * j + lo < q.N;
+            for (int j = 0; j < IN; ++j, to += 16 * end.ldc) {
+                const bool on = n0 + wn + 16 * j + lo < end.N;
                 pin(j);
 #pragma unroll
                 for (int i = 0; i < IM; i += 2) {
@@ -495,12 +530,12 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
                 }
             }
         } else {
-            const int left = (int)(q.M - m0 - wm < 4 * BM ? q.M - m0 - wm : 4 * BM) - 4 * hi;   // elements of the row
+            const int left = (int)(end.M - m0 - wm < 4 * BM ? end.M - m0 - wm : 4 * BM) - 4 * hi;   // elements of the row
             to += 4 * hi;
 #pragma unroll
-            for (int j = 0; j < IN; ++j, to += 16 * q.ldc) {
+            for (int j = 0; j < IN; ++j, to += 16 * end.ldc) {
                 pin(j);
-                if (n0 + wn + 16 * j + lo >= q.N) continue;
+                if (n0 + wn + 16 * j + lo >= end.N) continue;
 #pragma unroll
                 for (int i = 0; i < IM; ++i)
 #pragma unroll
