@@ -666,15 +666,44 @@ __global__ __launch_bounds__(256) void k_few(const ProductArgs q) {
     }
 }
 
+struct Scalars {
+    uint32_t zeros[4];
+    float alpha;    // what dx and dW are multiplied by
+    float per;      // what the sum of the losses is multiplied by
+    float w_scale;  // G holds the weights times this (a power of 2: the largest weight to [1, 2))
+};
+
+// the sum (or mean) of the tokens' losses by one workgroup, in a fixed order
+__device__ __forceinline__ void total(const float* loss, long N, const Scalars* scal, float* out) {
+    __shared__ double slot[4];
+    double sum = 0.0;
+    long i = threadIdx.x;
+    for (; i + 7 * 256 < N; i += 8 * 256) {   // (eight loads together)
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = loss[i + 256 * k];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += (double)v[k];
+    }
+    for (; i < N; i += 256) sum += (double)loss[i];
+    sum = reduce_threads<256, Sum>(sum, slot);
+    if (threadIdx.x == 0) *out = (float)(sum * (double)scal->per);
+}
+__global__ __launch_bounds__(256) void k_total(const float* loss, long N, const Scalars* scal, float* out) {
+    total(loss, N, scal, out);
+}
+
 // C = alpha times the sum of the splits' parts, in their order, of `rows` rows each; two: of twice as many, the second
-// half added to the first
+// half added to the first. Where `loss` is given, one workgroup more than JOINERS has the N tokens' total.
+constexpr unsigned JOINERS = 2048;
 template <typename T>
 __global__ __launch_bounds__(256) void k_join(const float* acc, int splits, bool two, long rows, long M, long Mp, void* C,
-                                              const float* alpha) {
+                                              const Scalars* scal, const float* loss, long N, float* out) {
+    if (blockIdx.x == JOINERS) return total(loss, N, scal, out);
     const long n = rows * Mp / 4;
     const int parts = two ? 2 * splits : splits;
-    const float a = *alpha;
-    for (long i = blockIdx.x * 256l + threadIdx.x; i < n; i += 256l * gridDim.x) {
+    const float a = scal->alpha;
+    for (long i = blockIdx.x * 256l + threadIdx.x; i < n; i += 256l * JOINERS) {
         f32x4 v = ((const f32x4*)acc)[i];
         int s = 1;
         for (; s + 8 <= parts; s += 8) {   // (their loads together)
@@ -699,13 +728,6 @@ __device__ __forceinline__ float weight_of(long target, long ignore, long V, con
     if (target < 0 || target >= V) return NAN;
     return row_weight == nullptr ? 1.0f : row_weight[i];
 }
-
-struct Scalars {
-    uint32_t zeros[4];
-    float alpha;    // what dx and dW are multiplied by
-    float per;      // what the sum of the losses is multiplied by
-    float w_scale;  // G holds the weights times this (a power of 2: the largest weight to [1, 2))
-};
 
 // counts the tokens that are not ignored; one workgroup
 __global__ __launch_bounds__(1024) void k_prepare(const long* target, long N, long ignore, int mean, const float* row_weight,
@@ -806,15 +828,6 @@ __global__ __launch_bounds__(256) void k_finish(const FinishArgs q) {
     }
 }
 
-// the sum (or mean) of the tokens' losses; one workgroup, a fixed order
-__global__ __launch_bounds__(1024) void k_total(const float* loss, long N, const Scalars* scal, float* out) {
-    __shared__ double slot[16];
-    double sum = 0.0;
-    for (long i = threadIdx.x; i < N; i += 1024) sum += (double)loss[i];
-    sum = reduce_threads<1024, Sum>(sum, slot);
-    if (threadIdx.x == 0) *out = (float)(sum * (double)scal->per);
-}
-
 // rows of H elements to rows of Hp (the next multiple of 8), the rest 0: operands whose rows do not start on 16 bytes.
 // `times` the same rows, one lot after the other.
 template <typename T>
@@ -837,8 +850,9 @@ long over(long v, long by) { return (v + by - 1) / by; }
 enum { BIG, MID, NARROW };
 constexpr int TILE_M[] = {256, 128, 128}, TILE_N[] = {256, 128, 64};
 constexpr int SLOTS[] = {256, 512, 768};        // workgroups the device holds at once
-constexpr double STEP_US[] = {1.65, 1.0, 0.95}; // 64 k of a full device, at the clock that it keeps under this load
-constexpr double ENDS_US[] = {11.0, 4.5, 3.5};  // a workgroup's first loads and its epilogue
+constexpr double STEP_US[] = {1.6, 1.0, 0.95};  // 64 k of a full device, at the clock that it keeps under this load
+constexpr double ALONE_US[] = {1.6, 0.6, 0.5};  // and with one workgroup a compute unit
+constexpr double ENDS_US[][3] = {{9.5, 5.0, 4.0}, {8.7, 3.8, 3.5}};   // a workgroup's first loads and its epilogue: logits, others
 
 struct Shape {
     int kind;
@@ -848,19 +862,19 @@ struct Shape {
 };
 
 // Microseconds of C [N][M] over K in tiles of `kind`, in `splits` parts of K. Measured, in us, for 256 / 128 / 64-wide
-// tiles: logits of 512 x 768 x 32000 40 / 35 / 41, of 128 x 1024 x 32000 37 / 19 / 16, of 2000 x 2048 x 50257 435 / 462 / 538, of
-// 4000 x 1024 x 50257 475 / 493 / 544; dW of the same 43 / 35 / 42, 28 / 24 / 28, 384 / 428 / 525, 398 / 413 / 521; dx (and
-// the sum of its parts) of 512 x 768 x 32000 in 16 parts 50 + 7 / 32 + 7 / 35 + 7, in 8 78 + 5 / 43 + 5 / 40 + 5, of 2000 x
-// 2048 x 50257 in 4 parts 327 + 13 / 414 + 14 / 590 + 15, in 2 547 + 9 / 401 + 9 / 642 + 9.
-double time_of(int kind, long M, long N, long K, long splits) {
+// tiles: logits of 512 x 768 x 32000 30 / 33 / 40, of 128 x 1024 x 32000 29 / 18 / 16, of 2000 x 2048 x 50257 410 / 465 /
+// 537, of 4000 x 1024 x 50257 425 / 484 / 550; dW of the same 38 / 34 / 40, 24 / 24 / 27, 370 / 428 / 531, 385 / 419 / 529; dx
+// and the sum of its parts, of 512 x 768 x 32000 in 16 parts 50 + 6 / 33 + 6 / 34 + 6, in 8 80 + 5 / 44 + 5 / 39 + 5, of
+// 2000 x 2048 x 50257 in 4 parts 357 + 13 / 430 + 14 / 580 + 14.
+double time_of(int epilogue, int kind, long M, long N, long K, long splits) {
     const double tiles = (double)(over(M, TILE_M[kind]) * over(N, TILE_N[kind]) * splits);
-    double rounds = tiles / SLOTS[kind], step = STEP_US[kind], ends = ENDS_US[kind];
-    if (tiles <= 256) {   // one a compute unit: nothing fills a gap, and small tiles have it to themselves
-        step = kind == BIG ? step : kind == MID ? 0.6 : 0.5;
-        ends += 3.0;
-    }
+    // workgroups beside each other on the compute units that have most; where there is one, nothing fills its gaps
+    const double most = SLOTS[kind] / 256, beside = tiles >= SLOTS[kind] ? most : ceil(tiles / 256);
+    const double step = beside <= 1 ? ALONE_US[kind] : ALONE_US[kind] + (STEP_US[kind] - ALONE_US[kind]) * (beside - 1) / (most - 1);
+    const double ends = ENDS_US[epilogue][kind] + (tiles <= 256 ? 3.0 : 0.0);
     // the last round of the largest starts as workgroups end, one after the other; tiles that share a compute unit fill
     // each other's gaps
+    double rounds = tiles / SLOTS[kind];
     rounds = rounds <= 1.0 ? 1.0 : kind == BIG ? 0.5 * (rounds + ceil(rounds)) : rounds;
     const double join = splits > 1 ? 3.0 + 1e-6 * (double)(M * N * splits) : 0.0;
     return rounds * (step * (double)over(over(K, 64), splits) + ends) + join;
@@ -875,12 +889,12 @@ long split_rows(long tokens) {
 }
 
 // the fastest by time_of, in at most `most` parts of K
-Shape shape_of(long M, long N, long K, long most) {
+Shape shape_of(int epilogue, long M, long N, long K, long most) {
     Shape best = {};
     double least = 1e300;
     for (int kind = BIG; kind <= NARROW; ++kind)
         for (long splits = 1; splits <= most && (splits == 1 || over(K, 64) >= 4 * splits); ++splits) {
-            const double t = time_of(kind, M, N, K, splits);
+            const double t = time_of(epilogue, kind, M, N, K, splits);
             if (t < least * 0.98) {
                 least = t;
                 best = {kind, over(M, TILE_M[kind]), over(N, TILE_N[kind]), (int)splits, 64 * over(over(K, 64), splits)};
@@ -899,10 +913,10 @@ struct Layout {
 };
 Layout layout_of(long N, long H, long V, int grads, bool pad, long tokens) {
     Layout l;
-    l.logits = shape_of(V, tokens, H, 1);
+    l.logits = shape_of(LOGITS, V, tokens, H, 1);
     l.few = tokens <= FEW_TOKENS;
     const long rows = l.few ? 2 * tokens : tokens;   // of p
-    l.dx = shape_of(H, rows, V, rows > 0 ? split_rows(tokens) / rows : 1);
+    l.dx = shape_of(OUT, H, rows, V, rows > 0 ? split_rows(tokens) / rows : 1);
     l.seg = l.few ? 5 : l.logits.kind == BIG ? 7 : 6;
     l.segs = over(V, 1l << l.seg);
     l.ldp = up(V, 64);
@@ -1005,6 +1019,7 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
     base.ldp = l.ldp, base.segs = l.segs;
     base.ldc = c.H, base.ldacc = l.Hp;
     base.alpha = &scal->alpha;
+    bool totalled = false;
     // no tokens: dW is a product over nothing
     for (long at = 0; at < c.N || (at == 0 && c.dw != nullptr); at += tokens > 0 ? tokens : 1) {
         const long n = c.N - at < tokens ? c.N - at : tokens;
@@ -1052,8 +1067,11 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
             Shape s = l.dx;
             s.n_tiles = over(d.N, TILE_N[s.kind]);
             product<T, false, true, OUT>(s, d, st);
-            if (d.acc != nullptr)
-                k_join<T><<<2048, 256, 0, st>>>(d.acc, s.splits, two, n, c.H, l.Hp, C, &scal->alpha);
+            if (d.acc != nullptr) {
+                const bool last = c.reduced && at + n == c.N;   // the losses are all there
+                k_join<T><<<JOINERS + last, 256, 0, st>>>(d.acc, s.splits, two, n, c.H, l.Hp, C, scal, loss, c.N, c.loss);
+                totalled |= last;
+            }
         }
         if (c.dw != nullptr) {
             ProductArgs d = base;
@@ -1064,12 +1082,12 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
             d.vector = c.H % 8 == 0 && (uintptr_t)c.dw % 16 == 0;
             d.acc = tokens < c.N ? (float*)(ws + l.dw_acc) : nullptr;
             d.add = at > 0;
-            product<T, false, false, OUT>(shape_of(c.H, c.V, d.K, 1), d, st);
+            product<T, false, false, OUT>(shape_of(OUT, c.H, c.V, d.K, 1), d, st);
             if (d.acc != nullptr && at + n == c.N)
-                k_join<T><<<2048, 256, 0, st>>>(d.acc, 1, false, c.V, c.H, l.Hp, c.dw, &scal->alpha);
+                k_join<T><<<JOINERS, 256, 0, st>>>(d.acc, 1, false, c.V, c.H, l.Hp, c.dw, scal, nullptr, 0, nullptr);
         }
     }
-    if (c.reduced) k_total<<<1, 1024, 0, st>>>(loss, c.N, scal, c.loss);
+    if (c.reduced && !totalled) k_total<<<1, 256, 0, st>>>(loss, c.N, scal, c.loss);
     return launched("linear_cross_entropy");
 }
 
