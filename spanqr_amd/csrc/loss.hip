@@ -903,6 +903,16 @@ Shape shape_of(int epilogue, long M, long N, long K, long most) {
     return best;
 }
 
+// How many rows of C [N][M] to leave to the largest tiles, so that those come out in whole rounds over the device, where
+// `all` has them: the rest takes smaller tiles in a launch of its own. dW of 4000 x 1024 x 50257 are 788 tiles, 20 more than
+// three rounds: 350 + 50 us so, 421 in one launch.
+long rows_of_rounds(const Shape& all, long M, long N, long K) {
+    const long tiles = all.m_tiles * all.n_tiles, rows = TILE_N[BIG] * (tiles / SLOTS[BIG] * SLOTS[BIG] / all.m_tiles);
+    if (all.kind != BIG || all.splits > 1 || rows == 0 || rows >= N) return N;
+    const Shape rest = shape_of(OUT, M, N - rows, K, 1);
+    return time_of(OUT, BIG, M, rows, K, 1) + time_of(OUT, rest.kind, M, N - rows, K, 1) < time_of(OUT, BIG, M, N, K, 1) ? rows : N;
+}
+
 // where things lie in the workspace, for `tokens` tokens at a time
 struct Layout {
     long scal, loss, zt, stat, p, dx_acc, dw_acc, x, w, bytes;
@@ -1082,9 +1092,20 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
             d.vector = c.H % 8 == 0 && (uintptr_t)c.dw % 16 == 0;
             d.acc = tokens < c.N ? (float*)(ws + l.dw_acc) : nullptr;
             d.add = at > 0;
-            product<T, false, false, OUT>(shape_of(OUT, c.H, c.V, d.K, 1), d, st);
+            Shape s = shape_of(OUT, c.H, c.V, d.K, 1);
+            const long rows = rows_of_rounds(s, c.H, c.V, d.K);
+            if (rows < c.V) {
+                d.N = rows, s.n_tiles = rows / TILE_N[BIG];
+                product<T, false, false, OUT>(s, d, st);
+                d.N = c.V - rows;
+                d.B = (const T*)d.B + rows;
+                d.C = (T*)d.C + rows * c.H;
+                if (d.acc != nullptr) d.acc += rows * l.Hp;
+                s = shape_of(OUT, c.H, d.N, d.K, 1);
+            }
+            product<T, false, false, OUT>(s, d, st);
             if (d.acc != nullptr && at + n == c.N)
-                k_join<T><<<JOINERS, 256, 0, st>>>(d.acc, 1, false, c.V, c.H, l.Hp, c.dw, scal, nullptr, 0, nullptr);
+                k_join<T><<<JOINERS, 256, 0, st>>>((const float*)(ws + l.dw_acc), 1, false, c.V, c.H, l.Hp, c.dw, scal, nullptr, 0, nullptr);
         }
     }
     if (c.reduced && !totalled) k_total<<<1, 256, 0, st>>>(loss, c.N, scal, c.loss);
