@@ -782,14 +782,16 @@ __global__ __launch_bounds__(256) void k_finish(const FinishArgs q) {
     float sum = 0.0f;
     for (long s = threadIdx.x; s < q.segs; s += 256) sum += stat[s].y * __builtin_amdgcn_exp2f(stat[s].x - m);
     sum = reduce_threads<256, Sum>(sum, slot);
-    const float lse2 = m + log2f(sum), lse = lse2 * LN2;
+    const float l = log2f(sum), lse2 = m + l;
     const long t = q.target[i];
     const float w = weight_of(t, q.ignore, q.V, q.row_weight, i);
     const bool in = t >= 0 && t < q.V && t != q.ignore;
-    const float d = in ? q.zt[i] - lse : w;   // log of the target's probability (or 0, or NaN)
+    // Log of the target's probability (or 0, or NaN), from what is small where that is: z - m and the sum, not lse. Below
+    // 2^-23 it is the rounding of a sum of 1.
+    const float d2 = in ? fmaf(q.zt[i], LOG2E, -m) - l : w, d = fabsf(d2) < 0x1p-23f ? 0.0f : d2 * LN2;
     if (blockIdx.y == 0 && threadIdx.x == 0) {
         q.loss[i] = w == 0.0f ? 0.0f : -w * d;
-        if (q.lse != nullptr) q.lse[i] = lse;
+        if (q.lse != nullptr) q.lse[i] = lse2 * LN2;
     }
     if (q.p == nullptr) return;
     T* p = (T*)q.p + i * q.ldp;
