@@ -284,10 +284,11 @@ __device__ __forceinline__ float reduce_rows(float v, OP op) {
 // the halves every wavefront has read the whole step, so there is the one barrier: behind it the next step's first half is
 // read and the step after that is loaded into the buffer that became free.
 // A 128 x 128 part for each wavefront (one per SIMD) reads LDS least: 64 KB for 64 matrix instructions a SIMD and 32 k,
-// where eight wavefronts of 128 x 64 read 96 (8.6 / 8.0 / 8.65 ms for the three products of the size below).
+// where eight wavefronts of 128 x 64 read 96 (8.6 / 8.0 / 8.65 ms for the three products of the size below, when four
+// took 8.1 / 8.1 / 8.3).
 // Bound by the matrix pipe and the clock that it leaves (1.7 to 1.85 GHz under this load): logits, dx and dW of
-// 8192 x 5120 x 128000 in 8.0, 8.1 and 8.3 ms, 1300 to 1350 TFLOP/s; with a short k by what surrounds the loop, the first
-// loads and the epilogue: 4000 x 1024 x 50257 in 490, 350 and 415 us, 1180 TFLOP/s at most.
+// 8192 x 5120 x 128000 in 7.9, 8.15 and 8.3 ms, 1290 to 1360 TFLOP/s; with a short k by what surrounds the loop, the first
+// loads and the epilogue: 4000 x 1024 x 50257 in 465, 350 and 390 us, 890 to 1180 TFLOP/s.
 template <typename T, bool A_ROWS, bool B_ROWS, int EPILOGUE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const ProductArgs q) {
     typedef typename Vec<T>::x8 x8;
