@@ -491,7 +491,6 @@ __global__ __launch_bounds__(1024) void k_rms_dw(const float* part, int parts, l
 constexpr long LONG_ROW = 32768;    // longest row that stays in registers
 constexpr long LONG_GRAD = 16384;   // and in the gradient
 constexpr long MAX_D = 1l << 24;
-constexpr int GRAD_PARTS = 1024;    // most workgroups of the gradient, and so rows of partial sums
 
 // Threads of a row and pieces a thread. Measured, forward / backward in us: 16384 x 2048 bf16 as 256 threads of one
 // piece 51 / 50, as 128 of two 53 / 53, as a wavefront of four 60 / 55; 4096 x 5120 with 8 bits as 640 of one 40, as 320
@@ -515,9 +514,13 @@ int grid_of(long rows, const Split& s, int most) {
     return turns < 1 ? 0 : (int)((need + turns - 1) / turns);
 }
 
+// The gradient's workgroups, and so rows of partial sums: as many as the compute units hold at once, since each of them ends
+// with a row of sums that is written and read again. The gradient and dw, in us, with 1024 / 512 / 256: rows of 4000 (256
+// threads) 49 + 7 / 54 + 6 / 84 + 4, 4096 of 5120 (320) 46 + 9 / 34 + 6 / 49 + 4, 2000 of 12000 (768) 59 + 18 / 51 + 13 / 46 + 7.
 int grad_parts(long rows, long D) {
     if (D > LONG_GRAD) return (int)(rows < 256 ? rows : 256);
-    return grid_of(rows, split_of(rows, D), GRAD_PARTS);
+    const Split s = split_of(rows, D);
+    return grid_of(rows, s, !s.block || s.group <= 256 ? 1024 : s.group <= 512 ? 512 : 256);
 }
 
 #define SPANQR_SPLITS(LAUNCH)                                       \
