@@ -132,6 +132,26 @@ def test_largest_tiles(cuda, N, H, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,H,V", [(1, 512, 1111), (2, 136, 40), (15, 72, 3000), (16, 640, 257), (31, 65, 500), (32, 264, 2001)])
+def test_few_tokens_round_once(cuda, N, H, V, dtype):
+    """up to 32 tokens p and G have a second row with what their rounding drops: what is left of an element's error is the
+    square of one rounding, twice. Rounding is monotone, so a gradient lies between the rounded ends of what that allows."""
+    print(f"linear_cross_entropy {N}x{H}x{V} {dtype}", flush=True)
+    x, W, t = make(N, H, V, dtype, 23, ignored=0.0)
+    loss, dx, dw = sp.linear_cross_entropy_grad(x, W, t, reduction="sum")
+    L, tol, G, d, w, _ = reference(x, W, t)
+    check("loss", loss, L.sum(), tol.sum() + 2 * E * L.sum().abs())
+    u = U[dtype]
+    small = 2.0 ** -24 + 2.0 ** -35 if dtype == torch.float16 else 0.0   # float16's absolute part, as in bounds()
+    dG = G.abs() * (2.1 * u * u + 2.1 * d[:, None] + 64 * E) + 2.1 * d[:, None] + small
+    X, Y = x.double(), W.double()
+    for what, got, want, error in (("dx", dx, G @ Y, dG @ Y.abs() + (V + 16) * E * (G.abs() @ Y.abs())),
+                                   ("dw", dw, G.T @ X, dG.T @ X.abs() + (N + 16) * E * (G.abs().T @ X.abs()))):
+        low, high = (want - error).to(dtype), (want + error).to(dtype)
+        assert bool(((got >= low) & (got <= high)).all()), what
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("N,H,V", [(7, 65, 33), (300, 128, 520), (64, 200, 1000)])
 def test_weights_and_scale(cuda, N, H, V, dtype):
     x, W, t = make(N, H, V, dtype, 2)
