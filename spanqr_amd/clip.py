@@ -121,7 +121,7 @@ def clip_grad_norm(grads, max_norm, out=None):
         out, out_types = grads, types
     else:
         out, _, out_types = _tensors("clip_grad_norm", "every tensor of out", out, dev)
-        if [g.shape for g in grads] != [o.shape for o in out]:
+        if len(out) != len(grads) or not all(map(torch.Tensor.is_same_size, grads, out)):
             if len(out) != len(grads):
                 raise ValueError(f"clip_grad_norm: {len(grads)} gradients but {len(out)} tensors in out")
             for g, o in zip(grads, out):
