@@ -29,7 +29,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 fp16x8 __attribute__((ext_vector_type(8)));
 
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float LOG2E = 1.44269504088896340736f;
 
 template <typename T>
 struct Vec;
@@ -116,7 +116,7 @@ struct ProductArgs {
     // logits
     const long* target;          // of token 0 of this piece
     float* zt;                   // the target's logit
-    float2* stat;                // [token][segs]: maximum (of z log2 e), sum
+    float2* stat;                // [token][segs]: maximum (-inf: no logit), sum of the exponentials
     long segs;
     void* p;                     // exponentials [token][ldp], or null
     long ldp;
@@ -278,6 +278,19 @@ __device__ __forceinline__ float reduce_rows(float v, OP op) {
     u = __builtin_bit_cast(uint32_t, both(__builtin_amdgcn_permlane16_swap(u, u, false, false)));
     return both(__builtin_amdgcn_permlane32_swap(u, u, false, false));
 }
+
+// A group of a token's columns with maximum m has the exponentials 2^(z log2 e - top), top = m log2 e rounded: one fma for
+// each. They are exp(z - m) 2^off, off being what top's rounding leaves: below 2^-7. Where m is larger (up to where
+// m log2 e overflows), and where it is -inf (no logit: k_finish passes the group by), they are 2^((z - sub) log2 e). That
+// form for all would cost the logits of 4000 x 1024 x 50257 7 us of 465.
+struct Base {
+    float sub, top;
+};
+__device__ __forceinline__ bool within(float m) { return fabsf(m) < 65536.0f; }
+__device__ __forceinline__ Base base_of(float m) {
+    return within(m) ? Base{0.0f, m * LOG2E} : Base{m == -INFINITY ? 0.0f : m, 0.0f};
+}
+__device__ __forceinline__ float off_of(float m) { return within(m) ? fmaf(m, LOG2E, -(m * LOG2E)) : 0.0f; }
 
 // A workgroup's tile is BM x BN, each of its four wavefronts' WM x WN in 16 x 16 subtiles. A step of 64 k has two
 // halves: while one half's matrix instructions run, the other half's operands come from LDS, in its first rows. Between
@@ -459,9 +472,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
             for (int i = 0; i < 4 * IM; i += 2) m = max3(m, z[i], z[i + 1]);
             // (fmaxf, not the asm of max3: the compiler has to see what a permlane reads, which needs a wait behind it)
             m = reduce_rows(fmaxf(m, z[0]), [](float a, float b) { return fmaxf(a, b); });
-            // exponentials are 2^(z log2 e - top): top is kept rounded as it is used here, so that its rounding
-            // cancels where the parts are put together
-            const float top = m == -INFINITY ? 0.0f : m * LOG2E;
+            const Base base = base_of(m);
             const long target = on ? t[j] - first : -1;
             const int at = target >= 0 && target < inside ? (int)target : -1;
             const bool here = at >= 0 && at < 64 * (IM / 4) && (at & 63) < 16;
@@ -471,9 +482,13 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
                 for (int i = 0; i < 4 * IM; ++i) zt = at == 64 * (i >> 4) + (i & 15) ? z[i] : zt;
                 if (here) end.zt[n] = zt;
             }
+            if (__builtin_expect(__ballot(!within(m)) != 0, 0)) {
+#pragma unroll
+                for (int i = 0; i < 4 * IM; ++i) z[i] -= base.sub;
+            }
             float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4 * IM; ++i) z[i] = __builtin_amdgcn_exp2f(fmaf(z[i], LOG2E, -top));
+            for (int i = 0; i < 4 * IM; ++i) z[i] = __builtin_amdgcn_exp2f(fmaf(z[i], LOG2E, -base.top));
 #pragma unroll
             for (int i = 0; i < 4 * IM; ++i) sum += z[i];
             if (end.p != nullptr && on) {
@@ -490,7 +505,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
             }
             to += 16 * end.ldp;
             sum = reduce_rows(sum, [](float a, float b) { return a + b; });
-            if (hi == 0 && on && m0 + wm < end.M) end.stat[n * end.segs + (m0 + wm) / WM] = make_float2(top, sum);
+            if (hi == 0 && on && m0 + wm < end.M) end.stat[n * end.segs + (m0 + wm) / WM] = make_float2(m, sum);
         }
     } else if (end.acc != nullptr) {
         float* to = end.acc + (split * end.N + n0 + wn + lo) * end.ldacc + m0 + wm + 4 * hi;
@@ -644,7 +659,7 @@ __global__ __launch_bounds__(256) void k_few(const ProductArgs q) {
         }
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        const float top = m == -INFINITY ? 0.0f : m * LOG2E;
+        const Base base = base_of(m);
         const bool on = n < q.N;
         const long tgt = on ? q.target[n] : -1;
         typedef T x4 __attribute__((ext_vector_type(4)));
@@ -652,7 +667,7 @@ __global__ __launch_bounds__(256) void k_few(const ProductArgs q) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             if (v + r == tgt && v + r < q.M) q.zt[n] = z[r];
-            const float x = __builtin_amdgcn_exp2f(fmaf(z[r], LOG2E, -top));
+            const float x = __builtin_amdgcn_exp2f(fmaf(z[r] - base.sub, LOG2E, -base.top));
             sum += x;
             e[r] = (T)x;
             rest[r] = (T)(x - (float)e[r]);
@@ -663,7 +678,7 @@ __global__ __launch_bounds__(256) void k_few(const ProductArgs q) {
             *(x4*)((T*)q.p + n * q.ldp + v) = e;
             *(x4*)((T*)q.p + (q.N + n) * q.ldp + v) = rest;
         }
-        if ((threadIdx.x & 7) == 0) q.stat[n * q.segs + blockIdx.x] = make_float2(top, sum);
+        if ((threadIdx.x & 7) == 0) q.stat[n * q.segs + blockIdx.x] = make_float2(m, sum);
     }
 }
 
@@ -780,19 +795,22 @@ __global__ __launch_bounds__(256) void k_finish(const FinishArgs q) {
     float m = -INFINITY;
     for (long s = threadIdx.x; s < q.segs; s += 256) m = nan_max(m, stat[s].x);
     m = reduce_threads<256, NanMax>(m, slot);
+    // segments without a logit above -inf: exp(-inf) times their sum, 0 or NaN
+    const float top = m == -INFINITY ? 0.0f : m;
     float sum = 0.0f;
-    for (long s = threadIdx.x; s < q.segs; s += 256) sum += stat[s].y * __builtin_amdgcn_exp2f(stat[s].x - m);
+    for (long s = threadIdx.x; s < q.segs; s += 256)
+        sum += stat[s].y * __builtin_amdgcn_exp2f(fmaf(stat[s].x - top, LOG2E, -off_of(stat[s].x)));
     sum = reduce_threads<256, Sum>(sum, slot);
-    const float l = log2f(sum), lse2 = m + l;
+    const float l = logf(sum);
     const long t = q.target[i];
     const float w = weight_of(t, q.ignore, q.V, q.row_weight, i);
     const bool in = t >= 0 && t < q.V && t != q.ignore;
     // Log of the target's probability (or 0, or NaN), from what is small where that is: z - m and the sum, not lse. Below
     // 2^-23 it is the rounding of a sum of 1.
-    const float d2 = in ? fmaf(q.zt[i], LOG2E, -m) - l : w, d = fabsf(d2) < 0x1p-23f ? 0.0f : d2 * LN2;
+    const float far = in ? (q.zt[i] - top) - l : w, d = fabsf(far) < 0x1p-23f ? 0.0f : far;
     if (blockIdx.y == 0 && threadIdx.x == 0) {
         q.loss[i] = w == 0.0f ? 0.0f : -w * d;
-        if (q.lse != nullptr) q.lse[i] = lse2 * LN2;
+        if (q.lse != nullptr) q.lse[i] = top + l;
     }
     if (q.p == nullptr) return;
     T* p = (T*)q.p + i * q.ldp;
@@ -810,7 +828,8 @@ __global__ __launch_bounds__(256) void k_finish(const FinishArgs q) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) e[k] += r[k];
             }
-            const float s = v < q.V ? f * __builtin_amdgcn_exp2f(stat[v >> q.seg].x - lse2) : 0.0f;
+            const float seg = stat[v < q.V ? v >> q.seg : 0].x;
+            const float s = v < q.V ? f * __builtin_amdgcn_exp2f(fmaf((seg - top) - l, LOG2E, -off_of(seg))) : 0.0f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) e[k] = v + k < q.V ? e[k] * s : 0.0f;
             if (in && t >= v && t < v + 8) {

@@ -1,0 +1,100 @@
+"""linear_cross_entropy where the ordinary cases do not reach: groups of columns without a finite logit, logits near the
+ends of float32, tokens that are sure of their target, the log of the sum of exponentials.
+
+The logits here are exact: a token is one number in the first place of x, a column one in the first of W, so a logit is one
+product of at most 22 bits. What is left are the exponentials and their sum: the distance D of a logit from the maximum is
+rounded, multiplied by a rounded constant and rounded again (3 E D of the exponential), the exponential itself within 2 E,
+in a group and once more from the group to the whole; at most 80 additions stand behind each other. So a sum of
+exponentials is within (3 D + 100) E of itself."""
+import math
+
+import pytest
+import torch
+
+import spanqr_amd as sp
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+DTYPES = [torch.bfloat16, torch.float16]
+# few tokens (1 to 16, 17 to 32), and the three tiles of the others
+SIZES = [(1, 8, 33), (3, 8, 500), (20, 8, 1000), (32, 72, 4000), (33, 8, 130), (70, 136, 1111), (300, 64, 5000),
+         (2048, 8, 20000)]
+
+
+def place(column, H):
+    """[n] as [n, H] with zeros behind"""
+    t = torch.zeros(column.shape[0], H, dtype=column.dtype, device=column.device)
+    t[:, 0] = column
+    return t
+
+
+def exact(s, w, t):
+    """loss, softmax and the largest distance of a logit from the maximum, in 64 bits, for z = s w^T; -inf logits allowed"""
+    z = s.double()[:, None] * w.double()[None]
+    z = torch.where(z.abs() >= 2.0 ** 128, torch.sign(z) * math.inf, z)   # as float32 has it
+    zt = z.gather(1, t[:, None])
+    m = z.amax(1, keepdim=True)
+    others = z.clone().scatter_(1, t[:, None], -math.inf)
+    M = torch.maximum(others.amax(1, keepdim=True), zt)
+    loss = torch.where(zt == M, torch.log1p(torch.exp(others - M).sum(1, keepdim=True)),
+                       M - zt + torch.log(torch.exp(z - M).sum(1, keepdim=True)))[:, 0]
+    far = torch.where(z > m - 200, m - z, torch.zeros_like(z)).amax(1)   # further ones add nothing
+    return loss, torch.softmax(z - m, 1), far
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,H,V", SIZES)
+def test_groups_without_a_finite_logit(cuda, N, H, V, dtype):
+    """columns that are out (-inf), whole groups of them, beside logits far below 0: they take no part"""
+    print(f"linear_cross_entropy {N}x{H}x{V} {dtype}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(31)
+    w = (-100.0 + 5.0 * torch.randn(V, generator=g, device="cuda")).to(dtype)
+    s = (1.0 + 1.5 * torch.rand(N, generator=g, device="cuda")).to(dtype)
+    out = torch.rand(V, generator=g, device="cuda") < 0.1
+    out[V // 4:V // 4 + (V + 1) // 2] = True
+    t = torch.nonzero(~out)[:, 0][torch.randint(0, int((~out).sum()), (N,), generator=g, device="cuda")]
+    w[out] = -math.inf
+    want, p, far = exact(s, w, t)
+    tol = want.abs() * E * 4 + (3 * far + 100) * E
+    x, W = place(s, H), place(w, H)
+    loss = sp.linear_cross_entropy(x, W, t, reduction="none")
+    assert bool(((loss.double() - want).abs() <= tol).all()), float((loss.double() - want).abs().max())
+    total, none, dw = sp.linear_cross_entropy_grad(x, W, t, reduction="sum", need_dx=False)
+    assert bool(torch.isfinite(dw).all()) and not dw[out].any() and not dw[:, 1:].any()
+    G = p.scatter_add(1, t[:, None], -torch.ones(N, 1, device=cuda, dtype=torch.float64))
+    X = s.double()
+    # two roundings of an element to 16 bits, float16's absolute part, the sum over the tokens, the result's own rounding
+    small = 2.0 ** -24 + 2.0 ** -35 if dtype == torch.float16 else 0.0
+    dG = G.abs() * (2.1 * U[dtype] + 2 * (3 * far[:, None] + 100) * E) + small * (p > 0)
+    dG += 4 * (3 * far[:, None] + 100) * E * (G < 0)   # the target's: of 1, not of 1 - p
+    want_w = (G * X[:, None]).sum(0)
+    tol_w = (dG * X[:, None]).sum(0) + (N + 16) * E * (G.abs() * X[:, None]).sum(0) + U[dtype] * want_w.abs() * 1.01 + 2.0 ** -25
+    assert bool(((dw[:, 0].double() - want_w).abs() <= tol_w).all())
+    assert bool(((total.double() - want.sum()).abs() <= tol.sum() + 2 * E * want.sum()).all())
+
+
+@pytest.mark.parametrize("N", [1, 20, 40, 300])
+def test_logits_at_the_ends_of_float32(cuda, N):
+    """bfloat16's lowest value as a mask (finite or -inf as a logit), and rows whose largest logit is near float32's ends"""
+    H, V, dtype = 8, 700, torch.bfloat16
+    lowest = torch.finfo(dtype).min
+    g = torch.Generator(device="cuda").manual_seed(32)
+    w = torch.randn(V, generator=g, device="cuda").to(dtype)
+    w[100:420] = lowest
+    t = torch.randint(0, 100, (N,), generator=g, device="cuda")
+    for at in (1.0, 2.0):                       # the masked logits: lowest itself, -inf
+        s = torch.full((N,), at, dtype=dtype, device=cuda)
+        want, p, far = exact(s, w, t)
+        x, W = place(s, H), place(w, H)
+        loss, dx, dw = sp.linear_cross_entropy_grad(x, W, t, reduction="none")
+        assert bool(((loss.double() - want).abs() <= 4 * E * want + (3 * far + 100) * E).all())
+        assert bool(torch.isfinite(dx).all()) and bool(torch.isfinite(dw).all()) and not dw[100:420].any()
+    s = torch.ones(N, dtype=dtype, device=cuda)
+    for top in (-3.0e38, 3.0e38, -2.0e38, 2.5e38, 1e30, -1e30, 1e8, -1e8, 69632.0, -60000.0):
+        w = torch.full((V,), lowest, dtype=dtype, device=cuda)
+        w[::7] = top                            # 100 of one size, the others far below
+        t = 7 * torch.randint(0, 100, (N,), generator=g, device="cuda")
+        loss = sp.linear_cross_entropy(place(s, H), place(w, H), t, reduction="none")
+        assert bool(((loss.double() - math.log(100.0)).abs() <= 200 * E).all()), (top, loss[:3])
