@@ -6,11 +6,13 @@
 //
 // Three products of 2 N H V operations each. The product of the logits ends in its own softmax statistics: for 64 or
 // 128 neighbouring columns of a token it leaves the maximum m and the sum of exp(z - m), and, where gradients are wanted,
-// the exponentials p = exp(z - m) themselves, rounded to the 16-bit type once. One pass over p turns them into G
-// (times exp(m - lse), the target's element from its fp32 logit), and G goes into the other two products. So nothing
-// is multiplied twice, and what is held is 16 bits an element for as many tokens at a time as the workspace takes. The
-// gradients' error is then that of G's elements, rounded twice, and of one rounding at the end: 1.3 times the error of
-// a result that is rounded at the end alone (1.0 times for up to 32 tokens, whose p and G keep what is rounded off).
+// the exponentials p = exp(z - m) themselves, rounded to the 16-bit type once. The target's column is left out of all
+// three and its logit kept: with R the sum over the others of exp(z_ij - z_i,t) the loss is log1p R, within 1e-6 of itself
+// also where the token is sure (next to the target's 1 a sum would lose R). One pass over p turns it into G (times
+// exp(m - lse); the target's element from the loss), and G goes into the other two products. So nothing is multiplied
+// twice, and what is held is 16 bits an element for as many tokens at a time as the workspace takes. The gradients' error
+// is then that of G's elements, rounded twice, and of one rounding at the end: 1.3 times the error of a result that is
+// rounded at the end alone (1.0 times for up to 32 tokens, whose p and G keep what is rounded off).
 #include <math.h>
 
 #include <type_traits>
@@ -466,22 +468,31 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void k_product(const Produc
 #pragma unroll
                 for (int i = 0; i < 4 * IM; ++i) z[i] = 64 * (i >> 4) + (i & 15) < inside ? z[i] : -INFINITY;
             }
-            // (a maximum that passes NaN by: the sum has it)
-            float m = -INFINITY;
+            auto largest = [&] {   // (passes NaN by: the sum has it)
+                float m = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4 * IM; i += 2) m = max3(m, z[i], z[i + 1]);
-            // (fmaxf, not the asm of max3: the compiler has to see what a permlane reads, which needs a wait behind it)
-            m = reduce_rows(fmaxf(m, z[0]), [](float a, float b) { return fmaxf(a, b); });
-            const Base base = base_of(m);
+                for (int i = 0; i < 4 * IM; i += 2) m = max3(m, z[i], z[i + 1]);
+                // (fmaxf, not the asm of max3: the compiler has to see what a permlane reads, which needs a wait behind it)
+                return reduce_rows(fmaxf(m, z[0]), [](float a, float b) { return fmaxf(a, b); });
+            };
+            float m = largest();
+            // The target's logit stands alone: k_finish adds its exponential to a maximum and a sum of the others, so that
+            // what they leave of a sure prediction's loss is not lost beside it.
             const long target = on ? t[j] - first : -1;
             const int at = target >= 0 && target < inside ? (int)target : -1;
             const bool here = at >= 0 && at < 64 * (IM / 4) && (at & 63) < 16;
             if (__builtin_expect(__ballot(here) != 0, 0)) {
                 float zt = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4 * IM; ++i) zt = at == 64 * (i >> 4) + (i & 15) ? z[i] : zt;
+                for (int i = 0; i < 4 * IM; ++i) {
+                    const bool is = at == 64 * (i >> 4) + (i & 15);
+                    zt = is ? z[i] : zt;
+                    z[i] = is ? -INFINITY : z[i];
+                }
                 if (here) end.zt[n] = zt;
+                m = largest();
             }
+            const Base base = base_of(m);
             if (__builtin_expect(__ballot(!within(m)) != 0, 0)) {
 #pragma unroll
                 for (int i = 0; i < 4 * IM; ++i) z[i] -= base.sub;
@@ -650,23 +661,23 @@ __global__ __launch_bounds__(256) void k_few(const ProductArgs q) {
     for (int n = threadIdx.x >> 3; n < 16 * NB; n += 32) {
         const int col = 4 * (threadIdx.x & 7);
         const long v = m0 + col;
+        const bool on = n < q.N;
+        const long tgt = on ? q.target[n] : -1;
         float z[4], m = -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             z[r] = (part[0][n][col + r] + part[1][n][col + r]) + (part[2][n][col + r] + part[3][n][col + r]);
-            if (v + r >= q.M) z[r] = -INFINITY;
+            if (v + r == tgt && v + r < q.M) q.zt[n] = z[r];   // it stands alone, as in the other kernel
+            if (v + r >= q.M || v + r == tgt) z[r] = -INFINITY;
             m = fmaxf(m, z[r]);
         }
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
         const Base base = base_of(m);
-        const bool on = n < q.N;
-        const long tgt = on ? q.target[n] : -1;
         typedef T x4 __attribute__((ext_vector_type(4)));
         x4 e, rest;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            if (v + r == tgt && v + r < q.M) q.zt[n] = z[r];
             const float x = __builtin_amdgcn_exp2f(fmaf(z[r] - base.sub, LOG2E, -base.top));
             sum += x;
             e[r] = (T)x;
@@ -795,21 +806,22 @@ __global__ __launch_bounds__(256) void k_finish(const FinishArgs q) {
     float m = -INFINITY;
     for (long s = threadIdx.x; s < q.segs; s += 256) m = nan_max(m, stat[s].x);
     m = reduce_threads<256, NanMax>(m, slot);
-    // segments without a logit above -inf: exp(-inf) times their sum, 0 or NaN
-    const float top = m == -INFINITY ? 0.0f : m;
-    float sum = 0.0f;
-    for (long s = threadIdx.x; s < q.segs; s += 256)
-        sum += stat[s].y * __builtin_amdgcn_exp2f(fmaf(stat[s].x - top, LOG2E, -off_of(stat[s].x)));
-    sum = reduce_threads<256, Sum>(sum, slot);
-    const float l = logf(sum);
     const long t = q.target[i];
     const float w = weight_of(t, q.ignore, q.V, q.row_weight, i);
-    const bool in = t >= 0 && t < q.V && t != q.ignore;
-    // Log of the target's probability (or 0, or NaN), from what is small where that is: z - m and the sum, not lse. Below
-    // 2^-23 it is the rounding of a sum of 1.
-    const float far = in ? (q.zt[i] - top) - l : w, d = fabsf(far) < 0x1p-23f ? 0.0f : far;
+    const bool column = t >= 0 && t < q.V, in = column && t != q.ignore;
+    const float zt = column ? q.zt[i] : -INFINITY;
+    // The segments have all but the target. Relative to the larger of their maximum and the target's logit (NaN if either is;
+    // segments without a logit above -inf add exp(-inf) times their sum, 0 or NaN):
+    const float most = nan_max(m, zt), top = most == -INFINITY ? 0.0f : most;
+    float rest = 0.0f;
+    for (long s = threadIdx.x; s < q.segs; s += 256)
+        rest += stat[s].y * __builtin_amdgcn_exp2f(fmaf(stat[s].x - top, LOG2E, -off_of(stat[s].x)));
+    rest = reduce_threads<256, Sum>(rest, slot);
+    // log of the sum of all exponentials: of 1 + rest where the target is the largest; of at least 1 otherwise
+    const float far = zt - top, l = log1pf(rest + expm1f(far));
+    const float d = in ? l - far : w;   // the token's loss (or 0, or NaN)
     if (blockIdx.y == 0 && threadIdx.x == 0) {
-        q.loss[i] = w == 0.0f ? 0.0f : -w * d;
+        q.loss[i] = w == 0.0f ? 0.0f : w * d;
         if (q.lse != nullptr) q.lse[i] = top + l;
     }
     if (q.p == nullptr) return;
@@ -835,7 +847,7 @@ __global__ __launch_bounds__(256) void k_finish(const FinishArgs q) {
             if (in && t >= v && t < v + 8) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    if (t == v + k) e[k] = f * expm1f(d);
+                    if (t == v + k) e[k] = f * expm1f(-d);
             }
         }
         store8(p + v, 8, e);

@@ -98,3 +98,65 @@ def test_logits_at_the_ends_of_float32(cuda, N):
         t = 7 * torch.randint(0, 100, (N,), generator=g, device="cuda")
         loss = sp.linear_cross_entropy(place(s, H), place(w, H), t, reduction="none")
         assert bool(((loss.double() - math.log(100.0)).abs() <= 200 * E).all()), (top, loss[:3])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,H,V", SIZES)
+def test_small_losses(cuda, N, H, V, dtype):
+    """a token that is sure of its target: what the other columns leave, from a tenth of a nat to 1e-20, as exactly as a
+    large loss (relative, not beside the logits), and the gradients of such tokens"""
+    print(f"linear_cross_entropy {N}x{H}x{V} {dtype}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(33)
+    best = int(torch.randint(0, V, (1,), generator=g, device="cuda"))
+    w = (0.5 * torch.randn(V, generator=g, device="cuda")).clamp(-1.5, 1.5).to(dtype)
+    w[best] = math.log(V) + 1.0
+    s = (1.0 + 2.0 * torch.rand(N, generator=g, device="cuda")).to(dtype)
+    s[0] = 1.0
+    t = torch.full((N,), best, device=cuda)
+    want, p, far = exact(s, w, t)
+    assert float(want.max()) < 0.9 and float(far.max()) < 60.0
+    c = (3 * far + 100) * E
+    x, W = place(s, H), place(w, H)
+    loss = sp.linear_cross_entropy(x, W, t, reduction="none")
+    rel = (loss.double() - want).abs() / want
+    assert bool((rel <= c).all()), float((rel / c).max())
+    one, none, dw = sp.linear_cross_entropy_grad(x[:1], W, t[:1], reduction="sum", need_dx=False)
+    assert torch.equal(one, loss[0]) or abs(float(one) - float(want[0])) <= float(c[0] * want[0])
+    total, dx, dw = sp.linear_cross_entropy_grad(x, W, t, reduction="sum")
+    assert abs(float(total) - float(want.sum())) <= float((c * want).sum() + 2 * E * want.sum())
+    # the target's element of G is expm1(-loss): relative, too (float16 has G times 2^10 and then its smallest number)
+    u, small = U[dtype], 2.0 ** -24 if dtype == torch.float16 else 0.0
+    G = p.clone()
+    G[:, best] = torch.expm1(-want)
+    X, Y = s.double(), w.double()
+    # (float16's p is relative to its group's largest, the target not among them: that is below 1 / V^0.5 here)
+    dG = G.abs() * (2.1 * u + 2 * c[:, None]) + small * (G.abs().amax(1, keepdim=True) + 2.0 ** -11)
+    want_x, want_w = (G * Y).sum(1), (G * X[:, None]).sum(0)
+    tol_x = (dG * Y.abs()).sum(1) + (V + 16) * E * (G.abs() * Y.abs()).sum(1) + u * want_x.abs() * 1.01 + small
+    tol_w = (dG * X[:, None]).sum(0) + (N + 16) * E * (G.abs() * X[:, None]).sum(0) + u * want_w.abs() * 1.01 + small
+    assert bool(((dx[:, 0].double() - want_x).abs() <= tol_x).all())
+    assert bool(((dw[:, 0].double() - want_w).abs() <= tol_w).all())
+
+
+@pytest.mark.parametrize("N", [3, 300])
+def test_small_gradients_under_a_scale(cuda, N):
+    """float16, losses of 1e-9 to 1e-6 and a loss scale that takes their gradients into range: the other columns' share, which
+    lies below float16's numbers next to the target's, is there"""
+    H, V, dtype, scale = 8, 256, torch.float16, 2.0 ** 20
+    g = torch.Generator(device="cuda").manual_seed(34)
+    w = torch.randn(V, generator=g, device="cuda").to(dtype)
+    w[5] = 22.0
+    s = torch.linspace(0.9, 1.0, N, device=cuda).to(dtype)
+    t = torch.full((N,), 5, device=cuda)
+    want, p, far = exact(s, w, t)
+    assert 1e-9 < float(want.min()) and float(want.max()) < 1e-6
+    _, _, dw = sp.linear_cross_entropy_grad(place(s, H), place(w, H), t, reduction="sum", grad_scale=scale, need_dx=False)
+    G = p.clone()
+    G[:, 5] = torch.expm1(-want)
+    want_w = (G * s.double()[:, None]).sum(0) * scale
+    # G is held times 2^10, and a smallest number of float16 is 2^-24
+    tol = (G.abs() * (2.1 * U[dtype] + 400 * E) + 2.0 ** -34).sum(0) * scale + U[dtype] * want_w.abs() * 1.01 + 2.0 ** -24
+    off = (dw[:, 0].double() - want_w).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
+    # and no column is lost
+    assert bool((dw[:, 0] != 0).all())
