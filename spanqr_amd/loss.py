@@ -5,7 +5,7 @@ gradients begin that end in the optimizer's orth.
 import torch
 
 from . import _lib
-from .tensors import TYPES, check_same, check_tensor, on, workspace
+from .tensors import TYPES, check_same, check_tensor, on, once, workspace
 
 IGNORE_INDEX = -100
 MAX_WORKSPACE = 4 << 30   # bytes: 16-bit exponentials of 16384 tokens over 128000 columns
@@ -78,10 +78,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def backward(ctx, g):
         x, weight, target = ctx.saved_tensors
         reduction, ignore_index, max_workspace = ctx.how
-        g = g.to(torch.float32)
-        _, _, dx, dw = _run(x, weight, target, reduction, ignore_index, g.contiguous() if reduction == "none" else None,
-                            None if reduction == "none" else g, ctx.needs_input_grad[0], ctx.needs_input_grad[1],
+        f = g.detach().to(torch.float32)
+        _, _, dx, dw = _run(x, weight, target, reduction, ignore_index, f.contiguous() if reduction == "none" else None,
+                            None if reduction == "none" else f, ctx.needs_input_grad[0], ctx.needs_input_grad[1],
                             max_workspace)
+        dx, dw = (once("linear_cross_entropy", d, x, weight, g) for d in (dx, dw))
         return dx, dw, None, None, None, None
 
 
@@ -91,9 +92,10 @@ def linear_cross_entropy(x, weight, target, reduction="mean", ignore_index=IGNOR
     none), the sum, or ("none") each token's loss [N], 0 where ignored. The logits are not kept. A target that is neither a
     column nor ignore_index gives NaN.
 
-    Differentiable in x and weight; the backward pass forms the logits again with the incoming gradient at hand.
-    A training step that wants the gradients at once takes linear_cross_entropy_grad, which forms the logits once.
-    max_workspace: bytes of scratch memory that bound how many tokens are taken at a time."""
+    Differentiable in x and weight, once (gradients of the gradients raise RuntimeError); the backward pass forms the
+    logits again with the incoming gradient at hand. A training step that wants the gradients at once takes
+    linear_cross_entropy_grad, which forms the logits once. max_workspace: bytes of scratch memory that bound how many
+    tokens are taken at a time."""
     _check("linear_cross_entropy", x, weight, target, reduction, None)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _LinearCrossEntropy.apply(x, weight, target, reduction, ignore_index, max_workspace)

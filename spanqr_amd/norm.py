@@ -5,7 +5,7 @@ whose gradients the optimizer that calls orth works on.
 import torch
 
 from . import _lib
-from .tensors import TYPES, check_like, check_same, check_tensor, like, on, rows_of, workspace
+from .tensors import TYPES, check_like, check_same, check_tensor, like, on, once, rows_of, workspace
 
 QUANT = {None: (_lib.QUANT_NONE, None), "fp8": (_lib.QUANT_FP8, torch.float8_e4m3fn), "int8": (_lib.QUANT_INT8, torch.int8)}
 
@@ -60,6 +60,7 @@ class _RmsNorm(torch.autograd.Function):
         if dy is None:                       # only the stream went on
             return dh, None if weight is None else torch.zeros_like(weight), dh if ctx.residual else None, None
         dx, dw = rms_norm_backward(dy, h, weight, ctx.eps, dh, ctx.needs_input_grad[1])
+        dx, dw = (once("rms_norm", d, h, weight, dy, dh) for d in (dx, dw))
         return dx, dw, dx if ctx.residual else None, None
 
 
@@ -72,8 +73,9 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, quant=None):
     comes with its scale [...] float32, (y, scale) or (y, scale, h): y * scale is the norm, the scale is max|norm| / 448 or
     / 127 of each row. A row of zeros has scale 0; a row with a NaN has scale NaN.
 
-    Differentiable in x, weight and residual without quant; with it the result carries no gradient (rms_norm_backward
-    takes the gradient of the unrounded norm, as a straight-through step does)."""
+    Differentiable in x, weight and residual without quant, once (gradients of the gradients raise RuntimeError); with
+    quant the result carries no gradient (rms_norm_backward takes the gradient of the unrounded norm, as a
+    straight-through step does)."""
     _check("rms_norm", x, weight)
     if quant not in QUANT:
         raise ValueError(f"rms_norm: quant must be None, 'fp8' or 'int8', got {quant!r}")

@@ -48,6 +48,26 @@ def rows_of(t, D):
     return t
 
 
+class _Once(torch.autograd.Function):
+    """a gradient as it is, behind what it was formed from: its own gradient is refused"""
+
+    @staticmethod
+    def forward(ctx, what, grad, *formed_from):
+        ctx.what = what
+        ctx.mark_dirty(grad)
+        return grad
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"{ctx.what}: its gradients cannot be differentiated again")
+
+
+def once(what, grad, *formed_from):
+    """grad as a backward pass returns it. Where that pass records (create_graph) the kernels' result would look like a
+    constant, and a function of it would train without its share: it depends on formed_from, and says so when asked."""
+    return grad if grad is None or not torch.is_grad_enabled() else _Once.apply(what, grad, *formed_from)
+
+
 # the current stream's handle by the device's index: what torch.cuda.current_stream(device).cuda_stream gives, without
 # the stream object around it (0.1 us instead of 1.9)
 _stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None

@@ -1,0 +1,70 @@
+"""What autograd may not overlook in the training operators: gradients of gradients"""
+import pytest
+import torch
+
+import spanqr_amd as sp
+
+pytestmark = pytest.mark.gpu
+
+
+def loss_inputs(N=6, H=16, V=40, dtype=torch.bfloat16):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(N, H, generator=g, device="cuda").to(dtype).requires_grad_()
+    W = (0.3 * torch.randn(V, H, generator=g, device="cuda")).to(dtype).requires_grad_()
+    return x, W, torch.randint(0, V, (N,), generator=g, device="cuda")
+
+
+def norm_inputs(rows=5, D=40, dtype=torch.bfloat16):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x, r = (torch.randn(rows, D, generator=g, device="cuda").to(dtype).requires_grad_() for _ in range(2))
+    return x, torch.ones(D, device="cuda", dtype=dtype, requires_grad=True), r
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_loss_is_not_differentiated_twice(cuda, reduction):
+    x, W, t = loss_inputs()
+    loss = sp.linear_cross_entropy(x, W, t, reduction=reduction).sum()
+    plain = torch.autograd.grad(loss, (x, W), retain_graph=True)
+    gx, gw = torch.autograd.grad(loss, (x, W), create_graph=True)
+    assert torch.equal(gx, plain[0]) and torch.equal(gw, plain[1])
+    for g in (gx, gw):
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (loss + g.float().square().sum()).backward(retain_graph=True)
+    # one of the two alone
+    W2 = W.detach()
+    loss = sp.linear_cross_entropy(x, W2, t, reduction=reduction).sum()
+    gx, = torch.autograd.grad(loss, x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        gx.float().square().sum().backward()
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_is_not_differentiated_twice(cuda, residual):
+    x, w, r = norm_inputs()
+    y = sp.rms_norm(x, w, residual=r)[0] if residual else sp.rms_norm(x, w)
+    loss = y.float().square().sum()
+    inputs = (x, w, r) if residual else (x, w)
+    plain = torch.autograd.grad(loss, inputs, retain_graph=True)
+    grads = torch.autograd.grad(loss, inputs, create_graph=True)
+    for g, p in zip(grads, plain):
+        assert torch.equal(g, p)
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (loss + g.float().square().sum()).backward(retain_graph=True)
+
+
+def test_create_graph_alone_is_fine(cuda):
+    """steps that record the backward pass and do not use what it recorded, with the gradients added up and set to zero"""
+    x, W, t = loss_inputs()
+    w = torch.ones(16, device=cuda, dtype=torch.bfloat16, requires_grad=True)
+    for _ in range(2):
+        loss = sp.linear_cross_entropy(sp.rms_norm(x, w), W, t)
+        loss.backward(create_graph=True)
+    for p in (x, W, w):
+        assert p.grad.requires_grad
+        p.grad = p.grad.detach()
+    twice = [p.grad.clone() for p in (x, W, w)]
+    for p in (x, W, w):
+        p.grad.zero_()
+    for _ in range(2):
+        sp.linear_cross_entropy(sp.rms_norm(x, w), W, t).backward()
+    assert all(torch.equal(p.grad, v) for p, v in zip((x, W, w), twice))
