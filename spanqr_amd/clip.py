@@ -6,7 +6,7 @@ from array import array
 import torch
 
 from . import _lib
-from .tensors import TYPES, check_same, check_tensor, on, workspace
+from .tensors import TYPES, check_same, check_tensor, no_tangents, on, workspace
 
 
 def _dense(t):
@@ -28,6 +28,7 @@ _device_of, _dtype_of = torch.Tensor.get_device, torch.Tensor.dtype.__get__
 def _tensors(what, name, ts, device=None):
     """ts as a list of tensors of the three types on one GPU, that device, and the tensors' types for the C ABI"""
     ts = [ts] if isinstance(ts, torch.Tensor) else list(ts)
+    no_tangents(what, *ts)
     if not ts:
         return ts, device or torch.device("cuda", torch.cuda.current_device()), array("i")
     first = ts[0]

@@ -5,7 +5,7 @@ gradients begin that end in the optimizer's orth.
 import torch
 
 from . import _lib
-from .tensors import TYPES, check_same, check_tensor, on, once, workspace
+from .tensors import TYPES, check_same, check_tensor, no_tangents, on, once, workspace
 
 IGNORE_INDEX = -100
 MAX_WORKSPACE = 4 << 30   # bytes: 16-bit exponentials of 16384 tokens over 128000 columns
@@ -20,7 +20,8 @@ def _rows(t):
     return t
 
 
-def _check(what, x, weight, target, reduction, row_weight):
+def _check(what, x, weight, target, reduction, row_weight, grad_scale=None):
+    no_tangents(what, x, weight, row_weight, grad_scale)
     check_tensor(what, "x", x, (torch.bfloat16, torch.float16))
     check_tensor(what, "weight", weight, (torch.bfloat16, torch.float16))
     if x.dim() != 2 or weight.dim() != 2:
@@ -108,7 +109,7 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
     each token's loss (not the count that the mean is over). grad_scale (a number, or a float32 tensor of one element on
     the device: a loss scale) multiplies the gradients before they are rounded, not the loss. With reduction "none" the
     gradients are of the sum. dx or dw is None with need_dx=False or need_dw=False."""
-    _check("linear_cross_entropy_grad", x, weight, target, reduction, row_weight)
+    _check("linear_cross_entropy_grad", x, weight, target, reduction, row_weight, grad_scale)
     if grad_scale is not None:
         if not isinstance(grad_scale, torch.Tensor):
             grad_scale = torch.full((), float(grad_scale), dtype=torch.float32, device=x.device)

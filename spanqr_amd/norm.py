@@ -5,12 +5,13 @@ whose gradients the optimizer that calls orth works on.
 import torch
 
 from . import _lib
-from .tensors import TYPES, check_like, check_same, check_tensor, like, on, once, rows_of, workspace
+from .tensors import TYPES, check_like, check_same, check_tensor, like, no_tangents, on, once, rows_of, workspace
 
 QUANT = {None: (_lib.QUANT_NONE, None), "fp8": (_lib.QUANT_FP8, torch.float8_e4m3fn), "int8": (_lib.QUANT_INT8, torch.int8)}
 
 
-def _check(what, x, weight):
+def _check(what, x, weight, *others):
+    no_tangents(what, x, weight, *others)
     check_tensor(what, "x", x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what}: x must be [..., D] with D >= 1, got {list(x.shape)}")
@@ -76,7 +77,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, quant=None):
     Differentiable in x, weight and residual without quant, once (gradients of the gradients raise RuntimeError); with
     quant the result carries no gradient (rms_norm_backward takes the gradient of the unrounded norm, as a
     straight-through step does)."""
-    _check("rms_norm", x, weight)
+    _check("rms_norm", x, weight, residual)
     if quant not in QUANT:
         raise ValueError(f"rms_norm: quant must be None, 'fp8' or 'int8', got {quant!r}")
     if residual is not None:
@@ -95,7 +96,7 @@ def rms_norm_backward(dy, h, weight=None, eps=1e-6, dh=None, need_dw=True):
     """(dx, dw) of rms_norm from the gradient dy of y and the normed stream h (x itself where there was no residual):
     dx is the gradient of x and of the residual alike. dh: the gradient that reaches h on the stream's own way, added to
     dx. dw is None without a weight or with need_dw=False; it has the weight's type."""
-    _check("rms_norm_backward", h, weight)
+    _check("rms_norm_backward", h, weight, dy, dh)
     D, dev = h.shape[-1], h.device
     check_like("rms_norm_backward", "dy", dy, h, h.shape)
     if dh is not None:

@@ -3,6 +3,7 @@ and stream a call runs on."""
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -36,6 +37,16 @@ def check_like(what, name, t, x, shape):
     if not like(t, x, shape):
         check_tensor(what, name, t)
         check_same(what, name, t, x.device, shape, x.dtype)
+
+
+def no_tangents(what, *ts):
+    """Refuses tensors with a tangent of forward-mode differentiation, which the kernels would leave behind. Outside of it
+    (no dual level) nothing is looked at."""
+    if forward_ad._current_level < 0:
+        return
+    for t in ts:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: forward-mode differentiation is not implemented")
 
 
 def rows_of(t, D):

@@ -1,6 +1,8 @@
-"""What autograd may not overlook in the training operators: gradients of gradients"""
+"""What autograd may not overlook in the training operators: gradients of gradients, tangents of forward-mode
+differentiation"""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import spanqr_amd as sp
 
@@ -68,3 +70,23 @@ def test_create_graph_alone_is_fine(cuda):
     for _ in range(2):
         sp.linear_cross_entropy(sp.rms_norm(x, w), W, t).backward()
     assert all(torch.equal(p.grad, v) for p, v in zip((x, W, w), twice))
+
+
+def test_tangents_are_refused(cuda):
+    x, W, t = loss_inputs()
+    x, W = x.detach(), W.detach()
+    h, w, r = (v.detach() for v in norm_inputs())
+    calls = [(x, lambda d: sp.linear_cross_entropy(d, W, t)), (W, lambda d: sp.linear_cross_entropy(x, d, t)),
+             (x, lambda d: sp.linear_cross_entropy_grad(d, W, t)),
+             (torch.ones(len(t), device=cuda), lambda d: sp.linear_cross_entropy_grad(x, W, t, row_weight=d)),
+             (torch.ones((), device=cuda), lambda d: sp.linear_cross_entropy_grad(x, W, t, grad_scale=d)),
+             (h, lambda d: sp.rms_norm(d, w)), (w, lambda d: sp.rms_norm(h, d)), (r, lambda d: sp.rms_norm(h, w, residual=d)),
+             (h, lambda d: sp.rms_norm(d, w, quant="int8")), (r, lambda d: sp.rms_norm_backward(d, h, w)),
+             (r, lambda d: sp.rms_norm_backward(r, h, w, dh=d)), (h, lambda d: sp.grad_norm([r, d])),
+             (h, lambda d: sp.clip_grad_norm(d, 1.0)), (h, lambda d: sp.clip_grad_norm([r.clone()], 1.0, out=[d]))]
+    for v, call in calls:
+        want = call(v.clone())
+        with forward_ad.dual_level():
+            assert torch.equal(*(c[0] if isinstance(c, tuple) else c for c in (call(v.clone()), want)))   # no tangent
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(forward_ad.make_dual(v.clone(), torch.ones_like(v)))
