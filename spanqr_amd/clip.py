@@ -141,6 +141,9 @@ def clip_grad_norm(grads, max_norm, out=None):
         ws = workspace(nbytes, dev)
         _lib.check(lib.spanqr_clip_grad_norm(n, _at(at), _at(numel), _at(types), _at(to), _at(out_types), max_norm,
                                              norm.data_ptr(), ws.data_ptr(), nbytes, stream))
+    # written behind autograd's back, which has to notice if it keeps one of them (whether the norm was within max_norm is
+    # not known here)
+    torch.autograd.graph.increment_version(out)
     for o, copy in back:
         o.copy_(copy)
     return norm

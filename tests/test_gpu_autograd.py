@@ -1,5 +1,5 @@
 """What autograd may not overlook in the training operators: gradients of gradients, tangents of forward-mode
-differentiation"""
+differentiation, tensors that are written in place"""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -90,3 +90,31 @@ def test_tangents_are_refused(cuda):
             assert torch.equal(*(c[0] if isinstance(c, tuple) else c for c in (call(v.clone()), want)))   # no tangent
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call(forward_ad.make_dual(v.clone(), torch.ones_like(v)))
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_clipping_is_seen(cuda, strided):
+    """a tensor that autograd keeps and that is clipped in place, or written as out, is not the one it kept"""
+    def kept():
+        a = torch.ones(6, 8, device=cuda, requires_grad=True)
+        b = a * 3.0
+        c = b.square().sum()         # keeps b
+        b = b.detach()
+        return b[:, ::2] if strided else b, c
+
+    b, c = kept()
+    sp.grad_norm([b])                # reads alone
+    c.backward()
+    for write in (lambda t: sp.clip_grad_norm([t], 1.0), lambda t: sp.clip_grad_norm([torch.ones_like(t)], 1.0, out=[t])):
+        b, c = kept()
+        was = b._version
+        write(b)
+        assert b._version > was
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            c.backward()
+    g = torch.ones(5, device=cuda)
+    was = g._version
+    sp.clip_grad_norm([g], 1.0, out=[torch.empty_like(g)])
+    assert g._version == was
+    with torch.inference_mode():     # such tensors have no version
+        sp.clip_grad_norm([torch.ones(5, device=cuda)], 1.0)
