@@ -144,6 +144,8 @@ def clip_grad_norm(grads, max_norm, out=None):
     # written behind autograd's back, which has to notice if it keeps one of them (whether the norm was within max_norm is
     # not known here)
     torch.autograd.graph.increment_version(out)
-    for o, copy in back:
-        o.copy_(copy)
+    if back:
+        with torch.no_grad():   # as the others are written
+            for o, copy in back:
+                o.copy_(copy)
     return norm

@@ -118,3 +118,18 @@ def test_clipping_is_seen(cuda, strided):
     assert g._version == was
     with torch.inference_mode():     # such tensors have no version
         sp.clip_grad_norm([torch.ones(5, device=cuda)], 1.0)
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_clipping_records_nothing(cuda, strided):
+    """gradients that require a gradient (of a recorded backward pass, or leaves) are clipped as others are, in any order"""
+    whole = torch.ones(6, 8, device=cuda)
+    leaf = (whole[:, ::2] if strided else whole).requires_grad_()
+    sp.clip_grad_norm([leaf], 1.0)
+    assert leaf.is_leaf and abs(float(leaf.detach().norm()) - 1.0) < 1e-6
+    a = torch.ones(6, 8, device=cuda, requires_grad=True)
+    b = (a * 1.0)[:, ::2] if strided else a * 1.0
+    sp.clip_grad_norm([b], 1.0)
+    assert abs(float(b.detach().norm()) - 1.0) < 1e-6
+    b.sum().backward()               # as before: the factor is no part of it
+    assert float(a.grad.sum()) == b.numel()
