@@ -112,8 +112,9 @@ def clip_grad_norm(grads, max_norm, out=None):
     any of the three types), into out, the gradients left as they are: float32 copies of 16-bit gradients in the same
     pass, for an optimizer that works in float32. In place a norm within max_norm writes nothing.
 
-    A NaN norm makes every result NaN, an infinite norm makes finite gradients 0: look at the norm before the step. out
-    may share no memory with the gradients, other than out[i] being grads[i]."""
+    Each tensor to write to is listed once (a shared parameter's gradient, too): two that start at the same address raise
+    ValueError. out may share no memory with the gradients, other than out[i] being grads[i]. A NaN norm makes every
+    result NaN, an infinite norm makes finite gradients 0: look at the norm before the step."""
     grads, dev, types = _tensors("clip_grad_norm", "every gradient", grads)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
@@ -134,6 +135,10 @@ def clip_grad_norm(grads, max_norm, out=None):
     n = len(src)
     at, numel = _pointers(src), _sizes(src)
     to = at if dst is src else _pointers(dst)
+    if len(set(to)) < n:   # (empty tensors have no address)
+        full = [p for p, k in zip(to, numel) if k]
+        if len(set(full)) < len(full):
+            raise ValueError("clip_grad_norm: two of the tensors to write to lie in the same memory")
     norm = torch.empty((), dtype=torch.float32, device=dev)
     lib = _lib.lib()
     with on(dev) as stream:
