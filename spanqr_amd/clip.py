@@ -70,7 +70,7 @@ def _at(values):
 def grad_norm(grads):
     """sqrt of the sum of squares over all tensors of a list (or of one tensor): float32, bfloat16 and float16 mixed, of
     any shapes and strides, on one ROCm device. A float32 tensor without axes on that device, no host synchronisation;
-    squares and sums in float64. An empty list gives 0."""
+    squares and sums in float64. An empty list gives 0. The norm carries no gradient, also of tensors that require one."""
     ts, dev, types = _tensors("grad_norm", "every gradient", grads)
     if not _contiguous(ts):
         ts = [t if _dense(t) else t.contiguous() for t in ts]
@@ -114,7 +114,8 @@ def clip_grad_norm(grads, max_norm, out=None):
 
     Each tensor to write to is listed once (a shared parameter's gradient, too): two that start at the same address raise
     ValueError. out may share no memory with the gradients, other than out[i] being grads[i]. A NaN norm makes every
-    result NaN, an infinite norm makes finite gradients 0: look at the norm before the step."""
+    result NaN, an infinite norm makes finite gradients 0: look at the norm before the step. Neither the norm nor what is
+    written carries a gradient."""
     grads, dev, types = _tensors("clip_grad_norm", "every gradient", grads)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

@@ -108,7 +108,7 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
     """(loss, dx, dw): linear_cross_entropy and its gradients in one pass, in x's type. row_weight [N] float32 multiplies
     each token's loss (not the count that the mean is over). grad_scale (a number, or a float32 tensor of one element on
     the device: a loss scale) multiplies the gradients before they are rounded, not the loss. With reduction "none" the
-    gradients are of the sum. dx or dw is None with need_dx=False or need_dw=False."""
+    gradients are of the sum. dx or dw is None with need_dx=False or need_dw=False. None of them carries a gradient."""
     _check("linear_cross_entropy_grad", x, weight, target, reduction, row_weight, grad_scale)
     if grad_scale is not None:
         if not isinstance(grad_scale, torch.Tensor):

@@ -95,7 +95,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, quant=None):
 def rms_norm_backward(dy, h, weight=None, eps=1e-6, dh=None, need_dw=True):
     """(dx, dw) of rms_norm from the gradient dy of y and the normed stream h (x itself where there was no residual):
     dx is the gradient of x and of the residual alike. dh: the gradient that reaches h on the stream's own way, added to
-    dx. dw is None without a weight or with need_dw=False; it has the weight's type."""
+    dx. dw is None without a weight or with need_dw=False; it has the weight's type. Neither carries a gradient."""
     _check("rms_norm_backward", h, weight, dy, dh)
     D, dev = h.shape[-1], h.device
     check_like("rms_norm_backward", "dy", dy, h, h.shape)
