@@ -985,13 +985,21 @@ Layout layout_of(long N, long H, long V, int grads, bool pad, long tokens) {
     return l;
 }
 
+// A launch has fewer than 2^32 threads: 256 for each of k_finish's tokens, and for each tile of the logits.
+constexpr long MAX_TOKENS = 1l << 23, MAX_TILES = 1l << 24;
+
 // most tokens at a time within `most` bytes: all, or a multiple of 256 (at least 256)
 long tokens_of(long N, long H, long V, int grads, bool pad, long most) {
-    if (N <= 256 || layout_of(N, H, V, grads, pad, N).bytes <= most) return N;
+    auto fit = [&](long tokens) {
+        if (tokens > MAX_TOKENS) return false;
+        const Layout l = layout_of(N, H, V, grads, pad, tokens);
+        return l.bytes <= most && l.logits.m_tiles * l.logits.n_tiles < MAX_TILES;
+    };
+    if (N <= 256 || fit(N)) return N;
     long lo = 1, hi = over(N, 256);   // in units of 256: lo is taken, hi is too many
     while (hi - lo > 1) {
         const long mid = (lo + hi) / 2;
-        if (layout_of(N, H, V, grads, pad, 256 * mid).bytes <= most)
+        if (fit(256 * mid))
             lo = mid;
         else
             hi = mid;

@@ -160,3 +160,16 @@ def test_small_gradients_under_a_scale(cuda, N):
     assert bool((off <= tol).all()), float((off / tol).max())
     # and no column is lost
     assert bool((dw[:, 0] != 0).all())
+
+
+def test_more_tokens_than_a_launch_takes(cuda):
+    """2^24 tokens and some: pieces, each of fewer than 2^32 threads"""
+    N, H, V, dtype = (1 << 24) + 5, 8, 16, torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(35)
+    s = (torch.rand(N, generator=g, device="cuda") + 1.0).to(dtype)
+    w = torch.randn(V, generator=g, device="cuda").to(dtype)
+    t = torch.randint(0, V, (N,), generator=g, device="cuda")
+    loss = sp.linear_cross_entropy(place(s, H), place(w, H), t, reduction="none")
+    for at in range(0, N, 1 << 22):
+        want, _, far = exact(s[at:at + (1 << 22)], w, t[at:at + (1 << 22)])
+        assert bool(((loss[at:at + (1 << 22)].double() - want).abs() <= 4 * E * want + (3 * far + 100) * E).all()), at
