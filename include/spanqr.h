@@ -346,7 +346,7 @@ int spanqr_clip_grad_norm(int n, const void* const* grads, const long* numel, co
  * `type`, each or null: the gradients of the sum (none, sum) or of the mean, times *grad_scale (device, or null for 1).
  * workspace: what spanqr_linear_cross_entropy_workspace gives for `grads` (1: dx, 2: dw, 3: both, 0: neither;
  * plus 4 where rows of x or w do not all start on 16 bytes: they are copied into rows that do) and most_bytes, which
- * bounds it: the tokens go through in pieces whose 16-bit exponentials fit (256 tokens at least). H and V up to 2^22. */
+ * bounds it: the tokens go through in pieces whose 16-bit exponentials fit (256 tokens at least). H and V up to 2^22, N below 2^31. */
 long spanqr_linear_cross_entropy_workspace(int type, long N, long H, long V, int grads, long most_bytes);
 int spanqr_linear_cross_entropy(int type, int reduction, long N, long H, long V, const void* x, long ldx, const void* w,
                                 long ldw, const long* target, long ignore_index, const float* row_weight,

@@ -875,7 +875,7 @@ __global__ __launch_bounds__(256) void k_pad(const T* src, long ld, long rows, i
     }
 }
 
-constexpr long MAX_N = 1l << 31, MAX_HV = 1l << 22;   // 256 rows stay within 32-bit byte offsets
+constexpr long MAX_N = (1l << 31) - 1, MAX_HV = 1l << 22;   // counted in int; 256 rows stay within 32-bit byte offsets
 
 long up(long v, long to) { return (v + to - 1) / to * to; }
 long over(long v, long by) { return (v + by - 1) / by; }

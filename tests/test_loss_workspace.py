@@ -27,3 +27,8 @@ def test_tiles_of_one_launch():
     one = need((1 << 18) - 256, 8, V, 0, huge)      # 2^24 tiles but 2^14
     N = 1 << 21
     assert 0 < need(N, 8, V, 0, huge) <= one + 4 * N
+
+
+def test_tokens_are_counted_in_int():
+    assert need((1 << 31) - 1, 8, 16, 0) > 0
+    assert need(1 << 31, 8, 16, 0) == -1   # SPANQR_EINVAL
