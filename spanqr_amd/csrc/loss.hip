@@ -13,8 +13,10 @@
 // twice, and what is held is 16 bits an element for as many tokens at a time as the workspace takes. The gradients' error
 // is then that of G's elements, rounded twice, and of one rounding at the end: 1.3 times the error of a result that is
 // rounded at the end alone (1.0 times for up to 32 tokens, whose p and G keep what is rounded off).
+#include <limits.h>
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -914,8 +916,7 @@ double time_of(int epilogue, int kind, long M, long N, long K, long splits) {
     return rounds * (step * (double)over(over(K, 64), splits) + ends) + join;
 }
 
-// rows of fp32 sums that dx over several parts of K may take. Like all of the workspace it does not shrink with more
-// tokens, so that what fits for some fits for fewer.
+// rows of fp32 sums that dx over several parts of K may take
 long split_rows(long tokens) {
     const long most = 2 * tokens > 16384 ? 2 * tokens : 16384;
     const long rows = tokens <= FEW_TOKENS ? 128 * tokens : tokens <= 2 * FEW_TOKENS ? 128 * FEW_TOKENS : 64 * tokens;
@@ -947,20 +948,20 @@ long rows_of_rounds(const Shape& all, long M, long N, long K) {
     return time_of(OUT, BIG, M, rows, K, 1) + time_of(OUT, rest.kind, M, N - rows, K, 1) < time_of(OUT, BIG, M, N, K, 1) ? rows : N;
 }
 
-// where things lie in the workspace, for `tokens` tokens at a time
+// Where things lie in the workspace, for `tokens` tokens at a time. It does not shrink with more tokens, so that what fits for
+// some fits for fewer. The sums of dx's parts come last: there are as many parts as the rest of the workspace holds.
 struct Layout {
-    long scal, loss, zt, stat, p, dx_acc, dw_acc, x, w, bytes;
-    long segs, ldp, Hp;
+    long scal, loss, zt, stat, p, dw_acc, x, w, dx_acc, bytes;
+    long rows, segs, ldp, Hp;    // (rows of p)
     int seg;                     // columns that share a maximum, 2^seg
     bool few;                    // the logits by k_few, p and G in two rows a token
-    Shape logits, dx;            // of a full piece of the tokens
+    Shape logits;                // of a full piece of the tokens
 };
 Layout layout_of(long N, long H, long V, int grads, bool pad, long tokens) {
     Layout l;
     l.logits = shape_of(LOGITS, V, tokens, H, 1);
     l.few = tokens <= FEW_TOKENS;
-    const long rows = l.few ? 2 * tokens : tokens;   // of p
-    l.dx = shape_of(OUT, H, rows, V, rows > 0 ? split_rows(tokens) / rows : 1);
+    l.rows = l.few ? 2 * tokens : tokens;
     l.seg = l.few ? 5 : l.logits.kind == BIG ? 7 : 6;
     l.segs = over(V, 1l << l.seg);
     l.ldp = up(V, 64);
@@ -974,15 +975,21 @@ Layout layout_of(long N, long H, long V, int grads, bool pad, long tokens) {
     l.scal = take(sizeof(Scalars));
     l.loss = take(4 * N);
     l.zt = take(4 * tokens);
-    const long most = l.few || tokens > 2 * FEW_TOKENS ? rows : 2 * FEW_TOKENS;   // (not below what fewer tokens need)
+    const long most = l.few || tokens > 2 * FEW_TOKENS ? l.rows : 2 * FEW_TOKENS;   // (not below what fewer tokens need)
     l.stat = take(8 * (l.few ? tokens * over(V, FEW_ROWS) : most * over(V, 64)));
     l.p = take(grads ? 2 * most * l.ldp : 0);
-    l.dx_acc = take((grads & 1) ? 4 * split_rows(tokens) * l.Hp : 0);
     l.dw_acc = take((grads & 2) && tokens < N ? 4 * l.Hp * V : 0);
-    l.x = take(pad ? 2 * most * l.Hp : (grads & 2) ? 2 * (l.few ? rows : 2 * FEW_TOKENS) * l.Hp : 0);
+    l.x = take(pad ? 2 * most * l.Hp : (grads & 2) ? 2 * (l.few ? l.rows : 2 * FEW_TOKENS) * l.Hp : 0);
     l.w = take(pad ? 2 * V * l.Hp : 0);
+    l.dx_acc = take((grads & 1) ? 4 * (l.few ? l.rows : 2 * FEW_TOKENS) * l.Hp : 0);
     l.bytes = at;
     return l;
+}
+
+// dx of a full piece of the tokens, with sums in `bytes` bytes where there are several parts or few tokens
+Shape dx_of(const Layout& l, long H, long V, long tokens, long bytes) {
+    const long most = l.rows > 0 ? std::min(split_rows(tokens) / l.rows, bytes / (4 * l.rows * l.Hp)) : 1;
+    return shape_of(OUT, H, l.rows, V, most > 1 ? most : 1);
 }
 
 // A launch has fewer than 2^32 threads: 256 for each of k_finish's tokens, and for each tile of the logits.
@@ -990,23 +997,23 @@ constexpr long MAX_TOKENS = 1l << 23, MAX_TILES = 1l << 24;
 
 // most tokens at a time within `most` bytes: all, or a multiple of 256 (at least 256)
 long tokens_of(long N, long H, long V, int grads, bool pad, long most) {
-    auto fit = [&](long tokens) {
+    auto fit = [&](long tokens, long bytes) {
         if (tokens > MAX_TOKENS) return false;
         const Layout l = layout_of(N, H, V, grads, pad, tokens);
-        return l.bytes <= most && l.logits.m_tiles * l.logits.n_tiles < MAX_TILES;
+        return l.bytes <= bytes && l.logits.m_tiles * l.logits.n_tiles < MAX_TILES;
     };
-    if (N <= 256 || fit(N)) return N;
+    if (N <= 256 || fit(N, most)) return N;
     long lo = 1, hi = over(N, 256);   // in units of 256: lo is taken, hi is too many
     while (hi - lo > 1) {
         const long mid = (lo + hi) / 2;
-        if (fit(256 * mid))
+        if (fit(256 * mid, most))
             lo = mid;
         else
             hi = mid;
     }
-    // the pieces alike
-    const long pieces = over(N, 256 * lo), even = up(over(N, pieces), 256);
-    return even < 256 * lo ? even : 256 * lo;
+    // the pieces alike; or all at once after all, where the pieces' sums of dW take more
+    const long pieces = over(N, 256 * lo), even = std::min(up(over(N, pieces), 256), 256 * lo);
+    return fit(N, layout_of(N, H, V, grads, pad, even).bytes) ? N : even;
 }
 
 int check_sizes(int type, long N, long H, long V) {
@@ -1049,9 +1056,10 @@ void product(const Shape& s, ProductArgs q, hipStream_t st) {
 }
 
 template <typename T>
-int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
+int enqueue(const Call& c, char* ws, long bytes, long tokens, hipStream_t st) {
     const int grads = (c.dx != nullptr ? 1 : 0) | (c.dw != nullptr ? 2 : 0);
     const Layout l = layout_of(c.N, c.H, c.V, grads, c.pad, tokens);
+    const Shape dx = grads & 1 ? dx_of(l, c.H, c.V, tokens, bytes - l.dx_acc) : Shape{};
     Scalars* scal = (Scalars*)(ws + l.scal);
     float* loss = c.reduced ? (float*)(ws + l.loss) : c.loss;
     const T *x = (const T*)c.x, *w = (const T*)c.w;
@@ -1115,8 +1123,8 @@ int enqueue(const Call& c, char* ws, long tokens, hipStream_t st) {
             T* C = (T*)c.dx + at * c.H;
             d.C = C;
             d.vector = c.H % 8 == 0 && (uintptr_t)C % 16 == 0;
-            d.acc = two || l.dx.splits > 1 ? (float*)(ws + l.dx_acc) : nullptr;
-            Shape s = l.dx;
+            d.acc = two || dx.splits > 1 ? (float*)(ws + l.dx_acc) : nullptr;
+            Shape s = dx;
             s.n_tiles = over(d.N, TILE_N[s.kind]);
             product<T, false, true, OUT>(s, d, st);
             if (d.acc != nullptr) {
@@ -1162,7 +1170,12 @@ long spanqr_linear_cross_entropy_workspace(int type, long N, long H, long V, int
     const int rc = check_sizes(type, N, H, V);
     if (rc != SPANQR_OK) return rc;
     const bool pad = ((grads & 4) || H % 8 != 0) && ((grads & 3) || N > FEW_TOKENS);
-    return layout_of(N, H, V, grads & 3, pad, tokens_of(N, H, V, grads & 3, pad, most_bytes)).bytes;
+    const long tokens = tokens_of(N, H, V, grads & 3, pad, most_bytes);
+    const Layout l = layout_of(N, H, V, grads & 3, pad, tokens);
+    if (!(grads & 1)) return l.bytes;
+    // (what is beyond most_bytes anyway has room for all parts of dx)
+    const Shape dx = dx_of(l, H, V, tokens, N > 256 && l.bytes <= most_bytes ? most_bytes - l.dx_acc : LONG_MAX);
+    return std::max(l.bytes, dx.splits > 1 ? l.dx_acc + 4 * dx.splits * l.rows * l.Hp : 0);
 }
 
 int spanqr_linear_cross_entropy(int type, int reduction, long N, long H, long V, const void* x, long ldx, const void* w,
@@ -1187,8 +1200,8 @@ int spanqr_linear_cross_entropy(int type, int reduction, long N, long H, long V,
     const Call c = {reduction == SPANQR_REDUCE_MEAN, reduced, pad, N, H, V, x, w, ldx, ldw, target, ignore_index,
                     row_weight, grad_scale, loss, lse, dx, dw};
     hipStream_t st = (hipStream_t)stream;
-    return type == SPANQR_BF16 ? enqueue<bf16>(c, (char*)workspace, tokens, st)
-                               : enqueue<fp16>(c, (char*)workspace, tokens, st);
+    return type == SPANQR_BF16 ? enqueue<bf16>(c, (char*)workspace, workspace_bytes, tokens, st)
+                               : enqueue<fp16>(c, (char*)workspace, workspace_bytes, tokens, st);
 }
 
 }  // extern "C"

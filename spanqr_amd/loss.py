@@ -8,7 +8,7 @@ from . import _lib
 from .tensors import TYPES, check_same, check_tensor, no_tangents, on, once, workspace
 
 IGNORE_INDEX = -100
-MAX_WORKSPACE = 4 << 30   # bytes: 16-bit exponentials of 16384 tokens over 128000 columns
+MAX_WORKSPACE = 4 << 30   # bytes: 16-bit exponentials of 15000 tokens over 128000 columns, with their statistics
 MAX_STRIDE = 1 << 22
 REDUCTIONS = {"none": _lib.REDUCE_NONE, "sum": _lib.REDUCE_SUM, "mean": _lib.REDUCE_MEAN}
 

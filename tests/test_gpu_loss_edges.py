@@ -173,3 +173,45 @@ def test_more_tokens_than_a_launch_takes(cuda):
     for at in range(0, N, 1 << 22):
         want, _, far = exact(s[at:at + (1 << 22)], w, t[at:at + (1 << 22)])
         assert bool(((loss[at:at + (1 << 22)].double() - want).abs() <= 4 * E * want + (3 * far + 100) * E).all()), at
+
+
+def abi_call(x, W, t, reduction, ws, grads, lse=None):
+    """the C entry point with a workspace that is given"""
+    from spanqr_amd import _lib
+    N, H, V = x.shape[0], x.shape[1], W.shape[0]
+    loss = torch.full((N if reduction == _lib.REDUCE_NONE else 1,), 7.0, device=x.device)
+    dx, dw = (torch.empty_like(v) if grads & bit else None for v, bit in ((x, 1), (W, 2)))
+    ptr = lambda v: None if v is None else v.data_ptr()   # noqa: E731
+    rc = _lib.lib().spanqr_linear_cross_entropy(
+        _lib.BF16 if x.dtype == torch.bfloat16 else _lib.FP16, reduction, N, H, V, x.data_ptr(), x.stride(0), W.data_ptr(),
+        W.stride(0), t.data_ptr(), -100, None, None, loss.data_ptr(), ptr(lse), ptr(dx), ptr(dw), ws.data_ptr(), ws.numel(),
+        torch.cuda.current_stream().cuda_stream)
+    _lib.check(rc)
+    return loss, dx, dw
+
+
+@pytest.mark.parametrize("grads", [1, 3])
+@pytest.mark.parametrize("N,H,V", [(1000, 136, 5000), (300, 768, 1024), (64, 64, 3000)])
+def test_a_workspace_for_more_tokens(cuda, N, H, V, grads):
+    """what the query gives for N tokens, and the least that it gives, hold fewer tokens; the bytes behind the workspace stay,
+    and dx's parts, which adapt to it, change no more than their sums' order"""
+    from spanqr_amd import _lib
+    g = torch.Generator(device="cuda").manual_seed(36)
+    x = torch.randn(N, H, generator=g, device="cuda").bfloat16()
+    W = (torch.randn(V, H, generator=g, device="cuda") * (2.5 / math.sqrt(H))).bfloat16()
+    t = torch.randint(0, V, (N,), generator=g, device="cuda")
+    for most in (0, 16 << 20, 1 << 32):
+        nbytes = _lib.lib().spanqr_linear_cross_entropy_workspace(_lib.BF16, N, H, V, grads, most)
+        room = torch.full((nbytes + 4096,), 77, dtype=torch.uint8, device=cuda)
+        for n in sorted({1, 2, 17, 32, 33, 64, 65, 255, 256, 257, N - 1, N}):
+            if n > N:
+                continue
+            print(f"linear_cross_entropy {n} of {N}x{H}x{V}, {nbytes} bytes", flush=True)
+            loss, dx, dw = abi_call(x[:n], W, t[:n], _lib.REDUCE_SUM, room[:nbytes], grads)
+            assert bool((room[nbytes:] == 77).all())
+            want = sp.linear_cross_entropy_grad(x[:n], W, t[:n], reduction="sum")
+            for a, b in ((loss[0], want[0]), (dx, want[1]), (dw, want[2])):
+                if a is not None:
+                    a, b = a.double(), b.double()
+                    # (one rounding to bfloat16 of sums that differ in their order)
+                    assert float((a - b).norm()) <= 2.0 ** -8 * float(b.norm()) + 1e-6

@@ -32,3 +32,40 @@ def test_tiles_of_one_launch():
 def test_tokens_are_counted_in_int():
     assert need((1 << 31) - 1, 8, 16, 0) > 0
     assert need(1 << 31, 8, 16, 0) == -1   # SPANQR_EINVAL
+
+
+def p_bytes(N, V):
+    return 2 * N * ((V + 63) // 64 * 64)
+
+
+@pytest.mark.parametrize("N,H,V", [(65536, 5120, 32000), (8192, 5120, 1000), (16384, 5120, 128000), (300, 4096, 1000)])
+def test_only_what_is_used(N, H, V):
+    """beside the exponentials and their statistics (16 bytes for 64 columns at most) nothing of their size that no launch touches"""
+    rest = N * (16 * (V // 64 + 1) + 16) + 4 * 128 * H + 4096
+    whole = need(N, H, V, 3, 1 << 45)
+    assert p_bytes(N, V) <= whole <= p_bytes(N, V) + rest + (4 * 16384 * H if N == 300 else 0)
+
+
+def test_pieces_take_no_more_than_the_whole():
+    """dW over pieces has sums in fp32 that all tokens at once do without"""
+    for N in (257, 300, 500, 900, 4000):
+        for H, V in ((4096, 1000), (1024, 50257), (5120, 512)):
+            for most in (0, 10 << 20, 100 << 20):
+                assert need(N, H, V, 3, most) <= max(most, need(N, H, V, 3, 1 << 45)), (N, H, V, most)
+
+
+@pytest.mark.parametrize("grads", [0, 1, 2, 3])
+def test_what_fits_for_some_fits_for_fewer(grads):
+    """a workspace for N tokens, whole or in pieces, is enough for fewer (all of the workspace but the sums of dx's parts,
+    which adapt to it, is what the least query gives)"""
+    for H, V in ((768, 32000), (64, 100), (5120, 1000), (1000, 50257)):
+        last = 0
+        for N in (1, 2, 16, 17, 31, 32, 33, 63, 64, 65, 100, 256, 257, 512, 1000, 4096, 10000, 40000):
+            least = need(N, H, V, grads, 1 << 45)
+            if not grads & 1:
+                assert least >= last, (H, V, N)
+            last = least
+            for most in (64 << 20, 1 << 30):
+                got = need(N, H, V, grads, most)
+                # the same call again, with what the query gave as its bound, needs no more
+                assert need(N, H, V, grads, got) <= got, (H, V, N, most)
