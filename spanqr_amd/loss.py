@@ -40,15 +40,13 @@ def _check(what, x, weight, target, reduction, row_weight, grad_scale=None):
         check_same(what, "row_weight", row_weight, x.device, (x.shape[0],))
 
 
-def _run(x, weight, target, reduction, ignore_index, row_weight, grad_scale, need_dx, need_dw, max_workspace,
-         need_lse=False):
+def _run(x, weight, target, reduction, ignore_index, row_weight, grad_scale, need_dx, need_dw, max_workspace):
     x, weight = _rows(x.detach()), _rows(weight.detach())
     (N, H), V, dev = x.shape, weight.shape[0], x.device
     target = target.to(torch.int64).contiguous()
     if row_weight is not None:
         row_weight = row_weight.contiguous()
     loss = torch.empty((N,) if reduction == "none" else (), dtype=torch.float32, device=dev)
-    lse = torch.empty(N, dtype=torch.float32, device=dev) if need_lse else None
     dx = torch.empty(N, H, dtype=x.dtype, device=dev) if need_dx else None
     dw = torch.empty(V, H, dtype=x.dtype, device=dev) if need_dw else None
     t, grads = TYPES[x.dtype], int(need_dx) + 2 * int(need_dw)
@@ -62,15 +60,15 @@ def _run(x, weight, target, reduction, ignore_index, row_weight, grad_scale, nee
         _lib.check(_lib.lib().spanqr_linear_cross_entropy(
             t, REDUCTIONS[reduction], N, H, V, x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0),
             target.data_ptr(), int(ignore_index), None if row_weight is None else row_weight.data_ptr(),
-            None if grad_scale is None else grad_scale.data_ptr(), loss.data_ptr(), None if lse is None else lse.data_ptr(),
+            None if grad_scale is None else grad_scale.data_ptr(), loss.data_ptr(), None,
             None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(), ws.data_ptr(), nbytes, stream))
-    return loss, lse, dx, dw
+    return loss, dx, dw
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, reduction, ignore_index, max_workspace):
-        loss, _, _, _ = _run(x, weight, target, reduction, ignore_index, None, None, False, False, max_workspace)
+        loss, _, _ = _run(x, weight, target, reduction, ignore_index, None, None, False, False, max_workspace)
         ctx.save_for_backward(x, weight, target)
         ctx.how = reduction, ignore_index, max_workspace
         return loss
@@ -80,9 +78,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         x, weight, target = ctx.saved_tensors
         reduction, ignore_index, max_workspace = ctx.how
         f = g.detach().to(torch.float32)
-        _, _, dx, dw = _run(x, weight, target, reduction, ignore_index, f.contiguous() if reduction == "none" else None,
-                            None if reduction == "none" else f, ctx.needs_input_grad[0], ctx.needs_input_grad[1],
-                            max_workspace)
+        _, dx, dw = _run(x, weight, target, reduction, ignore_index, f.contiguous() if reduction == "none" else None,
+                         None if reduction == "none" else f, ctx.needs_input_grad[0], ctx.needs_input_grad[1],
+                         max_workspace)
         dx, dw = (once("linear_cross_entropy", d, x, weight, g) for d in (dx, dw))
         return dx, dw, None, None, None, None
 
@@ -117,6 +115,4 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
         check_same("linear_cross_entropy_grad", "grad_scale", grad_scale, x.device)
         if grad_scale.numel() != 1:
             raise ValueError("linear_cross_entropy_grad: grad_scale must have one element")
-    loss, _, dx, dw = _run(x, weight, target, reduction, ignore_index, row_weight, grad_scale, need_dx, need_dw,
-                           max_workspace)
-    return loss, dx, dw
+    return _run(x, weight, target, reduction, ignore_index, row_weight, grad_scale, need_dx, need_dw, max_workspace)

@@ -215,3 +215,30 @@ def test_a_workspace_for_more_tokens(cuda, N, H, V, grads):
                     a, b = a.double(), b.double()
                     # (one rounding to bfloat16 of sums that differ in their order)
                     assert float((a - b).norm()) <= 2.0 ** -8 * float(b.norm()) + 1e-6
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,H,V", SIZES)
+def test_log_of_the_sum_of_exponentials(cuda, N, H, V, dtype):
+    """the C entry point's lse: of every token, whatever its target, with and without gradients, in pieces of the tokens"""
+    from spanqr_amd import _lib
+    print(f"linear_cross_entropy {N}x{H}x{V} {dtype}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(37)
+    w = (4.0 * torch.randn(V, generator=g, device="cuda")).to(dtype)
+    w[1::5] = -math.inf
+    s = (0.5 + torch.rand(N, generator=g, device="cuda")).to(dtype)
+    z = s.double()[:, None] * w.double()[None]
+    want = torch.logsumexp(z, 1)
+    far = torch.where(z > -math.inf, z.amax(1, keepdim=True) - z, torch.zeros_like(z)).amax(1)
+    tol = 4 * E * want.abs() + 4 * E * z.amax(1).abs() + (3 * far + 100) * E
+    x, W = place(s, H), place(w, H)
+    best = z.argmax(1)
+    for t in (best, torch.full_like(best, -100), torch.full_like(best, V + 3),
+              torch.where(torch.arange(N, device=cuda) % 2 == 0, best, torch.full_like(best, -100)),
+              torch.ones_like(best) if V > 1 else best):       # (column 1 is out)
+        for grads in (0, 2):
+            nbytes = _lib.lib().spanqr_linear_cross_entropy_workspace(_lib.BF16, N, H, V, grads, 0)
+            lse = torch.full((N + 8,), 7.0, device=cuda)
+            abi_call(x, W, t, _lib.REDUCE_MEAN, torch.empty(nbytes, dtype=torch.uint8, device=cuda), grads, lse)
+            assert bool((lse[N:] == 7.0).all())
+            assert bool(((lse[:N].double() - want).abs() <= tol).all()), float(((lse[:N].double() - want).abs() / tol).max())
