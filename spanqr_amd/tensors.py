@@ -81,7 +81,7 @@ def once(what, grad, *formed_from):
 
 # the current stream's handle by the device's index: what torch.cuda.current_stream(device).cuda_stream gives, without
 # the stream object around it (0.1 us instead of 1.9)
-_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 @contextlib.contextmanager
