@@ -111,6 +111,8 @@ def rms_norm_backward(dy, h, weight=None, eps=1e-6, dh=None, need_dw=True):
         if need_dw:
             dw = torch.empty_like(weight)
             nbytes = _lib.lib().spanqr_rms_norm_backward_workspace(h2.shape[0], D)
+            if nbytes < 0:
+                _lib.check(nbytes)
     t = TYPES[h.dtype]
     with on(dev) as stream:
         if nbytes:
