@@ -333,7 +333,7 @@ int spanqr_grad_norm(int n, const void* const* grads, const long* numel, const i
 
 /* The same, and out[i] = grads[i] min(1, max_norm / norm), of type out_type[i], element for element in memory order;
  * out[i] may be grads[i] itself (in place, and then nothing is written where the norm is within max_norm), but not
- * overlap it otherwise. A NaN norm makes every element NaN; an infinite one makes finite elements 0. */
+ * overlap it otherwise, nor another out. A NaN gradient makes every element NaN; an infinite one the finite elements 0. */
 int spanqr_clip_grad_norm(int n, const void* const* grads, const long* numel, const int* type, void* const* out,
                           const int* out_type, float max_norm, float* norm, void* workspace, long workspace_bytes,
                           void* stream);
@@ -346,7 +346,8 @@ int spanqr_clip_grad_norm(int n, const void* const* grads, const long* numel, co
  * `type`, each or null: the gradients of the sum (none, sum) or of the mean, times *grad_scale (device, or null for 1).
  * workspace: what spanqr_linear_cross_entropy_workspace gives for `grads` (1: dx, 2: dw, 3: both, 0: neither;
  * plus 4 where rows of x or w do not all start on 16 bytes: they are copied into rows that do) and most_bytes, which
- * bounds it: the tokens go through in pieces whose 16-bit exponentials fit (256 tokens at least). H and V up to 2^22, N below 2^31. */
+ * bounds it: the tokens go through in pieces whose 16-bit exponentials fit (256 tokens at least). What holds a number of
+ * tokens holds fewer; more than what is needed lets dx have more parts. H and V up to 2^22, N below 2^31. */
 long spanqr_linear_cross_entropy_workspace(int type, long N, long H, long V, int grads, long most_bytes);
 int spanqr_linear_cross_entropy(int type, int reduction, long N, long H, long V, const void* x, long ldx, const void* w,
                                 long ldw, const long* target, long ignore_index, const float* row_weight,

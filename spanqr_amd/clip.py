@@ -113,8 +113,8 @@ def clip_grad_norm(grads, max_norm, out=None):
     pass, for an optimizer that works in float32. In place a norm within max_norm writes nothing.
 
     Each tensor to write to is listed once (a shared parameter's gradient, too): two that start at the same address raise
-    ValueError. out may share no memory with the gradients, other than out[i] being grads[i]. A NaN norm makes every
-    result NaN, an infinite norm makes finite gradients 0: look at the norm before the step. Neither the norm nor what is
+    ValueError. out may share no memory with the gradients, other than out[i] being grads[i]. A NaN gradient makes
+    every result NaN, an infinite one makes the finite ones 0: look at the norm before the step. Neither the norm nor what is
     written carries a gradient."""
     grads, dev, types = _tensors("clip_grad_norm", "every gradient", grads)
     max_norm = float(max_norm)

@@ -11,8 +11,9 @@
 // also where the token is sure (next to the target's 1 a sum would lose R). One pass over p turns it into G (times
 // exp(m - lse); the target's element from the loss), and G goes into the other two products. So nothing is multiplied
 // twice, and what is held is 16 bits an element for as many tokens at a time as the workspace takes. The gradients' error
-// is then that of G's elements, rounded twice, and of one rounding at the end: 1.3 times the error of a result that is
-// rounded at the end alone (1.0 times for up to 32 tokens, whose p and G keep what is rounded off).
+// is then that of G's elements, rounded twice, and of one rounding at the end: 1.0 to 1.3 times the error of a result that
+// is rounded at the end alone where many elements add up, up to 1.7 (three roundings) where one makes a gradient; 1.0
+// times for up to 32 tokens, whose p and G keep what is rounded off. A G in fp32 would take the products' rate.
 #include <limits.h>
 #include <math.h>
 

@@ -106,7 +106,11 @@ def linear_cross_entropy_grad(x, weight, target, reduction="mean", ignore_index=
     """(loss, dx, dw): linear_cross_entropy and its gradients in one pass, in x's type. row_weight [N] float32 multiplies
     each token's loss (not the count that the mean is over). grad_scale (a number, or a float32 tensor of one element on
     the device: a loss scale) multiplies the gradients before they are rounded, not the loss. With reduction "none" the
-    gradients are of the sum. dx or dw is None with need_dx=False or need_dw=False. None of them carries a gradient."""
+    gradients are of the sum. dx or dw is None with need_dx=False or need_dw=False. None of them carries a gradient.
+
+    Sums are float32. Above 32 tokens each element of softmax - onehot is rounded to x's type twice on its way into the
+    gradients: their error is 1.0 to 1.3 times that of a float32 result that is rounded once, 1.7 times at most. x of ignored
+    tokens has to be finite for dw, where it is multiplied by 0."""
     _check("linear_cross_entropy_grad", x, weight, target, reduction, row_weight, grad_scale)
     if grad_scale is not None:
         if not isinstance(grad_scale, torch.Tensor):
