@@ -284,7 +284,7 @@ int spanqr_chol64(spanqr_chol64_plan* plan, const double* G, long ldg, const dou
                   float* Lf, float* Lif, void* stream);
 int spanqr_chol64_status(spanqr_chol64_plan* plan, void* stream);
 
-/* ---- training operators beside orth: the loss over the vocabulary, root-mean-square norm, clipping ----
+/* ---- training operators beside orth: loss over the vocabulary, norms, clipping, dropout, attention ----
  * No counterpart in the reference, whose caller's training step forms the gradients that its optimizer turns into X
  * (README.md:19-30). Conventions: matrices are row-major in device memory with row strides in elements and neighbouring
  * elements in a row; element alignment is enough. Types are SPANQR_BF16, SPANQR_FP16 and SPANQR_FP32. Calls enqueue on
@@ -305,6 +305,11 @@ enum {
     SPANQR_REDUCE_NONE = 0,
     SPANQR_REDUCE_SUM = 1,
     SPANQR_REDUCE_MEAN = 2,      /* over the tokens that are not ignored (0 if there are none) */
+};
+enum {                           /* act(g) of a gate */
+    SPANQR_GATE_LINEAR = 0,      /* g */
+    SPANQR_GATE_SIGMOID = 1,     /* 1 / (1 + exp(-g)) */
+    SPANQR_GATE_SILU = 2,        /* g / (1 + exp(-g)) */
 };
 
 /* y = norm(h) weight for each of `rows` rows of D elements (1 to 2^24): h = x, or with `residual` h = x + residual,
@@ -353,6 +358,35 @@ int spanqr_linear_cross_entropy(int type, int reduction, long N, long H, long V,
                                 long ldw, const long* target, long ignore_index, const float* row_weight,
                                 const float* grad_scale, float* loss, float* lse, void* dx, void* dw, void* workspace,
                                 long workspace_bytes, void* stream);
+
+/* Dropout of x [rows, D] into y, contiguous: element (row, column) is 0 where its 16-bit number is below P = round(65536 p)
+ * (to nearest even; p from 0 to 1 - 2^-16), and x 65536 / (65536 - P) elsewhere. The number is half (column % 2) (low half
+ * first) of word (column % 8) / 2 of Philox-4x32-10 with counter (column / 8, row mod 2^32, row / 2^32, index) and key (low,
+ * high word of the seed): the same call on the gradient is the backward pass, and nothing else is kept. The seed is
+ * *seed_at (device, 64 bits, read when the kernel runs) or, with null, `seed`. D up to 2^32. */
+int spanqr_dropout(int type, long rows, long D, const void* x, long ldx, double p, unsigned long seed, const void* seed_at,
+                   unsigned index, void* y, void* stream);
+
+/* Between two blocks: t = norm(x) post_weight act(gate), h = residual + a dropout(t), rounded to the type, y = norm(h) weight,
+ * y normed as h is rounded. x, residual, gate (or null: act(gate) = 1), h and y are [rows, D] (h and y contiguous);
+ * post_weight and weight [D] of type wtype, each or null for 1; a is *scale_at (device) or, with null, `scale`; norm and
+ * dropout as above, p = 0 drops nothing. D up to 2^24. */
+int spanqr_block_norm(int type, int wtype, int act, long rows, long D, const void* x, long ldx, const void* residual, long ldr,
+                      const void* gate, long ldg, const void* post_weight, const void* weight, float eps, float scale,
+                      const float* scale_at, double p, unsigned long seed, const void* seed_at, unsigned index, void* h,
+                      void* y, void* stream);
+
+/* Gradient of it from dy and dh (the gradient that reaches h on the stream's own way; each or null for 0), x, h and gate:
+ * dx, dresidual, and dgate where there is a gate, contiguous; dpost_weight and dweight [D] of type wtype and dscale (one
+ * fp32, that of a), each or null. These three are also written for rows = 0 (zeros). workspace:
+ * spanqr_block_norm_backward_workspace(rows, D) bytes, needed where one of the three is wanted. */
+long spanqr_block_norm_backward_workspace(long rows, long D);
+int spanqr_block_norm_backward(int type, int wtype, int act, long rows, long D, const void* dy, long lddy, const void* dh,
+                               long lddh, const void* x, long ldx, const void* h, long ldh, const void* gate, long ldg,
+                               const void* post_weight, const void* weight, float eps, float scale, const float* scale_at,
+                               double p, unsigned long seed, const void* seed_at, unsigned index, void* dx, void* dresidual,
+                               void* dgate, void* dpost_weight, void* dweight, float* dscale, void* workspace,
+                               long workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

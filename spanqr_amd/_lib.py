@@ -11,7 +11,7 @@ import tempfile
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libspanqr.so")
 # orth's path, and the training operators beside it
-SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("spanqr.hip", "loss.hip", "norm.hip", "clip.hip")]
+SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("spanqr.hip", "loss.hip", "norm.hip", "clip.hip", "block.hip")]
 INCLUDE = os.path.join(os.path.dirname(_HERE), "include", "spanqr.h")
 
 # hipcc flags: gfx950 only; packed fp32 VALU ops disabled (the kernels never rely on them); no fast-math so every
@@ -28,13 +28,15 @@ MAX_R = 4096     # SPANQR_MAX_R
 (K_AMAX, K_GRAM_PASS1, K_GRAM, K_REDUCE, K_CHOL, K_TRSM_PASS1, K_TRSM, K_NS_APPLY, K_CHOL_SOLVE_PASS1,
  K_CHOL_SOLVE) = range(10)
 
-# types, 8-bit forms and reductions of the training operators
+# types, 8-bit forms, reductions and gates of the training operators
 FP32, BF16, FP16 = range(3)
 QUANT_NONE, QUANT_FP8, QUANT_INT8 = range(3)
 REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = range(3)
+GATE_LINEAR, GATE_SIGMOID, GATE_SILU = range(3)
 
 # every exported symbol of include/spanqr.h: (restype, argtypes)
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
+_D, _U, _UL = ctypes.c_double, ctypes.c_uint, ctypes.c_ulong
 SIGNATURES = {
     "spanqr_plan_create": (_I, [_I, _I, _I, ctypes.POINTER(ctypes.c_void_p)]),
     "spanqr_plan_create_batched": (_I, [_I, _I, _I, _I, ctypes.POINTER(ctypes.c_void_p)]),
@@ -76,6 +78,11 @@ SIGNATURES = {
     "spanqr_linear_cross_entropy_workspace": (_L, [_I, _L, _L, _L, _I, _L]),
     "spanqr_linear_cross_entropy": (_I, [_I, _I, _L, _L, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _L,
                                          _P]),
+    "spanqr_dropout": (_I, [_I, _L, _L, _P, _L, _D, _UL, _P, _U, _P, _P]),
+    "spanqr_block_norm": (_I, [_I, _I, _I, _L, _L, _P, _L, _P, _L, _P, _L, _P, _P, _F, _F, _P, _D, _UL, _P, _U, _P, _P, _P]),
+    "spanqr_block_norm_backward_workspace": (_L, [_L, _L]),
+    "spanqr_block_norm_backward": (_I, [_I, _I, _I, _L, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _F, _F, _P, _D,
+                                        _UL, _P, _U, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
 }
 
 _lib = None

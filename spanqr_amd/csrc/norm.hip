@@ -11,8 +11,8 @@
 // All sums are fp32 per thread over at most 32 elements, then a tree in a fixed order.
 // 16384 x 2048 bf16 with the residual: forward 52 us (5.2 TB/s), gradient 49 and 5 for dw's parts (5.0 TB/s; part of both
 // from the memory-side cache); 4096 x 5120 to 8 bits 30 us (4.9 TB/s), a copy's rate; one token of 5120 4 us.
-#include "elements.h"
 #include "host.h"
+#include "rows.h"
 
 using namespace spanqr_dev;
 using spanqr_host::error;
@@ -38,23 +38,6 @@ struct GradArgs {
     void* dx;
     float* part;                         // [gridDim.x, D] sums of dy n over the block's rows, or null
 };
-
-// eight weights as fp32; 1 without weights
-__device__ __forceinline__ void load_weight(const void* w, int type, long at, int n, float (&f)[8]) {
-    if (w == nullptr) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = 1.0f;
-    } else if (type == SPANQR_BF16) {
-        load8((const bf16*)w + at, n, f);
-    } else if (type == SPANQR_FP16) {
-        load8((const fp16*)w + at, n, f);
-    } else {
-        load8((const float*)w + at, n, f);
-    }
-}
-
-// elements of the piece at `at` that are inside the row (0 to 8)
-__device__ __forceinline__ int inside(long D, long at) { return D - at >= 8 ? 8 : D > at ? (int)(D - at) : 0; }
 
 __device__ __forceinline__ float quant_max(int quant) { return quant == SPANQR_QUANT_FP8 ? 448.0f : 127.0f; }
 
@@ -88,56 +71,6 @@ __device__ __forceinline__ void store_quant(int quant, uint8_t* q, int n, const 
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i < n) q[i] = (uint8_t)((i < 4 ? lo : hi) >> 8 * (i & 3));
-    }
-}
-
-// Threads of a row: GROUP lanes of a wavefront (16 or 64; then a workgroup of 256 threads has several rows), or with GROUP
-// 0 the whole workgroup, of any number of wavefronts.
-template <int GROUP>
-struct Group {
-    static constexpr int MOST = GROUP ? 256 : 1024;
-    __device__ __forceinline__ static int size() { return GROUP ? GROUP : (int)blockDim.x; }
-    __device__ __forceinline__ static int rows() { return GROUP ? 256 / GROUP : 1; }
-    __device__ __forceinline__ static int lane() { return GROUP ? threadIdx.x % GROUP : threadIdx.x; }
-    __device__ __forceinline__ static int index() { return GROUP ? threadIdx.x / GROUP : 0; }
-    // N values over the group's threads. One barrier: `slot` ([N][16]) may be used again only behind another one.
-    template <typename OP, int N>
-    __device__ __forceinline__ static void reduce(float (&v)[N], float (*slot)[16]) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = reduce_lanes<GROUP ? GROUP : 64, OP>(v[i]);
-        if constexpr (GROUP == 0) {
-            const int waves = blockDim.x >> 6;
-            if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) slot[i][threadIdx.x >> 6] = v[i];
-            }
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = slot[i][0];
-            for (int w = 1; w < waves; ++w) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) v[i] = OP::of(v[i], slot[i][w]);
-            }
-        }
-    }
-};
-
-// piece `at` of a row; WHOLE: the row has 8 elements at least (shorter ones are read one by one)
-template <bool WHOLE, typename T>
-__device__ __forceinline__ Pack8<T> piece(const T* row, long D, long at, int n) {
-    if constexpr (WHOLE) return fetch8(row, D, at);
-    Pack8<T> k;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) k.v[i] = i < n ? row[at + i] : (T)0.0f;
-    return k;
-}
-template <bool WHOLE, typename T>
-__device__ __forceinline__ void settle(const Pack8<T>& k, int n, float (&f)[8]) {
-    if constexpr (WHOLE) {
-        settle8(k, n, f);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = (float)k.v[i];
     }
 }
 
@@ -495,23 +428,12 @@ constexpr long MAX_D = 1l << 24;
 // Threads of a row and pieces a thread. Measured, forward / backward in us: 16384 x 2048 bf16 as 256 threads of one
 // piece 51 / 50, as 128 of two 53 / 53, as a wavefront of four 60 / 55; 4096 x 5120 with 8 bits as 640 of one 40, as 320
 // of two 31, as 192 of four 35. One token of 5120 as 640 of one 3.8, as 256 of four 6.7.
-struct Split {
-    int group, nch;   // group 16 or 64: lanes of a wavefront; else (64 and `block`) a workgroup
-    bool block;
-};
 Split split_of(long rows, long D) {
     const long pieces = (D + 7) / 8;
     if (D <= 128) return {16, 1, false};
     if (D <= 512) return {64, 1, false};
     const int nch = D <= 2048 || (rows <= 512 && D <= 8192) ? 1 : D <= 16384 ? 2 : 4;
     return {(int)(((pieces + nch - 1) / nch + 63) / 64 * 64), nch, true};
-}
-
-// workgroups for `rows` rows, each of about as many rows as the others, `most` at most
-int grid_of(long rows, const Split& s, int most) {
-    const int per = s.block ? 1 : 256 / s.group;
-    const long need = (rows + per - 1) / per, turns = (need + most - 1) / most;
-    return turns < 1 ? 0 : (int)((need + turns - 1) / turns);
 }
 
 // The gradient's workgroups, and so rows of partial sums: as many as the compute units hold at once, since each of them ends
