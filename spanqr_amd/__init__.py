@@ -5,9 +5,10 @@
 
 The hot path is hand-written HIP in csrc/spanqr.hip behind the C ABI of include/spanqr.h, loaded with ctypes. Beside it
 stand the operators of the training step that calls orth: the loss over the vocabulary (csrc/loss.hip), the
-root-mean-square norm (csrc/norm.hip), clipping by the global norm (csrc/clip.hip), and the norms around a block with gate
-and dropout (csrc/block.hip).
+root-mean-square norm (csrc/norm.hip), clipping by the global norm (csrc/clip.hip), the norms around a block with gate
+and dropout (csrc/block.hip), and attention (csrc/attention.hip).
 """
+from .attention import attention, attention_backward  # noqa: F401
 from .block import block_norm, block_norm_backward, dropout  # noqa: F401
 from .clip import clip_grad_norm, grad_norm  # noqa: F401
 from .kcholqr import borth, kcholqr_f, kcholqr_f_many, orth, orth_many, set_checked, status  # noqa: F401
@@ -17,4 +18,5 @@ from .plan import clear_plans, get_plan  # noqa: F401
 
 __all__ = ["orth", "orth_many", "kcholqr_f", "kcholqr_f_many", "borth", "get_plan", "clear_plans", "set_checked",
            "status", "linear_cross_entropy", "linear_cross_entropy_grad", "rms_norm", "rms_norm_backward", "grad_norm",
-           "clip_grad_norm", "block_norm", "block_norm_backward", "dropout"]
+           "clip_grad_norm", "block_norm", "block_norm_backward", "dropout",
+           "attention", "attention_backward"]

@@ -11,7 +11,7 @@ import tempfile
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libspanqr.so")
 # orth's path, and the training operators beside it
-SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("spanqr.hip", "loss.hip", "norm.hip", "clip.hip", "block.hip")]
+SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("spanqr.hip", "loss.hip", "norm.hip", "clip.hip", "block.hip", "attention.hip")]
 INCLUDE = os.path.join(os.path.dirname(_HERE), "include", "spanqr.h")
 
 # hipcc flags: gfx950 only; packed fp32 VALU ops disabled (the kernels never rely on them); no fast-math so every
@@ -83,6 +83,12 @@ SIGNATURES = {
     "spanqr_block_norm_backward_workspace": (_L, [_L, _L]),
     "spanqr_block_norm_backward": (_I, [_I, _I, _I, _L, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _F, _F, _P, _D,
                                         _UL, _P, _U, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
+    "spanqr_attention_workspace": (_L, [_L, _L, _L, _L, _L, _L, _I, _L, _L]),
+    "spanqr_attention": (_I, [_I, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _L, _L, _I, _L, _F, _P, _P, _P, _L,
+                              _P]),
+    "spanqr_attention_backward_workspace": (_L, [_L, _L, _L, _L, _L, _L, _I]),
+    "spanqr_attention_backward": (_I, [_I, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _L,
+                                       _I, _L, _F, _P, _P, _P, _P, _L, _P]),
 }
 
 _lib = None

@@ -1,0 +1,866 @@
+// attention.hip -- softmax attention with heads that share keys and values, for padded batches and packed sequences, and its
+// gradient, which makes the probabilities again.
+//
+//   S = c Q K^T,  lse_i = log sum_j exp S_ij,  P_ij = exp(S_ij - lse_i),  O = P V
+//   D_i = sum_d dO_id O_id,  dP = dO V^T,  dS = P (dP - D),  dV = P^T dO,  dK = c dS^T Q,  dQ = c dS K
+//   query i of a sequence stands at p = i + Lk - Lq; causal: j <= p, with a window w also j > p - w; a query that sees no key
+//   has O = 0, lse = -inf and no gradient
+//
+// A group of G heads shares a key head; its queries are taken as Lq G rows (row m is query m / G of head m % G), so that
+// what is read of K and V serves the whole group, one token of a group fills a tile, and the gradient of shared heads is a sum
+// over rows like any other: no atomics, the same bits in every call.
+//
+// All products are of 32 x 32 x 16 matrix instructions, arranged so that what one leaves in registers is what the next one
+// takes: a lane of S^T (K's rows against Q's) has 16 keys of one query, which are the softmax's to reduce (one lane swap joins
+// the two halves) and, rounded to 16 bits, the second operand of O^T = V^T P^T, the sum over keys going in the order in
+// which they lie in the registers. V^T comes from LDS by the transposing read in that order. The gradient of K and V
+// holds its keys by lanes and streams Q and dO; that of Q holds queries and streams K and V. P is rounded to 16 bits before
+// the product with V or dO, and dS before those with K and Q; all sums are fp32.
+#include <limits.h>
+#include <math.h>
+
+#include "elements.h"
+#include "host.h"
+
+using namespace spanqr_dev;
+using spanqr_host::error;
+using spanqr_host::launched;
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 fp16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
+constexpr int TILE = 64;     // rows of a tile in LDS
+constexpr int WAVES = 4;
+constexpr int BLOCK = 32 * WAVES;   // rows that a workgroup holds, a wavefront 32
+
+template <typename T>
+struct Vec;
+template <>
+struct Vec<bf16> {
+    typedef bf16x8 x8;
+};
+template <>
+struct Vec<fp16> {
+    typedef fp16x8 x8;
+};
+
+// c + a b, 32 x 32 x 16: lane l has row l % 32 of a and column l % 32 of b, k = 8 (l / 32) + 0..7 of both, and of c the column
+// l % 32, register i being row 8 (i / 4) + 4 (l / 32) + i % 4
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma(fp16x8 a, fp16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// registers 8 s to 8 s + 7 in 16 bits
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::x8 half_of(const f32x16& v, int s) {
+    typename Vec<T>::x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (T)v[8 * s + i];
+    return r;
+}
+
+// of the lane with the same l % 32 in the other half, and this one's
+template <typename OP>
+__device__ __forceinline__ float both_halves(float v, OP op) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = r[0], b = r[1];   // (a bit_cast of a vector's element takes the first one)
+    return op(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
+// One of q, k, v, out, dout: elements between batches, rows and heads; 16-byte alignment, neighbouring elements of a head.
+struct Heads {
+    const void* p;
+    long batch, row, head;
+};
+
+struct Shape {
+    int B, Hk, G, D;              // sequences, key heads, heads a key head, elements a head
+    long Tq, Tk;                  // rows of all sequences; of each one where nothing is packed
+    const int *q_starts, *k_starts;   // packed: B + 1 each, ascending; or null
+    int causal, window;           // window 0: none
+    float scale2;                 // c log2 e
+};
+
+// where a sequence's rows lie: the first one among all, and how many
+struct Seq {
+    long q0, k0;
+    int lq, lk;
+};
+__device__ __forceinline__ void span(const int* starts, int b, long T, long& at, int& n) {
+    const long a = starts[b] < 0 ? 0 : starts[b] > T ? T : starts[b];
+    const long e = starts[b + 1] < a ? a : starts[b + 1] > T ? T : starts[b + 1];
+    at = a;
+    n = (int)(e - a);
+}
+__device__ __forceinline__ Seq seq_of(const Shape& s, int b) {
+    Seq r;
+    if (s.q_starts != nullptr) {
+        span(s.q_starts, b, s.Tq, r.q0, r.lq);
+        span(s.k_starts, b, s.Tk, r.k0, r.lk);
+    } else {
+        r = {b * s.Tq, b * s.Tk, (int)s.Tq, (int)s.Tk};
+    }
+    return r;
+}
+// the first row of a sequence and a head
+template <typename T>
+__device__ __forceinline__ const char* head_of(const Heads& h, bool packed, int b, long row0, int head) {
+    return (const char*)h.p + (long)sizeof(T) * ((packed ? row0 * h.row : b * h.batch) + head * h.head);
+}
+
+// what a load reads outside a matrix: elements past D, rows past the end
+__device__ const uint32_t __attribute__((aligned(16))) nothing[4] = {0, 0, 0, 0};
+__device__ const float no_row[2] = {INFINITY, 0.0f};   // lse and D of a row past the end
+
+// 16 bytes (4) a lane to LDS at `lds` + 16 lane (4 lane), asynchronously: counted by vmcnt, which `arrived` waits for
+__device__ __forceinline__ void load_lds(const char* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds(const void* at, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "memory");
+}
+__device__ __forceinline__ void load_lds4(const void* at, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(at) : "memory");
+}
+// this wavefront's loads are there and its reads are done; then everybody's
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Tiles of 64 rows of DP elements in LDS (DP: D rounded up to 64 or 128, zeros behind D) and the way there and into
+// registers. The 16-byte chunk c of a row lies at c ^ swizzle(row): LDS serves lanes 0-3, 12-15, 20-27 of each 32 together and
+// then the others, 256 bytes at a time, and for reads of rows (16 rows, the same chunk) as for transposing reads (4 rows,
+// 64 bytes of each) those fill the 256 bytes exactly.
+template <int DP>
+__device__ __forceinline__ int swizzle(int row) {
+    return DP == 128 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3);
+}
+
+template <typename T, int DP>
+struct Reader {
+    typedef typename Vec<T>::x8 x8;
+    static constexpr int ROW = 2 * DP;            // bytes
+    static constexpr int BYTES = TILE * ROW;
+    uint32_t rows, cols[2];
+    __device__ __forceinline__ explicit Reader(int lane) {
+        const int r = lane & 31, h = lane >> 5, lo = lane & 15, g = lane >> 4 & 1;
+        rows = r * ROW + ((swizzle<DP>(r) ^ h) << 4);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int k = 8 * j + 4 * h + (lo >> 2);
+            cols[j] = k * ROW + (((2 * g + (lo >> 1 & 1)) ^ swizzle<DP>(k)) << 4) + 8 * (lo & 1);
+        }
+    }
+    // rows 32 t + lane % 32, elements 16 ks + 8 (lane / 32) + 0..7
+    __device__ __forceinline__ x8 row(uint32_t tile, int t, int ks) const {
+        return *(__attribute__((address_space(3))) const x8*)(uintptr_t)(tile + (rows ^ 32 * ks) + t * 32 * ROW);
+    }
+    // element 32 dt + lane % 32 of the rows 16 s + 4 (lane / 32) + 0..3 and those + 8: the order of a result's registers
+    __device__ __forceinline__ x8 col(uint32_t tile, int s, int dt) const {
+        typedef __attribute__((address_space(3))) s16x4 lds_s4;
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(tile + (cols[0] ^ 64 * dt) + s * 16 * ROW));
+        const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(tile + (cols[1] ^ 64 * dt) + s * 16 * ROW));
+        return __builtin_bit_cast(x8, __builtin_shufflevector(v, w, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
+
+// Loads of tiles of 64 rows m of one sequence and key head, m / G being the row in memory and m % G the head. Where G divides
+// 64 a lane's places in a tile are the same in every tile, and a tile inside the matrix is loaded from a base that
+// moves; otherwise, at the end and where D < DP every lane finds its own.
+template <typename T, int DP>
+struct Loader {
+    static constexpr int CHUNKS = DP / 8, LOADS = TILE * CHUNKS / 64 / WAVES;
+    const char* base;
+    long row, head;       // bytes
+    int G, D;
+    bool even;
+    uint32_t off[LOADS];
+    int at[LOADS];        // row and chunk of a load: 16 row + chunk
+    __device__ __forceinline__ Loader(const char* base, const Heads& h, int G, int D, int wave, int lane)
+        : base(base), row((long)sizeof(T) * h.row), head((long)sizeof(T) * h.head), G(G), D(D), even(D == DP && TILE % G == 0) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int slot = (wave * LOADS + i) * 64 + lane, r = slot / CHUNKS, c = slot % CHUNKS ^ swizzle<DP>(r);
+            at[i] = 16 * r + c;
+            off[i] = (uint32_t)(r / G) * (uint32_t)row + (uint32_t)(r % G) * (uint32_t)head + 16 * c;
+        }
+    }
+    // rows m0 (a multiple of 64) to m0 + 63 of M into the tile at lds
+    __device__ __forceinline__ void load(int m0, int M, uint32_t lds, int wave) const {
+        const uint32_t to = lds + wave * LOADS * 1024;
+        if (even && m0 + TILE <= M) {
+            const char* from = base + (m0 / G) * row;
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) load_lds(from, off[i], to + i * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int m = m0 + (at[i] >> 4), c = at[i] & 15, q = m / G;
+                const void* from = m < M && 8 * c < D ? (const void*)(base + q * row + (m - q * G) * head + 16 * c) : (const void*)nothing;
+                load_lds(from, to + i * 1024);
+            }
+        }
+    }
+};
+
+// the second operand straight from memory: a lane's row at p (or nothing)
+template <typename T, int DP>
+__device__ __forceinline__ void load_row(const char* p, bool on, int D, int lane, typename Vec<T>::x8 (&f)[DP / 16]) {
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+        const int d = 16 * ks + 8 * (lane >> 5);
+        const char* from = on && d < D ? p + sizeof(T) * d : (const char*)nothing;
+        f[ks] = *(const typename Vec<T>::x8*)from;
+    }
+}
+
+// a result's column (a row of D elements in memory at p) times f, 16 bytes a lane
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(T* p, bool on, int D, int lane, const f32x16 (&c)[DP / 32], float f) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    typedef T x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+            x4 v, w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = (T)(c[dt][4 * q + i] * f);
+                w[i] = (T)(c[dt][4 * q + 4 + i] * f);
+            }
+            const u32x2 a = __builtin_bit_cast(u32x2, v), b = __builtin_bit_cast(u32x2, w);
+            // the lower half of the lanes gets both halves' elements 8 q + 0..7, the upper one 8 q + 8..15
+            const auto lo = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+            const auto hi = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+            const int d = 32 * dt + 8 * q + 8 * (lane >> 5);
+            const u32x4 out = {lo[0], hi[0], lo[1], hi[1]};
+            if (on && d < D) *(u32x4*)(p + d) = out;
+        }
+}
+
+// Zeros in rows [0, from) and [to, T) of `width` elements (a multiple of 8), by workgroups `me` of `all`; rest (or null): -inf
+// for each of the `per` heads of such a row
+template <typename T>
+__device__ void outside(T* p, float* rest, long from, long to, long rows, long width, int per, long me, long all) {
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const long t = me * 256 + threadIdx.x, step = all * 256;
+    for (long i = t; i < from * width / 8; i += step) ((uint4*)p)[i] = zero;
+    for (long i = to * width / 8 + t; i < rows * width / 8; i += step) ((uint4*)p)[i] = zero;
+    if (rest == nullptr) return;
+    for (long i = t; i < from * per; i += step) rest[i] = -INFINITY;
+    for (long i = to * per + t; i < rows * per; i += step) rest[i] = -INFINITY;
+}
+__device__ __forceinline__ long clip_start(int s, long T) { return s < 0 ? 0 : s > T ? T : s; }
+
+struct ForwardArgs {
+    Shape s;
+    Heads q, k, v;
+    void* out;            // [rows of all][heads][D]
+    float* lse;           // [rows of all][heads], or null
+    int tiles, splits;
+    float* part;          // splits > 1: [split][rows of all x heads][D] sums, and behind them float2 (base, sum) for each
+    long rows;            // rows of all x heads
+};
+
+// A workgroup has 128 rows, a wavefront 32 of them in registers (a lane one query), and goes over the keys in tiles of 64 in
+// two LDS buffers. The softmax's base moves only where a tile's maximum is more than 2^8 above it: sums and products are
+// relative to it anyway, and 64 multiplications a tile and lane are left out.
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) {
+    typedef typename Vec<T>::x8 x8;
+    typedef Reader<T, DP> R;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * R::BYTES];
+    const Shape& s = a.s;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    const bool packed = s.q_starts != nullptr;
+    // all heads' longest rows of keys first; neighbouring heads go round the XCDs, so that a head's tiles meet in one L2
+    const int many = (s.B + (packed && a.splits == 1 ? 1 : 0)) * s.Hk;
+    const int which = blockIdx.x % many, turn = blockIdx.x / many;
+    const int split = turn / a.tiles, first = a.tiles - 1 - turn % a.tiles;
+    const int b = which / s.Hk, hk = which % s.Hk;
+    if (b == s.B) {
+        outside((T*)a.out, a.lse, clip_start(s.q_starts[0], s.Tq), clip_start(s.q_starts[s.B], s.Tq), s.Tq, (long)s.Hk * s.G * s.D,
+                s.Hk * s.G, first * s.Hk + hk, a.tiles * s.Hk);
+        return;
+    }
+    const Seq seq = seq_of(s, b);
+    const int M = seq.lq * s.G, ahead = seq.lk - seq.lq;   // query i stands at i + ahead
+    const R read(lane);
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)smem;
+    const Loader<T, DP> K(head_of<T>(a.k, packed, b, seq.k0, hk), a.k, 1, s.D, wave, lane);
+    const Loader<T, DP> V(head_of<T>(a.v, packed, b, seq.k0, hk), a.v, 1, s.D, wave, lane);
+    const char* q = head_of<T>(a.q, packed, b, seq.q0, hk * s.G);
+    // keys of this split
+    const int chunk = a.splits == 1 ? seq.lk : ((seq.lk + a.splits - 1) / a.splits + TILE - 1) / TILE * TILE;
+    const int k_from = split * chunk < seq.lk ? split * chunk : seq.lk, k_to = k_from + chunk < seq.lk ? k_from + chunk : seq.lk;
+
+    for (int tile = first; (long)tile * BLOCK < M; tile += a.tiles) {
+        const int m0 = tile * BLOCK, w0 = m0 + 32 * wave, m = w0 + (lane & 31);
+        const int i = (m < M ? m : M - 1) / s.G, g = m - i * s.G;
+        const bool on = m < M;
+        x8 fq[DP / 16];
+        load_row<T, DP>(q + (long)sizeof(T) * (i * a.q.row + g * a.q.head), on, s.D, lane, fq);
+        // the keys [lo, hi) that this lane's query sees, this wavefront's queries see, and the workgroup's
+        const int hi = s.causal ? (i + ahead + 1 < k_to ? i + ahead + 1 : k_to) : k_to;
+        const int lo = s.window && i + ahead - s.window + 1 > k_from ? i + ahead - s.window + 1 : k_from;
+        const int i_first = w0 / s.G, i_last = ((w0 + 31 < M ? w0 + 31 : M - 1)) / s.G;
+        const int all_hi = s.causal ? (i_first + ahead + 1 < k_to ? i_first + ahead + 1 : k_to) : k_to;
+        const int any_hi = w0 >= M ? 0 : s.causal ? (i_last + ahead + 1 < k_to ? i_last + ahead + 1 : k_to) : k_to;
+        const int any_lo = s.window && i_first + ahead - s.window + 1 > k_from ? i_first + ahead - s.window + 1 : k_from;
+        const int all_lo = s.window && i_last + ahead - s.window + 1 > k_from ? i_last + ahead - s.window + 1 : k_from;
+        const int block_last = (m0 + BLOCK < M ? m0 + BLOCK : M) - 1;
+        const int to = k_from == k_to ? 0 : s.causal ? (block_last / s.G + ahead + 1 < k_to ? block_last / s.G + ahead + 1 : k_to) : k_to;
+        int from = s.window && m0 / s.G + ahead - s.window + 1 > k_from ? m0 / s.G + ahead - s.window + 1 : k_from;
+        from &= ~(TILE - 1);
+
+        f32x16 o[DP / 32] = {};
+        float base = -INFINITY, sum = 0.0f;   // the base is in units of log2
+        if (from < to) {
+            K.load(from, seq.lk, lds, wave);
+            V.load(from, seq.lk, lds + R::BYTES, wave);
+        }
+        uint32_t now = lds;
+        for (int n0 = from; n0 < to; n0 += TILE, now ^= 2 * R::BYTES) {
+            arrived();
+            if (n0 + TILE < to) {
+                K.load(n0 + TILE, seq.lk, now ^ 2 * R::BYTES, wave);
+                V.load(n0 + TILE, seq.lk, (now ^ 2 * R::BYTES) + R::BYTES, wave);
+            }
+            if (n0 >= any_hi || n0 + TILE <= any_lo) continue;
+            f32x16 z[2] = {};
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) z[t] = mfma(read.row(now, t, ks), fq[ks], z[t]);
+            if (n0 + TILE > all_hi || n0 < all_lo) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = n0 + 32 * t + 8 * (r / 4) + 4 * h + r % 4;
+                        z[t][r] = j >= lo && j < hi ? z[t][r] : -INFINITY;
+                    }
+            }
+            float top = z[0][0];
+#pragma unroll
+            for (int r = 1; r < 32; ++r) top = fmaxf(top, z[r / 16][r % 16]);
+            top = both_halves(top, [](float x, float y) { return fmaxf(x, y); }) * s.scale2;
+            if (__any(top > base + 8.0f)) {
+                const float next = fmaxf(base, top), down = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - next);
+                base = next;
+                sum *= down;
+#pragma unroll
+                for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[dt][r] *= down;
+            }
+            const float off = base == -INFINITY ? 0.0f : base;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    z[t][r] = __builtin_amdgcn_exp2f(fmaf(z[t][r], s.scale2, -off));
+                    sum += z[t][r];
+                }
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                const x8 p = half_of<T>(z[st / 2], st % 2);
+#pragma unroll
+                for (int dt = 0; dt < DP / 32; ++dt) o[dt] = mfma(read.col(now + R::BYTES, st, dt), p, o[dt]);
+            }
+        }
+        sum = both_halves(sum, [](float x, float y) { return x + y; });
+        const long at = (seq.q0 + i) * (s.Hk * s.G) + hk * s.G + g;
+        if (a.splits == 1) {
+            store_row<T, DP>((T*)a.out + at * s.D, on, s.D, lane, o, sum == 0.0f ? 0.0f : 1.0f / sum);
+            if (on && h == 0 && a.lse != nullptr) a.lse[at] = sum == 0.0f ? -INFINITY : (base + __builtin_amdgcn_logf(sum)) * LN2;
+        } else if (on) {
+            float* part = a.part + (split * a.rows + at) * s.D;
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const int d = 32 * dt + 8 * q4 + 4 * h;
+                    if (d < s.D) *(float4*)(part + d) = make_float4(o[dt][4 * q4], o[dt][4 * q4 + 1], o[dt][4 * q4 + 2], o[dt][4 * q4 + 3]);
+                }
+            if (h == 0) ((float2*)(a.part + a.splits * a.rows * s.D))[split * a.rows + at] = make_float2(base, sum);
+        }
+        arrived();   // (nobody reads the buffers any more)
+    }
+}
+
+// The splits' sums joined: a wavefront a row, a lane two elements (D <= 128).
+template <typename T>
+__global__ __launch_bounds__(256) void k_join(const ForwardArgs a) {
+    const Shape& s = a.s;
+    const int lane = threadIdx.x & 63, heads = s.Hk * s.G;
+    const float2* stat = (const float2*)(a.part + a.splits * a.rows * s.D);
+    for (long r = blockIdx.x * 4l + (threadIdx.x >> 6); r < a.rows; r += gridDim.x * 4l) {
+        bool in = true;
+        if (s.q_starts != nullptr) {
+            const long row = r / heads;
+            in = row >= clip_start(s.q_starts[0], s.Tq) && row < clip_start(s.q_starts[s.B], s.Tq);
+        }
+        float top = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
+        if (in) {
+            for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, stat[i * a.rows + r].x);
+            top = reduce_lanes<64, NanMax>(top);
+            for (int i = 0; i < a.splits; ++i) {
+                const float2 v = stat[i * a.rows + r];
+                // (a split without a visible key has base -inf, and its sums may be anything but they are zeros)
+                const float w = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v.x - top);
+                sum = fmaf(v.y, w, sum);
+                if (2 * lane < s.D) {
+                    const float2 p = *(const float2*)(a.part + (i * a.rows + r) * s.D + 2 * lane);
+                    x = fmaf(p.x, w, x);
+                    y = fmaf(p.y, w, y);
+                }
+            }
+        }
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (2 * lane < s.D) {
+            T* out = (T*)a.out + r * s.D + 2 * lane;
+            out[0] = (T)(x * f);
+            out[1] = (T)(y * f);
+        }
+        if (lane == 0 && a.lse != nullptr) a.lse[r] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
+    }
+}
+
+struct BackwardArgs {
+    Shape s;
+    Heads q, k, v, out, dout;
+    const float* lse;
+    void *dq, *dk, *dv;   // contiguous
+    float* stat;          // [2][rows of all x heads]: lse log2 e (inf where nothing is seen), D
+    long rows;
+    int q_tiles, k_tiles;
+    float scale;
+};
+
+// D, and lse as the gradients take it: 16 lanes a head's row, eight elements a lane
+template <typename T>
+__global__ __launch_bounds__(256) void k_delta(const BackwardArgs a) {
+    const Shape& s = a.s;
+    const int heads = s.Hk * s.G, lane = threadIdx.x & 15;
+    const int n = (int)(s.Tq * heads);   // of a sequence, or of all that are packed
+    for (int b = blockIdx.y; b < (s.q_starts != nullptr ? 1 : s.B); b += gridDim.y)
+        for (int r = blockIdx.x * 16 + (threadIdx.x >> 4); r < n; r += gridDim.x * 16) {
+            const int i = r / heads, hq = r - i * heads;
+            float o[8], d[8], sum = 0.0f;
+            const int here = s.D - 8 * lane >= 8 ? 8 : 0;
+            load8((const T*)a.out.p + b * a.out.batch + i * a.out.row + hq * a.out.head + 8 * lane, here, o);
+            load8((const T*)a.dout.p + b * a.dout.batch + i * a.dout.row + hq * a.dout.head + 8 * lane, here, d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fmaf(o[e], d[e], sum);
+            sum = reduce_lanes<16, Sum>(sum);
+            if (lane == 0) {
+                const long at = (long)b * n + r;
+                const float lse = a.lse[at];
+                a.stat[at] = lse == -INFINITY ? INFINITY : lse * LOG2E;
+                a.stat[a.rows + at] = sum;
+            }
+        }
+}
+
+// dQ: as the forward pass, 128 rows a workgroup; a lane has one query
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
+    typedef typename Vec<T>::x8 x8;
+    typedef Reader<T, DP> R;
+    __shared__ __attribute__((aligned(1024))) char smem[4 * R::BYTES];
+    const Shape& s = a.s;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    const bool packed = s.q_starts != nullptr;
+    const int many = (s.B + (packed ? 1 : 0)) * s.Hk;
+    const int which = blockIdx.x % many, first = a.q_tiles - 1 - blockIdx.x / many;
+    const int b = which / s.Hk, hk = which % s.Hk;
+    if (b == s.B) {
+        outside((T*)a.dq, nullptr, clip_start(s.q_starts[0], s.Tq), clip_start(s.q_starts[s.B], s.Tq), s.Tq, (long)s.Hk * s.G * s.D, 0,
+                first * s.Hk + hk, a.q_tiles * s.Hk);
+        return;
+    }
+    const Seq seq = seq_of(s, b);
+    const int M = seq.lq * s.G, ahead = seq.lk - seq.lq;
+    const R read(lane);
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)smem;
+    const Loader<T, DP> K(head_of<T>(a.k, packed, b, seq.k0, hk), a.k, 1, s.D, wave, lane);
+    const Loader<T, DP> V(head_of<T>(a.v, packed, b, seq.k0, hk), a.v, 1, s.D, wave, lane);
+    const char* q = head_of<T>(a.q, packed, b, seq.q0, hk * s.G);
+    const char* d_out = head_of<T>(a.dout, packed, b, seq.q0, hk * s.G);
+
+    for (int tile = first; (long)tile * BLOCK < M; tile += a.q_tiles) {
+        const int m0 = tile * BLOCK, w0 = m0 + 32 * wave, m = w0 + (lane & 31);
+        const int i = (m < M ? m : M - 1) / s.G, g = m - i * s.G;
+        const bool on = m < M;
+        const long at = (seq.q0 + i) * (s.Hk * s.G) + hk * s.G + g;
+        x8 fq[DP / 16], fd[DP / 16];
+        load_row<T, DP>(q + (long)sizeof(T) * (i * a.q.row + g * a.q.head), on, s.D, lane, fq);
+        load_row<T, DP>(d_out + (long)sizeof(T) * (i * a.dout.row + g * a.dout.head), on, s.D, lane, fd);
+        const float lse = on ? a.stat[at] : INFINITY, delta = on ? a.stat[a.rows + at] : 0.0f;
+        const int k_to = seq.lk;
+        const int hi = s.causal ? (i + ahead + 1 < k_to ? i + ahead + 1 : k_to) : k_to;
+        const int lo = s.window && i + ahead - s.window + 1 > 0 ? i + ahead - s.window + 1 : 0;
+        const int i_first = w0 / s.G, i_last = ((w0 + 31 < M ? w0 + 31 : M - 1)) / s.G;
+        const int all_hi = s.causal ? (i_first + ahead + 1 < k_to ? i_first + ahead + 1 : k_to) : k_to;
+        const int any_hi = w0 >= M ? 0 : s.causal ? (i_last + ahead + 1 < k_to ? i_last + ahead + 1 : k_to) : k_to;
+        const int any_lo = s.window && i_first + ahead - s.window + 1 > 0 ? i_first + ahead - s.window + 1 : 0;
+        const int all_lo = s.window && i_last + ahead - s.window + 1 > 0 ? i_last + ahead - s.window + 1 : 0;
+        const int block_last = (m0 + BLOCK < M ? m0 + BLOCK : M) - 1;
+        const int to = s.causal ? (block_last / s.G + ahead + 1 < k_to ? block_last / s.G + ahead + 1 : k_to) : k_to;
+        int from = s.window && m0 / s.G + ahead - s.window + 1 > 0 ? m0 / s.G + ahead - s.window + 1 : 0;
+        from &= ~(TILE - 1);
+
+        f32x16 dq[DP / 32] = {};
+        if (from < to) {
+            K.load(from, seq.lk, lds, wave);
+            V.load(from, seq.lk, lds + R::BYTES, wave);
+        }
+        uint32_t now = lds;
+        for (int n0 = from; n0 < to; n0 += TILE, now ^= 2 * R::BYTES) {
+            arrived();
+            if (n0 + TILE < to) {
+                K.load(n0 + TILE, seq.lk, now ^ 2 * R::BYTES, wave);
+                V.load(n0 + TILE, seq.lk, (now ^ 2 * R::BYTES) + R::BYTES, wave);
+            }
+            if (n0 >= any_hi || n0 + TILE <= any_lo) continue;
+            const bool masked = n0 + TILE > all_hi || n0 < all_lo;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f32x16 z = {}, dp = {};
+#pragma unroll
+                for (int ks = 0; ks < DP / 16; ++ks) {
+                    z = mfma(read.row(now, t, ks), fq[ks], z);
+                    dp = mfma(read.row(now + R::BYTES, t, ks), fd[ks], dp);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], s.scale2, -lse)) * (dp[r] - delta);
+                if (masked) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = n0 + 32 * t + 8 * (r / 4) + 4 * h + r % 4;
+                        z[r] = j >= lo && j < hi ? z[r] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    const x8 ds = half_of<T>(z, st);
+#pragma unroll
+                    for (int dt = 0; dt < DP / 32; ++dt) dq[dt] = mfma(read.col(now, 2 * t + st, dt), ds, dq[dt]);
+                }
+            }
+        }
+        store_row<T, DP>((T*)a.dq + at * s.D, on, s.D, lane, dq, a.scale);
+        arrived();
+    }
+}
+
+// dK and dV: 128 keys a workgroup, a wavefront 32 of them in registers (a lane one key), over all rows of the group's
+// queries that see them, in tiles of 64
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_dkv(const BackwardArgs a) {
+    typedef typename Vec<T>::x8 x8;
+    typedef Reader<T, DP> R;
+    constexpr int BUFFER = 2 * R::BYTES;
+    __shared__ __attribute__((aligned(1024))) char smem[2 * BUFFER + 2 * 2 * TILE * 4];
+    const Shape& s = a.s;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    const bool packed = s.q_starts != nullptr;
+    const int many = (s.B + (packed ? 1 : 0)) * s.Hk;
+    const int which = blockIdx.x % many, first = blockIdx.x / many;   // (the first keys are seen by most)
+    const int b = which / s.Hk, hk = which % s.Hk;
+    if (b == s.B) {
+        const long from = clip_start(s.k_starts[0], s.Tk), to = clip_start(s.k_starts[s.B], s.Tk), width = (long)s.Hk * s.D;
+        outside((T*)a.dk, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, a.k_tiles * s.Hk);
+        outside((T*)a.dv, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, a.k_tiles * s.Hk);
+        return;
+    }
+    const Seq seq = seq_of(s, b);
+    const int M = seq.lq * s.G, ahead = seq.lk - seq.lq;
+    const R read(lane);
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)smem, stats = lds + 2 * BUFFER;
+    const Loader<T, DP> Q(head_of<T>(a.q, packed, b, seq.q0, hk * s.G), a.q, s.G, s.D, wave, lane);
+    const Loader<T, DP> DO(head_of<T>(a.dout, packed, b, seq.q0, hk * s.G), a.dout, s.G, s.D, wave, lane);
+    const float* stat = a.stat + seq.q0 * (s.Hk * s.G) + hk * s.G;
+    const char* k = head_of<T>(a.k, packed, b, seq.k0, hk);
+    const char* v = head_of<T>(a.v, packed, b, seq.k0, hk);
+    auto load = [&](int m0, int buffer) {
+        Q.load(m0, M, lds + buffer * BUFFER, wave);
+        DO.load(m0, M, lds + buffer * BUFFER + R::BYTES, wave);
+        if (wave < 2) {   // lse by one wavefront, D by another
+            const int m = m0 + lane, i = m / s.G;
+            const float* from = m < M ? stat + wave * a.rows + i * (s.Hk * s.G) + (m - i * s.G) : no_row + wave;
+            load_lds4(from, stats + (2 * buffer + wave) * TILE * 4);
+        }
+    };
+
+    for (int tile = first; (long)tile * BLOCK < seq.lk; tile += a.k_tiles) {
+        const int n0 = tile * BLOCK, w0 = n0 + 32 * wave, j = w0 + (lane & 31);
+        const bool on = j < seq.lk;
+        const long row = on ? j : 0;
+        x8 fk[DP / 16], fv[DP / 16];
+        load_row<T, DP>(k + (long)sizeof(T) * row * a.k.row, on, s.D, lane, fk);
+        load_row<T, DP>(v + (long)sizeof(T) * row * a.v.row, on, s.D, lane, fv);
+        // the rows [lo, hi) that see this lane's key, this wavefront's keys, and the workgroup's
+        auto first_row = [&](int key) {   // of those that see it
+            const long m = s.causal ? (long)(key - ahead) * s.G : 0;
+            return m < 0 ? 0 : m < M ? (int)m : M;
+        };
+        auto end_row = [&](int key) {
+            const long m = s.window ? (long)(key - ahead + s.window) * s.G : M;
+            return m < 0 ? 0 : m < M ? (int)m : M;
+        };
+        const int last = w0 + 31 < seq.lk ? w0 + 31 : seq.lk - 1, block_last = n0 + BLOCK < seq.lk ? n0 + BLOCK - 1 : seq.lk - 1;
+        const int lo = first_row(j), hi = on ? end_row(j) : 0;
+        const int any_lo = first_row(w0), any_hi = w0 < seq.lk ? end_row(last) : 0;
+        const int all_lo = first_row(last), all_hi = w0 + 32 <= seq.lk ? end_row(w0) : 0;
+        const int from = first_row(n0) & ~(TILE - 1), to = end_row(block_last);
+
+        f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+        if (from < to) load(from, 0);
+        int buffer = 0;
+        for (int m0 = from; m0 < to; m0 += TILE, buffer ^= 1) {
+            arrived();
+            if (m0 + TILE < to) load(m0 + TILE, buffer ^ 1);
+            const uint32_t now = lds + buffer * BUFFER;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int r0 = m0 + 32 * t;
+                if (r0 >= any_hi || r0 + 32 <= any_lo) continue;
+                f32x16 z = {}, dp = {};
+#pragma unroll
+                for (int ks = 0; ks < DP / 16; ++ks) {
+                    z = mfma(read.row(now, t, ks), fk[ks], z);
+                    dp = mfma(read.row(now + R::BYTES, t, ks), fv[ks], dp);
+                }
+                const bool masked = r0 < all_lo || r0 + 32 > all_hi;
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const uint32_t at = stats + 2 * buffer * TILE * 4 + (32 * t + 8 * q4 + 4 * h) * 4;
+                    typedef float f32x4 __attribute__((ext_vector_type(4)));
+                    const f32x4 lse = *(__attribute__((address_space(3))) const f32x4*)(uintptr_t)at;
+                    const f32x4 delta = *(__attribute__((address_space(3))) const f32x4*)(uintptr_t)(at + TILE * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = 4 * q4 + e;
+                        z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], s.scale2, -lse[e]));
+                        if (masked) {
+                            const int m = r0 + 8 * q4 + 4 * h + e;
+                            z[r] = m >= lo && m < hi ? z[r] : 0.0f;
+                        }
+                        dp[r] = z[r] * (dp[r] - delta[e]);
+                    }
+                }
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    const x8 p = half_of<T>(z, st), ds = half_of<T>(dp, st);
+#pragma unroll
+                    for (int dt = 0; dt < DP / 32; ++dt) {
+                        dv[dt] = mfma(read.col(now + R::BYTES, 2 * t + st, dt), p, dv[dt]);
+                        dk[dt] = mfma(read.col(now, 2 * t + st, dt), ds, dk[dt]);
+                    }
+                }
+            }
+        }
+        const long at = ((seq.k0 + row) * s.Hk + hk) * s.D;
+        store_row<T, DP>((T*)a.dk + at, on, s.D, lane, dk, a.scale);
+        store_row<T, DP>((T*)a.dv + at, on, s.D, lane, dv, 1.0f);
+        arrived();
+    }
+}
+
+constexpr long MAX_ROWS = 1l << 30;      // queries x group, or keys, of a sequence
+constexpr long MAX_STRIDE = 1l << 24;    // of rows and heads: a tile's offsets stay within 32 bits
+
+long blocks(long n) { return (n + BLOCK - 1) / BLOCK; }
+
+// Where there are few workgroups the keys are split among several, so that 512 (two for each compute unit) run, each with
+// 128 keys at least; the sums are joined by a second kernel.
+long splits_of(long B, long Hk, long tiles, long max_k) {
+    const long have = B * Hk * tiles;
+    if (have == 0 || have >= 256) return 1;
+    const long want = (512 + have - 1) / have, most = max_k / 128;
+    const long n = want < most ? want : most;
+    return n < 1 ? 1 : n;
+}
+
+struct Call {
+    Shape s;
+    long rows;                 // of all sequences, times heads
+    long q_tiles, k_tiles;     // tiles a head that workgroups are launched for
+    long splits;
+};
+
+int check_shape(const char* what, int type, long B, long Hk, long G, long D, long Tq, long Tk, const int* q_starts,
+                const int* k_starts, long max_q, long max_k, int causal, long window, float scale, Call& c) {
+    if (type != SPANQR_BF16 && type != SPANQR_FP16) return error(SPANQR_EINVAL, "%s: the type must be bf16 or fp16", what);
+    if (D < 8 || D > 128 || D % 8 != 0) return error(SPANQR_EINVAL, "%s: D = %ld (multiples of 8 up to 128)", what, D);
+    if (B < 0 || Hk < 1 || G < 1 || Tq < 0 || Tk < 0 || B > INT_MAX / 2 || Hk > INT_MAX / G || (B + 1) > INT_MAX / Hk ||
+        Tq >= MAX_ROWS / G || Tk >= MAX_ROWS || (Tq > 0 && Hk * G > INT_MAX / Tq))
+        return error(SPANQR_EINVAL, "%s: B = %ld, heads = %ld x %ld, rows = %ld and %ld", what, B, Hk, G, Tq, Tk);
+    if ((q_starts != nullptr) != (k_starts != nullptr)) return error(SPANQR_EINVAL, "%s: q_starts and k_starts belong together", what);
+    if (window < 0 || (window > 0 && !causal)) return error(SPANQR_EINVAL, "%s: a window needs causal, and one key at least", what);
+    if (!(scale > 0.0f && scale < INFINITY)) return error(SPANQR_EINVAL, "%s: scale must be positive and finite", what);
+    const bool packed = q_starts != nullptr;
+    if (!packed || max_q < 1 || max_q > Tq) max_q = Tq;
+    if (!packed || max_k < 1 || max_k > Tk) max_k = Tk;
+    c.s = {(int)B, (int)Hk, (int)G, (int)D, Tq, Tk, q_starts, k_starts, causal ? 1 : 0, (int)(window < MAX_ROWS ? window : MAX_ROWS),
+           scale * LOG2E};
+    c.rows = (packed ? 1 : B) * Tq * Hk * G;
+    c.q_tiles = blocks(max_q * G) < 1 ? 1 : blocks(max_q * G);
+    c.k_tiles = blocks(max_k) < 1 ? 1 : blocks(max_k);
+    c.splits = splits_of(B, Hk, c.q_tiles, max_k);
+    if ((B + 1) * Hk > INT_MAX / (c.q_tiles * c.splits) || (B + 1) * Hk > INT_MAX / c.k_tiles)
+        return error(SPANQR_EINVAL, "%s: too many workgroups", what);
+    return SPANQR_OK;
+}
+
+// strides: {batch, row, head}
+int check_heads(const char* what, const char* name, const void* p, const long* strides, bool empty, Heads& h) {
+    if (empty) {
+        h = {p, 0, 0, 0};
+        return SPANQR_OK;
+    }
+    if (p == nullptr || strides == nullptr) return error(SPANQR_EINVAL, "%s: %s is missing", what, name);
+    h = {p, strides[0], strides[1], strides[2]};
+    if ((uintptr_t)p % 16 != 0 || h.batch % 8 != 0 || h.row % 8 != 0 || h.head % 8 != 0 || h.batch < 0 || h.row < 0 || h.head < 0 ||
+        h.row >= MAX_STRIDE || h.head >= MAX_STRIDE)
+        return error(SPANQR_EINVAL, "%s: %s needs 16-byte alignment and strides that are multiples of 8, of rows and heads below %ld", what,
+                     name, MAX_STRIDE);
+    return SPANQR_OK;
+}
+bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+template <typename T>
+void launch_forward(const ForwardArgs& a, hipStream_t st) {
+    const Shape& s = a.s;
+    const bool tail = s.q_starts != nullptr && a.splits == 1;
+    const int grid = (s.B + (tail ? 1 : 0)) * s.Hk * a.tiles * a.splits;
+    if (s.D <= 64)
+        k_forward<T, 64><<<grid, 64 * WAVES, 0, st>>>(a);
+    else
+        k_forward<T, 128><<<grid, 64 * WAVES, 0, st>>>(a);
+    if (a.splits > 1) k_join<T><<<(int)(a.rows < 4 * 4096 ? (a.rows + 3) / 4 : 4096), 256, 0, st>>>(a);
+}
+
+template <typename T>
+void launch_backward(const BackwardArgs& a, hipStream_t st) {
+    const Shape& s = a.s;
+    const bool packed = s.q_starts != nullptr;
+    const long n = s.Tq * s.Hk * s.G;
+    if (a.rows > 0)
+        k_delta<T><<<dim3((int)(n < 16 * 65536 ? (n + 15) / 16 : 65536), packed ? 1 : s.B < 65535 ? s.B : 65535), 256, 0, st>>>(a);
+    const int heads = (s.B + (packed ? 1 : 0)) * s.Hk;
+    if (a.dk != nullptr && heads > 0 && s.Tk > 0) {
+        if (s.D <= 64)
+            k_dkv<T, 64><<<heads * a.k_tiles, 64 * WAVES, 0, st>>>(a);
+        else
+            k_dkv<T, 128><<<heads * a.k_tiles, 64 * WAVES, 0, st>>>(a);
+    }
+    if (a.dq != nullptr && a.rows > 0) {
+        if (s.D <= 64)
+            k_dq<T, 64><<<heads * a.q_tiles, 64 * WAVES, 0, st>>>(a);
+        else
+            k_dq<T, 128><<<heads * a.q_tiles, 64 * WAVES, 0, st>>>(a);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+long spanqr_attention_workspace(long B, long Hk, long G, long D, long Tq, long Tk, int packed, long max_q, long max_k) {
+    Call c;
+    const int none = 0;
+    const int rc = check_shape("attention", SPANQR_BF16, B, Hk, G, D, Tq, Tk, packed ? &none : nullptr, packed ? &none : nullptr, max_q,
+                               max_k, 0, 0, 1.0f, c);
+    if (rc != SPANQR_OK) return rc;
+    return c.splits > 1 ? 4 * c.splits * c.rows * (D + 2) : 0;
+}
+
+int spanqr_attention(int type, long B, long Hk, long G, long D, long Tq, long Tk, const void* q, const long* q_strides, const void* k,
+                     const long* k_strides, const void* v, const long* v_strides, const int* q_starts, const int* k_starts, long max_q,
+                     long max_k, int causal, long window, float scale, void* out, float* lse, void* workspace, long workspace_bytes,
+                     void* stream) {
+    Call c;
+    int rc = check_shape("attention", type, B, Hk, G, D, Tq, Tk, q_starts, k_starts, max_q, max_k, causal, window, scale, c);
+    if (rc != SPANQR_OK || c.rows == 0) return rc;
+    ForwardArgs a = {};
+    const bool none = Tk == 0 || (B == 0 && q_starts == nullptr);
+    if ((rc = check_heads("attention", "q", q, q_strides, false, a.q)) != SPANQR_OK ||
+        (rc = check_heads("attention", "k", k, k_strides, none, a.k)) != SPANQR_OK ||
+        (rc = check_heads("attention", "v", v, v_strides, none, a.v)) != SPANQR_OK)
+        return rc;
+    if (out == nullptr || !aligned(out)) return error(SPANQR_EINVAL, "attention: out is missing or not on 16 bytes");
+    const long need = c.splits > 1 ? 4 * c.splits * c.rows * (D + 2) : 0;
+    if (need > 0 && (workspace == nullptr || !aligned(workspace) || workspace_bytes < need))
+        return error(SPANQR_EINVAL, "attention: the workspace needs %ld bytes", need);
+    a.s = c.s;
+    a.out = out;
+    a.lse = lse;
+    a.tiles = (int)c.q_tiles;
+    a.splits = (int)c.splits;
+    a.part = (float*)workspace;
+    a.rows = c.rows;
+    if (type == SPANQR_BF16)
+        launch_forward<bf16>(a, (hipStream_t)stream);
+    else
+        launch_forward<fp16>(a, (hipStream_t)stream);
+    return launched("attention");
+}
+
+long spanqr_attention_backward_workspace(long B, long Hk, long G, long D, long Tq, long Tk, int packed) {
+    Call c;
+    const int none = 0;
+    const int rc = check_shape("attention_backward", SPANQR_BF16, B, Hk, G, D, Tq, Tk, packed ? &none : nullptr, packed ? &none : nullptr,
+                               0, 0, 0, 0, 1.0f, c);
+    return rc != SPANQR_OK ? rc : 8 * c.rows;
+}
+
+int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq, long Tk, const void* dout, const long* dout_strides,
+                              const void* q, const long* q_strides, const void* k, const long* k_strides, const void* v,
+                              const long* v_strides, const void* out, const long* out_strides, const float* lse, const int* q_starts,
+                              const int* k_starts, long max_q, long max_k, int causal, long window, float scale, void* dq, void* dk,
+                              void* dv, void* workspace, long workspace_bytes, void* stream) {
+    const char* what = "attention_backward";
+    Call c;
+    int rc = check_shape(what, type, B, Hk, G, D, Tq, Tk, q_starts, k_starts, max_q, max_k, causal, window, scale, c);
+    if (rc != SPANQR_OK) return rc;
+    const bool packed = q_starts != nullptr, no_q = c.rows == 0, no_k = Tk == 0 || (B == 0 && !packed);
+    BackwardArgs a = {};
+    if ((rc = check_heads(what, "q", q, q_strides, no_q, a.q)) != SPANQR_OK ||
+        (rc = check_heads(what, "k", k, k_strides, no_k, a.k)) != SPANQR_OK ||
+        (rc = check_heads(what, "v", v, v_strides, no_k, a.v)) != SPANQR_OK ||
+        (rc = check_heads(what, "out", out, out_strides, no_q, a.out)) != SPANQR_OK ||
+        (rc = check_heads(what, "dout", dout, dout_strides, no_q, a.dout)) != SPANQR_OK)
+        return rc;
+    if ((dk != nullptr) != (dv != nullptr) || !aligned(dq) || !aligned(dk) || !aligned(dv))
+        return error(SPANQR_EINVAL, "%s: dk and dv belong together, and gradients lie on 16 bytes", what);
+    if (c.rows > 0 && (lse == nullptr || workspace == nullptr || !aligned(workspace) || workspace_bytes < 8 * c.rows))
+        return error(SPANQR_EINVAL, "%s: lse is missing, or the workspace, which needs %ld bytes", what, 8 * c.rows);
+    a.s = c.s;
+    a.lse = lse;
+    a.dq = dq;
+    a.dk = dk;
+    a.dv = dv;
+    a.stat = (float*)workspace;
+    a.rows = c.rows;
+    a.q_tiles = (int)c.q_tiles;
+    a.k_tiles = (int)c.k_tiles;
+    a.scale = scale;
+    if (type == SPANQR_BF16)
+        launch_backward<bf16>(a, (hipStream_t)stream);
+    else
+        launch_backward<fp16>(a, (hipStream_t)stream);
+    return launched(what);
+}
+
+}  // extern "C"
