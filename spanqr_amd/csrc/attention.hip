@@ -28,8 +28,8 @@ using spanqr_host::launched;
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 fp16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -147,7 +147,7 @@ struct Reader {
     typedef typename Vec<T>::x8 x8;
     static constexpr int ROW = 2 * DP;            // bytes
     static constexpr int BYTES = TILE * ROW;
-    uint32_t rows, cols[2];
+    uint32_t rows, cols[2];                       // a lane's places in a tile, or with the tile's address added
     __device__ __forceinline__ explicit Reader(int lane) {
         const int r = lane & 31, h = lane >> 5, lo = lane & 15, g = lane >> 4 & 1;
         rows = r * ROW + ((swizzle<DP>(r) ^ h) << 4);
@@ -157,52 +157,65 @@ struct Reader {
             cols[j] = k * ROW + (((2 * g + (lo >> 1 & 1)) ^ swizzle<DP>(k)) << 4) + 8 * (lo & 1);
         }
     }
-    // rows 32 t + lane % 32, elements 16 ks + 8 (lane / 32) + 0..7
-    __device__ __forceinline__ x8 row(uint32_t tile, int t, int ks) const {
-        return *(__attribute__((address_space(3))) const x8*)(uintptr_t)(tile + (rows ^ 32 * ks) + t * 32 * ROW);
+    __device__ __forceinline__ Reader(const Reader& r, uint32_t tile) : rows(r.rows + tile), cols{r.cols[0] + tile, r.cols[1] + tile} {}
+    // makes the compiler form the places below again behind this point: kept, they take the registers of two results
+    __device__ __forceinline__ void fresh() { asm volatile("" : "+v"(rows), "+v"(cols[0]), "+v"(cols[1])); }
+    // rows 32 t + lane % 32, elements 16 ks + 8 (lane / 32) + 0..7, of the tile `off` bytes on
+    __device__ __forceinline__ x8 row(int off, int t, int ks) const {
+        return *(__attribute__((address_space(3))) const x8*)(uintptr_t)((rows ^ 32 * ks) + off + t * 32 * ROW);
     }
     // element 32 dt + lane % 32 of the rows 16 s + 4 (lane / 32) + 0..3 and those + 8: the order of a result's registers
-    __device__ __forceinline__ x8 col(uint32_t tile, int s, int dt) const {
+    __device__ __forceinline__ x8 col(int off, int s, int dt) const {
         typedef __attribute__((address_space(3))) s16x4 lds_s4;
-        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(tile + (cols[0] ^ 64 * dt) + s * 16 * ROW));
-        const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)(tile + (cols[1] ^ 64 * dt) + s * 16 * ROW));
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)((cols[0] ^ 64 * dt) + off + s * 16 * ROW));
+        const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)((cols[1] ^ 64 * dt) + off + s * 16 * ROW));
         return __builtin_bit_cast(x8, __builtin_shufflevector(v, w, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 };
 
 // Loads of tiles of 64 rows m of one sequence and key head, m / G being the row in memory and m % G the head. Where G divides
 // 64 a lane's places in a tile are the same in every tile, and a tile inside the matrix is loaded from a base that
-// moves; otherwise, at the end and where D < DP every lane finds its own.
-template <typename T, int DP>
+// moves (what it has behind D is the row's last 16 bytes again: the other operand is 0 there, or the result is not used);
+// otherwise, and at the end, every lane finds its own, and reads zeros past the end.
+// KEPT: the places stay in registers; otherwise they are formed for each tile.
+template <typename T, int DP, bool KEPT>
 struct Loader {
     static constexpr int CHUNKS = DP / 8, LOADS = TILE * CHUNKS / 64 / WAVES;
     const char* base;
     long row, head;       // bytes
-    int G, D;
-    bool even;
-    uint32_t off[LOADS];
-    int at[LOADS];        // row and chunk of a load: 16 row + chunk
+    int G, shift, last;   // shift: of a G that divides 64; last: the row's last chunk
+    uint32_t off[KEPT ? LOADS : 1];
+    __device__ __forceinline__ static int row_of(int i, int wave, int lane) { return (wave * LOADS + i) * (64 / CHUNKS) + lane / CHUNKS; }
+    __device__ __forceinline__ int chunk_of(int r, int lane) const {
+        const int c = lane % CHUNKS ^ swizzle<DP>(r);
+        return c < last ? c : last;
+    }
+    // (strides are multiples of 16 bytes, below 2^25)
+    __device__ __forceinline__ uint32_t place(int i, int wave, int lane) const {
+        const int r = row_of(i, wave, lane);
+        return 16 * (__umul24(r >> shift, (uint32_t)row >> 4) + __umul24(r & (1 << shift) - 1, (uint32_t)head >> 4) + chunk_of(r, lane));
+    }
     __device__ __forceinline__ Loader(const char* base, const Heads& h, int G, int D, int wave, int lane)
-        : base(base), row((long)sizeof(T) * h.row), head((long)sizeof(T) * h.head), G(G), D(D), even(D == DP && TILE % G == 0) {
+        : base(base), row((long)sizeof(T) * h.row), head((long)sizeof(T) * h.head), G(G), shift(__builtin_ctz(G)), last(D / 8 - 1) {
+        if constexpr (KEPT) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int slot = (wave * LOADS + i) * 64 + lane, r = slot / CHUNKS, c = slot % CHUNKS ^ swizzle<DP>(r);
-            at[i] = 16 * r + c;
-            off[i] = (uint32_t)(r / G) * (uint32_t)row + (uint32_t)(r % G) * (uint32_t)head + 16 * c;
+            for (int i = 0; i < LOADS; ++i) off[i] = place(i, wave, lane);
         }
     }
     // rows m0 (a multiple of 64) to m0 + 63 of M into the tile at lds
-    __device__ __forceinline__ void load(int m0, int M, uint32_t lds, int wave) const {
+    __device__ __forceinline__ void load(int m0, int M, uint32_t lds, int wave, int lane) const {
         const uint32_t to = lds + wave * LOADS * 1024;
-        if (even && m0 + TILE <= M) {
-            const char* from = base + (m0 / G) * row;
+        const bool inside = TILE % G == 0 && m0 + TILE <= M;
+        if (!KEPT || !inside) asm volatile("" : "+v"(lane));   // (formed here: hoisted, the places would fill the registers)
+        if (inside) {
+            const char* from = base + (m0 >> shift) * row;
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) load_lds(from, off[i], to + i * 1024);
+            for (int i = 0; i < LOADS; ++i) load_lds(from, KEPT ? off[KEPT ? i : 0] : place(i, wave, lane), to + i * 1024);
         } else {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const int m = m0 + (at[i] >> 4), c = at[i] & 15, q = m / G;
-                const void* from = m < M && 8 * c < D ? (const void*)(base + q * row + (m - q * G) * head + 16 * c) : (const void*)nothing;
+                const int r = row_of(i, wave, lane), m = m0 + r, q = m / G;
+                const void* from = m < M ? (const void*)(base + q * row + (m - q * G) * head + 16 * chunk_of(r, lane)) : (const void*)nothing;
                 load_lds(from, to + i * 1024);
             }
         }
@@ -212,6 +225,7 @@ struct Loader {
 // the second operand straight from memory: a lane's row at p (or nothing)
 template <typename T, int DP>
 __device__ __forceinline__ void load_row(const char* p, bool on, int D, int lane, typename Vec<T>::x8 (&f)[DP / 16]) {
+    asm volatile("" : "+v"(lane));   // (nothing of it is kept for the next block)
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
         const int d = 16 * ks + 8 * (lane >> 5);
@@ -295,8 +309,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
     const int M = seq.lq * s.G, ahead = seq.lk - seq.lq;   // query i stands at i + ahead
     const R read(lane);
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)smem;
-    const Loader<T, DP> K(head_of<T>(a.k, packed, b, seq.k0, hk), a.k, 1, s.D, wave, lane);
-    const Loader<T, DP> V(head_of<T>(a.v, packed, b, seq.k0, hk), a.v, 1, s.D, wave, lane);
+    const Loader<T, DP, true> K(head_of<T>(a.k, packed, b, seq.k0, hk), a.k, 1, s.D, wave, lane);
+    const Loader<T, DP, true> V(head_of<T>(a.v, packed, b, seq.k0, hk), a.v, 1, s.D, wave, lane);
     const char* q = head_of<T>(a.q, packed, b, seq.q0, hk * s.G);
     // keys of this split
     const int chunk = a.splits == 1 ? seq.lk : ((seq.lk + a.splits - 1) / a.splits + TILE - 1) / TILE * TILE;
@@ -324,22 +338,23 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
         f32x16 o[DP / 32] = {};
         float base = -INFINITY, sum = 0.0f;   // the base is in units of log2
         if (from < to) {
-            K.load(from, seq.lk, lds, wave);
-            V.load(from, seq.lk, lds + R::BYTES, wave);
+            K.load(from, seq.lk, lds, wave, lane);
+            V.load(from, seq.lk, lds + R::BYTES, wave, lane);
         }
         uint32_t now = lds;
         for (int n0 = from; n0 < to; n0 += TILE, now ^= 2 * R::BYTES) {
             arrived();
             if (n0 + TILE < to) {
-                K.load(n0 + TILE, seq.lk, now ^ 2 * R::BYTES, wave);
-                V.load(n0 + TILE, seq.lk, (now ^ 2 * R::BYTES) + R::BYTES, wave);
+                K.load(n0 + TILE, seq.lk, now ^ 2 * R::BYTES, wave, lane);
+                V.load(n0 + TILE, seq.lk, (now ^ 2 * R::BYTES) + R::BYTES, wave, lane);
             }
             if (n0 >= any_hi || n0 + TILE <= any_lo) continue;
+            const R in(read, now);
             f32x16 z[2] = {};
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) z[t] = mfma(read.row(now, t, ks), fq[ks], z[t]);
+                for (int t = 0; t < 2; ++t) z[t] = mfma(in.row(0, t, ks), fq[ks], z[t]);
             if (n0 + TILE > all_hi || n0 < all_lo) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -374,7 +389,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
             for (int st = 0; st < 4; ++st) {
                 const x8 p = half_of<T>(z[st / 2], st % 2);
 #pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt) o[dt] = mfma(read.col(now + R::BYTES, st, dt), p, o[dt]);
+                for (int dt = 0; dt < DP / 32; ++dt) o[dt] = mfma(in.col(R::BYTES, st, dt), p, o[dt]);
             }
         }
         sum = both_halves(sum, [](float x, float y) { return x + y; });
@@ -397,13 +412,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
     }
 }
 
-// The splits' sums joined: a wavefront a row, a lane two elements (D <= 128).
+// The splits' sums joined: a workgroup a row, each wavefront every fourth split, a lane two elements (D <= 128); in a fixed order.
 template <typename T>
-__global__ __launch_bounds__(256) void k_join(const ForwardArgs a) {
+__global__ __launch_bounds__(64 * WAVES) void k_join(const ForwardArgs a) {
+    __shared__ float add[WAVES][3][64];
     const Shape& s = a.s;
-    const int lane = threadIdx.x & 63, heads = s.Hk * s.G;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, heads = s.Hk * s.G;
     const float2* stat = (const float2*)(a.part + a.splits * a.rows * s.D);
-    for (long r = blockIdx.x * 4l + (threadIdx.x >> 6); r < a.rows; r += gridDim.x * 4l) {
+    for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         bool in = true;
         if (s.q_starts != nullptr) {
             const long row = r / heads;
@@ -413,25 +429,36 @@ __global__ __launch_bounds__(256) void k_join(const ForwardArgs a) {
         if (in) {
             for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, stat[i * a.rows + r].x);
             top = reduce_lanes<64, NanMax>(top);
-            for (int i = 0; i < a.splits; ++i) {
-                const float2 v = stat[i * a.rows + r];
-                // (a split without a visible key has base -inf, and its sums may be anything but they are zeros)
-                const float w = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v.x - top);
+            const long d = r * s.D + (2 * lane < s.D ? 2 * lane : 0);
+#pragma unroll 8
+            for (int i = wave; i < a.splits; i += WAVES) {
+                const float2 v = stat[i * a.rows + r], p = *(const float2*)(a.part + i * a.rows * s.D + d);
+                const float w = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v.x - top);   // (no visible key: zeros)
                 sum = fmaf(v.y, w, sum);
-                if (2 * lane < s.D) {
-                    const float2 p = *(const float2*)(a.part + (i * a.rows + r) * s.D + 2 * lane);
-                    x = fmaf(p.x, w, x);
-                    y = fmaf(p.y, w, y);
-                }
+                x = fmaf(p.x, w, x);
+                y = fmaf(p.y, w, y);
             }
         }
-        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-        if (2 * lane < s.D) {
-            T* out = (T*)a.out + r * s.D + 2 * lane;
-            out[0] = (T)(x * f);
-            out[1] = (T)(y * f);
+        add[wave][0][lane] = sum;
+        add[wave][1][lane] = x;
+        add[wave][2][lane] = y;
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) {
+                sum += add[w][0][lane];
+                x += add[w][1][lane];
+                y += add[w][2][lane];
+            }
+            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+            if (2 * lane < s.D) {
+                T* out = (T*)a.out + r * s.D + 2 * lane;
+                out[0] = (T)(x * f);
+                out[1] = (T)(y * f);
+            }
+            if (lane == 0 && a.lse != nullptr) a.lse[r] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
         }
-        if (lane == 0 && a.lse != nullptr) a.lse[r] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * LN2;
+        __syncthreads();
     }
 }
 
@@ -492,8 +519,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
     const int M = seq.lq * s.G, ahead = seq.lk - seq.lq;
     const R read(lane);
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)smem;
-    const Loader<T, DP> K(head_of<T>(a.k, packed, b, seq.k0, hk), a.k, 1, s.D, wave, lane);
-    const Loader<T, DP> V(head_of<T>(a.v, packed, b, seq.k0, hk), a.v, 1, s.D, wave, lane);
+    const Loader<T, DP, true> K(head_of<T>(a.k, packed, b, seq.k0, hk), a.k, 1, s.D, wave, lane);
+    const Loader<T, DP, true> V(head_of<T>(a.v, packed, b, seq.k0, hk), a.v, 1, s.D, wave, lane);
     const char* q = head_of<T>(a.q, packed, b, seq.q0, hk * s.G);
     const char* d_out = head_of<T>(a.dout, packed, b, seq.q0, hk * s.G);
 
@@ -521,25 +548,27 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
 
         f32x16 dq[DP / 32] = {};
         if (from < to) {
-            K.load(from, seq.lk, lds, wave);
-            V.load(from, seq.lk, lds + R::BYTES, wave);
+            K.load(from, seq.lk, lds, wave, lane);
+            V.load(from, seq.lk, lds + R::BYTES, wave, lane);
         }
         uint32_t now = lds;
         for (int n0 = from; n0 < to; n0 += TILE, now ^= 2 * R::BYTES) {
             arrived();
             if (n0 + TILE < to) {
-                K.load(n0 + TILE, seq.lk, now ^ 2 * R::BYTES, wave);
-                V.load(n0 + TILE, seq.lk, (now ^ 2 * R::BYTES) + R::BYTES, wave);
+                K.load(n0 + TILE, seq.lk, now ^ 2 * R::BYTES, wave, lane);
+                V.load(n0 + TILE, seq.lk, (now ^ 2 * R::BYTES) + R::BYTES, wave, lane);
             }
             if (n0 >= any_hi || n0 + TILE <= any_lo) continue;
             const bool masked = n0 + TILE > all_hi || n0 < all_lo;
+            R in(read, now);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
+                in.fresh();
                 f32x16 z = {}, dp = {};
 #pragma unroll
                 for (int ks = 0; ks < DP / 16; ++ks) {
-                    z = mfma(read.row(now, t, ks), fq[ks], z);
-                    dp = mfma(read.row(now + R::BYTES, t, ks), fd[ks], dp);
+                    z = mfma(in.row(0, t, ks), fq[ks], z);
+                    dp = mfma(in.row(R::BYTES, t, ks), fd[ks], dp);
                 }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], s.scale2, -lse)) * (dp[r] - delta);
@@ -554,7 +583,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
                 for (int st = 0; st < 2; ++st) {
                     const x8 ds = half_of<T>(z, st);
 #pragma unroll
-                    for (int dt = 0; dt < DP / 32; ++dt) dq[dt] = mfma(read.col(now, 2 * t + st, dt), ds, dq[dt]);
+                    for (int dt = 0; dt < DP / 32; ++dt) dq[dt] = mfma(in.col(0, 2 * t + st, dt), ds, dq[dt]);
                 }
             }
         }
@@ -587,14 +616,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dkv(const BackwardArgs a) {
     const int M = seq.lq * s.G, ahead = seq.lk - seq.lq;
     const R read(lane);
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)smem, stats = lds + 2 * BUFFER;
-    const Loader<T, DP> Q(head_of<T>(a.q, packed, b, seq.q0, hk * s.G), a.q, s.G, s.D, wave, lane);
-    const Loader<T, DP> DO(head_of<T>(a.dout, packed, b, seq.q0, hk * s.G), a.dout, s.G, s.D, wave, lane);
+    const Loader<T, DP, DP == 64> Q(head_of<T>(a.q, packed, b, seq.q0, hk * s.G), a.q, s.G, s.D, wave, lane);
+    const Loader<T, DP, DP == 64> DO(head_of<T>(a.dout, packed, b, seq.q0, hk * s.G), a.dout, s.G, s.D, wave, lane);
     const float* stat = a.stat + seq.q0 * (s.Hk * s.G) + hk * s.G;
     const char* k = head_of<T>(a.k, packed, b, seq.k0, hk);
     const char* v = head_of<T>(a.v, packed, b, seq.k0, hk);
     auto load = [&](int m0, int buffer) {
-        Q.load(m0, M, lds + buffer * BUFFER, wave);
-        DO.load(m0, M, lds + buffer * BUFFER + R::BYTES, wave);
+        Q.load(m0, M, lds + buffer * BUFFER, wave, lane);
+        DO.load(m0, M, lds + buffer * BUFFER + R::BYTES, wave, lane);
         if (wave < 2) {   // lse by one wavefront, D by another
             const int m = m0 + lane, i = m / s.G;
             const float* from = m < M ? stat + wave * a.rows + i * (s.Hk * s.G) + (m - i * s.G) : no_row + wave;
@@ -609,8 +638,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dkv(const BackwardArgs a) {
         x8 fk[DP / 16], fv[DP / 16];
         load_row<T, DP>(k + (long)sizeof(T) * row * a.k.row, on, s.D, lane, fk);
         load_row<T, DP>(v + (long)sizeof(T) * row * a.v.row, on, s.D, lane, fv);
-        // the rows [lo, hi) that see this lane's key, this wavefront's keys, and the workgroup's
-        auto first_row = [&](int key) {   // of those that see it
+        // the rows that see a key; then those that see any and all of this wavefront's keys, and the workgroup's
+        auto first_row = [&](int key) {
             const long m = s.causal ? (long)(key - ahead) * s.G : 0;
             return m < 0 ? 0 : m < M ? (int)m : M;
         };
@@ -619,7 +648,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dkv(const BackwardArgs a) {
             return m < 0 ? 0 : m < M ? (int)m : M;
         };
         const int last = w0 + 31 < seq.lk ? w0 + 31 : seq.lk - 1, block_last = n0 + BLOCK < seq.lk ? n0 + BLOCK - 1 : seq.lk - 1;
-        const int lo = first_row(j), hi = on ? end_row(j) : 0;
         const int any_lo = first_row(w0), any_hi = w0 < seq.lk ? end_row(last) : 0;
         const int all_lo = first_row(last), all_hi = w0 + 32 <= seq.lk ? end_row(w0) : 0;
         const int from = first_row(n0) & ~(TILE - 1), to = end_row(block_last);
@@ -630,42 +658,52 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dkv(const BackwardArgs a) {
         for (int m0 = from; m0 < to; m0 += TILE, buffer ^= 1) {
             arrived();
             if (m0 + TILE < to) load(m0 + TILE, buffer ^ 1);
-            const uint32_t now = lds + buffer * BUFFER;
+            R in(read, lds + buffer * BUFFER);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int r0 = m0 + 32 * t;
                 if (r0 >= any_hi || r0 + 32 <= any_lo) continue;
+                in.fresh();
                 f32x16 z = {}, dp = {};
 #pragma unroll
                 for (int ks = 0; ks < DP / 16; ++ks) {
-                    z = mfma(read.row(now, t, ks), fk[ks], z);
-                    dp = mfma(read.row(now + R::BYTES, t, ks), fv[ks], dp);
+                    z = mfma(in.row(0, t, ks), fk[ks], z);
+                    dp = mfma(in.row(R::BYTES, t, ks), fv[ks], dp);
                 }
-                const bool masked = r0 < all_lo || r0 + 32 > all_hi;
+                // four rows' lse or D
+                auto stat4 = [&](int which, int q4) {
+                    const uint32_t at = stats + ((2 * buffer + which) * TILE + 32 * t + 8 * q4 + 4 * h) * 4;
+                    return *(__attribute__((address_space(3))) const f32x4*)(uintptr_t)at;
+                };
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) {
-                    const uint32_t at = stats + 2 * buffer * TILE * 4 + (32 * t + 8 * q4 + 4 * h) * 4;
-                    typedef float f32x4 __attribute__((ext_vector_type(4)));
-                    const f32x4 lse = *(__attribute__((address_space(3))) const f32x4*)(uintptr_t)at;
-                    const f32x4 delta = *(__attribute__((address_space(3))) const f32x4*)(uintptr_t)(at + TILE * 4);
+                    const f32x4 lse = stat4(0, q4);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = 4 * q4 + e;
-                        z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], s.scale2, -lse[e]));
-                        if (masked) {
-                            const int m = r0 + 8 * q4 + 4 * h + e;
-                            z[r] = m >= lo && m < hi ? z[r] : 0.0f;
-                        }
-                        dp[r] = z[r] * (dp[r] - delta[e]);
+                    for (int e = 0; e < 4; ++e) z[4 * q4 + e] = __builtin_amdgcn_exp2f(fmaf(z[4 * q4 + e], s.scale2, -lse[e]));
+                }
+                if (r0 < all_lo || r0 + 32 > all_hi) {
+                    int key = j;
+                    asm volatile("" : "+v"(key));   // (formed here)
+                    const int lo = first_row(key), hi = key < seq.lk ? end_row(key) : 0;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int m = r0 + 8 * (r / 4) + 4 * h + r % 4;
+                        z[r] = m >= lo && m < hi ? z[r] : 0.0f;
                     }
+                }
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const f32x4 delta = stat4(1, q4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = z[4 * q4 + e] * (dp[4 * q4 + e] - delta[e]);
                 }
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
                     const x8 p = half_of<T>(z, st), ds = half_of<T>(dp, st);
 #pragma unroll
                     for (int dt = 0; dt < DP / 32; ++dt) {
-                        dv[dt] = mfma(read.col(now + R::BYTES, 2 * t + st, dt), p, dv[dt]);
-                        dk[dt] = mfma(read.col(now, 2 * t + st, dt), ds, dk[dt]);
+                        dv[dt] = mfma(in.col(R::BYTES, 2 * t + st, dt), p, dv[dt]);
+                        dk[dt] = mfma(in.col(0, 2 * t + st, dt), ds, dk[dt]);
                     }
                 }
             }
@@ -748,7 +786,7 @@ void launch_forward(const ForwardArgs& a, hipStream_t st) {
         k_forward<T, 64><<<grid, 64 * WAVES, 0, st>>>(a);
     else
         k_forward<T, 128><<<grid, 64 * WAVES, 0, st>>>(a);
-    if (a.splits > 1) k_join<T><<<(int)(a.rows < 4 * 4096 ? (a.rows + 3) / 4 : 4096), 256, 0, st>>>(a);
+    if (a.splits > 1) k_join<T><<<(int)(a.rows < 65536 ? a.rows : 65536), 64 * WAVES, 0, st>>>(a);
 }
 
 template <typename T>
