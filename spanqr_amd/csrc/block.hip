@@ -31,6 +31,7 @@ struct BlockArgs {
     const float* scale_at;                       // read instead of scale where it is not null
     Dropout drop;
     void *h, *y;
+    bool past;                                   // the outputs do not fit the caches
 };
 
 struct BlockGradArgs {
@@ -41,36 +42,100 @@ struct BlockGradArgs {
     const float* scale_at;
     Dropout drop;
     void *dx, *dr, *dg;                          // dg null without a gate
+    bool past;
     float* part;                                 // [gridDim.x][2 D + 1] sums over the workgroup's rows for dw1, dw2, da, or null
 };
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
-
-// act(g), and its slope
-__device__ __forceinline__ float gate_of(int act, float g) {
-    if (act == SPANQR_GATE_LINEAR) return g;
-    const float s = sigmoid(g);
-    return act == SPANQR_GATE_SIGMOID ? s : g * s;
+// the factor of what is added to the stream, in a scalar register
+template <typename ARGS>
+__device__ __forceinline__ float factor_of(const ARGS& p) {
+    const float a = p.scale_at != nullptr ? *p.scale_at : p.scale;
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, a)));
 }
-__device__ __forceinline__ float gate_of(int act, float g, float& slope) {
-    slope = 1.0f;
-    if (act == SPANQR_GATE_LINEAR) return g;
-    const float s = sigmoid(g);
-    if (act == SPANQR_GATE_SIGMOID) {
-        slope = s * (1.0f - s);
-        return s;
+
+// Both weights of a thread's columns in fp32 in LDS, each thread's own words: read from memory in every row they would be two
+// more latencies, in registers 16 a piece. 64 bytes for each thread and piece.
+template <int NCH>
+struct Weights {
+    float4* at;
+    __device__ __forceinline__ Weights(float4* lds, const void* w1, const void* w2, int type, long D, int lane, int size) : at(lds + threadIdx.x) {
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            const long from = 8l * (lane + c * size);
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                float w[8];
+                load_weight(which ? w2 : w1, type, from, inside(D, from), w);
+                at[(4 * c + 2 * which) * blockDim.x] = make_float4(w[0], w[1], w[2], w[3]);
+                at[(4 * c + 2 * which + 1) * blockDim.x] = make_float4(w[4], w[5], w[6], w[7]);
+            }
+        }
     }
-    slope = s * (1.0f + g * (1.0f - s));
-    return g * s;
+    __device__ __forceinline__ void get(int which, int c, float (&w)[8]) const {
+        const float4 a = at[(4 * c + 2 * which) * blockDim.x], b = at[(4 * c + 2 * which + 1) * blockDim.x];
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    }
+};
+
+// 1 / (1 + exp(-g)): in fp32's full precision, or within 2^-20 of itself for what is rounded to 16 bits (2^-11 at best)
+template <typename T>
+__device__ __forceinline__ float sigmoid(float g) {
+    if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-g));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * g));
 }
 
-template <typename T, int GROUP, int NCH, bool WHOLE>
+// v act(g)
+template <typename T>
+__device__ __forceinline__ void times_gate(int act, const float (&g)[8], float (&v)[8]) {
+    if (act == SPANQR_GATE_LINEAR) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= g[i];
+    } else if (act == SPANQR_GATE_SIGMOID) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= sigmoid<T>(g[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= g[i] * sigmoid<T>(g[i]);
+    }
+}
+// v act(g) in v, and u act'(g) in g
+template <typename T>
+__device__ __forceinline__ void gate_slope(int act, float (&g)[8], float (&v)[8], const float (&u)[8]) {
+    if (act == SPANQR_GATE_LINEAR) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[i] *= g[i];
+            g[i] = u[i];
+        }
+    } else if (act == SPANQR_GATE_SIGMOID) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float s = sigmoid<T>(g[i]);
+            v[i] *= s;
+            g[i] = u[i] * (s * (1.0f - s));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float s = sigmoid<T>(g[i]), a = g[i] * s;
+            v[i] *= a;
+            g[i] = u[i] * (s + a * (1.0f - s));
+        }
+    }
+}
+
+template <typename T, int GROUP, int NCH, int WHOLE>
 __global__ __launch_bounds__(Group<GROUP>::MOST) void k_block(const BlockArgs p) {
     typedef Group<GROUP> G;
     __shared__ float slot[2][2][1][16];   // both sums', by turns
+    extern __shared__ float4 weights[];
     const int lane = G::lane(), size = G::size();
-    const float scale = p.scale_at != nullptr ? *p.scale_at : p.scale;
+    const Weights<NCH> weight(weights, p.w1, p.w2, p.wtype, p.D, lane, size);
+    const float scale = factor_of(p);
     const uint64_t key = p.drop.key();
+    // (a load under a condition would be waited for before the next one: without a gate x is read again, from the cache)
+    const void* gate = p.gate != nullptr ? p.gate : p.x;
+    const long ldg = p.gate != nullptr ? p.ldg : p.ldx;
     int turn = 0;
     for (long base = (long)blockIdx.x * G::rows(); base < p.rows; base += (long)gridDim.x * G::rows(), turn ^= 1) {
         const long row = base + G::index();
@@ -83,7 +148,7 @@ __global__ __launch_bounds__(Group<GROUP>::MOST) void k_block(const BlockArgs p)
             const int n = inside(p.D, at);
             kx[c] = piece<WHOLE>((const T*)p.x + from * p.ldx, p.D, at, n);
             kr[c] = piece<WHOLE>((const T*)p.residual + from * p.ldr, p.D, at, n);
-            if (p.gate != nullptr) kg[c] = piece<WHOLE>((const T*)p.gate + from * p.ldg, p.D, at, n);
+            kg[c] = piece<WHOLE>((const T*)gate + from * ldg, p.D, at, n);
         }
         float sum[1] = {0.0f};
 #pragma unroll
@@ -93,7 +158,7 @@ __global__ __launch_bounds__(Group<GROUP>::MOST) void k_block(const BlockArgs p)
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[0] = fmaf(x[i], x[i], sum[0]);
         }
-        G::template reduce<Sum>(sum, slot[turn][0]);
+        G::sum(sum, slot[turn][0]);
         const float s1 = rsqrtf(sum[0] / (float)p.D + p.eps);
         float h[NCH][8];
         sum[0] = 0.0f;
@@ -101,88 +166,89 @@ __global__ __launch_bounds__(Group<GROUP>::MOST) void k_block(const BlockArgs p)
         for (int c = 0; c < NCH; ++c) {
             const long at = 8l * (lane + c * size);
             const int n = on ? inside(p.D, at) : 0;
-            float x[8], w[8], f[8];
+            float x[8], w[8];
             settle<WHOLE>(kx[c], n, x);
             settle<WHOLE>(kr[c], n, h[c]);
-            load_weight(p.w1, p.wtype, at, n, w);
-            p.drop.factors(key, row, lane + c * size, f);
+            weight.get(0, c, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = x[i] * s1 * w[i];
             if (p.gate != nullptr) {
                 float g[8];
                 settle<WHOLE>(kg[c], n, g);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] *= gate_of(p.act, g[i]);
+                times_gate<T>(p.act, g, x);
             }
+            p.drop.thin(key, row, lane + c * size, x);
             // the stream is rounded as it is kept; the norm is of the rounded values
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                h[c][i] = i < n ? (float)(T)fmaf(scale, thin(x[i], f[i]), h[c][i]) : 0.0f;
+                h[c][i] = i < n ? (float)(T)fmaf(scale, x[i], h[c][i]) : 0.0f;
                 sum[0] = fmaf(h[c][i], h[c][i], sum[0]);
             }
-            store8((T*)p.h + row * p.D + at, n, h[c]);
+            store8((T*)p.h + row * p.D + at, n, h[c], p.past);
         }
-        G::template reduce<Sum>(sum, slot[turn][1]);
+        G::sum(sum, slot[turn][1]);
         const float s2 = rsqrtf(sum[0] / (float)p.D + p.eps);
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
             const long at = 8l * (lane + c * size);
             const int n = on ? inside(p.D, at) : 0;
             float w[8];
-            load_weight(p.w2, p.wtype, at, n, w);
+            weight.get(1, c, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * s2 * w[i];
-            store8((T*)p.y + row * p.D + at, n, h[c]);
+            store8((T*)p.y + row * p.D + at, n, h[c], p.past);
         }
     }
 }
 
-// rows longer than 16384: one workgroup a row, the row read again for each step (from the cache where it fits)
+// Rows longer than 8192: one workgroup a row, x and h read twice (from the cache the second time). Keeping h of up to 24576
+// elements in registers took 235 us where this takes 207 (4096 x 14336 bf16).
 template <typename T>
 __global__ __launch_bounds__(1024) void k_block_long(const BlockArgs p) {
-    __shared__ float slot[16];
-    const float scale = p.scale_at != nullptr ? *p.scale_at : p.scale;
+    __shared__ float slot[3][1][16];
+    typedef Group<0> G;
+    const float scale = factor_of(p);
     const uint64_t key = p.drop.key();
-    for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    int turn = 0;
+    for (long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const T* x = (const T*)p.x + row * p.ldx;
         T* h = (T*)p.h + row * p.D;
-        float sum = 0.0f, v[8], w[8], f[8], g[8];
+        float sum[1] = {0.0f}, v[8], w[8], u[8];
 #pragma unroll 2
         for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
             settle8(fetch8(x, p.D, at), inside(p.D, at), v);
             float part = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) part = fmaf(v[i], v[i], part);
-            sum += part;
+            sum[0] += part;
         }
-        sum = reduce_threads<1024, Sum>(sum, slot);
-        const float s1 = rsqrtf(sum / (float)p.D + p.eps);
-        sum = 0.0f;
+        G::sum(sum, slot[turn]);
+        const float s1 = rsqrtf(sum[0] / (float)p.D + p.eps);
+        sum[0] = 0.0f;
         for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
             const int n = inside(p.D, at);
             const Pack8<T> kx = fetch8(x, p.D, at), kr = fetch8((const T*)p.residual + row * p.ldr, p.D, at);
             settle8(kx, n, v);
             load_weight(p.w1, p.wtype, at, n, w);
-            p.drop.factors(key, row, at >> 3, f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = v[i] * s1 * w[i];
             if (p.gate != nullptr) {
-                settle8(fetch8((const T*)p.gate + row * p.ldg, p.D, at), n, g);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= gate_of(p.act, g[i]);
+                settle8(fetch8((const T*)p.gate + row * p.ldg, p.D, at), n, w);
+                times_gate<T>(p.act, w, v);
             }
-            settle8(kr, n, g);
+            p.drop.thin(key, row, at >> 3, v);
+            settle8(kr, n, u);
             float part = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                v[i] = i < n ? (float)(T)fmaf(scale, thin(v[i], f[i]), g[i]) : 0.0f;
-                part = fmaf(v[i], v[i], part);
+                u[i] = i < n ? (float)(T)fmaf(scale, v[i], u[i]) : 0.0f;
+                part = fmaf(u[i], u[i], part);
             }
-            store8(h + at, n, v);
-            sum += part;
+            store8(h + at, n, u);
+            sum[0] += part;
         }
-        sum = reduce_threads<1024, Sum>(sum, slot);
-        const float s2 = rsqrtf(sum / (float)p.D + p.eps);
+        G::sum(sum, slot[2]);   // (the next row's first barrier stands between its reads and the next writes)
+        const float s2 = rsqrtf(sum[0] / (float)p.D + p.eps);
         // a thread reads back only what it wrote itself
         for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
             const int n = inside(p.D, at);
@@ -190,57 +256,68 @@ __global__ __launch_bounds__(1024) void k_block_long(const BlockArgs p) {
             load_weight(p.w2, p.wtype, at, n, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = v[i] * s2 * w[i];
-            store8((T*)p.y + row * p.D + at, n, v);
+            store8((T*)p.y + row * p.D + at, n, v, p.past);
         }
     }
 }
 
-
 // The weights' gradients are sums over rows: a workgroup keeps its rows' part in registers (each thread always holds the same
 // columns), adds its groups through LDS and writes one row of partial sums; k_block_sums adds those.
-template <typename T, int GROUP, int NCH, bool WHOLE>
+template <typename T, int GROUP, int NCH, int WHOLE>
 __global__ __launch_bounds__(GROUP ? 256 : 512) void k_block_grad(const BlockGradArgs p) {
     typedef Group<GROUP> G;
     __shared__ float slot[2][3][16], slot2[2][1][16];
     constexpr int ROWS = GROUP ? 256 / GROUP : 1;
     __shared__ float add[ROWS > 1 ? (ROWS - 1) * GROUP * NCH * 16 : 1];
     __shared__ float add_scale[ROWS];
+    extern __shared__ float4 weights[];
     const int lane = G::lane(), group = G::index(), size = G::size();
-    const float scale = p.scale_at != nullptr ? *p.scale_at : p.scale;
+    const Weights<NCH> weight(weights, p.w1, p.w2, p.wtype, p.D, lane, size);
+    const float scale = factor_of(p);
     const uint64_t key = p.drop.key();
     float dw1[NCH][8], dw2[NCH][8], da = 0.0f;
 #pragma unroll
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) dw1[c][i] = dw2[c][i] = 0.0f;
-    int turn = 0;
-    for (long base = (long)blockIdx.x * ROWS; base < p.rows; base += (long)gridDim.x * ROWS, turn ^= 1) {
-        const long row = base + group;
-        const bool on = row < p.rows;
-        const long from = on ? row : base;
-        Pack8<T> kx[NCH], kh[NCH], ky[NCH], kd[NCH], kg[NCH];
+    // (a load under a condition would be waited for before the next one: for what is absent h is read again, from the cache)
+    const void *dy = p.dy != nullptr ? p.dy : p.h, *dh = p.dh != nullptr ? p.dh : p.h, *gate = p.gate != nullptr ? p.gate : p.h;
+    const long lddy = p.dy != nullptr ? p.lddy : p.ldh, lddh = p.dh != nullptr ? p.lddh : p.ldh, ldg = p.gate != nullptr ? p.ldg : p.ldh;
+    struct Row {
+        Pack8<T> x[NCH], h[NCH], y[NCH], d[NCH], g[NCH];
+    };
+    auto fetch = [&](long base, Row& k) {
+        const long from = base + group < p.rows ? base + group : base;
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
             const long at = 8l * (lane + c * size);
             const int n = inside(p.D, at);
-            kx[c] = piece<WHOLE>((const T*)p.x + from * p.ldx, p.D, at, n);
-            kh[c] = piece<WHOLE>((const T*)p.h + from * p.ldh, p.D, at, n);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ky[c].v[i] = kd[c].v[i] = (T)0.0f;
-            if (p.dy != nullptr) ky[c] = piece<WHOLE>((const T*)p.dy + from * p.lddy, p.D, at, n);
-            if (p.dh != nullptr) kd[c] = piece<WHOLE>((const T*)p.dh + from * p.lddh, p.D, at, n);
-            if (p.gate != nullptr) kg[c] = piece<WHOLE>((const T*)p.gate + from * p.ldg, p.D, at, n);
+            k.x[c] = piece<WHOLE>((const T*)p.x + from * p.ldx, p.D, at, n);
+            k.h[c] = piece<WHOLE>((const T*)p.h + from * p.ldh, p.D, at, n);
+            k.y[c] = piece<WHOLE>((const T*)dy + from * lddy, p.D, at, n);
+            k.d[c] = piece<WHOLE>((const T*)dh + from * lddh, p.D, at, n);
+            k.g[c] = piece<WHOLE>((const T*)gate + from * ldg, p.D, at, n);
         }
+    };
+    const long step = (long)gridDim.x * ROWS;
+    int turn = 0;
+    Row k, next;
+    if ((long)blockIdx.x * ROWS < p.rows) fetch((long)blockIdx.x * ROWS, next);
+    for (long base = (long)blockIdx.x * ROWS; base < p.rows; base += step, turn ^= 1) {
+        const long row = base + group;
+        const bool on = row < p.rows;
+        k = next;
+        if (base + step < p.rows) fetch(base + step, next);
         float sum[3] = {0.0f, 0.0f, 0.0f};   // of x^2, h^2 and dy w2 h
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
             const long at = 8l * (lane + c * size);
             const int n = on ? inside(p.D, at) : 0;
             float x[8], h[8], u[8], w[8];
-            settle<WHOLE>(kx[c], n, x);
-            settle<WHOLE>(kh[c], n, h);
-            settle<WHOLE>(ky[c], n, u);
-            load_weight(p.w2, p.wtype, at, n, w);
+            settle<WHOLE>(k.x[c], n, x);
+            settle<WHOLE>(k.h[c], n, h);
+            settle<WHOLE>(k.y[c], p.dy != nullptr ? n : 0, u);
+            weight.get(1, c, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 sum[0] = fmaf(x[i], x[i], sum[0]);
@@ -248,7 +325,7 @@ __global__ __launch_bounds__(GROUP ? 256 : 512) void k_block_grad(const BlockGra
                 sum[2] = fmaf(u[i] * w[i], h[i], sum[2]);
             }
         }
-        G::template reduce<Sum>(sum, slot[turn]);
+        G::sum(sum, slot[turn]);
         // a group without a row adds zeros, also where eps is 0
         const float s1 = on ? rsqrtf(sum[0] / (float)p.D + p.eps) : 0.0f;
         const float s2 = on ? rsqrtf(sum[1] / (float)p.D + p.eps) : 0.0f;
@@ -256,42 +333,38 @@ __global__ __launch_bounds__(GROUP ? 256 : 512) void k_block_grad(const BlockGra
         float q[NCH][8], last[1] = {0.0f};
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            again(kx[c]);   // (packed they take half the registers until here)
-            again(kh[c]);
-            again(ky[c]);
+            again(k.x[c]);   // (packed they take half the registers until here)
+            again(k.h[c]);
+            again(k.y[c]);
             const long at = 8l * (lane + c * size);
             const int n = on ? inside(p.D, at) : 0;
-            float a[8], b[8], w[8], d[8], f[8];
-            settle<WHOLE>(kh[c], n, a);
-            settle<WHOLE>(ky[c], n, b);
-            settle<WHOLE>(kd[c], n, d);
-            load_weight(p.w2, p.wtype, at, n, w);
+            float a[8], b[8], w[8], d[8];
+            settle<WHOLE>(k.h[c], n, a);
+            settle<WHOLE>(k.y[c], p.dy != nullptr ? n : 0, b);
+            settle<WHOLE>(k.d[c], p.dh != nullptr ? n : 0, d);
+            weight.get(1, c, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float n2 = a[i] * s2;
                 dw2[c][i] = fmaf(b[i], n2, dw2[c][i]);
                 d[i] = fmaf(s2, b[i] * w[i] - n2 * m2, d[i]);
             }
-            store8((T*)p.dr + row * p.D + at, n, d);
-            p.drop.factors(key, row, lane + c * size, f);
-            settle<WHOLE>(kx[c], n, a);
-            load_weight(p.w1, p.wtype, at, n, w);
+            store8((T*)p.dr + row * p.D + at, n, d, p.past);
+            p.drop.thin(key, row, lane + c * size, d);
+            settle<WHOLE>(k.x[c], n, a);
+            weight.get(0, c, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                d[i] = i < n ? thin(d[i], f[i]) : 0.0f;
+                d[i] = i < n ? d[i] : 0.0f;
                 a[i] *= s1;
             }
             if (p.gate != nullptr) {
                 float g[8];
-                settle<WHOLE>(kg[c], n, g);
+                settle<WHOLE>(k.g[c], n, g);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float slope;
-                    const float act = gate_of(p.act, g[i], slope);
-                    b[i] = scale * d[i] * a[i] * w[i] * slope;
-                    d[i] *= act;
-                }
-                store8((T*)p.dg + row * p.D + at, n, b);
+                for (int i = 0; i < 8; ++i) b[i] = scale * d[i] * a[i] * w[i];
+                gate_slope<T>(p.act, g, d, b);
+                store8((T*)p.dg + row * p.D + at, n, g, p.past);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -300,19 +373,19 @@ __global__ __launch_bounds__(GROUP ? 256 : 512) void k_block_grad(const BlockGra
                 last[0] = fmaf(q[c][i], a[i], last[0]);
             }
         }
-        G::template reduce<Sum>(last, slot2[turn]);
+        G::sum(last, slot2[turn]);
         const float m1 = last[0] / (float)p.D;   // the mean of q n1
         if (lane == 0) da += last[0];
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-            again(kx[c]);
+            again(k.x[c]);
             const long at = 8l * (lane + c * size);
             const int n = on ? inside(p.D, at) : 0;
             float x[8];
-            settle<WHOLE>(kx[c], n, x);
+            settle<WHOLE>(k.x[c], n, x);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = scale * s1 * (q[c][i] - x[i] * s1 * m1);
-            store8((T*)p.dx + row * p.D + at, n, x);
+            store8((T*)p.dx + row * p.D + at, n, x, p.past);
         }
     }
     if (p.part == nullptr) return;
@@ -352,125 +425,135 @@ __global__ __launch_bounds__(GROUP ? 256 : 512) void k_block_grad(const BlockGra
     if (lane == 0) part[2 * p.D] = da;
 }
 
-// The gradient of rows longer than 8192, which do not stay in registers: the row is read once for each step, from L2
-// behind the first one; the sums for the weights are in the partial sums' own memory, a thread's own words.
-template <typename T>
+// The gradient of rows longer than 8192: one workgroup a row, which is read for each of three steps (from L2 behind the first
+// one). The sums for the weights are in LDS (up to LONG_LDS columns), or in the partial sums' own memory; a thread's own words
+// either way. With the sums in registers and q kept in LDS for the third step it took 1082 us (4096 x 14336 bf16: they spill).
+constexpr int LONG_LDS = 18432;
+template <typename T, bool IN_LDS>
 __global__ __launch_bounds__(1024) void k_block_grad_long(const BlockGradArgs p) {
     __shared__ float slot[2][3][16], slot2[2][1][16];
+    __shared__ __attribute__((aligned(16))) float add[IN_LDS ? 2 * LONG_LDS : 4];
     typedef Group<0> G;
-    const float scale = p.scale_at != nullptr ? *p.scale_at : p.scale;
+    const float scale = factor_of(p);
     const uint64_t key = p.drop.key();
     float* part = p.part == nullptr ? nullptr : p.part + blockIdx.x * (2 * p.D + 1);
+    const void *dy = p.dy != nullptr ? p.dy : p.h, *dh = p.dh != nullptr ? p.dh : p.h, *gate = p.gate != nullptr ? p.gate : p.h;
+    const long lddy = p.dy != nullptr ? p.lddy : p.ldh, lddh = p.dh != nullptr ? p.lddh : p.ldh, ldg = p.gate != nullptr ? p.ldg : p.ldh;
+    const int n_y = p.dy != nullptr ? 8 : 0, n_d = p.dh != nullptr ? 8 : 0, t = threadIdx.x;
+    // adds v to the sums of piece `at`: the weight behind the block (0) or in front of the next one (1)
+    auto sums = [&](int which, long at, int n, bool start, const float (&v)[8]) {
+        float* mine = IN_LDS ? add + which * LONG_LDS + at : part + which * p.D + at;
+        if (!IN_LDS && part == nullptr) return;
+        float old[8];
+        load8(mine, start ? 0 : n, old);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) old[i] += v[i];
+        store8(mine, n, old);
+    };
     float da = 0.0f;
     int turn = 0;
     for (long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const T* xr = (const T*)p.x + row * p.ldx;
         const T* hr = (const T*)p.h + row * p.ldh;
-        const T* yr = p.dy == nullptr ? nullptr : (const T*)p.dy + row * p.lddy;
-        const T* dr = p.dh == nullptr ? nullptr : (const T*)p.dh + row * p.lddh;
-        const T* gr = p.gate == nullptr ? nullptr : (const T*)p.gate + row * p.ldg;
-        // eight elements of a row, 0 where there is none
-        auto load = [&](const T* from, long at, int n, float (&f)[8]) {
-            if (from != nullptr) {
-                settle8(fetch8(from, p.D, at), n, f);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = 0.0f;
-            }
-        };
+        const T* yr = (const T*)dy + row * lddy;
+        const T* dr = (const T*)dh + row * lddh;
+        const T* gr = (const T*)gate + row * ldg;
         float sum[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll 2
-        for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
+        for (long at = 8l * t; at < p.D; at += 8192) {
             const int n = inside(p.D, at);
-            float x[8], h[8], u[8], w[8], a = 0.0f, b = 0.0f, c = 0.0f;
-            load(xr, at, n, x);
-            load(hr, at, n, h);
-            load(yr, at, n, u);
+            const Pack8<T> kx = fetch8(xr, p.D, at), kh = fetch8(hr, p.D, at), ky = fetch8(yr, p.D, at);
+            float a[8], b[8], w[8], e = 0.0f, f = 0.0f, g = 0.0f;
+            settle8(kx, n, a);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e = fmaf(a[i], a[i], e);
+            settle8(kh, n, a);
+            settle8(ky, n < n_y ? n : n_y, b);
             load_weight(p.w2, p.wtype, at, n, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                a = fmaf(x[i], x[i], a);
-                b = fmaf(h[i], h[i], b);
-                c = fmaf(u[i] * w[i], h[i], c);
+                f = fmaf(a[i], a[i], f);
+                g = fmaf(b[i] * w[i], a[i], g);
             }
-            sum[0] += a;
-            sum[1] += b;
-            sum[2] += c;
+            sum[0] += e;
+            sum[1] += f;
+            sum[2] += g;
         }
-        G::template reduce<Sum>(sum, slot[turn]);
+        G::sum(sum, slot[turn]);
         const float s1 = rsqrtf(sum[0] / (float)p.D + p.eps), s2 = rsqrtf(sum[1] / (float)p.D + p.eps);
         const float m2 = s2 * sum[2] / (float)p.D;
         // q and n1 of a piece; in the first of two steps with everything else that the piece gives
-        auto piece_of = [&](long at, int n, bool first, float (&q)[8], float (&n1)[8]) {
-            float a[8], b[8], w[8], d[8], f[8], g[8];
-            load(hr, at, n, a);
-            load(yr, at, n, b);
-            load(dr, at, n, d);
-            load(gr, at, n, g);
-            load(xr, at, n, n1);
+        auto piece_of = [&](long at, bool first, float (&q)[8], float (&n1)[8]) __attribute__((always_inline)) {
+            const int n = inside(p.D, at);
+            const Pack8<T> kh = fetch8(hr, p.D, at), ky = fetch8(yr, p.D, at), kd = fetch8(dr, p.D, at), kx = fetch8(xr, p.D, at),
+                           kg = fetch8(gr, p.D, at);
+            float a[8], b[8], w[8];
+            settle8(kh, n, a);
+            settle8(ky, n < n_y ? n : n_y, b);
+            settle8(kd, n < n_d ? n : n_d, q);
             load_weight(p.w2, p.wtype, at, n, w);
-            float dw2[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float n2 = a[i] * s2;
-                dw2[i] = b[i] * n2;
-                d[i] = fmaf(s2, b[i] * w[i] - n2 * m2, d[i]);
+                a[i] *= s2;
+                q[i] = fmaf(s2, b[i] * w[i] - a[i] * m2, q[i]);
+                a[i] *= b[i];
             }
-            if (first) store8((T*)p.dr + row * p.D + at, n, d);
-            p.drop.factors(key, row, at >> 3, f);
+            if (first) {
+                store8((T*)p.dr + row * p.D + at, n, q, p.past);
+                sums(1, at, n, row == blockIdx.x, a);
+            }
+            p.drop.thin(key, row, at >> 3, q);
+            settle8(kx, n, n1);
             load_weight(p.w1, p.wtype, at, n, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                d[i] = i < n ? thin(d[i], f[i]) : 0.0f;
+                q[i] = i < n ? q[i] : 0.0f;
                 n1[i] *= s1;
             }
-            if (gr != nullptr) {
+            if (p.gate != nullptr) {
+                settle8(kg, n, b);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float slope;
-                    const float act = gate_of(p.act, g[i], slope);
-                    g[i] = scale * d[i] * n1[i] * w[i] * slope;
-                    d[i] *= act;
-                }
-                if (first) store8((T*)p.dg + row * p.D + at, n, g);
+                for (int i = 0; i < 8; ++i) a[i] = scale * q[i] * n1[i] * w[i];
+                gate_slope<T>(p.act, b, q, a);
+                if (first) store8((T*)p.dg + row * p.D + at, n, b, p.past);
             }
-            if (first && part != nullptr) {
-                float old[8];
-                const bool start = row == blockIdx.x;
+            if (first) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) old[i] = 0.0f;
-                if (!start) load8(part + at, n, old);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) old[i] = fmaf(scale * d[i], n1[i], old[i]);
-                store8(part + at, n, old);
-                if (!start) load8(part + p.D + at, n, old);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) old[i] = start ? dw2[i] : old[i] + dw2[i];
-                store8(part + p.D + at, n, old);
+                for (int i = 0; i < 8; ++i) a[i] = scale * q[i] * n1[i];
+                sums(0, at, n, row == blockIdx.x, a);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = i < n ? d[i] * w[i] : 0.0f;
+            for (int i = 0; i < 8; ++i) q[i] = i < n ? q[i] * w[i] : 0.0f;
         };
         float last[1] = {0.0f}, q[8], n1[8];
-        for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
-            piece_of(at, inside(p.D, at), true, q, n1);
+        for (long at = 8l * t; at < p.D; at += 8192) {
+            piece_of(at, true, q, n1);
             float a = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) a = fmaf(q[i], n1[i], a);
             last[0] += a;
         }
-        G::template reduce<Sum>(last, slot2[turn]);
+        G::sum(last, slot2[turn]);
         const float m1 = last[0] / (float)p.D;
         da += last[0];
-        for (long at = 8l * threadIdx.x; at < p.D; at += 8192) {
-            const int n = inside(p.D, at);
-            piece_of(at, n, false, q, n1);
+        for (long at = 8l * t; at < p.D; at += 8192) {
+            piece_of(at, false, q, n1);
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[i] = scale * s1 * (q[i] - n1[i] * m1);
-            store8((T*)p.dx + row * p.D + at, n, q);
+            store8((T*)p.dx + row * p.D + at, inside(p.D, at), q, p.past);
         }
     }
-    if (part != nullptr && threadIdx.x == 0) part[2 * p.D] = da;
+    if (part == nullptr) return;
+    if constexpr (IN_LDS) {
+        for (long at = 8l * t; at < p.D; at += 8192)
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                float v[8];
+                load8(add + which * LONG_LDS + at, inside(p.D, at), v);
+                store8(part + which * p.D + at, inside(p.D, at), v);
+            }
+    }
+    if (t == 0) part[2 * p.D] = da;
 }
 
 // columns [0, D) of the parts are dw1's, [D, 2 D) dw2's, the last is da's: 16 columns a workgroup, 64 threads a column, added in
@@ -506,11 +589,14 @@ __global__ __launch_bounds__(1024) void k_block_sums(const float* part, int part
         ((float*)dw)[d] = sum;
 }
 
+// outputs of more than the eight L2s' 32 MB are written past them
+bool past_caches(long rows, long D, long bytes) { return rows * D * bytes > 32l << 20; }
+
 // Dropout alone: a workgroup takes DROP_PIECES neighbouring pieces at a time, a thread every 256th of them, so that its loads
 // are under way together. pieces: of a row.
-constexpr int DROP_PIECES = 1024;
+constexpr int DROP_PIECES = 512;
 template <typename T>
-__global__ __launch_bounds__(256) void k_dropout(long rows, long D, uint32_t pieces, const T* x, long ldx, Dropout drop, T* y) {
+__global__ __launch_bounds__(256) void k_dropout(long rows, long D, uint32_t pieces, const T* x, long ldx, Dropout drop, T* y, bool past) {
     constexpr int N = DROP_PIECES / 256;
     const uint64_t key = drop.key();
     const long all = rows * pieces;
@@ -531,21 +617,18 @@ __global__ __launch_bounds__(256) void k_dropout(long rows, long D, uint32_t pie
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            float v[8], f[8];
+            float v[8];
             if (D >= 8)
                 settle8(k[i], n[i], v);
             else
                 settle<false>(k[i], n[i], v);
-            drop.factors(key, row[i], at[i] >> 3, f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = thin(v[j], f[j]);
-            store8(y + row[i] * D + at[i], n[i], v);
+            drop.thin(key, row[i], at[i] >> 3, v);
+            store8(y + row[i] * D + at[i], n[i], v, past);
         }
     }
 }
 
-constexpr long LONG_ROW = 16384;   // longest row that stays in registers
-constexpr long LONG_GRAD = 8192;   // and in the gradient
+constexpr long LONG_ROW = 8192;   // longest row that stays in registers
 constexpr long MAX_D = 1l << 24;
 constexpr long MAX_DROP_D = 1l << 32;   // dropout alone
 
@@ -564,12 +647,32 @@ Split grad_split_of(long D) {
     return {(int)(((pieces + nch - 1) / nch + 63) / 64 * 64), nch, true};
 }
 
-// the gradient's workgroups, and so rows of partial sums: as many as the compute units hold at once
+// The gradient's workgroups, and so rows of partial sums: as many as the compute units hold at once (12 wavefronts of one
+// piece a thread each, 8 of two), but where there are few rows at least four for each, since each workgroup ends with a row of sums
+// that is written and read again. Forward and gradient in us with 768 / 1536: 16384 x 1024 bf16 115 / 103, 3001 x 769 fp32 37 / 43.
 int grad_parts(long rows, long D) {
-    if (D > LONG_GRAD) return (int)(rows < 256 ? rows : 256);
+    if (D > LONG_ROW) return (int)(rows < 256 ? rows : 256);
     const Split s = grad_split_of(D);
-    return grid_of(rows, s, !s.block || s.group <= 256 ? 1024 : 512);
+    const long most = !s.block ? 1024 : s.group <= 128 ? 1536 : s.group <= 256 ? 768 : 256, few = rows / 4 > 256 ? rows / 4 : 256;
+    return grid_of(rows, s, (int)(most < few ? most : few));
 }
+
+#define SPANQR_BLOCK_SPLITS(LAUNCH)                       \
+    if (s.block && s.nch == 2) {                          \
+        if (p.D % 8 == 0) LAUNCH(0, 2, 2);                \
+        else LAUNCH(0, 2, 1);                             \
+    } else if (s.block) {                                 \
+        if (p.D % 8 == 0) LAUNCH(0, 1, 2);                \
+        else LAUNCH(0, 1, 1);                             \
+    } else if (s.group == 64) {                           \
+        if (p.D % 8 == 0) LAUNCH(64, 1, 2);               \
+        else LAUNCH(64, 1, 1);                            \
+    } else if (p.D >= 8) {                                \
+        if (p.D % 8 == 0) LAUNCH(16, 1, 2);               \
+        else LAUNCH(16, 1, 1);                            \
+    } else {                                              \
+        LAUNCH(16, 1, 0);                                 \
+    }
 
 template <typename T>
 void launch_block(const BlockArgs& p, hipStream_t st) {
@@ -579,41 +682,33 @@ void launch_block(const BlockArgs& p, hipStream_t st) {
     }
     const Split s = split_of(p.rows, p.D);
     const int grid = grid_of(p.rows, s, s.block ? 1024 : 2048);
-    if (s.block && s.nch == 2)
-        k_block<T, 0, 2, true><<<grid, s.group, 0, st>>>(p);
-    else if (s.block)
-        k_block<T, 0, 1, true><<<grid, s.group, 0, st>>>(p);
-    else if (s.group == 64)
-        k_block<T, 64, 1, true><<<grid, 256, 0, st>>>(p);
-    else if (p.D >= 8)
-        k_block<T, 16, 1, true><<<grid, 256, 0, st>>>(p);
-    else
-        k_block<T, 16, 1, false><<<grid, 256, 0, st>>>(p);
+    const int threads = s.block ? s.group : 256;
+#define LAUNCH(G, C, W) k_block<T, G, C, W><<<grid, threads, 64 * C * threads, st>>>(p)
+    SPANQR_BLOCK_SPLITS(LAUNCH)
+#undef LAUNCH
 }
 
 template <typename T>
 void launch_grad(const BlockGradArgs& p, int grid, hipStream_t st) {
-    if (p.D > LONG_GRAD) {
-        k_block_grad_long<T><<<grid, 1024, 0, st>>>(p);
+    if (p.D > LONG_ROW) {
+        if (p.D <= LONG_LDS)
+            k_block_grad_long<T, true><<<grid, 1024, 0, st>>>(p);
+        else
+            k_block_grad_long<T, false><<<grid, 1024, 0, st>>>(p);
         return;
     }
     const Split s = grad_split_of(p.D);
-    if (s.block && s.nch == 2)
-        k_block_grad<T, 0, 2, true><<<grid, s.group, 0, st>>>(p);
-    else if (s.block)
-        k_block_grad<T, 0, 1, true><<<grid, s.group, 0, st>>>(p);
-    else if (s.group == 64)
-        k_block_grad<T, 64, 1, true><<<grid, 256, 0, st>>>(p);
-    else if (p.D >= 8)
-        k_block_grad<T, 16, 1, true><<<grid, 256, 0, st>>>(p);
-    else
-        k_block_grad<T, 16, 1, false><<<grid, 256, 0, st>>>(p);
+    const int threads = s.block ? s.group : 256;
+#define LAUNCH(G, C, W) k_block_grad<T, G, C, W><<<grid, threads, 64 * C * threads, st>>>(p)
+    SPANQR_BLOCK_SPLITS(LAUNCH)
+#undef LAUNCH
 }
 
 template <typename T>
 void launch_dropout(long rows, long D, const void* x, long ldx, const Dropout& drop, void* y, hipStream_t st) {
     const long pieces = (D + 7) / 8, need = (rows * pieces + DROP_PIECES - 1) / DROP_PIECES;
-    k_dropout<T><<<(int)(need < 65536 ? need : 65536), 256, 0, st>>>(rows, D, (uint32_t)pieces, (const T*)x, ldx, drop, (T*)y);
+    k_dropout<T><<<(int)(need < 65536 ? need : 65536), 256, 0, st>>>(rows, D, (uint32_t)pieces, (const T*)x, ldx, drop, (T*)y,
+                                                                             past_caches(rows, D, sizeof(T)));
 }
 
 bool known(int type) { return type == SPANQR_BF16 || type == SPANQR_FP16 || type == SPANQR_FP32; }
@@ -678,7 +773,7 @@ int spanqr_block_norm(int type, int wtype, int act, long rows, long D, const voi
     if (rows > 1 && (ldx < D || ldr < D || (gate != nullptr && ldg < D)))
         return error(SPANQR_EINVAL, "block_norm: a row stride below D");
     const BlockArgs a = {rows, D, ldx, ldr, ldg, x, residual, gate, post_weight, weight, wtype, act, eps, scale, scale_at, drop,
-                         h, y};
+                         h, y, past_caches(rows, D, type == SPANQR_FP32 ? 4 : 2)};
     hipStream_t st = (hipStream_t)stream;
     if (type == SPANQR_BF16)
         launch_block<bf16>(a, st);
@@ -718,7 +813,8 @@ int spanqr_block_norm_backward(int type, int wtype, int act, long rows, long D, 
                          (gate != nullptr && ldg < D)))
             return error(SPANQR_EINVAL, "block_norm_backward: a row stride below D");
         const BlockGradArgs a = {rows, D, lddy, lddh, ldx, ldh, ldg, dy, dh, x, h, gate, post_weight, weight, wtype, act, eps,
-                                 scale, scale_at, drop, dx, dresidual, dgate, sums ? (float*)workspace : nullptr};
+                                 scale, scale_at, drop, dx, dresidual, dgate, past_caches(rows, D, type == SPANQR_FP32 ? 4 : 2),
+                                 sums ? (float*)workspace : nullptr};
         if (type == SPANQR_BF16)
             launch_grad<bf16>(a, parts, st);
         else if (type == SPANQR_FP16)

@@ -46,6 +46,22 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&f)[8]) {
     }
 }
 
+// store8 past the caches (where `past`): outputs that the L2s do not hold for whoever reads them next
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int n, const float (&f)[8], bool past) {
+    typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+    if (n < 8 || !past) {
+        store8(p, n, f);
+        return;
+    }
+    Pack8<T> k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k.v[i] = (T)f[i];
+    struct { Words w[sizeof(T) / 2]; } b = __builtin_bit_cast(decltype(b), k);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) __builtin_nontemporal_store(b.w[i], (Words*)p + i);
+}
+
 // Eight elements of a row of D >= 8 from `at` on, in two steps, so that many loads can be under way at once: fetch8 reads
 // the last eight where fewer are left (no branch, nothing past the row), and settle8 moves those to their place and
 // puts 0 behind them. n: how many are left, 0 to 8.

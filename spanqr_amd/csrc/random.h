@@ -24,15 +24,15 @@ struct Dropout {
     const uint64_t* seed_at;   // on the device, read instead where it is not null
     uint32_t index;
 
-    __device__ __forceinline__ uint64_t key() const { return below != 0 && seed_at != nullptr ? *seed_at : seed; }
+    // the seed, in scalar registers (the rounds' keys too, then)
+    __device__ __forceinline__ uint64_t key() const {
+        const uint64_t k = below != 0 && seed_at != nullptr ? *seed_at : seed;
+        return (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(k >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)k);
+    }
 
-    // what elements 8 piece to 8 piece + 7 of a row are multiplied by: 0 where dropped
-    __device__ __forceinline__ void factors(uint64_t key, long row, long piece, float (&f)[8]) const {
-        if (below == 0) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = 1.0f;
-            return;
-        }
+    // elements 8 piece to 8 piece + 7 of a row: 0 where dropped (also what is infinite or NaN), the others times the factor
+    __device__ __forceinline__ void thin(uint64_t key, long row, long piece, float (&v)[8]) const {
+        if (below == 0) return;
         uint32_t c0 = (uint32_t)piece, c1 = (uint32_t)row, c2 = (uint32_t)((uint64_t)row >> 32), c3 = index;
         uint32_t k0 = (uint32_t)key, k1 = (uint32_t)(key >> 32);
 #pragma unroll
@@ -49,13 +49,10 @@ struct Dropout {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const uint32_t number = i & 1 ? word[i >> 1] >> 16 : word[i >> 1] & 0xFFFFu;
-            f[i] = number < below ? 0.0f : factor;
+            v[i] = number < below ? 0.0f : v[i] * factor;
         }
     }
 };
-
-// v times its factor; what is dropped is 0 also where v is infinite or NaN
-__device__ __forceinline__ float thin(float v, float f) { return f == 0.0f ? 0.0f : v * f; }
 
 // p in 16 bits, to nearest even; -1 where it leaves nothing or is no probability
 inline int dropped_below(double p) {
