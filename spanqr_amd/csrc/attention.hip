@@ -133,28 +133,28 @@ __device__ __forceinline__ void load_lds4(const void* at, uint32_t lds) {
 // this wavefront's loads are there and its reads are done; then everybody's
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Tiles of 64 rows of DP elements in LDS (DP: D rounded up to 64 or 128, zeros behind D) and the way there and into
-// registers. The 16-byte chunk c of a row lies at c ^ swizzle(row): LDS serves lanes 0-3, 12-15, 20-27 of each 32 together and
+// Tiles of 64 rows of PITCH elements (64 or 128) in LDS, of which DP (D rounded up to a multiple of 32) are used, and the way
+// there and into registers. The 16-byte chunk c of a row lies at c ^ swizzle(row): LDS serves lanes 0-3, 12-15, 20-27 of each 32 together and
 // then the others, 256 bytes at a time, and for reads of rows (16 rows, the same chunk) as for transposing reads (4 rows,
 // 64 bytes of each) those fill the 256 bytes exactly.
-template <int DP>
+template <int PITCH>
 __device__ __forceinline__ int swizzle(int row) {
-    return DP == 128 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3);
+    return PITCH == 128 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3);
 }
 
-template <typename T, int DP>
+template <typename T, int PITCH>
 struct Reader {
     typedef typename Vec<T>::x8 x8;
-    static constexpr int ROW = 2 * DP;            // bytes
+    static constexpr int ROW = 2 * PITCH;            // bytes
     static constexpr int BYTES = TILE * ROW;
     uint32_t rows, cols[2];                       // a lane's places in a tile, or with the tile's address added
     __device__ __forceinline__ explicit Reader(int lane) {
         const int r = lane & 31, h = lane >> 5, lo = lane & 15, g = lane >> 4 & 1;
-        rows = r * ROW + ((swizzle<DP>(r) ^ h) << 4);
+        rows = r * ROW + ((swizzle<PITCH>(r) ^ h) << 4);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int k = 8 * j + 4 * h + (lo >> 2);
-            cols[j] = k * ROW + (((2 * g + (lo >> 1 & 1)) ^ swizzle<DP>(k)) << 4) + 8 * (lo & 1);
+            cols[j] = k * ROW + (((2 * g + (lo >> 1 & 1)) ^ swizzle<PITCH>(k)) << 4) + 8 * (lo & 1);
         }
     }
     __device__ __forceinline__ Reader(const Reader& r, uint32_t tile) : rows(r.rows + tile), cols{r.cols[0] + tile, r.cols[1] + tile} {}
@@ -178,16 +178,16 @@ struct Reader {
 // moves (what it has behind D is the row's last 16 bytes again: the other operand is 0 there, or the result is not used);
 // otherwise, and at the end, every lane finds its own, and reads zeros past the end.
 // KEPT: the places stay in registers; otherwise they are formed for each tile.
-template <typename T, int DP, bool KEPT>
+template <typename T, int PITCH, bool KEPT>
 struct Loader {
-    static constexpr int CHUNKS = DP / 8, LOADS = TILE * CHUNKS / 64 / WAVES;
+    static constexpr int CHUNKS = PITCH / 8, LOADS = TILE * CHUNKS / 64 / WAVES;
     const char* base;
     long row, head;       // bytes
     int G, shift, last;   // shift: of a G that divides 64; last: the row's last chunk
     uint32_t off[KEPT ? LOADS : 1];
     __device__ __forceinline__ static int row_of(int i, int wave, int lane) { return (wave * LOADS + i) * (64 / CHUNKS) + lane / CHUNKS; }
     __device__ __forceinline__ int chunk_of(int r, int lane) const {
-        const int c = lane % CHUNKS ^ swizzle<DP>(r);
+        const int c = lane % CHUNKS ^ swizzle<PITCH>(r);
         return c < last ? c : last;
     }
     // (strides are multiples of 16 bytes, below 2^25)
@@ -290,7 +290,8 @@ struct ForwardArgs {
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) {
     typedef typename Vec<T>::x8 x8;
-    typedef Reader<T, DP> R;
+    constexpr int PITCH = DP <= 64 ? 64 : 128;
+    typedef Reader<T, PITCH> R;
     __shared__ __attribute__((aligned(1024))) char smem[4 * R::BYTES];
     const Shape& s = a.s;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -309,8 +310,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
     const int M = seq.lq * s.G, ahead = seq.lk - seq.lq;   // query i stands at i + ahead
     const R read(lane);
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)smem;
-    const Loader<T, DP, true> K(head_of<T>(a.k, packed, b, seq.k0, hk), a.k, 1, s.D, wave, lane);
-    const Loader<T, DP, true> V(head_of<T>(a.v, packed, b, seq.k0, hk), a.v, 1, s.D, wave, lane);
+    const Loader<T, PITCH, true> K(head_of<T>(a.k, packed, b, seq.k0, hk), a.k, 1, s.D, wave, lane);
+    const Loader<T, PITCH, true> V(head_of<T>(a.v, packed, b, seq.k0, hk), a.v, 1, s.D, wave, lane);
     const char* q = head_of<T>(a.q, packed, b, seq.q0, hk * s.G);
     // keys of this split
     const int chunk = a.splits == 1 ? seq.lk : ((seq.lk + a.splits - 1) / a.splits + TILE - 1) / TILE * TILE;
@@ -467,42 +468,20 @@ struct BackwardArgs {
     Heads q, k, v, out, dout;
     const float* lse;
     void *dq, *dk, *dv;   // contiguous
-    float* stat;          // [2][rows of all x heads]: lse log2 e (inf where nothing is seen), D
+    float* stat;          // [2][rows of all x heads], from k_dq: lse log2 e (inf where nothing is seen), D
     long rows;
     int q_tiles, k_tiles;
     float scale;
 };
 
-// D, and lse as the gradients take it: 16 lanes a head's row, eight elements a lane
-template <typename T>
-__global__ __launch_bounds__(256) void k_delta(const BackwardArgs a) {
-    const Shape& s = a.s;
-    const int heads = s.Hk * s.G, lane = threadIdx.x & 15;
-    const int n = (int)(s.Tq * heads);   // of a sequence, or of all that are packed
-    for (int b = blockIdx.y; b < (s.q_starts != nullptr ? 1 : s.B); b += gridDim.y)
-        for (int r = blockIdx.x * 16 + (threadIdx.x >> 4); r < n; r += gridDim.x * 16) {
-            const int i = r / heads, hq = r - i * heads;
-            float o[8], d[8], sum = 0.0f;
-            const int here = s.D - 8 * lane >= 8 ? 8 : 0;
-            load8((const T*)a.out.p + b * a.out.batch + i * a.out.row + hq * a.out.head + 8 * lane, here, o);
-            load8((const T*)a.dout.p + b * a.dout.batch + i * a.dout.row + hq * a.dout.head + 8 * lane, here, d);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(o[e], d[e], sum);
-            sum = reduce_lanes<16, Sum>(sum);
-            if (lane == 0) {
-                const long at = (long)b * n + r;
-                const float lse = a.lse[at];
-                a.stat[at] = lse == -INFINITY ? INFINITY : lse * LOG2E;
-                a.stat[a.rows + at] = sum;
-            }
-        }
-}
-
-// dQ: as the forward pass, 128 rows a workgroup; a lane has one query
+// dQ: as the forward pass, 128 rows a workgroup; a lane has one query. It has dO in registers, so it forms D first, and leaves it
+// and lse as the gradients take it for the keys' kernel (a pass of its own over O and dO took 15 us of 200 at 16 x 1024 x 12 x 64).
+// Without dq that is all it does.
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
     typedef typename Vec<T>::x8 x8;
-    typedef Reader<T, DP> R;
+    constexpr int PITCH = DP <= 64 ? 64 : 128;
+    typedef Reader<T, PITCH> R;
     __shared__ __attribute__((aligned(1024))) char smem[4 * R::BYTES];
     const Shape& s = a.s;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -511,18 +490,20 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
     const int which = blockIdx.x % many, first = a.q_tiles - 1 - blockIdx.x / many;
     const int b = which / s.Hk, hk = which % s.Hk;
     if (b == s.B) {
-        outside((T*)a.dq, nullptr, clip_start(s.q_starts[0], s.Tq), clip_start(s.q_starts[s.B], s.Tq), s.Tq, (long)s.Hk * s.G * s.D, 0,
-                first * s.Hk + hk, a.q_tiles * s.Hk);
+        if (a.dq != nullptr)
+            outside((T*)a.dq, nullptr, clip_start(s.q_starts[0], s.Tq), clip_start(s.q_starts[s.B], s.Tq), s.Tq, (long)s.Hk * s.G * s.D, 0,
+                    first * s.Hk + hk, a.q_tiles * s.Hk);
         return;
     }
     const Seq seq = seq_of(s, b);
     const int M = seq.lq * s.G, ahead = seq.lk - seq.lq;
     const R read(lane);
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)smem;
-    const Loader<T, DP, true> K(head_of<T>(a.k, packed, b, seq.k0, hk), a.k, 1, s.D, wave, lane);
-    const Loader<T, DP, true> V(head_of<T>(a.v, packed, b, seq.k0, hk), a.v, 1, s.D, wave, lane);
+    const Loader<T, PITCH, true> K(head_of<T>(a.k, packed, b, seq.k0, hk), a.k, 1, s.D, wave, lane);
+    const Loader<T, PITCH, true> V(head_of<T>(a.v, packed, b, seq.k0, hk), a.v, 1, s.D, wave, lane);
     const char* q = head_of<T>(a.q, packed, b, seq.q0, hk * s.G);
     const char* d_out = head_of<T>(a.dout, packed, b, seq.q0, hk * s.G);
+    const char* out = head_of<T>(a.out, packed, b, seq.q0, hk * s.G);
 
     for (int tile = first; (long)tile * BLOCK < M; tile += a.q_tiles) {
         const int m0 = tile * BLOCK, w0 = m0 + 32 * wave, m = w0 + (lane & 31);
@@ -532,7 +513,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
         x8 fq[DP / 16], fd[DP / 16];
         load_row<T, DP>(q + (long)sizeof(T) * (i * a.q.row + g * a.q.head), on, s.D, lane, fq);
         load_row<T, DP>(d_out + (long)sizeof(T) * (i * a.dout.row + g * a.dout.head), on, s.D, lane, fd);
-        const float lse = on ? a.stat[at] : INFINITY, delta = on ? a.stat[a.rows + at] : 0.0f;
+        float lse = INFINITY, delta = 0.0f;
+        {
+            x8 fo[DP / 16];
+            load_row<T, DP>(out + (long)sizeof(T) * (i * a.out.row + g * a.out.head), on, s.D, lane, fo);
+            if (on) lse = a.lse[at] == -INFINITY ? INFINITY : a.lse[at] * LOG2E;
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) delta = fmaf((float)fo[ks][e], (float)fd[ks][e], delta);
+            delta = both_halves(delta, [](float x, float y) { return x + y; });
+            if (on && h == 0) {
+                a.stat[at] = lse;
+                a.stat[a.rows + at] = delta;
+            }
+        }
+        if (a.dq == nullptr) continue;
         const int k_to = seq.lk;
         const int hi = s.causal ? (i + ahead + 1 < k_to ? i + ahead + 1 : k_to) : k_to;
         const int lo = s.window && i + ahead - s.window + 1 > 0 ? i + ahead - s.window + 1 : 0;
@@ -597,7 +593,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_dkv(const BackwardArgs a) {
     typedef typename Vec<T>::x8 x8;
-    typedef Reader<T, DP> R;
+    constexpr int PITCH = DP <= 64 ? 64 : 128;
+    typedef Reader<T, PITCH> R;
     constexpr int BUFFER = 2 * R::BYTES;
     __shared__ __attribute__((aligned(1024))) char smem[2 * BUFFER + 2 * 2 * TILE * 4];
     const Shape& s = a.s;
@@ -616,8 +613,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dkv(const BackwardArgs a) {
     const int M = seq.lq * s.G, ahead = seq.lk - seq.lq;
     const R read(lane);
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)smem, stats = lds + 2 * BUFFER;
-    const Loader<T, DP, DP == 64> Q(head_of<T>(a.q, packed, b, seq.q0, hk * s.G), a.q, s.G, s.D, wave, lane);
-    const Loader<T, DP, DP == 64> DO(head_of<T>(a.dout, packed, b, seq.q0, hk * s.G), a.dout, s.G, s.D, wave, lane);
+    const Loader<T, PITCH, PITCH == 64> Q(head_of<T>(a.q, packed, b, seq.q0, hk * s.G), a.q, s.G, s.D, wave, lane);
+    const Loader<T, PITCH, PITCH == 64> DO(head_of<T>(a.dout, packed, b, seq.q0, hk * s.G), a.dout, s.G, s.D, wave, lane);
     const float* stat = a.stat + seq.q0 * (s.Hk * s.G) + hk * s.G;
     const char* k = head_of<T>(a.k, packed, b, seq.k0, hk);
     const char* v = head_of<T>(a.v, packed, b, seq.k0, hk);
@@ -777,37 +774,36 @@ int check_heads(const char* what, const char* name, const void* p, const long* s
 }
 bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
 
+#define SPANQR_HEADS(LAUNCH)            \
+    if (s.D <= 32) LAUNCH(32);          \
+    else if (s.D <= 64) LAUNCH(64);     \
+    else if (s.D <= 96) LAUNCH(96);     \
+    else LAUNCH(128);
+
 template <typename T>
 void launch_forward(const ForwardArgs& a, hipStream_t st) {
     const Shape& s = a.s;
     const bool tail = s.q_starts != nullptr && a.splits == 1;
     const int grid = (s.B + (tail ? 1 : 0)) * s.Hk * a.tiles * a.splits;
-    if (s.D <= 64)
-        k_forward<T, 64><<<grid, 64 * WAVES, 0, st>>>(a);
-    else
-        k_forward<T, 128><<<grid, 64 * WAVES, 0, st>>>(a);
+#define LAUNCH(DP) k_forward<T, DP><<<grid, 64 * WAVES, 0, st>>>(a)
+    SPANQR_HEADS(LAUNCH)
+#undef LAUNCH
     if (a.splits > 1) k_join<T><<<(int)(a.rows < 65536 ? a.rows : 65536), 64 * WAVES, 0, st>>>(a);
 }
 
 template <typename T>
 void launch_backward(const BackwardArgs& a, hipStream_t st) {
     const Shape& s = a.s;
-    const bool packed = s.q_starts != nullptr;
-    const long n = s.Tq * s.Hk * s.G;
-    if (a.rows > 0)
-        k_delta<T><<<dim3((int)(n < 16 * 65536 ? (n + 15) / 16 : 65536), packed ? 1 : s.B < 65535 ? s.B : 65535), 256, 0, st>>>(a);
-    const int heads = (s.B + (packed ? 1 : 0)) * s.Hk;
-    if (a.dk != nullptr && heads > 0 && s.Tk > 0) {
-        if (s.D <= 64)
-            k_dkv<T, 64><<<heads * a.k_tiles, 64 * WAVES, 0, st>>>(a);
-        else
-            k_dkv<T, 128><<<heads * a.k_tiles, 64 * WAVES, 0, st>>>(a);
+    const int heads = (s.B + (s.q_starts != nullptr ? 1 : 0)) * s.Hk;
+    if (a.rows > 0) {
+#define LAUNCH(DP) k_dq<T, DP><<<heads * a.q_tiles, 64 * WAVES, 0, st>>>(a)
+        SPANQR_HEADS(LAUNCH)
+#undef LAUNCH
     }
-    if (a.dq != nullptr && a.rows > 0) {
-        if (s.D <= 64)
-            k_dq<T, 64><<<heads * a.q_tiles, 64 * WAVES, 0, st>>>(a);
-        else
-            k_dq<T, 128><<<heads * a.q_tiles, 64 * WAVES, 0, st>>>(a);
+    if (a.dk != nullptr && heads > 0 && s.Tk > 0) {
+#define LAUNCH(DP) k_dkv<T, DP><<<heads * a.k_tiles, 64 * WAVES, 0, st>>>(a)
+        SPANQR_HEADS(LAUNCH)
+#undef LAUNCH
     }
 }
 
