@@ -118,7 +118,7 @@ __device__ __forceinline__ const char* head_of(const Heads& h, bool packed, int 
 
 // what a load reads outside a matrix: elements past D, rows past the end
 __device__ const uint32_t __attribute__((aligned(16))) nothing[4] = {0, 0, 0, 0};
-__device__ const float no_row[2] = {INFINITY, 0.0f};   // lse and D of a row past the end
+__device__ const float no_row[2] = {INFINITY, 0.0f};   // lse and -D of a row past the end
 
 // 16 bytes (4) a lane to LDS at `lds` + 16 lane (4 lane), asynchronously: counted by vmcnt, which `arrived` waits for
 __device__ __forceinline__ void load_lds(const char* base, uint32_t off, uint32_t lds) {
@@ -173,45 +173,65 @@ struct Reader {
     }
 };
 
-// Loads of tiles of 64 rows m of one sequence and key head, m / G being the row in memory and m % G the head. Where G divides
-// 64 a lane's places in a tile are the same in every tile, and a tile inside the matrix is loaded from a base that
-// moves (what it has behind D is the row's last 16 bytes again: the other operand is 0 there, or the result is not used);
-// otherwise, and at the end, every lane finds its own, and reads zeros past the end.
-// KEPT: the places stay in registers; otherwise they are formed for each tile.
+// Loads of tiles of rows m of one sequence and key head, m / G being the row in memory and m % G the head. A tile has
+// rows_of_tile(G) rows, whole rows in memory, so that a lane's places are the same in every tile, and a tile inside the matrix
+// is loaded from a base that moves. (What it has behind D is the row's last 16 bytes again: the other operand is 0 there, or
+// the result is not used. What it has behind its rows is the last one again: there the probabilities are 0.) At the matrix's end
+// every lane finds its own, and reads zeros past it. Groups of which a tile's whole rows would leave too much empty are
+// taken 64 rows a tile, each lane finding its own always.
+// KEPT: the places stay in registers; otherwise in LDS, a lane's own words.
+__device__ __forceinline__ int rows_of_tile(int G) {
+    const int n = G <= TILE ? TILE / G * G : 0;
+    return n >= TILE - 8 ? n : TILE;
+}
 template <typename T, int PITCH, bool KEPT>
 struct Loader {
     static constexpr int CHUNKS = PITCH / 8, LOADS = TILE * CHUNKS / 64 / WAVES;
+    static constexpr int TABLE = KEPT ? 0 : 16 * 64 * WAVES;   // bytes of LDS
+    static_assert(KEPT || LOADS == 4, "");
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) u32x4 lds_u4;
     const char* base;
     long row, head;       // bytes
-    int G, shift, last;   // shift: of a G that divides 64; last: the row's last chunk
-    uint32_t off[KEPT ? LOADS : 1];
+    int G, rows, last;    // last: the row's last chunk
+    uint32_t table, off[KEPT ? LOADS : 1];
     __device__ __forceinline__ static int row_of(int i, int wave, int lane) { return (wave * LOADS + i) * (64 / CHUNKS) + lane / CHUNKS; }
     __device__ __forceinline__ int chunk_of(int r, int lane) const {
         const int c = lane % CHUNKS ^ swizzle<PITCH>(r);
         return c < last ? c : last;
     }
-    // (strides are multiples of 16 bytes, below 2^25)
-    __device__ __forceinline__ uint32_t place(int i, int wave, int lane) const {
-        const int r = row_of(i, wave, lane);
-        return 16 * (__umul24(r >> shift, (uint32_t)row >> 4) + __umul24(r & (1 << shift) - 1, (uint32_t)head >> 4) + chunk_of(r, lane));
-    }
-    __device__ __forceinline__ Loader(const char* base, const Heads& h, int G, int D, int wave, int lane)
-        : base(base), row((long)sizeof(T) * h.row), head((long)sizeof(T) * h.head), G(G), shift(__builtin_ctz(G)), last(D / 8 - 1) {
-        if constexpr (KEPT) {
+    __device__ __forceinline__ Loader(const char* base, const Heads& h, int G, int D, int wave, int lane, uint32_t table = 0)
+        : base(base), row((long)sizeof(T) * h.row), head((long)sizeof(T) * h.head), G(G), rows(rows_of_tile(G)), last(D / 8 - 1), table(table) {
+        u32x4 all;
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) off[i] = place(i, wave, lane);
+        for (int i = 0; i < LOADS; ++i) {
+            const int r = row_of(i, wave, lane), m = r < rows ? r : rows - 1;
+            // (strides stay below 2^25 bytes)
+            const uint32_t at = (uint32_t)(m / G) * (uint32_t)row + (uint32_t)(m % G) * (uint32_t)head + 16 * chunk_of(r, lane);
+            if constexpr (KEPT)
+                off[i] = at;
+            else
+                all[i] = at;
         }
+        if constexpr (!KEPT) *(lds_u4*)(uintptr_t)(table + 16 * threadIdx.x) = all;
     }
-    // rows m0 (a multiple of 64) to m0 + 63 of M into the tile at lds
+    // the tile of rows from m0 (a multiple of `rows`) on, of M, into LDS
     __device__ __forceinline__ void load(int m0, int M, uint32_t lds, int wave, int lane) const {
         const uint32_t to = lds + wave * LOADS * 1024;
-        const bool inside = TILE % G == 0 && m0 + TILE <= M;
-        if (!KEPT || !inside) asm volatile("" : "+v"(lane));   // (formed here: hoisted, the places would fill the registers)
-        if (inside) {
-            const char* from = base + (m0 >> shift) * row;
+        if (rows % G == 0 && m0 + rows <= M) {
+            const char* from = base + (m0 / G) * row;
+            if constexpr (KEPT) {
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) load_lds(from, KEPT ? off[KEPT ? i : 0] : place(i, wave, lane), to + i * 1024);
+                for (int i = 0; i < LOADS; ++i) load_lds(from, off[i], to + i * 1024);
+            } else {
+                uint32_t mine = threadIdx.x;
+                asm volatile("" : "+v"(mine));
+                const u32x4 all = *(const lds_u4*)(uintptr_t)(table + 16 * mine);
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) load_lds(from, all[i], to + i * 1024);
+            }
         } else {
+            asm volatile("" : "+v"(lane));   // (formed here: hoisted, the places would fill the registers)
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int r = row_of(i, wave, lane), m = m0 + r, q = m / G;
@@ -343,11 +363,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
             V.load(from, seq.lk, lds + R::BYTES, wave, lane);
         }
         uint32_t now = lds;
-        for (int n0 = from; n0 < to; n0 += TILE, now ^= 2 * R::BYTES) {
+        for (int n0 = from; n0 < to; n0 += TILE, now = 2 * lds + 2 * R::BYTES - now) {
             arrived();
             if (n0 + TILE < to) {
-                K.load(n0 + TILE, seq.lk, now ^ 2 * R::BYTES, wave, lane);
-                V.load(n0 + TILE, seq.lk, (now ^ 2 * R::BYTES) + R::BYTES, wave, lane);
+                const uint32_t other = 2 * lds + 2 * R::BYTES - now;
+                K.load(n0 + TILE, seq.lk, other, wave, lane);
+                V.load(n0 + TILE, seq.lk, other + R::BYTES, wave, lane);
             }
             if (n0 >= any_hi || n0 + TILE <= any_lo) continue;
             const R in(read, now);
@@ -468,7 +489,7 @@ struct BackwardArgs {
     Heads q, k, v, out, dout;
     const float* lse;
     void *dq, *dk, *dv;   // contiguous
-    float* stat;          // [2][rows of all x heads], from k_dq: lse log2 e (inf where nothing is seen), D
+    float* stat;          // [2][rows of all x heads], from k_dq: lse log2 e (inf where nothing is seen), -D
     long rows;
     int q_tiles, k_tiles;
     float scale;
@@ -525,10 +546,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
             delta = both_halves(delta, [](float x, float y) { return x + y; });
             if (on && h == 0) {
                 a.stat[at] = lse;
-                a.stat[a.rows + at] = delta;
+                a.stat[a.rows + at] = -delta;
             }
         }
         if (a.dq == nullptr) continue;
+        f32x16 start;   // of dP - D's sum
+#pragma unroll
+        for (int r = 0; r < 16; ++r) start[r] = -delta;
         const int k_to = seq.lk;
         const int hi = s.causal ? (i + ahead + 1 < k_to ? i + ahead + 1 : k_to) : k_to;
         const int lo = s.window && i + ahead - s.window + 1 > 0 ? i + ahead - s.window + 1 : 0;
@@ -548,11 +572,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
             V.load(from, seq.lk, lds + R::BYTES, wave, lane);
         }
         uint32_t now = lds;
-        for (int n0 = from; n0 < to; n0 += TILE, now ^= 2 * R::BYTES) {
+        for (int n0 = from; n0 < to; n0 += TILE, now = 2 * lds + 2 * R::BYTES - now) {
             arrived();
             if (n0 + TILE < to) {
-                K.load(n0 + TILE, seq.lk, now ^ 2 * R::BYTES, wave, lane);
-                V.load(n0 + TILE, seq.lk, (now ^ 2 * R::BYTES) + R::BYTES, wave, lane);
+                const uint32_t other = 2 * lds + 2 * R::BYTES - now;
+                K.load(n0 + TILE, seq.lk, other, wave, lane);
+                V.load(n0 + TILE, seq.lk, other + R::BYTES, wave, lane);
             }
             if (n0 >= any_hi || n0 + TILE <= any_lo) continue;
             const bool masked = n0 + TILE > all_hi || n0 < all_lo;
@@ -560,14 +585,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 in.fresh();
-                f32x16 z = {}, dp = {};
+                f32x16 z = {}, dp = start;
 #pragma unroll
                 for (int ks = 0; ks < DP / 16; ++ks) {
                     z = mfma(in.row(0, t, ks), fq[ks], z);
                     dp = mfma(in.row(R::BYTES, t, ks), fd[ks], dp);
                 }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], s.scale2, -lse)) * (dp[r] - delta);
+                for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], s.scale2, -lse)) * dp[r];
                 if (masked) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
@@ -589,14 +614,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
 }
 
 // dK and dV: 128 keys a workgroup, a wavefront 32 of them in registers (a lane one key), over all rows of the group's
-// queries that see them, in tiles of 64
+// queries that see them, in tiles of 64 (or as many whole queries' rows as that holds)
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * WAVES, 2) void k_dkv(const BackwardArgs a) {
+__global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const BackwardArgs a) {
     typedef typename Vec<T>::x8 x8;
     constexpr int PITCH = DP <= 64 ? 64 : 128;
     typedef Reader<T, PITCH> R;
-    constexpr int BUFFER = 2 * R::BYTES;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * BUFFER + 2 * 2 * TILE * 4];
+    typedef Loader<T, PITCH, PITCH == 64> L;
+    constexpr int BUFFER = 2 * R::BYTES, STATS = 2 * 2 * TILE * 4 + 256;   // (and a lane's place in a tile's statistics)
+    __shared__ __attribute__((aligned(1024))) char smem[2 * BUFFER + STATS + 2 * L::TABLE];
     const Shape& s = a.s;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const bool packed = s.q_starts != nullptr;
@@ -613,18 +639,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dkv(const BackwardArgs a) {
     const int M = seq.lq * s.G, ahead = seq.lk - seq.lq;
     const R read(lane);
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)smem, stats = lds + 2 * BUFFER;
-    const Loader<T, PITCH, PITCH == 64> Q(head_of<T>(a.q, packed, b, seq.q0, hk * s.G), a.q, s.G, s.D, wave, lane);
-    const Loader<T, PITCH, PITCH == 64> DO(head_of<T>(a.dout, packed, b, seq.q0, hk * s.G), a.dout, s.G, s.D, wave, lane);
+    const L Q(head_of<T>(a.q, packed, b, seq.q0, hk * s.G), a.q, s.G, s.D, wave, lane, stats + STATS);
+    const L DO(head_of<T>(a.dout, packed, b, seq.q0, hk * s.G), a.dout, s.G, s.D, wave, lane, stats + STATS + L::TABLE);
+    const int rows = Q.rows;   // of a tile
+    typedef __attribute__((address_space(3))) int lds_int;
+    if (wave < 2) *(lds_int*)(uintptr_t)(stats + 1024 + 4 * lane) = lane / s.G * (s.Hk * s.G) + lane % s.G;   // (both the same)
     const float* stat = a.stat + seq.q0 * (s.Hk * s.G) + hk * s.G;
     const char* k = head_of<T>(a.k, packed, b, seq.k0, hk);
     const char* v = head_of<T>(a.v, packed, b, seq.k0, hk);
     auto load = [&](int m0, int buffer) {
         Q.load(m0, M, lds + buffer * BUFFER, wave, lane);
         DO.load(m0, M, lds + buffer * BUFFER + R::BYTES, wave, lane);
-        if (wave < 2) {   // lse by one wavefront, D by another
-            const int m = m0 + lane, i = m / s.G;
-            const float* from = m < M ? stat + wave * a.rows + i * (s.Hk * s.G) + (m - i * s.G) : no_row + wave;
-            load_lds4(from, stats + (2 * buffer + wave) * TILE * 4);
+        if (wave < 2) {   // lse by one wavefront, -D by another
+            int mine = lane;
+            asm volatile("" : "+v"(mine));   // (nothing of it is kept)
+            const int m = m0 + mine, heads = s.Hk * s.G;
+            const long at = rows % s.G == 0 ? (long)(m0 / s.G) * heads + *(const lds_int*)(uintptr_t)(stats + 1024 + 4 * mine)
+                                            : (long)(m / s.G) * heads + m % s.G;
+            load_lds4(m < M && mine < rows ? stat + wave * a.rows + at : no_row + wave, stats + (2 * buffer + wave) * TILE * 4);
         }
     };
 
@@ -647,31 +679,38 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dkv(const BackwardArgs a) {
         const int last = w0 + 31 < seq.lk ? w0 + 31 : seq.lk - 1, block_last = n0 + BLOCK < seq.lk ? n0 + BLOCK - 1 : seq.lk - 1;
         const int any_lo = first_row(w0), any_hi = w0 < seq.lk ? end_row(last) : 0;
         const int all_lo = first_row(last), all_hi = w0 + 32 <= seq.lk ? end_row(w0) : 0;
-        const int from = first_row(n0) & ~(TILE - 1), to = end_row(block_last);
+        const int from = first_row(n0) / rows * rows, to = end_row(block_last);
 
         f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
         if (from < to) load(from, 0);
         int buffer = 0;
-        for (int m0 = from; m0 < to; m0 += TILE, buffer ^= 1) {
+        for (int m0 = from; m0 < to; m0 += rows, buffer ^= 1) {
             arrived();
-            if (m0 + TILE < to) load(m0 + TILE, buffer ^ 1);
-            R in(read, lds + buffer * BUFFER);
+            if (m0 + rows < to) load(m0 + rows, buffer ^ 1);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int r0 = m0 + 32 * t;
                 if (r0 >= any_hi || r0 + 32 <= any_lo) continue;
+                R in(read, lds + buffer * BUFFER);
                 in.fresh();
-                f32x16 z = {}, dp = {};
+                // four rows' lse or -D
+                auto stat4 = [&](int which, int q4) {
+                    const uint32_t at = stats + ((2 * buffer + which) * TILE + 32 * t + 8 * q4 + 4 * h) * 4;
+                    return *(__attribute__((address_space(3))) const f32x4*)(uintptr_t)at;
+                };
+                // dP - D: the sum starts at -D
+                f32x16 z = {}, dp;
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const f32x4 d = stat4(1, q4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = d[e];
+                }
 #pragma unroll
                 for (int ks = 0; ks < DP / 16; ++ks) {
                     z = mfma(in.row(0, t, ks), fk[ks], z);
                     dp = mfma(in.row(R::BYTES, t, ks), fv[ks], dp);
                 }
-                // four rows' lse or D
-                auto stat4 = [&](int which, int q4) {
-                    const uint32_t at = stats + ((2 * buffer + which) * TILE + 32 * t + 8 * q4 + 4 * h) * 4;
-                    return *(__attribute__((address_space(3))) const f32x4*)(uintptr_t)at;
-                };
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) {
                     const f32x4 lse = stat4(0, q4);
@@ -689,11 +728,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dkv(const BackwardArgs a) {
                     }
                 }
 #pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) {
-                    const f32x4 delta = stat4(1, q4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = z[4 * q4 + e] * (dp[4 * q4 + e] - delta[e]);
-                }
+                for (int r = 0; r < 16; ++r) dp[r] *= z[r];
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
                     const x8 p = half_of<T>(z, st), ds = half_of<T>(dp, st);
