@@ -409,7 +409,8 @@ int spanqr_attention(int type, long B, long Hk, long G, long D, long Tq, long Tk
 /* Gradient of it, from dout, and from out and lse as they came out: dq as out lies, dk and dv [key rows][Hk][D] (both or
  * neither; dq or null), contiguous, zeros for rows of no sequence. P and dS are rounded to the type before the products that
  * they go into. workspace: spanqr_attention_backward_workspace bytes. */
-long spanqr_attention_backward_workspace(long B, long Hk, long G, long D, long Tq, long Tk, int packed);
+long spanqr_attention_backward_workspace(long B, long Hk, long G, long D, long Tq, long Tk, int packed, long max_q,
+                                         long max_k);
 int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq, long Tk, const void* dout,
                               const long* dout_strides, const void* q, const long* q_strides, const void* k,
                               const long* k_strides, const void* v, const long* v_strides, const void* out,

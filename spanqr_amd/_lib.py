@@ -86,7 +86,7 @@ SIGNATURES = {
     "spanqr_attention_workspace": (_L, [_L, _L, _L, _L, _L, _L, _I, _L, _L]),
     "spanqr_attention": (_I, [_I, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _L, _L, _I, _L, _F, _P, _P, _P, _L,
                               _P]),
-    "spanqr_attention_backward_workspace": (_L, [_L, _L, _L, _L, _L, _L, _I]),
+    "spanqr_attention_backward_workspace": (_L, [_L, _L, _L, _L, _L, _L, _I, _L, _L]),
     "spanqr_attention_backward": (_I, [_I, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _L,
                                        _I, _L, _F, _P, _P, _P, _P, _L, _P]),
 }

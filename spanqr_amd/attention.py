@@ -2,32 +2,32 @@
 makes the probabilities again, through the native library (csrc/attention.hip). No counterpart in the reference; its
 projections are among the layers that the optimizer keeps orthonormal with orth.
 """
-import ctypes
+import functools
+from array import array
 
 import torch
 
 from . import _lib
-from .tensors import TYPES, check_like, check_same, check_tensor, no_tangents, on, once, workspace
+from .tensors import TYPES, check_like, check_same, check_tensor, like, no_tangents, on, once, workspace
 
 MAX_STRIDE = 1 << 24   # of rows and heads, in elements
 MAX_HEAD = 128
 
 
 def _heads(t):
-    """t [..., heads, D] with neighbouring elements of a head, every head's row on 16 bytes, and strides that the library's
-    offsets reach: as it lies, or copied"""
-    strides = t.stride()
-    if (strides[-1] == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0 and all(
-            n == 1 or (s % 8 == 0 and (s < MAX_STRIDE or i == t.dim() - 4)) for i, (n, s) in
-            enumerate(zip(t.shape[:-1], strides))):
-        return t
-    return t.contiguous()
-
-
-def _strides(t):
-    """{batch, row, head} for the C ABI; axes of one element have none"""
-    s = [0 if n == 1 else v for n, v in zip(t.shape[:-1], t.stride())]
-    return (ctypes.c_long * 3)(*([0] * (3 - len(s)) + s))
+    """(t, its strides {batch, row, head}): neighbouring elements of a head, every head's row on 16 bytes, and strides that the
+    library's offsets reach; as it lies, or copied"""
+    s = t.stride()
+    if s[-1] != 1 or (s[0] | s[-2] | s[-3]) & 7 or s[-2] >= MAX_STRIDE or s[-3] >= MAX_STRIDE:
+        if not ((s[-1] == 1 or t.shape[-1] == 1) and all(
+                n == 1 or (v % 8 == 0 and (v < MAX_STRIDE or i == t.dim() - 4)) for i, (n, v) in enumerate(zip(t.shape[:-1], s)))):
+            t = t.contiguous()
+            s = t.stride()
+        s = tuple(0 if n == 1 else v for n, v in zip(t.shape, s))   # (axes of one element have any)
+    if t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s = t.stride()
+    return t, (s[:3] if t.dim() == 4 else (0, *s[:2]))
 
 
 def _check(what, q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_k):
@@ -42,13 +42,16 @@ def _check(what, q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_
         if t.dim() != axes:
             raise ValueError(f"{what}: {name} must be " + ("[rows, heads, D] with q_starts" if packed else "[B, S, heads, D]") +
                              f", got {list(t.shape)}")
-    D, heads, key_heads = q.shape[-1], q.shape[-2], k.shape[-2]
+    *lead, Tq, heads, D = q.shape
+    Tk, key_heads = k.shape[-3:-1]
     if D < 8 or D > MAX_HEAD or D % 8:
         raise ValueError(f"{what}: D must be a multiple of 8 from 8 to {MAX_HEAD}, got {D}")
     if heads < 1 or key_heads < 1 or heads % key_heads:
         raise ValueError(f"{what}: q's {heads} heads must be a multiple of k's {key_heads}, one at least")
-    check_same(what, "k", k, q.device, (*(() if packed else (q.shape[0],)), k.shape[-3], key_heads, D), q.dtype)
-    check_same(what, "v", v, q.device, k.shape, q.dtype)
+    key_shape = (*lead, Tk, key_heads, D)
+    if not (like(k, q, key_shape) and like(v, q, key_shape)):
+        check_same(what, "k", k, q.device, key_shape, q.dtype)
+        check_same(what, "v", v, q.device, key_shape, q.dtype)
     if window is not None:
         window = int(window)
         if window < 1 or not causal:
@@ -58,8 +61,8 @@ def _check(what, q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_
         raise ValueError(f"{what}: scale must be positive and finite, got {scale}")
     if packed:
         if k_starts is None:
-            if q.shape[0] != k.shape[0]:
-                raise ValueError(f"{what}: without k_starts q and k have the same rows, got {q.shape[0]} and {k.shape[0]}")
+            if Tq != Tk:
+                raise ValueError(f"{what}: without k_starts q and k have the same rows, got {Tq} and {Tk}")
             k_starts = q_starts
             max_k = max_q if max_k is None else max_k
         for name, t in (("q_starts", q_starts), ("k_starts", k_starts)):
@@ -69,17 +72,23 @@ def _check(what, q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_
             if t.dim() != 1 or t.numel() < 1 or t.numel() != q_starts.numel():
                 raise ValueError(f"{what}: q_starts and k_starts must be [B + 1], of one length")
         B = q_starts.numel() - 1
+        q_starts, k_starts = q_starts.contiguous(), k_starts.contiguous()
     else:
-        B = q.shape[0]
+        B = lead[0]
     for name, n in (("max_q", max_q), ("max_k", max_k)):
         if n is not None and int(n) < 0:
             raise ValueError(f"{what}: {name} must not be negative, got {n}")
-    shape = B, key_heads, heads // key_heads, D, q.shape[-3], k.shape[-3]
-    return shape, window or 0, scale, q_starts, k_starts, int(max_q or 0), int(max_k or 0)
+    return (B, key_heads, heads // key_heads, D, Tq, Tk), window or 0, scale, q_starts, k_starts, int(max_q or 0), int(max_k or 0)
 
 
-def _starts(t):
-    return None if t is None else t.contiguous()
+@functools.lru_cache(maxsize=256)
+def _workspace(backward, *sizes):
+    """bytes, by sizes alone"""
+    lib = _lib.lib()
+    nbytes = (lib.spanqr_attention_backward_workspace if backward else lib.spanqr_attention_workspace)(*sizes)
+    if nbytes < 0:
+        _lib.check(nbytes)
+    return nbytes
 
 
 def _at(t):
@@ -88,38 +97,38 @@ def _at(t):
 
 def _forward(q, k, v, causal, how, need_lse):
     shape, window, scale, q_starts, k_starts, max_q, max_k = how
-    q, k, v, q_starts, k_starts = _heads(q), _heads(k), _heads(v), _starts(q_starts), _starts(k_starts)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if need_lse else None
-    lib, ws = _lib.lib(), None
-    with on(q.device) as stream:
-        nbytes = lib.spanqr_attention_workspace(*shape, q_starts is not None, max_q, max_k)
-        if nbytes < 0:
-            _lib.check(nbytes)
-        if nbytes:
-            ws = workspace(nbytes, q.device)
-        _lib.check(lib.spanqr_attention(
-            TYPES[q.dtype], *shape, q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), _at(q_starts),
-            _at(k_starts), max_q, max_k, causal, window, scale, out.data_ptr(), _at(lse), _at(ws), nbytes, stream))
+    (q, qs), (k, ks), (v, vs) = _heads(q), _heads(k), _heads(v)
+    strides = array("q", qs + ks + vs)
+    at = strides.buffer_info()[0]
+    dev = q.device
+    with on(dev) as stream:
+        nbytes = _workspace(False, *shape, q_starts is not None, max_q, max_k)
+        ws = workspace(nbytes, dev) if nbytes else None
+        _lib.check(_lib.lib().spanqr_attention(
+            TYPES[q.dtype], *shape, q.data_ptr(), at, k.data_ptr(), at + 24, v.data_ptr(), at + 48, _at(q_starts), _at(k_starts),
+            max_q, max_k, causal, window, scale, out.data_ptr(), _at(lse), _at(ws), nbytes, stream))
     return out, lse
 
 
 def _backward(dout, q, k, v, out, lse, causal, how, need_dq, need_dkv):
     shape, window, scale, q_starts, k_starts, max_q, max_k = how
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_dq else None
-    dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) if need_dkv else None for _ in range(2))
-    dout, q, k, v, out = (_heads(t) for t in (dout, q, k, v, out))
-    lse, q_starts, k_starts = lse.contiguous(), _starts(q_starts), _starts(k_starts)
-    lib = _lib.lib()
-    with on(q.device) as stream:
-        nbytes = lib.spanqr_attention_backward_workspace(*shape, q_starts is not None)
-        if nbytes < 0:
-            _lib.check(nbytes)
-        ws = workspace(nbytes, q.device)
-        _lib.check(lib.spanqr_attention_backward(
-            TYPES[q.dtype], *shape, dout.data_ptr(), _strides(dout), q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
-            v.data_ptr(), _strides(v), out.data_ptr(), _strides(out), lse.data_ptr(), _at(q_starts), _at(k_starts), max_q, max_k,
-            causal, window, scale, _at(dq), _at(dk), _at(dv), ws.data_ptr(), nbytes, stream))
+    dev = q.device
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_dq else None
+    dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_dkv else None
+    dv = torch.empty_like(dk) if need_dkv else None
+    (dout, ds), (q, qs), (k, ks), (v, vs), (out, os) = map(_heads, (dout, q, k, v, out))
+    strides = array("q", ds + qs + ks + vs + os)
+    at = strides.buffer_info()[0]
+    lse = lse.contiguous()
+    with on(dev) as stream:
+        nbytes = _workspace(True, *shape, q_starts is not None, max_q, max_k)
+        ws = workspace(nbytes, dev)
+        _lib.check(_lib.lib().spanqr_attention_backward(
+            TYPES[q.dtype], *shape, dout.data_ptr(), at, q.data_ptr(), at + 24, k.data_ptr(), at + 48, v.data_ptr(), at + 72,
+            out.data_ptr(), at + 96, lse.data_ptr(), _at(q_starts), _at(k_starts), max_q, max_k, causal, window, scale, _at(dq),
+            _at(dk), _at(dv), ws.data_ptr(), nbytes, stream))
     return dq, dk, dv
 
 

@@ -34,13 +34,12 @@ def _numbers(what, p, seed, index, device):
     return p, int(seed) & (1 << 64) - 1, None, index
 
 
-def _dropout(x, p, seed, index):
+def _dropout(x, p, number, at, index):
     D = x.shape[-1] if x.dim() else 1
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if x.numel() == 0:
         return y
     x2 = rows_of(x, D)
-    p, number, at, index = _numbers("dropout", p, seed, index, x.device)
     with on(x.device) as stream:
         _lib.check(_lib.lib().spanqr_dropout(TYPES[x.dtype], x2.shape[0], D, x2.data_ptr(), x2.stride(0), p, number, at, index,
                                              y.data_ptr(), stream))
@@ -54,7 +53,7 @@ class _Dropout(torch.autograd.Function):
         ctx.number = None if isinstance(seed, torch.Tensor) else seed
         if ctx.number is None and seed is not None:
             ctx.save_for_backward(seed)   # (changed in place before the backward pass it would give another mask)
-        return _dropout(x, p, seed, index)
+        return _dropout(x, *_numbers("dropout", p, seed, index, x.device))
 
     @staticmethod
     def backward(ctx, dy):
@@ -77,10 +76,10 @@ def dropout(x, p, seed=None, index=0):
     Differentiable in x any number of times."""
     no_tangents("dropout", x)
     check_tensor("dropout", "x", x)
-    _numbers("dropout", p, seed, index, x.device)
+    numbers = _numbers("dropout", p, seed, index, x.device)
     if torch.is_grad_enabled() and x.requires_grad:
         return _Dropout.apply(x, p, seed, index)
-    return _dropout(x, p, seed, index)
+    return _dropout(x, *numbers)
 
 
 def _check(what, x, weights, gate, gate_act, scale):
@@ -124,18 +123,21 @@ def _ld(t):
     return 0 if t is None else t.stride(0)
 
 
+def _dense(w):
+    return None if w is None else w.contiguous()
+
+
 def _rows(t, D):
     return None if t is None else rows_of(t, D)
 
 
-def _forward(x, residual, post_weight, weight, wtype, gate, gate_act, scale, p, seed, index, eps):
+def _forward(x, residual, post_weight, weight, wtype, gate, gate_act, scale, numbers, eps):
     D, dev = x.shape[-1], x.device
     h = torch.empty_like(x, memory_format=torch.contiguous_format)
     y = torch.empty_like(h)
     x2, r2, g2 = rows_of(x, D), rows_of(residual, D), _rows(gate, D)
-    post_weight, weight = (None if w is None else w.contiguous() for w in (post_weight, weight))
+    post_weight, weight = _dense(post_weight), _dense(weight)
     number, at = _scale(scale)
-    numbers = _numbers("block_norm", p, seed, index, dev)
     with on(dev) as stream:
         _lib.check(_lib.lib().spanqr_block_norm(
             TYPES[x.dtype], wtype, GATES[gate_act], x2.shape[0], D, x2.data_ptr(), x2.stride(0), r2.data_ptr(), r2.stride(0),
@@ -149,9 +151,10 @@ def _backward(dy, dh, x, h, post_weight, weight, wtype, gate, gate_act, scale, p
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dr = torch.empty_like(dx)
     dg = None if gate is None else torch.empty_like(dx)
-    dys, dhs, x2, h2, g2 = (_rows(t, D) for t in (dy, dh, x, h, gate))
-    post_weight, weight = (None if w is None else w.contiguous() for w in (post_weight, weight))
-    dw1, dw2 = (torch.empty_like(w) if w is not None and need_weights else None for w in (post_weight, weight))
+    dys, dhs, x2, h2, g2 = _rows(dy, D), _rows(dh, D), rows_of(x, D), rows_of(h, D), _rows(gate, D)
+    post_weight, weight = _dense(post_weight), _dense(weight)
+    dw1 = torch.empty_like(post_weight) if post_weight is not None and need_weights else None
+    dw2 = torch.empty_like(weight) if weight is not None and need_weights else None
     da = torch.empty((), dtype=torch.float32, device=dev) if need_scale else None
     number, at = _scale(scale)
     numbers = _numbers("block_norm_backward", p, seed, index, dev)
@@ -172,7 +175,8 @@ def _backward(dy, dh, x, h, post_weight, weight, wtype, gate, gate_act, scale, p
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, post_weight, weight, gate, scale, wtype, gate_act, p, seed, index, eps):
-        y, h = _forward(x, residual, post_weight, weight, wtype, gate, gate_act, scale, p, seed, index, eps)
+        y, h = _forward(x, residual, post_weight, weight, wtype, gate, gate_act, scale,
+                        _numbers("block_norm", p, seed, index, x.device), eps)
         ctx.scale, ctx.seed = (None if isinstance(v, torch.Tensor) else v for v in (scale, seed))
         ctx.save_for_backward(x, h, post_weight, weight, gate, scale if ctx.scale is None else None,
                               seed if ctx.seed is None else None)
@@ -211,11 +215,12 @@ def block_norm(x, residual, post_weight=None, weight=None, gate=None, gate_act="
     no_tangents("block_norm", x, residual, post_weight, weight, gate, scale)
     wtype = _check("block_norm", x, (("post_weight", post_weight), ("weight", weight)), gate, gate_act, scale)
     check_like("block_norm", "residual", residual, x, x.shape)
-    _numbers("block_norm", p, seed, index, x.device)
-    inputs = (x, residual, post_weight, weight, gate, scale)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs):
-        return _BlockNorm.apply(*inputs, wtype, gate_act, p, seed, index, eps)
-    return _forward(x, residual, post_weight, weight, wtype, gate, gate_act, scale, p, seed, index, eps)
+    numbers = _numbers("block_norm", p, seed, index, x.device)
+    if torch.is_grad_enabled():
+        inputs = (x, residual, post_weight, weight, gate, scale)
+        if any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs):
+            return _BlockNorm.apply(*inputs, wtype, gate_act, p, seed, index, eps)
+    return _forward(x, residual, post_weight, weight, wtype, gate, gate_act, scale, numbers, eps)
 
 
 def block_norm_backward(dy, dh, x, h, post_weight=None, weight=None, gate=None, gate_act="silu", scale=1.0, p=0.0, seed=None,

@@ -16,8 +16,14 @@
 // which they lie in the registers. V^T comes from LDS by the transposing read in that order. The gradient of K and V
 // holds its keys by lanes and streams Q and dO; that of Q holds queries and streams K and V. P is rounded to 16 bits before
 // the product with V or dO, and dS before those with K and Q; all sums are fp32.
+//
+// fp16 holds nothing below 2^-24, and little below 2^-14. So there P goes into its products times a power of two that keeps it
+// below 2^15, and dS times one that a bound on it allows: |dP_ij - D_i| <= 2 |dO_i| |V_j|, the lane's own norm and the other
+// side's largest. The powers go into the exponent, and the results are divided by them. bf16 has fp32's exponents.
 #include <limits.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "elements.h"
 #include "host.h"
@@ -56,6 +62,25 @@ struct Vec<fp16> {
 // l % 32, register i being row 8 (i / 4) + 4 (l / 32) + i % 4
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(fp16x8 a, fp16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// log2 of what P is multiplied by: over a base that may be 2^8 too small in the forward pass, and at most 1 in the backward pass
+template <typename T>
+constexpr float raised(bool forward) { return std::is_same<T, fp16>::value ? (forward ? 7.0f : 14.0f) : 0.0f; }
+// log2 of what dS, at most 2 sqrt(a b), may be multiplied by to stay within 2^14
+__device__ __forceinline__ float room(float a, float b) {
+    const float most = 2.0f * sqrtf(a) * sqrtf(b);
+    if (!(most > 0.0f && most < INFINITY)) return 0.0f;
+    const float e = 13.0f - floorf(__builtin_amdgcn_logf(most));
+    return fminf(fmaxf(e, -60.0f), 60.0f);
+}
+// x, or 0 where it is not finite (a row of such numbers gives such gradients, whatever the others are multiplied by)
+__device__ __forceinline__ float finite(float x) { return x < INFINITY ? x : 0.0f; }
+// the largest of n partial maxima, in every lane
+__device__ __forceinline__ float largest(const float* p, int n, int lane) {
+    float m = 0.0f;
+    for (int i = lane; i < n; i += 64) m = fmaxf(m, p[i]);
+    return reduce_lanes<64, NanMax>(m);
+}
 
 // registers 8 s to 8 s + 7 in 16 bits
 template <typename T>
@@ -399,7 +424,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[dt][r] *= down;
             }
-            const float off = base == -INFINITY ? 0.0f : base;
+            const float off = base == -INFINITY ? 0.0f : base - raised<T>(true);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -415,6 +440,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
             }
         }
         sum = both_halves(sum, [](float x, float y) { return x + y; });
+        base -= raised<T>(true);
         const long at = (seq.q0 + i) * (s.Hk * s.G) + hk * s.G + g;
         if (a.splits == 1) {
             store_row<T, DP>((T*)a.out + at * s.D, on, s.D, lane, o, sum == 0.0f ? 0.0f : 1.0f / sum);
@@ -493,7 +519,30 @@ struct BackwardArgs {
     long rows;
     int q_tiles, k_tiles;
     float scale;
+    float *v_most, *d_most;   // fp16: the largest |V_j|^2 and |dO_i|^2 of a sequence, key head and workgroup's rows
 };
+
+// |V_j|^2's maxima over a workgroup's rows: 16 lanes a row, eight elements a lane
+template <typename T>
+__global__ __launch_bounds__(64 * WAVES) void k_v_most(const BackwardArgs a) {
+    __shared__ float slot[WAVES];
+    const Shape& s = a.s;
+    const int many = s.B * s.Hk, which = blockIdx.x % many, first = blockIdx.x / many, b = which / s.Hk, hk = which % s.Hk;
+    const Seq seq = seq_of(s, b);
+    const T* v = (const T*)head_of<T>(a.v, s.q_starts != nullptr, b, seq.k0, hk);
+    const int d = 8 * (threadIdx.x & 15), here = s.D - d >= 8 ? 8 : 0;
+    float most = 0.0f;
+    for (int tile = first; (long)tile * BLOCK < seq.lk; tile += a.k_tiles)
+        for (int j = tile * BLOCK + (threadIdx.x >> 4); j < (tile + 1) * BLOCK && j < seq.lk; j += 16) {
+            float x[8], sum = 0.0f;
+            load8(v + j * a.v.row + d, here, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+            most = fmaxf(most, finite(reduce_lanes<16, Sum>(sum)));
+        }
+    most = reduce_threads<64 * WAVES, NanMax>(most, slot);
+    if (threadIdx.x == 0) a.v_most[which * a.k_tiles + first] = most;
+}
 
 // dQ: as the forward pass, 128 rows a workgroup; a lane has one query. It has dO in registers, so it forms D first, and leaves it
 // and lse as the gradients take it for the keys' kernel (a pass of its own over O and dO took 15 us of 200 at 16 x 1024 x 12 x 64).
@@ -525,6 +574,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
     const char* q = head_of<T>(a.q, packed, b, seq.q0, hk * s.G);
     const char* d_out = head_of<T>(a.dout, packed, b, seq.q0, hk * s.G);
     const char* out = head_of<T>(a.out, packed, b, seq.q0, hk * s.G);
+    constexpr bool SMALL = std::is_same<T, fp16>::value;
+    const float v_most = SMALL ? largest(a.v_most + which * a.k_tiles, a.k_tiles, lane) : 0.0f;
+    float d_most = 0.0f;
 
     for (int tile = first; (long)tile * BLOCK < M; tile += a.q_tiles) {
         const int m0 = tile * BLOCK, w0 = m0 + 32 * wave, m = w0 + (lane & 31);
@@ -534,7 +586,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
         x8 fq[DP / 16], fd[DP / 16];
         load_row<T, DP>(q + (long)sizeof(T) * (i * a.q.row + g * a.q.head), on, s.D, lane, fq);
         load_row<T, DP>(d_out + (long)sizeof(T) * (i * a.dout.row + g * a.dout.head), on, s.D, lane, fd);
-        float lse = INFINITY, delta = 0.0f;
+        float lse = INFINITY, delta = 0.0f, up = 0.0f;
+        if constexpr (SMALL) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = fmaf((float)fd[ks][e], (float)fd[ks][e], sum);
+            sum = finite(both_halves(sum, [](float x, float y) { return x + y; }));
+            d_most = fmaxf(d_most, sum);
+            up = room(sum, v_most);
+        }
         {
             x8 fo[DP / 16];
             load_row<T, DP>(out + (long)sizeof(T) * (i * a.out.row + g * a.out.head), on, s.D, lane, fo);
@@ -545,11 +607,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
                 for (int e = 0; e < 8; ++e) delta = fmaf((float)fo[ks][e], (float)fd[ks][e], delta);
             delta = both_halves(delta, [](float x, float y) { return x + y; });
             if (on && h == 0) {
-                a.stat[at] = lse;
+                a.stat[at] = lse - raised<T>(false);
                 a.stat[a.rows + at] = -delta;
             }
         }
         if (a.dq == nullptr) continue;
+        lse -= up;
         f32x16 start;   // of dP - D's sum
 #pragma unroll
         for (int r = 0; r < 16; ++r) start[r] = -delta;
@@ -608,8 +671,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
                 }
             }
         }
-        store_row<T, DP>((T*)a.dq + at * s.D, on, s.D, lane, dq, a.scale);
+        store_row<T, DP>((T*)a.dq + at * s.D, on, s.D, lane, dq, SMALL ? a.scale * __builtin_amdgcn_exp2f(-up) : a.scale);
         arrived();
+    }
+    if constexpr (SMALL) {
+        d_most = reduce_threads<64 * WAVES, NanMax>(d_most, (float*)smem);
+        if (threadIdx.x == 0) a.d_most[which * a.q_tiles + first] = d_most;
     }
 }
 
@@ -647,6 +714,8 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
     const float* stat = a.stat + seq.q0 * (s.Hk * s.G) + hk * s.G;
     const char* k = head_of<T>(a.k, packed, b, seq.k0, hk);
     const char* v = head_of<T>(a.v, packed, b, seq.k0, hk);
+    constexpr bool SMALL = std::is_same<T, fp16>::value;
+    const float d_most = SMALL ? largest(a.d_most + which * a.q_tiles, a.q_tiles, lane) : 0.0f;
     auto load = [&](int m0, int buffer) {
         Q.load(m0, M, lds + buffer * BUFFER, wave, lane);
         DO.load(m0, M, lds + buffer * BUFFER + R::BYTES, wave, lane);
@@ -667,6 +736,16 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
         x8 fk[DP / 16], fv[DP / 16];
         load_row<T, DP>(k + (long)sizeof(T) * row * a.k.row, on, s.D, lane, fk);
         load_row<T, DP>(v + (long)sizeof(T) * row * a.v.row, on, s.D, lane, fv);
+        float up = 0.0f, times = 1.0f;   // dS is multiplied by 2^up, and P by 2^raised already
+        if constexpr (SMALL) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = fmaf((float)fv[ks][e], (float)fv[ks][e], sum);
+            up = room(finite(both_halves(sum, [](float x, float y) { return x + y; })), d_most);
+            times = __builtin_amdgcn_exp2f(up - raised<T>(false));
+        }
         // the rows that see a key; then those that see any and all of this wavefront's keys, and the workgroup's
         auto first_row = [&](int key) {
             const long m = s.causal ? (long)(key - ahead) * s.G : 0;
@@ -728,7 +807,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
                     }
                 }
 #pragma unroll
-                for (int r = 0; r < 16; ++r) dp[r] *= z[r];
+                for (int r = 0; r < 16; ++r) dp[r] *= SMALL ? z[r] * times : z[r];
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
                     const x8 p = half_of<T>(z, st), ds = half_of<T>(dp, st);
@@ -741,8 +820,8 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
             }
         }
         const long at = ((seq.k0 + row) * s.Hk + hk) * s.D;
-        store_row<T, DP>((T*)a.dk + at, on, s.D, lane, dk, a.scale);
-        store_row<T, DP>((T*)a.dv + at, on, s.D, lane, dv, 1.0f);
+        store_row<T, DP>((T*)a.dk + at, on, s.D, lane, dk, SMALL ? a.scale * __builtin_amdgcn_exp2f(-up) : a.scale);
+        store_row<T, DP>((T*)a.dv + at, on, s.D, lane, dv, SMALL ? __builtin_amdgcn_exp2f(-raised<T>(false)) : 1.0f);
         arrived();
     }
 }
@@ -793,6 +872,9 @@ int check_shape(const char* what, int type, long B, long Hk, long G, long D, lon
     return SPANQR_OK;
 }
 
+// two numbers a row, and the maxima of fp16
+long backward_bytes(const Call& c) { return 8 * c.rows + 4l * c.s.B * c.s.Hk * (c.q_tiles + c.k_tiles); }
+
 // strides: {batch, row, head}
 int check_heads(const char* what, const char* name, const void* p, const long* strides, bool empty, Heads& h) {
     if (empty) {
@@ -830,6 +912,8 @@ template <typename T>
 void launch_backward(const BackwardArgs& a, hipStream_t st) {
     const Shape& s = a.s;
     const int heads = (s.B + (s.q_starts != nullptr ? 1 : 0)) * s.Hk;
+    if (std::is_same<T, fp16>::value && s.B > 0 && s.Tk > 0 && a.rows > 0)
+        k_v_most<T><<<s.B * s.Hk * a.k_tiles, 64 * WAVES, 0, st>>>(a);
     if (a.rows > 0) {
 #define LAUNCH(DP) k_dq<T, DP><<<heads * a.q_tiles, 64 * WAVES, 0, st>>>(a)
         SPANQR_HEADS(LAUNCH)
@@ -886,12 +970,12 @@ int spanqr_attention(int type, long B, long Hk, long G, long D, long Tq, long Tk
     return launched("attention");
 }
 
-long spanqr_attention_backward_workspace(long B, long Hk, long G, long D, long Tq, long Tk, int packed) {
+long spanqr_attention_backward_workspace(long B, long Hk, long G, long D, long Tq, long Tk, int packed, long max_q, long max_k) {
     Call c;
     const int none = 0;
     const int rc = check_shape("attention_backward", SPANQR_BF16, B, Hk, G, D, Tq, Tk, packed ? &none : nullptr, packed ? &none : nullptr,
-                               0, 0, 0, 0, 1.0f, c);
-    return rc != SPANQR_OK ? rc : 8 * c.rows;
+                               max_q, max_k, 0, 0, 1.0f, c);
+    return rc != SPANQR_OK ? rc : backward_bytes(c);
 }
 
 int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq, long Tk, const void* dout, const long* dout_strides,
@@ -913,8 +997,8 @@ int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq
         return rc;
     if ((dk != nullptr) != (dv != nullptr) || !aligned(dq) || !aligned(dk) || !aligned(dv))
         return error(SPANQR_EINVAL, "%s: dk and dv belong together, and gradients lie on 16 bytes", what);
-    if (c.rows > 0 && (lse == nullptr || workspace == nullptr || !aligned(workspace) || workspace_bytes < 8 * c.rows))
-        return error(SPANQR_EINVAL, "%s: lse is missing, or the workspace, which needs %ld bytes", what, 8 * c.rows);
+    if (c.rows > 0 && (lse == nullptr || workspace == nullptr || !aligned(workspace) || workspace_bytes < backward_bytes(c)))
+        return error(SPANQR_EINVAL, "%s: lse is missing, or the workspace, which needs %ld bytes", what, backward_bytes(c));
     a.s = c.s;
     a.lse = lse;
     a.dq = dq;
@@ -925,6 +1009,8 @@ int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq
     a.q_tiles = (int)c.q_tiles;
     a.k_tiles = (int)c.k_tiles;
     a.scale = scale;
+    a.v_most = a.stat + 2 * c.rows;
+    a.d_most = a.v_most + B * Hk * c.k_tiles;
     if (type == SPANQR_BF16)
         launch_backward<bf16>(a, (hipStream_t)stream);
     else

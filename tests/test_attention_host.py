@@ -37,8 +37,8 @@ def test_forward_refusals():
 
 
 def test_backward_refusals():
-    need = _lib.lib().spanqr_attention_backward_workspace(2, 2, 2, 64, 10, 10, 0)
-    assert need == 8 * 2 * 10 * 4
+    need = _lib.lib().spanqr_attention_backward_workspace(2, 2, 2, 64, 10, 10, 0, 0, 0)
+    assert need == 8 * 2 * 10 * 4 + 4 * 2 * 2 * (1 + 1)
 
     def call(type=1, B=2, Hk=2, G=2, D=64, Tq=10, Tk=10, do=PTR, q=PTR, k=PTR, v=PTR, o=PTR, do_str=strides(), q_str=strides(),
              k_str=strides(), v_str=strides(), o_str=strides(), lse=PTR, qs=None, ks=None, causal=1, window=0, scale=1.0, dq=PTR, dk=PTR,

@@ -13,9 +13,13 @@ import spanqr_amd as sp
 pytestmark = pytest.mark.gpu
 
 HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
-# Half a step of fp16's subnormals. bf16 has fp32's exponents, and there the exponential instruction gives 0 below the smallest
-# normal number, 2^-126, as the matrix instructions take 0 for bf16's subnormals: a probability of 2^-127 is off by all of it.
+# Half a step of fp16's subnormals, of a result. P goes into its products at 2^7 times at least what it is relative to its row's
+# largest (PTINY), and dS times what brings 2 |dO| |V|, the largest ones', to 2^13 at least (2^-25 2 / 2^13 of it). bf16 has
+# fp32's exponents, and there the exponential instruction gives 0 below the smallest normal number, 2^-126, as the
+# matrix instructions take 0 for bf16's subnormals: a probability of 2^-127 is off by all of it.
 TINY = {torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25}
+PTINY = {torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -32}
+DSTINY = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -37}
 
 
 def visible(lq, lk, causal, window):
@@ -29,7 +33,7 @@ def visible(lq, lk, causal, window):
     return seen
 
 
-def one_head(q, k, v, dout, seen, scale, half, tiny, out=None):
+def one_head(q, k, v, dout, seen, scale, half=0.0, tiny=0.0, ptiny=0.0, dstiny=0.0):
     """in 64 bits, of one head: (result, bound) of out, dq and this head's part of dk and dv; bounds without the last rounding"""
     q, k, v = q.double(), k.double(), v.double()
     eps = (q.shape[1] + 16) * 2.0 ** -24
@@ -42,7 +46,7 @@ def one_head(q, k, v, dout, seen, scale, half, tiny, out=None):
         p = torch.softmax(s, 1).nan_to_num(0.0)
     # an exponent's error is the score's, and that of its own size; the rows' common part too
     p_err = p * (s_err + s_err.amax(1, keepdim=True) if s.shape[1] else s_err)
-    p_err = p_err + p * 2.0 ** -22 * (2.0 + s.abs().masked_fill(~seen, 0.0)) + half * p + tiny * seen
+    p_err = p_err + p * 2.0 ** -22 * (2.0 + s.abs().masked_fill(~seen, 0.0)) + half * p + ptiny * seen
     o, o_err = p @ v, p_err @ v.abs()
     if dout is None:
         return lse, (o, o_err)
@@ -53,7 +57,9 @@ def one_head(q, k, v, dout, seen, scale, half, tiny, out=None):
     rounded = half * o.abs() + tiny + o_err
     d_err = (g.abs() * rounded).sum(1, keepdim=True) + eps * (g.abs() * o.abs()).sum(1, keepdim=True)
     ds = p * (dp - delta)
-    ds_err = p_err * (dp - delta).abs() + p * (d_err + eps * (g.abs() @ v.abs().T)) + half * ds.abs() + tiny * seen
+    ds_err = p_err * (dp - delta).abs() + p * (d_err + eps * (g.abs() @ v.abs().T)) + half * ds.abs() + 2.0 ** -126 * seen
+    if v.numel() and g.numel():
+        ds_err = ds_err + dstiny * seen * float(g.norm(dim=1).max()) * float(v.norm(dim=1).max())
     return lse, (o, o_err), (scale * ds @ k, scale * ds_err @ k.abs()), (scale * ds.T @ q, scale * ds_err.T @ q.abs()), (
         p.T @ g, p_err.T @ g.abs())
 
@@ -69,7 +75,7 @@ def near(got, want, err, what):
 def check(q, k, v, dout=None, causal=False, window=None, scale=None, sequences=None, **packed):
     """runs the operator and compares; sequences: (first query, end, first key, end) of packed ones"""
     D, H, Hk = q.shape[-1], q.shape[-2], k.shape[-2]
-    half, tiny = HALF[q.dtype], TINY[q.dtype]
+    small = HALF[q.dtype], TINY[q.dtype], PTINY[q.dtype], DSTINY[q.dtype]
     out, lse = sp.attention(q, k, v, causal=causal, window=window, scale=scale, return_lse=True, **packed)
     grads = [] if dout is None else sp.attention_backward(dout, q, k, v, out, lse, causal=causal, window=window, scale=scale, **packed)
     got = {"out": out}
@@ -90,7 +96,7 @@ def check(q, k, v, dout=None, causal=False, window=None, scale=None, sequences=N
         seen = visible(lq, lk, causal, window)
         for h in range(H):
             hk = h // (H // Hk)
-            r = one_head(q[qa][:, h], k[ka][:, hk], v[ka][:, hk], None if dout is None else dout[qa][:, h], seen, c, half, tiny)
+            r = one_head(q[qa][:, h], k[ka][:, hk], v[ka][:, hk], None if dout is None else dout[qa][:, h], seen, c, *small)
             want_lse[qa][:, h] = r[0]
             for n, (value, err), where, head in zip(("out", "dq", "dk", "dv"), r[1:], (qa, qa, ka, ka), (h, h, hk, hk)):
                 want[n][0][where][:, head] += value
@@ -235,6 +241,21 @@ def test_sizes_of_scores(cuda):
     check(torch.ones_like(q), torch.ones_like(k) * ramp.flip(1), v, dout, True, scale=1.0 / D)
 
 
+@pytest.mark.parametrize("size", [1e-5, 1e-3, 30.0])
+def test_sizes_of_gradients(cuda, size):
+    """fp16: gradients far below its normal numbers, and large ones against large values, of long rows; heads of other sizes beside"""
+    S, D = 1000, 64
+    q, k, v, dout = (normal(2, S, h, D, seed=s, dtype=torch.float16) for s, h in ((1, 4), (2, 2), (3, 2), (4, 4)))
+    v[:, :, 1] *= 10.0
+    dout[1] *= 0.01
+    got, _ = check(q, k, v, (dout * size).half(), True)
+    if size < 1:
+        assert got["dq"].any() and got["dk"].any()
+    v[0, 5, 0] = 0.0
+    dout[0, 7] = 0.0
+    check(q, k, v, (dout * size).half(), False)
+
+
 def test_nothing_to_do(cuda):
     for B, Sq, Sk in ((0, 5, 5), (2, 0, 5), (2, 5, 0)):
         q, k, v = normal(B, Sq, 4, 64), normal(B, Sk, 2, 64), normal(B, Sk, 2, 64)
@@ -289,7 +310,7 @@ def test_gradient_against_differences(cuda):
     def loss(q, k, v):
         return float((torch.softmax((q @ k.T / 4).masked_fill(~seen, -math.inf), 1) @ v * dout).sum())
 
-    _, _, (dq, _), (dk, _), (dv, _) = one_head(q, k, v, dout, seen, 0.25, 0.0, 0.0)
+    _, _, (dq, _), (dk, _), (dv, _) = one_head(q, k, v, dout, seen, 0.25)
     for i, g in enumerate((dq, dk, dv)):
         d = normal(20, 16, seed=9).double()
         up, down = (loss(*(t + s * 1e-5 * d if j == i else t for j, t in enumerate((q, k, v)))) for s in (1, -1))
