@@ -100,6 +100,25 @@ __device__ __forceinline__ float both_halves(float v, OP op) {
     return op(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
 }
 
+// N products whose first operands come from LDS, AHEAD of them under way: the compiler left to itself reads each operand right
+// before its product and waits for it. between(i): what else goes behind product i.
+template <int N, int AHEAD, typename X8, typename READ, typename PRODUCT, typename BETWEEN>
+__device__ __forceinline__ void stream(X8 (&f)[AHEAD], READ read, PRODUCT product, BETWEEN between) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        product(i, f[i % AHEAD]);
+        if (i + AHEAD < N) f[i % AHEAD] = read(i + AHEAD);
+        between(i);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+template <int AHEAD, typename X8, typename READ>
+__device__ __forceinline__ void read_ahead(X8 (&f)[AHEAD], READ read) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) f[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // One of q, k, v, out, dout: elements between batches, rows and heads; 16-byte alignment, neighbouring elements of a head.
 struct Heads {
     const void* p;
@@ -183,6 +202,11 @@ struct Reader {
         }
     }
     __device__ __forceinline__ Reader(const Reader& r, uint32_t tile) : rows(r.rows + tile), cols{r.cols[0] + tile, r.cols[1] + tile} {}
+    __device__ __forceinline__ void move(int by) {
+        rows += by;
+        cols[0] += by;
+        cols[1] += by;
+    }
     // makes the compiler form the places below again behind this point: kept, they take the registers of two results
     __device__ __forceinline__ void fresh() { asm volatile("" : "+v"(rows), "+v"(cols[0]), "+v"(cols[1])); }
     // rows 32 t + lane % 32, elements 16 ks + 8 (lane / 32) + 0..7, of the tile `off` bytes on
@@ -337,6 +361,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
     typedef typename Vec<T>::x8 x8;
     constexpr int PITCH = DP <= 64 ? 64 : 128;
     typedef Reader<T, PITCH> R;
+    constexpr int AHEAD = 4;
     __shared__ __attribute__((aligned(1024))) char smem[4 * R::BYTES];
     const Shape& s = a.s;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -398,10 +423,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
             if (n0 >= any_hi || n0 + TILE <= any_lo) continue;
             const R in(read, now);
             f32x16 z[2] = {};
-#pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) z[t] = mfma(in.row(0, t, ks), fq[ks], z[t]);
+            x8 f[AHEAD];
+            const auto keys = [&](int i) { return in.row(0, i % 2, i / 2); };
+            read_ahead(f, keys);
+            stream<DP / 8>(f, keys, [&](int i, x8 k) { z[i % 2] = mfma(k, fq[i / 2], z[i % 2]); }, [](int) {});
+            // (the first of the values are read while the softmax goes on)
+            const auto values = [&](int i) { return in.col(R::BYTES, i / (DP / 32), i % (DP / 32)); };
+            read_ahead(f, values);
             if (n0 + TILE > all_hi || n0 < all_lo) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -425,19 +453,21 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
                     for (int r = 0; r < 16; ++r) o[dt][r] *= down;
             }
             const float off = base == -INFINITY ? 0.0f : base - raised<T>(true);
+            const auto exps = [&](int t, int from, int to) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
+                for (int r = from; r < to; ++r) {
                     z[t][r] = __builtin_amdgcn_exp2f(fmaf(z[t][r], s.scale2, -off));
                     sum += z[t][r];
                 }
-#pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                const x8 p = half_of<T>(z[st / 2], st % 2);
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt) o[dt] = mfma(in.col(R::BYTES, st, dt), p, o[dt]);
-            }
+            };
+            exps(0, 0, 16);
+            x8 p[2] = {half_of<T>(z[0], 0), half_of<T>(z[0], 1)};
+            __builtin_amdgcn_sched_barrier(0);
+            constexpr int DT = DP / 32, EACH = (16 + 2 * DT - 1) / (2 * DT);
+            stream<4 * DT>(f, values, [&](int i, x8 v) { o[i % DT] = mfma(v, p[i / DT % 2], o[i % DT]); }, [&](int i) {
+                if (i < 2 * DT) exps(1, EACH * i, EACH * (i + 1) < 16 ? EACH * (i + 1) : 16);
+                if (i == 2 * DT - 1) p[0] = half_of<T>(z[1], 0), p[1] = half_of<T>(z[1], 1);
+            });
         }
         sum = both_halves(sum, [](float x, float y) { return x + y; });
         base -= raised<T>(true);
@@ -552,6 +582,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
     typedef typename Vec<T>::x8 x8;
     constexpr int PITCH = DP <= 64 ? 64 : 128;
     typedef Reader<T, PITCH> R;
+    constexpr int AHEAD = DP == 32 ? 2 : 4, BEHIND = DP == 32 ? 2 : 4;
     __shared__ __attribute__((aligned(1024))) char smem[4 * R::BYTES];
     const Shape& s = a.s;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -649,13 +680,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
             for (int t = 0; t < 2; ++t) {
                 in.fresh();
                 f32x16 z = {}, dp = start;
+                x8 f[AHEAD];
+                const auto keys = [&](int i) { return in.row(0, t, i); };
+                const auto values = [&](int i) { return in.row(R::BYTES, t, i); };
+                read_ahead(f, keys);
+                stream<DP / 16>(f, keys, [&](int i, x8 x) { z = mfma(x, fq[i], z); }, [](int) {});
+                read_ahead(f, values);
+                constexpr int EACH = 256 / DP;
+                stream<DP / 16>(f, values, [&](int i, x8 x) { dp = mfma(x, fd[i], dp); }, [&](int i) {
 #pragma unroll
-                for (int ks = 0; ks < DP / 16; ++ks) {
-                    z = mfma(in.row(0, t, ks), fq[ks], z);
-                    dp = mfma(in.row(R::BYTES, t, ks), fd[ks], dp);
-                }
+                    for (int r = EACH * i; r < EACH * (i + 1) && r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], s.scale2, -lse));
+                });
 #pragma unroll
-                for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], s.scale2, -lse)) * dp[r];
+                for (int r = EACH * (DP / 16); r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], s.scale2, -lse));
+                const auto cols = [&](int i) { return in.col(0, 2 * t + i / (DP / 32), i % (DP / 32)); };
+                x8 c[BEHIND];
+                read_ahead(c, cols);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) z[r] *= dp[r];
                 if (masked) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
@@ -663,12 +705,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
                         z[r] = j >= lo && j < hi ? z[r] : 0.0f;
                     }
                 }
-#pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    const x8 ds = half_of<T>(z, st);
-#pragma unroll
-                    for (int dt = 0; dt < DP / 32; ++dt) dq[dt] = mfma(in.col(0, 2 * t + st, dt), ds, dq[dt]);
-                }
+                const x8 ds[2] = {half_of<T>(z, 0), half_of<T>(z, 1)};
+                __builtin_amdgcn_sched_barrier(0);
+                stream<DP / 16>(c, cols, [&](int i, x8 x) { dq[i % (DP / 32)] = mfma(x, ds[i / (DP / 32)], dq[i % (DP / 32)]); }, [](int) {});
             }
         }
         store_row<T, DP>((T*)a.dq + at * s.D, on, s.D, lane, dq, SMALL ? a.scale * __builtin_amdgcn_exp2f(-up) : a.scale);
@@ -688,10 +727,11 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
     constexpr int PITCH = DP <= 64 ? 64 : 128;
     typedef Reader<T, PITCH> R;
     typedef Loader<T, PITCH, PITCH == 64> L;
+    constexpr int AHEAD = 2;
     constexpr int BUFFER = 2 * R::BYTES, STATS = 2 * 2 * TILE * 4 + 256;   // (and a lane's place in a tile's statistics)
     __shared__ __attribute__((aligned(1024))) char smem[2 * BUFFER + STATS + 2 * L::TABLE];
     const Shape& s = a.s;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const bool packed = s.q_starts != nullptr;
     const int many = (s.B + (packed ? 1 : 0)) * s.Hk;
     const int which = blockIdx.x % many, first = blockIdx.x / many;   // (the first keys are seen by most)
@@ -704,7 +744,6 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
     }
     const Seq seq = seq_of(s, b);
     const int M = seq.lq * s.G, ahead = seq.lk - seq.lq;
-    const R read(lane);
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_char*)smem, stats = lds + 2 * BUFFER;
     const L Q(head_of<T>(a.q, packed, b, seq.q0, hk * s.G), a.q, s.G, s.D, wave, lane, stats + STATS);
     const L DO(head_of<T>(a.dout, packed, b, seq.q0, hk * s.G), a.dout, s.G, s.D, wave, lane, stats + STATS + L::TABLE);
@@ -763,18 +802,25 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
         f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
         if (from < to) load(from, 0);
         int buffer = 0;
-        for (int m0 = from; m0 < to; m0 += rows, buffer ^= 1) {
+        R in(R(lane), lds);
+        // (threadIdx and what follows from it: formed where it is used, the registers are full)
+        auto thread = [] {
+            uint32_t t = threadIdx.x;
+            asm volatile("" : "+v"(t));
+            return t;
+        };
+        for (int m0 = from; m0 < to; m0 += rows, in.move(buffer ? -BUFFER : BUFFER), buffer ^= 1) {
             arrived();
             if (m0 + rows < to) load(m0 + rows, buffer ^ 1);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int r0 = m0 + 32 * t;
                 if (r0 >= any_hi || r0 + 32 <= any_lo) continue;
-                R in(read, lds + buffer * BUFFER);
                 in.fresh();
+                const uint32_t half = (thread() >> 5 & 1) * 16 + stats + 2 * buffer * TILE * 4 + 32 * t * 4;
                 // four rows' lse or -D
                 auto stat4 = [&](int which, int q4) {
-                    const uint32_t at = stats + ((2 * buffer + which) * TILE + 32 * t + 8 * q4 + 4 * h) * 4;
+                    const uint32_t at = half + (which * TILE + 8 * q4) * 4;
                     return *(__attribute__((address_space(3))) const f32x4*)(uintptr_t)at;
                 };
                 // dP - D: the sum starts at -D
@@ -785,20 +831,25 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
 #pragma unroll
                     for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = d[e];
                 }
-#pragma unroll
-                for (int ks = 0; ks < DP / 16; ++ks) {
-                    z = mfma(in.row(0, t, ks), fk[ks], z);
-                    dp = mfma(in.row(R::BYTES, t, ks), fv[ks], dp);
-                }
-#pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) {
+                x8 f[AHEAD];
+                const auto q_rows = [&](int i) { return in.row(0, t, i); };
+                const auto do_rows = [&](int i) { return in.row(R::BYTES, t, i); };
+                read_ahead(f, q_rows);
+                stream<DP / 16>(f, q_rows, [&](int i, x8 x) { z = mfma(x, fk[i], z); }, [](int) {});
+                read_ahead(f, do_rows);
+                const auto exps = [&](int q4) {
                     const f32x4 lse = stat4(0, q4);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) z[4 * q4 + e] = __builtin_amdgcn_exp2f(fmaf(z[4 * q4 + e], s.scale2, -lse[e]));
-                }
+                };
+                constexpr int EVERY = DP >= 64 ? DP / 64 : 1;   // products between four rows' exponentials
+                stream<DP / 16>(f, do_rows, [&](int i, x8 x) { dp = mfma(x, fv[i], dp); }, [&](int i) {
+                    if (i % EVERY == 0 && i / EVERY < 4) exps(i / EVERY);
+                });
+#pragma unroll
+                for (int q4 = DP / 16 / EVERY; q4 < 4; ++q4) exps(q4);
                 if (r0 < all_lo || r0 + 32 > all_hi) {
-                    int key = j;
-                    asm volatile("" : "+v"(key));   // (formed here)
+                    const int key = w0 + (thread() & 31), h = thread() >> 5 & 1;
                     const int lo = first_row(key), hi = key < seq.lk ? end_row(key) : 0;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
@@ -806,17 +857,18 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
                         z[r] = m >= lo && m < hi ? z[r] : 0.0f;
                     }
                 }
+                constexpr int DT = DP / 32, EACH = (16 + 2 * DT - 1) / (2 * DT);
+                const x8 p[2] = {half_of<T>(z, 0), half_of<T>(z, 1)};
+                const auto do_cols = [&](int i) { return in.col(R::BYTES, 2 * t + i / DT, i % DT); };
+                const auto q_cols = [&](int i) { return in.col(0, 2 * t + i / DT, i % DT); };
+                read_ahead(f, do_cols);
+                stream<2 * DT>(f, do_cols, [&](int i, x8 x) { dv[i % DT] = mfma(x, p[i / DT], dv[i % DT]); }, [&](int i) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) dp[r] *= SMALL ? z[r] * times : z[r];
-#pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    const x8 p = half_of<T>(z, st), ds = half_of<T>(dp, st);
-#pragma unroll
-                    for (int dt = 0; dt < DP / 32; ++dt) {
-                        dv[dt] = mfma(in.col(R::BYTES, 2 * t + st, dt), p, dv[dt]);
-                        dk[dt] = mfma(in.col(0, 2 * t + st, dt), ds, dk[dt]);
-                    }
-                }
+                    for (int r = EACH * i; r < EACH * (i + 1) && r < 16; ++r) dp[r] *= SMALL ? z[r] * times : z[r];
+                });
+                const x8 ds[2] = {half_of<T>(dp, 0), half_of<T>(dp, 1)};
+                read_ahead(f, q_cols);
+                stream<2 * DT>(f, q_cols, [&](int i, x8 x) { dk[i % DT] = mfma(x, ds[i / DT], dk[i % DT]); }, [](int) {});
             }
         }
         const long at = ((seq.k0 + row) * s.Hk + hk) * s.D;
