@@ -8,7 +8,7 @@ stand the operators of the training step that calls orth: the loss over the voca
 root-mean-square norm (csrc/norm.hip), clipping by the global norm (csrc/clip.hip), the norms around a block with gate
 and dropout (csrc/block.hip), and attention (csrc/attention.hip).
 """
-from .attention import attention, attention_backward  # noqa: F401
+from .attn import attention, attention_backward  # noqa: F401
 from .block import block_norm, block_norm_backward, dropout  # noqa: F401
 from .clip import clip_grad_norm, grad_norm  # noqa: F401
 from .kcholqr import borth, kcholqr_f, kcholqr_f_many, orth, orth_many, set_checked, status  # noqa: F401
