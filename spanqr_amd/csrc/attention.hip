@@ -569,7 +569,7 @@ struct BackwardArgs {
     void *dq, *dk, *dv;   // contiguous
     float* stat;          // [2][rows of all x heads], from k_dq: lse log2 e (inf where nothing is seen), -D
     long rows;
-    int q_tiles, k_tiles;
+    int q_tiles, k_tiles, kv_tiles;
     float scale;
     float *v_most, *d_most;   // fp16: the largest |V_j|^2 and |dO_i|^2 of a sequence, key head and workgroup's rows
 };
@@ -744,14 +744,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
 }
 
 // dK and dV: 128 keys a workgroup, a wavefront 32 of them in registers (a lane one key), over all rows of the group's
-// queries that see them, in tiles of 64 (or as many whole queries' rows as that holds)
-template <typename T, int DP>
+// queries that see them; or (SPLIT 2, where 128 keys would leave too few workgroups) 64 keys, two wavefronts sharing 32 and each
+// taking half of every tile's rows. The rows come in tiles of 64, or as many whole queries' rows as that holds.
+template <typename T, int DP, int SPLIT>
 __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const BackwardArgs a) {
     typedef typename Vec<T>::x8 x8;
     constexpr int PITCH = DP <= 64 ? 64 : 128;
     typedef Reader<T, PITCH> R;
     typedef Loader<T, PITCH, PITCH == 64> L;
-    constexpr int AHEAD = 2;
+    constexpr int AHEAD = 2, KEYS = BLOCK / SPLIT;
     constexpr int BUFFER = 2 * R::BYTES, STATS = 2 * 2 * TILE * 4 + 256;   // (and a lane's place in a tile's statistics)
     __shared__ __attribute__((aligned(1024))) char smem[2 * BUFFER + STATS + 2 * L::TABLE];
     const Shape& s = a.s;
@@ -762,8 +763,8 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
     const int b = which / s.Hk, hk = which % s.Hk;
     if (b == s.B) {
         const long from = clip_start(s.k_starts[0], s.Tk), to = clip_start(s.k_starts[s.B], s.Tk), width = (long)s.Hk * s.D;
-        outside((T*)a.dk, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, a.k_tiles * s.Hk);
-        outside((T*)a.dv, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, a.k_tiles * s.Hk);
+        outside((T*)a.dk, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, a.kv_tiles * s.Hk);
+        outside((T*)a.dv, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, a.kv_tiles * s.Hk);
         return;
     }
     const Seq seq = seq_of(s, b);
@@ -792,8 +793,8 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
         }
     };
 
-    for (int tile = first; (long)tile * BLOCK < seq.lk; tile += a.k_tiles) {
-        const int n0 = tile * BLOCK, w0 = n0 + 32 * wave, j = w0 + (lane & 31);
+    for (int tile = first; (long)tile * KEYS < seq.lk; tile += a.kv_tiles) {
+        const int n0 = tile * KEYS, w0 = n0 + 32 * (wave % (WAVES / SPLIT)), j = w0 + (lane & 31);
         const bool on = j < seq.lk;
         const long row = on ? j : 0;
         x8 fk[DP / 16], fv[DP / 16];
@@ -818,7 +819,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
             const long m = s.window ? (long)(key - ahead + s.window) * s.G : M;
             return m < 0 ? 0 : m < M ? (int)m : M;
         };
-        const int last = w0 + 31 < seq.lk ? w0 + 31 : seq.lk - 1, block_last = n0 + BLOCK < seq.lk ? n0 + BLOCK - 1 : seq.lk - 1;
+        const int last = w0 + 31 < seq.lk ? w0 + 31 : seq.lk - 1, block_last = n0 + KEYS < seq.lk ? n0 + KEYS - 1 : seq.lk - 1;
         const int any_lo = first_row(w0), any_hi = w0 < seq.lk ? end_row(last) : 0;
         const int all_lo = first_row(last), all_hi = w0 + 32 <= seq.lk ? end_row(w0) : 0;
         const int from = first_row(n0) / rows * rows, to = end_row(block_last);
@@ -826,7 +827,8 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
         f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
         if (from < to) load(from, 0);
         int buffer = 0;
-        R in(R(lane), lds);
+        const int mine = SPLIT == 2 ? wave / 2 : 0;   // the half of a tile's rows that this wavefront takes
+        R in(R(lane), lds + mine * 32 * R::ROW);
         // (threadIdx and what follows from it: formed where it is used, the registers are full)
         auto thread = [] {
             uint32_t t = threadIdx.x;
@@ -837,11 +839,11 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
             arrived();
             if (m0 + rows < to) load(m0 + rows, buffer ^ 1);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int r0 = m0 + 32 * t;
+            for (int t = 0; t < 2 / SPLIT; ++t) {
+                const int r0 = m0 + 32 * (mine + t);
                 if (r0 >= any_hi || r0 + 32 <= any_lo) continue;
                 in.fresh();
-                const uint32_t half = (thread() >> 5 & 1) * 16 + stats + 2 * buffer * TILE * 4 + 32 * t * 4;
+                const uint32_t half = (thread() >> 5 & 1) * 16 + stats + 2 * buffer * TILE * 4 + 32 * (mine + t) * 4;
                 // four rows' lse or -D
                 auto stat4 = [&](int which, int q4) {
                     const uint32_t at = half + (which * TILE + 8 * q4) * 4;
@@ -895,6 +897,29 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
                 stream<2 * DT>(f, q_cols, [&](int i, x8 x) { dk[i % DT] = mfma(x, ds[i / DT], dk[i % DT]); }, [](int) {});
             }
         }
+        if constexpr (SPLIT == 2) {   // the other half's sums, through the tiles' memory
+            constexpr int N = 16 * (DP / 32);
+            typedef __attribute__((address_space(3))) float lds_float;
+            lds_float* sums = (lds_float*)(uintptr_t)lds + wave % 2 * 2 * N * 64 + lane;
+            arrived();
+            if (mine != 0) {
+#pragma unroll
+                for (int r = 0; r < N; ++r) {
+                    sums[64 * r] = dk[r / 16][r % 16];
+                    sums[64 * (N + r)] = dv[r / 16][r % 16];
+                }
+            }
+            arrived();
+            if (mine != 0) {
+                arrived();
+                continue;
+            }
+#pragma unroll
+            for (int r = 0; r < N; ++r) {
+                dk[r / 16][r % 16] += sums[64 * r];
+                dv[r / 16][r % 16] += sums[64 * (N + r)];
+            }
+        }
         const long at = ((seq.k0 + row) * s.Hk + hk) * s.D;
         store_row<T, DP>((T*)a.dk + at, on, s.D, lane, dk, SMALL ? a.scale * __builtin_amdgcn_exp2f(-up) : a.scale);
         store_row<T, DP>((T*)a.dv + at, on, s.D, lane, dv, SMALL ? __builtin_amdgcn_exp2f(-raised<T>(false)) : 1.0f);
@@ -916,6 +941,11 @@ long splits_of(long B, long Hk, long tiles, long max_k) {
     const long n = want < most ? want : most;
     return n < 1 ? 1 : n;
 }
+
+// Whether the gradient of K and V takes 64 keys a workgroup: where 128 make no more than the device runs at once (three
+// workgroups a compute unit of up to 64 wide heads, two of wider ones). Both ways in us with 128 / 64: 8 x 1024 x 8 x 128 on 4 heads
+// 160 / 139, 16 x 512 x 16 x 64 on 4 116 / 98, packed 24 x 2048 x 8 x 64 on 2 357 / 294; with more of them 16 x 1024 x 12 x 64 190 / 204.
+bool few_keys(long B, long Hk, long k_tiles, long D) { return B * Hk * k_tiles <= 256 * (D <= 64 ? 3 : 2); }
 
 struct Call {
     Shape s;
@@ -943,7 +973,7 @@ int check_shape(const char* what, int type, long B, long Hk, long G, long D, lon
     c.q_tiles = blocks(max_q * G) < 1 ? 1 : blocks(max_q * G);
     c.k_tiles = blocks(max_k) < 1 ? 1 : blocks(max_k);
     c.splits = splits_of(B, Hk, c.q_tiles, max_k);
-    if ((B + 1) * Hk > INT_MAX / (c.q_tiles * c.splits) || (B + 1) * Hk > INT_MAX / c.k_tiles)
+    if ((B + 1) * Hk > INT_MAX / (c.q_tiles * c.splits) || (B + 1) * Hk > INT_MAX / (2 * c.k_tiles))
         return error(SPANQR_EINVAL, "%s: too many workgroups", what);
     return SPANQR_OK;
 }
@@ -1002,9 +1032,15 @@ void launch_backward(const BackwardArgs& a, hipStream_t st) {
 #undef LAUNCH
     }
     if (a.dk != nullptr && heads > 0 && s.Tk > 0) {
-#define LAUNCH(DP) k_dkv<T, DP><<<heads * a.k_tiles, 64 * WAVES, 0, st>>>(a)
-        SPANQR_HEADS(LAUNCH)
+        if (a.kv_tiles != a.k_tiles) {
+#define LAUNCH(DP) k_dkv<T, DP, 2><<<heads * a.kv_tiles, 64 * WAVES, 0, st>>>(a)
+            SPANQR_HEADS(LAUNCH)
 #undef LAUNCH
+        } else {
+#define LAUNCH(DP) k_dkv<T, DP, 1><<<heads * a.kv_tiles, 64 * WAVES, 0, st>>>(a)
+            SPANQR_HEADS(LAUNCH)
+#undef LAUNCH
+        }
     }
 }
 
@@ -1090,6 +1126,7 @@ int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq
     a.rows = c.rows;
     a.q_tiles = (int)c.q_tiles;
     a.k_tiles = (int)c.k_tiles;
+    a.kv_tiles = few_keys(B, Hk, c.k_tiles, D) ? 2 * a.k_tiles : a.k_tiles;
     a.scale = scale;
     a.v_most = a.stat + 2 * c.rows;
     a.d_most = a.v_most + B * Hk * c.k_tiles;

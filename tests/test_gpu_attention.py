@@ -123,7 +123,9 @@ def normal(*shape, seed=0, dtype=torch.bfloat16, size=1.0):
     (2, 257, 257, 6, 2, 80, True, 64), (1, 64, 300, 3, 3, 24, False, None), (1, 300, 64, 4, 1, 128, True, None),
     (1, 300, 64, 4, 1, 64, False, None), (1, 200, 70, 1, 1, 72, True, 1), (3, 127, 129, 7, 7, 40, True, None),
     (1, 1000, 1000, 2, 1, 128, True, 100), (1, 700, 700, 2, 2, 64, True, None), (1, 90, 90, 65, 1, 64, True, None),
-    (2, 50, 513, 40, 8, 128, True, None)])
+    (2, 50, 513, 40, 8, 128, True, None),
+    # as many workgroups as make the gradient of K and V take 128 keys each
+    (33, 200, 300, 8, 8, 128, True, None), (50, 150, 260, 12, 6, 64, True, 40), (30, 129, 257, 9, 9, 96, False, None)])
 def test_batches(cuda, B, Sq, Sk, H, Hk, D, causal, window, dtype):
     q, k, v = normal(B, Sq, H, D, seed=1, dtype=dtype, size=1.5), normal(B, Sk, Hk, D, seed=2, dtype=dtype, size=1.5), normal(
         B, Sk, Hk, D, seed=3, dtype=dtype)
