@@ -11,8 +11,6 @@
 // Bound by memory: each input is read once and each output written once, the row stays in registers between the two sums
 // (threads and pieces as in norm.hip). Between them would be h, t, n1, dt and the mask in memory if these were operators of
 // their own. Sums are fp32: per thread over at most 16 elements, then a tree in a fixed order.
-#include <limits.h>
-
 #include "host.h"
 #include "random.h"
 #include "rows.h"
@@ -77,11 +75,19 @@ struct Weights {
     }
 };
 
-// 1 / (1 + exp(-g)): in fp32's full precision, or within 2^-20 of itself for what is rounded to 16 bits (2^-11 at best)
+// 1 / (1 + exp(-g)): in fp32's full precision, or for what is rounded to 16 bits from 2^t, t = -g log2 e. The product's rounding
+// makes that 2^-20 of itself for |g| up to 16, of which bf16 (2^-9 at best) sees nothing; fp16 has it taken out.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float g) {
     if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-g));
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * g));
+    constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+    const float t = -LOG2E * g;
+    float e = __builtin_amdgcn_exp2f(t);
+    if constexpr (std::is_same<T, fp16>::value) {
+        const float left = fmaf(-LOG2E, g, -t);
+        e = fabsf(g) < 88.0f ? fmaf(e, LN2 * left, e) : e;   // (beyond: infinite, or as good as 0)
+    }
+    return __builtin_amdgcn_rcpf(1.0f + e);
 }
 
 // v act(g)
@@ -315,7 +321,7 @@ __global__ __launch_bounds__(GROUP ? 256 : 512) void k_block_grad(const BlockGra
             const int n = on ? inside(p.D, at) : 0;
             float x[8], h[8], u[8], w[8];
             settle<WHOLE>(k.x[c], n, x);
-            settle<WHOLE>(k.h[c], n, h);
+            settle<WHOLE>(k.h[c], p.dy != nullptr ? n : 0, h);
             settle<WHOLE>(k.y[c], p.dy != nullptr ? n : 0, u);
             weight.get(1, c, w);
 #pragma unroll
@@ -328,7 +334,7 @@ __global__ __launch_bounds__(GROUP ? 256 : 512) void k_block_grad(const BlockGra
         G::sum(sum, slot[turn]);
         // a group without a row adds zeros, also where eps is 0
         const float s1 = on ? rsqrtf(sum[0] / (float)p.D + p.eps) : 0.0f;
-        const float s2 = on ? rsqrtf(sum[1] / (float)p.D + p.eps) : 0.0f;
+        const float s2 = on && p.dy != nullptr ? rsqrtf(sum[1] / (float)p.D + p.eps) : 0.0f;   // (without dy: dh alone)
         const float m2 = s2 * sum[2] / (float)p.D;   // the mean of dy w2 n2
         float q[NCH][8], last[1] = {0.0f};
 #pragma unroll
@@ -339,7 +345,7 @@ __global__ __launch_bounds__(GROUP ? 256 : 512) void k_block_grad(const BlockGra
             const long at = 8l * (lane + c * size);
             const int n = on ? inside(p.D, at) : 0;
             float a[8], b[8], w[8], d[8];
-            settle<WHOLE>(k.h[c], n, a);
+            settle<WHOLE>(k.h[c], p.dy != nullptr ? n : 0, a);   // (without dy h counts nothing, whatever it holds)
             settle<WHOLE>(k.y[c], p.dy != nullptr ? n : 0, b);
             settle<WHOLE>(k.d[c], p.dh != nullptr ? n : 0, d);
             weight.get(1, c, w);
@@ -467,7 +473,7 @@ __global__ __launch_bounds__(1024) void k_block_grad_long(const BlockGradArgs p)
             settle8(kx, n, a);
 #pragma unroll
             for (int i = 0; i < 8; ++i) e = fmaf(a[i], a[i], e);
-            settle8(kh, n, a);
+            settle8(kh, n < n_y ? n : n_y, a);
             settle8(ky, n < n_y ? n : n_y, b);
             load_weight(p.w2, p.wtype, at, n, w);
 #pragma unroll
@@ -480,7 +486,8 @@ __global__ __launch_bounds__(1024) void k_block_grad_long(const BlockGradArgs p)
             sum[2] += g;
         }
         G::sum(sum, slot[turn]);
-        const float s1 = rsqrtf(sum[0] / (float)p.D + p.eps), s2 = rsqrtf(sum[1] / (float)p.D + p.eps);
+        const float s1 = rsqrtf(sum[0] / (float)p.D + p.eps);
+        const float s2 = p.dy != nullptr ? rsqrtf(sum[1] / (float)p.D + p.eps) : 0.0f;   // (without dy: dh alone)
         const float m2 = s2 * sum[2] / (float)p.D;
         // q and n1 of a piece; in the first of two steps with everything else that the piece gives
         auto piece_of = [&](long at, bool first, float (&q)[8], float (&n1)[8]) __attribute__((always_inline)) {
@@ -488,7 +495,7 @@ __global__ __launch_bounds__(1024) void k_block_grad_long(const BlockGradArgs p)
             const Pack8<T> kh = fetch8(hr, p.D, at), ky = fetch8(yr, p.D, at), kd = fetch8(dr, p.D, at), kx = fetch8(xr, p.D, at),
                            kg = fetch8(gr, p.D, at);
             float a[8], b[8], w[8];
-            settle8(kh, n, a);
+            settle8(kh, n < n_y ? n : n_y, a);
             settle8(ky, n < n_y ? n : n_y, b);
             settle8(kd, n < n_d ? n : n_d, q);
             load_weight(p.w2, p.wtype, at, n, w);

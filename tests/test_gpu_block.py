@@ -1,6 +1,8 @@
 """block_norm, its backward pass and dropout against plain forms in 64 bits. Bounds: half a step of the type for each rounding
 to it, and 2^-18 of what is added up for fp32's sums (at most 16 elements in a row and a tree of 20 levels: below 40 steps
 of 2^-24, times what the reciprocal roots, the exponential and the products add)."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -259,6 +261,28 @@ def test_edges(cuda):
     assert y.shape == h.shape == (0, 300)
     g = sp.block_norm_backward(e, e, e, e, w1, w2, need_scale=True)
     assert not g.weight.any() and not g.post_weight.any() and g.scale == 0 and g.x.shape == (0, 300)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_gates(cuda, dtype):
+    """the gate's activations and slopes over their whole range, ends and NaN included"""
+    g = torch.cat([torch.linspace(-100, 100, 4001), torch.linspace(-8, 8, 4001),
+                   torch.tensor([0.0, -0.0, 1e-6, -1e-6, 6e4, -6e4, float("inf"), -float("inf"), float("nan")])]).to(dtype).cuda()[:, None]
+    x, r = torch.ones_like(g), torch.zeros_like(g)
+    dh = torch.ones_like(g)
+    for kind in ("sigmoid", "silu", None):
+        want, slope = act(g, kind)
+        y, h = sp.block_norm(x, r, gate=g, gate_act=kind, eps=0.0)
+        d = sp.block_norm_backward(None, dh, x, h, gate=g, gate_act=kind, eps=0.0).gate
+        # exp(-g)'s share: 2^-20 of it (less in fp32); s below 2^-126 may be 0, which times |g| < 2^7 is 2^-119. The slope has
+        # 1 - s, off by half a step of s, 2^-24, in s (1 - s) and, times g, in s (1 + g (1 - s)): a step of s and a rounding each
+        far = (g.double().abs().nan_to_num(posinf=0.0) + 1) * torch.sigmoid(g.double()) * 2.0 ** -23
+        for got, w, size, more in ((h, want, want.abs(), 0.0), (d, slope, slope.abs() + torch.sigmoid(g.double()), far)):
+            bound = (HALF[dtype] + 2.0 ** (-22 if dtype == torch.float32 else -19)) * size + max(TINY[dtype], 2.0 ** -119) + more
+            if kind == "silu":
+                w = torch.where(g.double() == -math.inf, got.double(), w)   # (-inf times 0)
+            same = (got.double() == w) | ((got.double() - w).abs() <= bound) | (torch.isnan(got) & torch.isnan(w))
+            assert same.all(), (kind, g[~same][:3], got[~same][:3], w[~same][:3])
 
 
 def test_autograd(cuda):
