@@ -928,6 +928,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
 }
 
 constexpr long MAX_ROWS = 1l << 30;      // queries x group, or keys, of a sequence
+constexpr long MAX_GRID = (1l << 24) - 1;
 constexpr long MAX_STRIDE = 1l << 24;    // of rows and heads: a tile's offsets stay within 32 bits
 
 long blocks(long n) { return (n + BLOCK - 1) / BLOCK; }
@@ -973,7 +974,8 @@ int check_shape(const char* what, int type, long B, long Hk, long G, long D, lon
     c.q_tiles = blocks(max_q * G) < 1 ? 1 : blocks(max_q * G);
     c.k_tiles = blocks(max_k) < 1 ? 1 : blocks(max_k);
     c.splits = splits_of(B, Hk, c.q_tiles, max_k);
-    if ((B + 1) * Hk > INT_MAX / (c.q_tiles * c.splits) || (B + 1) * Hk > INT_MAX / (2 * c.k_tiles))
+    // (a launch takes fewer than 2^32 threads, 2^24 workgroups)
+    if ((B + 1) * Hk > MAX_GRID / (c.q_tiles * c.splits) || (B + 1) * Hk > MAX_GRID / (2 * c.k_tiles))
         return error(SPANQR_EINVAL, "%s: too many workgroups", what);
     return SPANQR_OK;
 }
