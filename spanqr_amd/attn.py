@@ -12,6 +12,7 @@ from .tensors import TYPES, check_like, check_same, check_tensor, like, no_tange
 
 MAX_STRIDE = 1 << 24   # of rows and heads, in elements
 MAX_HEAD = 128
+MOST = 1 << 40         # more keys or rows than there are say the same, and this fits into the C ABI's numbers
 
 
 def _heads(t):
@@ -56,6 +57,7 @@ def _check(what, q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_
         window = int(window)
         if window < 1 or not causal:
             raise ValueError(f"{what}: a window is at least 1 and needs causal=True, got {window}")
+        window = min(window, MOST)
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"{what}: scale must be positive and finite, got {scale}")
@@ -78,7 +80,7 @@ def _check(what, q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_
     for name, n in (("max_q", max_q), ("max_k", max_k)):
         if n is not None and int(n) < 0:
             raise ValueError(f"{what}: {name} must not be negative, got {n}")
-    return (B, key_heads, heads // key_heads, D, Tq, Tk), window or 0, scale, q_starts, k_starts, int(max_q or 0), int(max_k or 0)
+    return (B, key_heads, heads // key_heads, D, Tq, Tk), window or 0, scale, q_starts, k_starts, *(min(int(n or 0), MOST) for n in (max_q, max_k))
 
 
 @functools.lru_cache(maxsize=256)

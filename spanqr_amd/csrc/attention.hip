@@ -683,7 +683,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
         from &= ~(TILE - 1);
 
         f32x16 dq[DP / 32] = {};
-        // both buffers at once: a split of a long cache has two tiles, and one memory latency then
         for (int i = 0; i < 2; ++i)
             if (from + i * TILE < to) {
                 K.load(from + i * TILE, seq.lk, lds + 2 * i * R::BYTES, wave, lane);
@@ -964,7 +963,7 @@ int check_shape(const char* what, int type, long B, long Hk, long G, long D, lon
         return error(SPANQR_EINVAL, "%s: B = %ld, heads = %ld x %ld, rows = %ld and %ld", what, B, Hk, G, Tq, Tk);
     if ((q_starts != nullptr) != (k_starts != nullptr)) return error(SPANQR_EINVAL, "%s: q_starts and k_starts belong together", what);
     if (window < 0 || (window > 0 && !causal)) return error(SPANQR_EINVAL, "%s: a window needs causal, and one key at least", what);
-    if (!(scale > 0.0f && scale < INFINITY)) return error(SPANQR_EINVAL, "%s: scale must be positive and finite", what);
+    if (!(scale > 0.0f && scale * LOG2E < INFINITY)) return error(SPANQR_EINVAL, "%s: scale must be positive and finite", what);
     const bool packed = q_starts != nullptr;
     if (!packed || max_q < 1 || max_q > Tq) max_q = Tq;
     if (!packed || max_k < 1 || max_k > Tk) max_k = Tk;
@@ -1117,8 +1116,10 @@ int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq
         return rc;
     if ((dk != nullptr) != (dv != nullptr) || !aligned(dq) || !aligned(dk) || !aligned(dv))
         return error(SPANQR_EINVAL, "%s: dk and dv belong together, and gradients lie on 16 bytes", what);
-    if (c.rows > 0 && (lse == nullptr || workspace == nullptr || !aligned(workspace) || workspace_bytes < backward_bytes(c)))
-        return error(SPANQR_EINVAL, "%s: lse is missing, or the workspace, which needs %ld bytes", what, backward_bytes(c));
+    if (c.rows > 0 && lse == nullptr) return error(SPANQR_EINVAL, "%s: lse is missing", what);
+    const long need = backward_bytes(c);
+    if (need > 0 && (workspace == nullptr || !aligned(workspace) || workspace_bytes < need))
+        return error(SPANQR_EINVAL, "%s: the workspace needs %ld bytes", what, need);
     a.s = c.s;
     a.lse = lse;
     a.dq = dq;

@@ -19,7 +19,7 @@ def strides(batch=64 * 4 * 10, row=64 * 4, head=64):
 BAD_SHAPES = [dict(type=0), dict(type=3), dict(B=-1), dict(Hk=0), dict(G=0), dict(D=0), dict(D=4), dict(D=136), dict(D=60), dict(Tq=-1),
               dict(Tk=-1), dict(Tk=1 << 30), dict(Tq=1 << 29), dict(G=1 << 31), dict(B=1 << 40), dict(B=1 << 23), dict(Tq=1 << 28, Hk=8),
               dict(qs=PTR), dict(ks=PTR), dict(window=-1, causal=1), dict(window=3, causal=0), dict(scale=0.0), dict(scale=-1.0),
-              dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(k=None), dict(v=None), dict(q=ctypes.c_void_p(4098)),
+              dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38), dict(q=None), dict(k=None), dict(v=None), dict(q=ctypes.c_void_p(4098)),
               dict(q_str=strides(row=65)), dict(q_str=strides(head=1 << 24)), dict(k_str=strides(row=-8)), dict(v_str=strides(batch=4)),
               dict(k_str=None)]
 
@@ -48,9 +48,10 @@ def test_backward_refusals():
 
     for kw in [*BAD_SHAPES, dict(do=None), dict(o=None), dict(do_str=strides(row=4)), dict(o_str=strides(head=12)), dict(lse=None),
                dict(ws=None), dict(nbytes=need - 1), dict(dk=None), dict(dv=None), dict(dq=ctypes.c_void_p(8)),
-               dict(dk=ctypes.c_void_p(24))]:
+               dict(dk=ctypes.c_void_p(24)), dict(type=2, Tq=0, ws=None), dict(Tq=0, nbytes=4 * 2 * 2 * 2 - 1)]:
         assert call(**kw) == EINVAL, kw
         assert b"attention_backward" in _lib.lib().spanqr_last_error()
+    assert call(B=0, ws=None, nbytes=0, lse=None) == 0
 
 
 def test_workspace():

@@ -320,6 +320,15 @@ def test_gradient_against_differences(cuda):
         assert abs((up - down) / 2e-5 - float((g * d).sum())) <= 1e-7 * (1 + float((g * d).abs().sum()))
 
 
+def test_limits_beyond_the_numbers_of_the_library(cuda):
+    """windows and lengths larger than any there are, 64 bits included"""
+    q, k, v = normal(1, 70, 2, 16), normal(1, 70, 1, 16, seed=1), normal(1, 70, 1, 16, seed=2)
+    want, starts = sp.attention(q, k, v, causal=True), torch.tensor([0, 70], dtype=torch.int32, device=cuda)
+    for n in (70, 1 << 31, (1 << 32) + 3, 1 << 63, (1 << 64) + 3):
+        assert torch.equal(sp.attention(q, k, v, causal=True, window=n), want), n
+        assert torch.equal(sp.attention(q[0], k[0], v[0], causal=True, q_starts=starts, max_q=n, max_k=n), want[0]), n
+
+
 def test_tangents_are_refused(cuda):
     q, k, v = normal(1, 4, 2, 16), normal(1, 4, 2, 16, seed=1), normal(1, 4, 2, 16, seed=2)
     out, lse = sp.attention(q, k, v, return_lse=True)
