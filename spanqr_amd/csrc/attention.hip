@@ -1120,6 +1120,7 @@ int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq
     const long need = backward_bytes(c);
     if (need > 0 && (workspace == nullptr || !aligned(workspace) || workspace_bytes < need))
         return error(SPANQR_EINVAL, "%s: the workspace needs %ld bytes", what, need);
+    if (no_q && (no_k || dk == nullptr)) return SPANQR_OK;
     a.s = c.s;
     a.lse = lse;
     a.dq = dq;
