@@ -391,32 +391,33 @@ int spanqr_block_norm_backward(int type, int wtype, int act, long rows, long D, 
 /* Softmax attention of bf16 or fp16, G heads to each of Hk key heads: out = softmax(scale q k^T) v. q, k and v are [.., Hk G or
  * Hk, D] by their strides {batch, row, head} in elements (host arrays, read at the call): multiples of 8, those of rows and
  * heads below 2^24, neighbouring elements of a head, 16-byte alignment. D: a multiple of 8 up to 128.
- * q_starts null: B sequences of Tq queries and Tk keys. Else packed: Tq and Tk rows in all, sequence b having the rows
+ * q_starts null: B sequences of Tq queries and Tk keys, of which with k_lens (device, B; read when the kernels run, taken as
+ * from 0 to Tk; or null) the first k_lens[b] are there, and the others are not read. Else packed: Tq and Tk rows in all, sequence b having the rows
  * q_starts[b] to q_starts[b + 1] - 1 and k_starts' (device, B + 1 each, ascending; read when the kernels run, and nothing outside
  * the rows is touched whatever they hold; batch strides are not used); max_q and max_k, the longest sequence's or 0,
  * set how much is launched alone. Query i stands at p = i + (its sequence's keys) - (queries); causal: it sees the
  * keys j <= p, with a window (0: none; needs causal) only those with j > p - window. One that sees none has out 0 and lse
  * -inf. out [rows][Hk G][D] contiguous, 16-byte aligned; lse [rows][Hk G] fp32, log sum exp of the scores, or null; rows of
  * no sequence are written as those that see no key. P is rounded to the type before the product with v.
- * A sequence's Tq G and Tk stay below 2^30, Tq Hk G below 2^31. workspace: spanqr_attention_workspace bytes (0 unless
+ * The elements of a sequence have to be finite, also where a mask hides them; scale is positive. A sequence's Tq G and Tk stay below 2^30, Tq Hk G below 2^31. workspace: spanqr_attention_workspace bytes (0 unless
  * the keys are split). */
 long spanqr_attention_workspace(long B, long Hk, long G, long D, long Tq, long Tk, int packed, long max_q, long max_k);
 int spanqr_attention(int type, long B, long Hk, long G, long D, long Tq, long Tk, const void* q, const long* q_strides,
                      const void* k, const long* k_strides, const void* v, const long* v_strides, const int* q_starts,
-                     const int* k_starts, long max_q, long max_k, int causal, long window, float scale, void* out, float* lse,
-                     void* workspace, long workspace_bytes, void* stream);
+                     const int* k_starts, const int* k_lens, long max_q, long max_k, int causal, long window, float scale,
+                     void* out, float* lse, void* workspace, long workspace_bytes, void* stream);
 
 /* Gradient of it, from dout, and from out and lse as they came out: dq as out lies, dk and dv [key rows][Hk][D] (both or
- * neither; dq or null), contiguous, zeros for rows of no sequence. P and dS are rounded to the type before the products that
+ * neither; dq or null), contiguous, zeros for rows of no sequence and keys behind k_lens. P and dS are rounded to the type before the products that
  * they go into. workspace: spanqr_attention_backward_workspace bytes. */
 long spanqr_attention_backward_workspace(long B, long Hk, long G, long D, long Tq, long Tk, int packed, long max_q,
                                          long max_k);
 int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq, long Tk, const void* dout,
                               const long* dout_strides, const void* q, const long* q_strides, const void* k,
                               const long* k_strides, const void* v, const long* v_strides, const void* out,
-                              const long* out_strides, const float* lse, const int* q_starts, const int* k_starts, long max_q,
-                              long max_k, int causal, long window, float scale, void* dq, void* dk, void* dv, void* workspace,
-                              long workspace_bytes, void* stream);
+                              const long* out_strides, const float* lse, const int* q_starts, const int* k_starts, const int* k_lens,
+                              long max_q, long max_k, int causal, long window, float scale, void* dq, void* dk, void* dv,
+                              void* workspace, long workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

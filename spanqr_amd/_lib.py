@@ -84,11 +84,11 @@ SIGNATURES = {
     "spanqr_block_norm_backward": (_I, [_I, _I, _I, _L, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _F, _F, _P, _D,
                                         _UL, _P, _U, _P, _P, _P, _P, _P, _P, _P, _L, _P]),
     "spanqr_attention_workspace": (_L, [_L, _L, _L, _L, _L, _L, _I, _L, _L]),
-    "spanqr_attention": (_I, [_I, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _L, _L, _I, _L, _F, _P, _P, _P, _L,
-                              _P]),
+    "spanqr_attention": (_I, [_I, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _L, _I, _L, _F, _P, _P, _P,
+                              _L, _P]),
     "spanqr_attention_backward_workspace": (_L, [_L, _L, _L, _L, _L, _L, _I, _L, _L]),
-    "spanqr_attention_backward": (_I, [_I, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _L,
-                                       _I, _L, _F, _P, _P, _P, _P, _L, _P]),
+    "spanqr_attention_backward": (_I, [_I, _L, _L, _L, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L,
+                                       _L, _I, _L, _F, _P, _P, _P, _P, _L, _P]),
 }
 
 _lib = None

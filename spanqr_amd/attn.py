@@ -31,12 +31,14 @@ def _heads(t):
     return t, (s[:3] if t.dim() == 4 else (0, *s[:2]))
 
 
-def _check(what, q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_k):
+def _check(what, q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_k, k_lens):
     """the shape as the C ABI takes it: B, key heads, group, D, Tq, Tk; and the other arguments settled"""
     check_tensor(what, "q", q, (torch.bfloat16, torch.float16))
     packed = q_starts is not None
     if not packed and (k_starts is not None or max_q is not None or max_k is not None):
         raise ValueError(f"{what}: k_starts, max_q and max_k belong to packed sequences, which need q_starts")
+    if packed and k_lens is not None:
+        raise ValueError(f"{what}: packed sequences have their lengths from k_starts, not from k_lens")
     axes = 3 if packed else 4
     for name, t in (("q", q), ("k", k), ("v", v)):
         check_tensor(what, name, t, (torch.bfloat16, torch.float16))
@@ -77,10 +79,16 @@ def _check(what, q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_
         q_starts, k_starts = q_starts.contiguous(), k_starts.contiguous()
     else:
         B = lead[0]
+        if k_lens is not None:
+            if not isinstance(k_lens, torch.Tensor) or k_lens.dtype != torch.int32:
+                raise TypeError(f"{what}: k_lens must be an int32 tensor")
+            check_same(what, "k_lens", k_lens, q.device, (B,))
+            k_lens = k_lens.contiguous()
     for name, n in (("max_q", max_q), ("max_k", max_k)):
         if n is not None and int(n) < 0:
             raise ValueError(f"{what}: {name} must not be negative, got {n}")
-    return (B, key_heads, heads // key_heads, D, Tq, Tk), window or 0, scale, q_starts, k_starts, *(min(int(n or 0), MOST) for n in (max_q, max_k))
+    return (B, key_heads, heads // key_heads, D, Tq, Tk), window or 0, scale, (q_starts, k_starts, k_lens), *(
+        min(int(n or 0), MOST) for n in (max_q, max_k))
 
 
 @functools.lru_cache(maxsize=256)
@@ -98,7 +106,7 @@ def _at(t):
 
 
 def _forward(q, k, v, causal, how, need_lse):
-    shape, window, scale, q_starts, k_starts, max_q, max_k = how
+    shape, window, scale, (q_starts, k_starts, k_lens), max_q, max_k = how
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if need_lse else None
     (q, qs), (k, ks), (v, vs) = _heads(q), _heads(k), _heads(v)
@@ -110,12 +118,12 @@ def _forward(q, k, v, causal, how, need_lse):
         ws = workspace(nbytes, dev) if nbytes else None
         _lib.check(_lib.lib().spanqr_attention(
             TYPES[q.dtype], *shape, q.data_ptr(), at, k.data_ptr(), at + 24, v.data_ptr(), at + 48, _at(q_starts), _at(k_starts),
-            max_q, max_k, causal, window, scale, out.data_ptr(), _at(lse), _at(ws), nbytes, stream))
+            _at(k_lens), max_q, max_k, causal, window, scale, out.data_ptr(), _at(lse), _at(ws), nbytes, stream))
     return out, lse
 
 
 def _backward(dout, q, k, v, out, lse, causal, how, need_dq, need_dkv):
-    shape, window, scale, q_starts, k_starts, max_q, max_k = how
+    shape, window, scale, (q_starts, k_starts, k_lens), max_q, max_k = how
     dev = q.device
     dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_dq else None
     dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_dkv else None
@@ -129,17 +137,17 @@ def _backward(dout, q, k, v, out, lse, causal, how, need_dq, need_dkv):
         ws = workspace(nbytes, dev)
         _lib.check(_lib.lib().spanqr_attention_backward(
             TYPES[q.dtype], *shape, dout.data_ptr(), at, q.data_ptr(), at + 24, k.data_ptr(), at + 48, v.data_ptr(), at + 72,
-            out.data_ptr(), at + 96, lse.data_ptr(), _at(q_starts), _at(k_starts), max_q, max_k, causal, window, scale, _at(dq),
-            _at(dk), _at(dv), ws.data_ptr(), nbytes, stream))
+            out.data_ptr(), at + 96, lse.data_ptr(), _at(q_starts), _at(k_starts), _at(k_lens), max_q, max_k, causal, window, scale,
+            _at(dq), _at(dk), _at(dv), ws.data_ptr(), nbytes, stream))
     return dq, dk, dv
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, q_starts, k_starts, causal, how):
+    def forward(ctx, q, k, v, causal, how):
         out, lse = _forward(q, k, v, causal, how, True)
-        ctx.save_for_backward(q, k, v, out, lse, q_starts, k_starts)
-        shape, window, scale, _, _, max_q, max_k = how
+        shape, window, scale, lengths, max_q, max_k = how
+        ctx.save_for_backward(q, k, v, out, lse, *lengths)
         ctx.how = causal, shape, window, scale, max_q, max_k
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -148,24 +156,26 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout, _):
         if dout is None:
-            return None, None, None, None, None, None, None
-        q, k, v, out, lse, q_starts, k_starts = ctx.saved_tensors
+            return None, None, None, None, None
+        q, k, v, out, lse, *lengths = ctx.saved_tensors
         causal, shape, window, scale, max_q, max_k = ctx.how
         need = ctx.needs_input_grad
-        grads = _backward(dout, q, k, v, out, lse, causal, (shape, window, scale, q_starts, k_starts, max_q, max_k), need[0],
+        grads = _backward(dout, q, k, v, out, lse, causal, (shape, window, scale, lengths, max_q, max_k), need[0],
                           need[1] or need[2])
-        return (*(once("attention", g, q, k, v, dout) for g in grads), None, None, None, None)
+        return (*(once("attention", g, q, k, v, dout) for g in grads), None, None)
 
 
 def attention(q, k, v, causal=False, window=None, scale=None, q_starts=None, k_starts=None, max_q=None, max_k=None,
-              return_lse=False):
+              return_lse=False, k_lens=None):
     """softmax(scale q k^T) v for each head: q [B, Sq, heads, D], k and v [B, Sk, key heads, D], bfloat16 or float16 on a ROCm
     device, heads a multiple of the key heads (head h reads key head h // (heads / key heads)), D a multiple of 8 up to
     128; scale (positive) is D^-1/2 unless given. Strided tensors, such as the columns of one product, are read as they lie
     where every head's row starts on 16 bytes. The result has q's shape and is contiguous.
 
     Query i stands at p = i + Sk - Sq, so that one token's query reads all that is cached. causal: it sees the keys j <= p;
-    window: only the last `window` of those. A query that sees no key has the result 0.
+    window: only the last `window` of those. A query that sees no key has the result 0. k_lens: int32 [B] on the device, the
+    number of keys that a sequence has of k's Sk (a cache with room); it stands for Sk in all this, and the rows behind are
+    not read.
 
     Packed sequences: q [Tq, heads, D], k and v [Tk, key heads, D], with the sequences' rows end to end: those of sequence b are
     q_starts[b] to q_starts[b + 1] - 1, and k_starts' for the keys (q_starts again where it is not given), int32 [B + 1] on
@@ -181,25 +191,25 @@ def attention(q, k, v, causal=False, window=None, scale=None, q_starts=None, k_s
     lse carries no gradient."""
     no_tangents("attention", q, k, v)
     causal = bool(causal)
-    how = _check("attention", q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_k)
+    how = _check("attention", q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_k, k_lens)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out, lse = _Attention.apply(q, k, v, how[3], how[4], causal, how)
+        out, lse = _Attention.apply(q, k, v, causal, how)
     else:
         out, lse = _forward(q, k, v, causal, how, return_lse)
     return (out, lse) if return_lse else out
 
 
 def attention_backward(dout, q, k, v, out, lse, causal=False, window=None, scale=None, q_starts=None, k_starts=None, max_q=None,
-                       max_k=None, need_dq=True, need_dkv=True):
+                       max_k=None, need_dq=True, need_dkv=True, k_lens=None):
     """(dq, dk, dv): attention's gradients from the gradient dout of its result, with out and lse as it returned them and the
-    other arguments as they were. Contiguous, in the inputs' type; rows of no sequence have the gradient 0. dq is None
+    other arguments as they were. Contiguous, in the inputs' type; rows of no sequence and keys behind k_lens have the gradient 0. dq is None
     with need_dq=False, dk and dv with need_dkv=False. The probabilities are made again from q, k and lse; they, and the
     scores' gradients, are rounded to 16 bits before the products that they go into. The sums over the heads that share
     keys are float32, in a fixed order: a call repeats its bits. None of the gradients carries a gradient."""
     what = "attention_backward"
     no_tangents(what, dout, q, k, v, out, lse)
     causal = bool(causal)
-    how = _check(what, q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_k)
+    how = _check(what, q, k, v, causal, window, scale, q_starts, k_starts, max_q, max_k, k_lens)
     check_like(what, "dout", dout, q, q.shape)
     check_like(what, "out", out, q, q.shape)
     check_tensor(what, "lse", lse, (torch.float32,))

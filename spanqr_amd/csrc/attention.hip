@@ -129,6 +129,7 @@ struct Shape {
     int B, Hk, G, D;              // sequences, key heads, heads a key head, elements a head
     long Tq, Tk;                  // rows of all sequences; of each one where nothing is packed
     const int *q_starts, *k_starts;   // packed: B + 1 each, ascending; or null
+    const int* k_lens;            // not packed: B numbers of keys, or null: Tk
     int causal, window;           // window 0: none
     float scale2;                 // c log2 e
 };
@@ -150,7 +151,8 @@ __device__ __forceinline__ Seq seq_of(const Shape& s, int b) {
         span(s.q_starts, b, s.Tq, r.q0, r.lq);
         span(s.k_starts, b, s.Tk, r.k0, r.lk);
     } else {
-        r = {b * s.Tq, b * s.Tk, (int)s.Tq, (int)s.Tk};
+        const int n = s.k_lens != nullptr ? s.k_lens[b] : (int)s.Tk;
+        r = {b * s.Tq, b * s.Tk, (int)s.Tq, n < 0 ? 0 : n < s.Tk ? n : (int)s.Tk};
     }
     return r;
 }
@@ -779,6 +781,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
     const char* v = head_of<T>(a.v, packed, b, seq.k0, hk);
     constexpr bool SMALL = std::is_same<T, fp16>::value;
     const float d_most = SMALL ? largest(a.d_most + which * a.q_tiles, a.q_tiles, lane) : 0.0f;
+    const int behind = packed ? seq.lk : (int)s.Tk;   // keys with gradients: those that lie behind k_lens have zeros
     auto load = [&](int m0, int buffer) {
         Q.load(m0, M, lds + buffer * BUFFER, wave, lane);
         DO.load(m0, M, lds + buffer * BUFFER + R::BYTES, wave, lane);
@@ -792,13 +795,12 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
         }
     };
 
-    for (int tile = first; (long)tile * KEYS < seq.lk; tile += a.kv_tiles) {
+    for (int tile = first; (long)tile * KEYS < behind; tile += a.kv_tiles) {
         const int n0 = tile * KEYS, w0 = n0 + 32 * (wave % (WAVES / SPLIT)), j = w0 + (lane & 31);
         const bool on = j < seq.lk;
-        const long row = on ? j : 0;
         x8 fk[DP / 16], fv[DP / 16];
-        load_row<T, DP>(k + (long)sizeof(T) * row * a.k.row, on, s.D, lane, fk);
-        load_row<T, DP>(v + (long)sizeof(T) * row * a.v.row, on, s.D, lane, fv);
+        load_row<T, DP>(k + (long)sizeof(T) * j * a.k.row, on, s.D, lane, fk);
+        load_row<T, DP>(v + (long)sizeof(T) * j * a.v.row, on, s.D, lane, fv);
         float up = 0.0f, times = 1.0f;   // dS is multiplied by 2^up, and P by 2^raised already
         if constexpr (SMALL) {
             float sum = 0.0f;
@@ -821,7 +823,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
         const int last = w0 + 31 < seq.lk ? w0 + 31 : seq.lk - 1, block_last = n0 + KEYS < seq.lk ? n0 + KEYS - 1 : seq.lk - 1;
         const int any_lo = first_row(w0), any_hi = w0 < seq.lk ? end_row(last) : 0;
         const int all_lo = first_row(last), all_hi = w0 + 32 <= seq.lk ? end_row(w0) : 0;
-        const int from = first_row(n0) / rows * rows, to = end_row(block_last);
+        const int from = first_row(n0) / rows * rows, to = n0 < seq.lk ? end_row(block_last) : 0;
 
         f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
         if (from < to) load(from, 0);
@@ -919,9 +921,10 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
                 dv[r / 16][r % 16] += sums[64 * (N + r)];
             }
         }
-        const long at = ((seq.k0 + row) * s.Hk + hk) * s.D;
-        store_row<T, DP>((T*)a.dk + at, on, s.D, lane, dk, SMALL ? a.scale * __builtin_amdgcn_exp2f(-up) : a.scale);
-        store_row<T, DP>((T*)a.dv + at, on, s.D, lane, dv, SMALL ? __builtin_amdgcn_exp2f(-raised<T>(false)) : 1.0f);
+        const int key = w0 + (thread() & 31);
+        const long at = ((seq.k0 + key) * s.Hk + hk) * s.D;
+        store_row<T, DP>((T*)a.dk + at, key < behind, s.D, lane, dk, SMALL ? a.scale * __builtin_amdgcn_exp2f(-up) : a.scale);
+        store_row<T, DP>((T*)a.dv + at, key < behind, s.D, lane, dv, SMALL ? __builtin_amdgcn_exp2f(-raised<T>(false)) : 1.0f);
         arrived();
     }
 }
@@ -955,19 +958,20 @@ struct Call {
 };
 
 int check_shape(const char* what, int type, long B, long Hk, long G, long D, long Tq, long Tk, const int* q_starts,
-                const int* k_starts, long max_q, long max_k, int causal, long window, float scale, Call& c) {
+                const int* k_starts, const int* k_lens, long max_q, long max_k, int causal, long window, float scale, Call& c) {
     if (type != SPANQR_BF16 && type != SPANQR_FP16) return error(SPANQR_EINVAL, "%s: the type must be bf16 or fp16", what);
     if (D < 8 || D > 128 || D % 8 != 0) return error(SPANQR_EINVAL, "%s: D = %ld (multiples of 8 up to 128)", what, D);
     if (B < 0 || Hk < 1 || G < 1 || Tq < 0 || Tk < 0 || B > INT_MAX / 2 || Hk > INT_MAX / G || (B + 1) > INT_MAX / Hk ||
         Tq >= MAX_ROWS / G || Tk >= MAX_ROWS || (Tq > 0 && Hk * G > INT_MAX / Tq))
         return error(SPANQR_EINVAL, "%s: B = %ld, heads = %ld x %ld, rows = %ld and %ld", what, B, Hk, G, Tq, Tk);
     if ((q_starts != nullptr) != (k_starts != nullptr)) return error(SPANQR_EINVAL, "%s: q_starts and k_starts belong together", what);
+    if (k_lens != nullptr && q_starts != nullptr) return error(SPANQR_EINVAL, "%s: packed sequences have their lengths from k_starts", what);
     if (window < 0 || (window > 0 && !causal)) return error(SPANQR_EINVAL, "%s: a window needs causal, and one key at least", what);
     if (!(scale > 0.0f && scale * LOG2E < INFINITY)) return error(SPANQR_EINVAL, "%s: scale must be positive and finite", what);
     const bool packed = q_starts != nullptr;
     if (!packed || max_q < 1 || max_q > Tq) max_q = Tq;
     if (!packed || max_k < 1 || max_k > Tk) max_k = Tk;
-    c.s = {(int)B, (int)Hk, (int)G, (int)D, Tq, Tk, q_starts, k_starts, causal ? 1 : 0, (int)(window < MAX_ROWS ? window : MAX_ROWS),
+    c.s = {(int)B, (int)Hk, (int)G, (int)D, Tq, Tk, q_starts, k_starts, k_lens, causal ? 1 : 0, (int)(window < MAX_ROWS ? window : MAX_ROWS),
            scale * LOG2E};
     c.rows = (packed ? 1 : B) * Tq * Hk * G;
     c.q_tiles = blocks(max_q * G) < 1 ? 1 : blocks(max_q * G);
@@ -1052,18 +1056,18 @@ extern "C" {
 long spanqr_attention_workspace(long B, long Hk, long G, long D, long Tq, long Tk, int packed, long max_q, long max_k) {
     Call c;
     const int none = 0;
-    const int rc = check_shape("attention", SPANQR_BF16, B, Hk, G, D, Tq, Tk, packed ? &none : nullptr, packed ? &none : nullptr, max_q,
-                               max_k, 0, 0, 1.0f, c);
+    const int rc = check_shape("attention", SPANQR_BF16, B, Hk, G, D, Tq, Tk, packed ? &none : nullptr, packed ? &none : nullptr, nullptr,
+                               max_q, max_k, 0, 0, 1.0f, c);
     if (rc != SPANQR_OK) return rc;
     return c.splits > 1 ? 4 * c.splits * c.rows * (D + 2) : 0;
 }
 
 int spanqr_attention(int type, long B, long Hk, long G, long D, long Tq, long Tk, const void* q, const long* q_strides, const void* k,
-                     const long* k_strides, const void* v, const long* v_strides, const int* q_starts, const int* k_starts, long max_q,
-                     long max_k, int causal, long window, float scale, void* out, float* lse, void* workspace, long workspace_bytes,
+                     const long* k_strides, const void* v, const long* v_strides, const int* q_starts, const int* k_starts, const int* k_lens,
+                     long max_q, long max_k, int causal, long window, float scale, void* out, float* lse, void* workspace, long workspace_bytes,
                      void* stream) {
     Call c;
-    int rc = check_shape("attention", type, B, Hk, G, D, Tq, Tk, q_starts, k_starts, max_q, max_k, causal, window, scale, c);
+    int rc = check_shape("attention", type, B, Hk, G, D, Tq, Tk, q_starts, k_starts, k_lens, max_q, max_k, causal, window, scale, c);
     if (rc != SPANQR_OK || c.rows == 0) return rc;
     ForwardArgs a = {};
     const bool none = Tk == 0 || (B == 0 && q_starts == nullptr);
@@ -1093,18 +1097,18 @@ long spanqr_attention_backward_workspace(long B, long Hk, long G, long D, long T
     Call c;
     const int none = 0;
     const int rc = check_shape("attention_backward", SPANQR_BF16, B, Hk, G, D, Tq, Tk, packed ? &none : nullptr, packed ? &none : nullptr,
-                               max_q, max_k, 0, 0, 1.0f, c);
+                               nullptr, max_q, max_k, 0, 0, 1.0f, c);
     return rc != SPANQR_OK ? rc : backward_bytes(c);
 }
 
 int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq, long Tk, const void* dout, const long* dout_strides,
                               const void* q, const long* q_strides, const void* k, const long* k_strides, const void* v,
                               const long* v_strides, const void* out, const long* out_strides, const float* lse, const int* q_starts,
-                              const int* k_starts, long max_q, long max_k, int causal, long window, float scale, void* dq, void* dk,
+                              const int* k_starts, const int* k_lens, long max_q, long max_k, int causal, long window, float scale, void* dq, void* dk,
                               void* dv, void* workspace, long workspace_bytes, void* stream) {
     const char* what = "attention_backward";
     Call c;
-    int rc = check_shape(what, type, B, Hk, G, D, Tq, Tk, q_starts, k_starts, max_q, max_k, causal, window, scale, c);
+    int rc = check_shape(what, type, B, Hk, G, D, Tq, Tk, q_starts, k_starts, k_lens, max_q, max_k, causal, window, scale, c);
     if (rc != SPANQR_OK) return rc;
     const bool packed = q_starts != nullptr, no_q = c.rows == 0, no_k = Tk == 0 || (B == 0 && !packed);
     BackwardArgs a = {};

@@ -18,7 +18,7 @@ def strides(batch=64 * 4 * 10, row=64 * 4, head=64):
 
 BAD_SHAPES = [dict(type=0), dict(type=3), dict(B=-1), dict(Hk=0), dict(G=0), dict(D=0), dict(D=4), dict(D=136), dict(D=60), dict(Tq=-1),
               dict(Tk=-1), dict(Tk=1 << 30), dict(Tq=1 << 29), dict(G=1 << 31), dict(B=1 << 40), dict(B=1 << 23), dict(Tq=1 << 28, Hk=8),
-              dict(qs=PTR), dict(ks=PTR), dict(window=-1, causal=1), dict(window=3, causal=0), dict(scale=0.0), dict(scale=-1.0),
+              dict(qs=PTR), dict(ks=PTR), dict(qs=PTR, ks=PTR, lens=PTR), dict(window=-1, causal=1), dict(window=3, causal=0), dict(scale=0.0), dict(scale=-1.0),
               dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38), dict(q=None), dict(k=None), dict(v=None), dict(q=ctypes.c_void_p(4098)),
               dict(q_str=strides(row=65)), dict(q_str=strides(head=1 << 24)), dict(k_str=strides(row=-8)), dict(v_str=strides(batch=4)),
               dict(k_str=None)]
@@ -26,9 +26,9 @@ BAD_SHAPES = [dict(type=0), dict(type=3), dict(B=-1), dict(Hk=0), dict(G=0), dic
 
 def test_forward_refusals():
     def call(type=1, B=2, Hk=2, G=2, D=64, Tq=10, Tk=10, q=PTR, k=PTR, v=PTR, q_str=strides(), k_str=strides(), v_str=strides(), qs=None,
-             ks=None, max_q=0, max_k=0, causal=1, window=0, scale=1.0, out=PTR, ws=None, nbytes=0):
-        return _lib.lib().spanqr_attention(type, B, Hk, G, D, Tq, Tk, q, q_str, k, k_str, v, v_str, qs, ks, max_q, max_k, causal, window,
-                                           scale, out, None, ws, nbytes, None)
+             ks=None, lens=None, max_q=0, max_k=0, causal=1, window=0, scale=1.0, out=PTR, ws=None, nbytes=0):
+        return _lib.lib().spanqr_attention(type, B, Hk, G, D, Tq, Tk, q, q_str, k, k_str, v, v_str, qs, ks, lens, max_q, max_k, causal,
+                                           window, scale, out, None, ws, nbytes, None)
 
     for kw in [*BAD_SHAPES, dict(out=None), dict(out=ctypes.c_void_p(8)), dict(Tk=4096), dict(Tk=4096, ws=PTR, nbytes=100)]:
         assert call(**kw) == EINVAL, kw
@@ -41,10 +41,10 @@ def test_backward_refusals():
     assert need == 8 * 2 * 10 * 4 + 4 * 2 * 2 * (1 + 1)
 
     def call(type=1, B=2, Hk=2, G=2, D=64, Tq=10, Tk=10, do=PTR, q=PTR, k=PTR, v=PTR, o=PTR, do_str=strides(), q_str=strides(),
-             k_str=strides(), v_str=strides(), o_str=strides(), lse=PTR, qs=None, ks=None, causal=1, window=0, scale=1.0, dq=PTR, dk=PTR,
+             k_str=strides(), v_str=strides(), o_str=strides(), lse=PTR, qs=None, ks=None, lens=None, causal=1, window=0, scale=1.0, dq=PTR, dk=PTR,
              dv=PTR, ws=PTR, nbytes=need):
         return _lib.lib().spanqr_attention_backward(type, B, Hk, G, D, Tq, Tk, do, do_str, q, q_str, k, k_str, v, v_str, o, o_str, lse,
-                                                    qs, ks, 0, 0, causal, window, scale, dq, dk, dv, ws, nbytes, None)
+                                                    qs, ks, lens, 0, 0, causal, window, scale, dq, dk, dv, ws, nbytes, None)
 
     for kw in [*BAD_SHAPES, dict(do=None), dict(o=None), dict(do_str=strides(row=4)), dict(o_str=strides(head=12)), dict(lse=None),
                dict(ws=None), dict(nbytes=need - 1), dict(dk=None), dict(dv=None), dict(dq=ctypes.c_void_p(8)),

@@ -72,9 +72,11 @@ def near(got, want, err, what):
                            f"{bad.nonzero()[0].tolist()}")
 
 
-def check(q, k, v, dout=None, causal=False, window=None, scale=None, sequences=None, **packed):
-    """runs the operator and compares; sequences: (first query, end, first key, end) of packed ones"""
+def check(q, k, v, dout=None, causal=False, window=None, scale=None, sequences=None, lens=None, **packed):
+    """runs the operator and compares; sequences: (first query, end, first key, end) of packed ones; lens: k_lens as numbers"""
     D, H, Hk = q.shape[-1], q.shape[-2], k.shape[-2]
+    if lens is not None:
+        packed["k_lens"] = torch.tensor(lens, dtype=torch.int32, device="cuda")
     small = HALF[q.dtype], TINY[q.dtype], PTINY[q.dtype], DSTINY[q.dtype]
     out, lse = sp.attention(q, k, v, causal=causal, window=window, scale=scale, return_lse=True, **packed)
     grads = [] if dout is None else sp.attention_backward(dout, q, k, v, out, lse, causal=causal, window=window, scale=scale, **packed)
@@ -88,7 +90,7 @@ def check(q, k, v, dout=None, causal=False, window=None, scale=None, sequences=N
     want = {n: zeros(t) for n, t in (("out", q), ("dq", q), ("dk", k), ("dv", v)) if n in got}
     want_lse = torch.full(q.shape[:-1], -math.inf, dtype=torch.float64, device="cuda")
     if sequences is None:
-        at = [((b,), (b,)) for b in range(q.shape[0])]
+        at = [((b,), (b, slice(0, k.shape[1] if lens is None else lens[b]))) for b in range(q.shape[0])]
     else:
         at = [((slice(a, e),), (slice(x, y),)) for a, e, x, y in sequences]
     for qa, ka in at:
@@ -146,6 +148,62 @@ def test_tokens_against_a_cache(cuda, B, Sq, Sk, H, Hk, D, window, dtype):
     check(q, k, v, causal=True, window=window)
     if window is None and Sq == 1:
         assert torch.equal(sp.attention(q, k, v), sp.attention(q, k, v, causal=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Sq,Sk,H,Hk,D,window,lens", [
+    (1, 5000, 16, 2, 128, None, [5000, 1, 0, 2500, 64, 65]), (1, 300, 4, 4, 64, None, [3, 0, 300, 128]), (4, 2000, 8, 1, 80, 100, [2, 1999, 700]),
+    (70, 200, 4, 2, 64, None, [200, 70, 13, 0, 129]), (130, 300, 3, 1, 128, 50, [0, 300, 299, 31, 64])])
+def test_lengths_of_a_cache(cuda, Sq, Sk, H, Hk, D, window, lens, dtype):
+    """what lies behind a sequence's keys is NaN, and neither read nor given a gradient"""
+    B = len(lens)
+    q, dout = normal(B, Sq, H, D, seed=1, dtype=dtype, size=1.5), normal(B, Sq, H, D, seed=4, dtype=dtype)
+    k, v = normal(B, Sk, Hk, D, seed=2, dtype=dtype, size=1.5), normal(B, Sk, Hk, D, seed=3, dtype=dtype)
+    for b, n in enumerate(lens):
+        k[b, n:] = v[b, n:] = float("nan")
+    check(q, k, v, dout, True, window, lens=lens)
+    if window is None:
+        check(q, k, v, dout, lens=lens)
+    # numbers outside 0 to Sk are taken as these
+    wild = torch.tensor([-5 if n == 0 else n if n < Sk else Sk + 7 for n in lens], dtype=torch.int32, device=cuda)
+    assert torch.equal(sp.attention(q, k, v, k_lens=wild), sp.attention(q, k, v, k_lens=wild.clamp(0, Sk)))
+
+
+def test_lengths_autograd_and_replays(cuda):
+    """k_lens changed between replays, as a cache grows; the gradient through autograd; batch strides"""
+    cache = normal(3, 500, 2, 2, 64)
+    q = normal(3, 1, 8, 64, seed=5)
+    lens = torch.tensor([1, 100, 499], dtype=torch.int32, device=cuda)
+    k, v = cache[:, :, 0], cache[:, :, 1]
+
+    def step():
+        return sp.attention(q, k, v, causal=True, k_lens=lens)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(4):
+        graph.replay()
+        eager = step()
+        assert torch.equal(got, eager)
+        for b, n in enumerate(lens.tolist()):
+            # (other splits of the keys, so other roundings: two calls, each half a step of the probabilities and of the result,
+            # which is below sum p |v|, known to 2 half steps of itself)
+            at = q[b:b + 1], k[b:b + 1, :n]
+            most = sp.attention(*at, v[b:b + 1, :n].abs()).float()
+            assert ((sp.attention(*at, v[b:b + 1, :n]) - eager[b]).float().abs() <= 4.1 * 2.0 ** -8 * most).all()
+        lens.add_(1).clamp_(max=500)
+    leaf = cache.clone().requires_grad_()
+    lens = torch.tensor([1, 0, 77], dtype=torch.int32, device=cuda)
+    out, lse = sp.attention(q, leaf[:, :, 0], leaf[:, :, 1], k_lens=lens, return_lse=True)
+    out.backward(q)
+    _, dk, dv = sp.attention_backward(q, q, k, v, out.detach(), lse, k_lens=lens)
+    assert torch.equal(leaf.grad, torch.stack([dk, dv], 2)) and not leaf.grad[1].any() and not leaf.grad[2, 77:].any()
 
 
 def packed_case(lq, lk, H, Hk, D, dtype, front=0, behind=0):
@@ -354,13 +412,16 @@ def test_refusals(cuda):
               lambda: sp.attention(q[0], k[0], v[0], q_starts=starts, k_starts=starts[:1]),
               lambda: sp.attention(q[0], k[0], v[0], q_starts=starts[:0]),
               lambda: sp.attention(q[0], k[0], v[0], q_starts=starts, max_q=-1),
+              lambda: sp.attention(q, k, v, k_lens=starts[:1]), lambda: sp.attention(q, k, v, k_lens=starts.cpu()),
+              lambda: sp.attention(q[0], k[0], v[0], q_starts=starts, k_lens=starts[:1]),
               lambda: sp.attention(normal(1, 2, 1, 136), normal(1, 2, 1, 136), normal(1, 2, 1, 136)),
               lambda: sp.attention_backward(q[:1], q, k, v, out, lse), lambda: sp.attention_backward(q, q, k, v, out[:1], lse),
               lambda: sp.attention_backward(q, q, k, v, out, lse[:1])):
         with pytest.raises(ValueError):
             f()
     for f in (lambda: sp.attention(q.float(), k.float(), v.float()), lambda: sp.attention(q, k.half(), v),
-              lambda: sp.attention(q[0], k[0], v[0], q_starts=starts.long()), lambda: sp.attention_backward(q.half(), q, k, v, out, lse),
+              lambda: sp.attention(q[0], k[0], v[0], q_starts=starts.long()), lambda: sp.attention(q, k, v, k_lens=starts.long()),
+              lambda: sp.attention_backward(q.half(), q, k, v, out, lse),
               lambda: sp.attention_backward(q, q, k, v, out, lse.half()), lambda: sp.attention(q.cpu(), k.cpu(), v.cpu())):
         with pytest.raises(TypeError):
             f()
