@@ -1,5 +1,5 @@
-"""What the training operators (loss.py, norm.py, clip.py) share: types of the C ABI, checks of tensors, and the device
-and stream a call runs on."""
+"""What the training operators (loss.py, norm.py, clip.py, block.py, attn.py) share: types of the C ABI, checks of tensors,
+and the device and stream a call runs on."""
 import contextlib
 
 import torch
