@@ -10,7 +10,9 @@
 //
 // Bound by memory: each input is read once and each output written once, the row stays in registers between the two sums
 // (threads and pieces as in norm.hip). Between them would be h, t, n1, dt and the mask in memory if these were operators of
-// their own. Sums are fp32: per thread over at most 16 elements, then a tree in a fixed order.
+// their own. Sums are fp32: per thread over at most 16 elements, then a tree in a fixed order. 16384 x 2048 bf16 with gate and
+// dropout: forward 61 us for 0.34 GB, gradient 91 for 0.54 GB and k_block_sums 7, with the 256 MB cache's help above a large
+// copy's 5.2 TB/s; without dropout's ten rounds of multiplications 161 us in all instead of 169.
 #include "host.h"
 #include "random.h"
 #include "rows.h"
@@ -600,7 +602,7 @@ __global__ __launch_bounds__(1024) void k_block_sums(const float* part, int part
 bool past_caches(long rows, long D, long bytes) { return rows * D * bytes > 32l << 20; }
 
 // Dropout alone: a workgroup takes DROP_PIECES neighbouring pieces at a time, a thread every 256th of them, so that its loads
-// are under way together. pieces: of a row.
+// are under way together. pieces: of a row. 16384 x 5120 bf16: 72 us, 4.7 TB/s.
 constexpr int DROP_PIECES = 512;
 template <typename T>
 __global__ __launch_bounds__(256) void k_dropout(long rows, long D, uint32_t pieces, const T* x, long ldx, Dropout drop, T* y, bool past) {
