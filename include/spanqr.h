@@ -392,10 +392,11 @@ int spanqr_block_norm_backward(int type, int wtype, int act, long rows, long D, 
  * Hk, D] by their strides {batch, row, head} in elements (host arrays, read at the call): multiples of 8, those of rows and
  * heads below 2^24, neighbouring elements of a head, 16-byte alignment. D: a multiple of 8 up to 128.
  * q_starts null: B sequences of Tq queries and Tk keys, of which with k_lens (device, B; read when the kernels run, taken as
- * from 0 to Tk; or null) the first k_lens[b] are there, and the others are not read. Else packed: Tq and Tk rows in all, sequence b having the rows
- * q_starts[b] to q_starts[b + 1] - 1 and k_starts' (device, B + 1 each, ascending; read when the kernels run, and nothing outside
- * the rows is touched whatever they hold; batch strides are not used); max_q and max_k, the longest sequence's or 0,
- * set how much is launched alone. Query i stands at p = i + (its sequence's keys) - (queries); causal: it sees the
+ * from 0 to Tk; or null) the first k_lens[b] are there, and the others are not read. Else packed: Tq and Tk rows in all,
+ * sequence b having the rows q_starts[b] to q_starts[b + 1] - 1 and k_starts' (device, B + 1 each, ascending; read when the
+ * kernels run, and nothing outside the rows is touched whatever they hold; batch strides are not used); max_q and max_k, the
+ * longest sequence's or 0, set how much is launched alone (and so the number of parts of a sum). Query i stands at
+ * p = i + (its sequence's keys) - (queries); causal: it sees the
  * keys j <= p, with a window (0: none; needs causal) only those with j > p - window. One that sees none has out 0 and lse
  * -inf. out [rows][Hk G][D] contiguous, 16-byte aligned; lse [rows][Hk G] fp32, log sum exp of the scores, or null; rows of
  * no sequence are written as those that see no key. P is rounded to the type before the product with v.

@@ -577,7 +577,63 @@ struct BackwardArgs {
     int q_tiles, k_tiles, kv_tiles;
     float scale;
     float *v_most, *d_most;   // fp16: the largest |V_j|^2 and |dO_i|^2 of a sequence, key head and workgroup's rows
+    int q_splits, kv_splits;  // workgroups that share a tile, each going over a part of the other side
+    float *q_part, *k_part, *v_part;   // [split][rows of all x heads][D], where there is more than one
 };
+
+// the split's share of [from, to), which it takes in steps of `step`
+__device__ __forceinline__ void share(int split, int splits, int step, int& from, int& to) {
+    if (splits == 1 || from >= to) return;
+    const int each = ((to - from + step - 1) / step + splits - 1) / splits * step;
+    const long at = from + (long)split * each;
+    from = at < to ? (int)at : to;
+    to = to - from > each ? from + each : to;
+}
+
+// a result's column as it is, times f, 16 bytes a lane
+template <int DP>
+__device__ __forceinline__ void store_part(float* p, bool on, int D, int lane, const f32x16 (&c)[DP / 32], float f) {
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int d = 32 * dt + 8 * q + 4 * (lane >> 5);
+            if (on && d < D) *(float4*)(p + d) = make_float4(c[dt][4 * q] * f, c[dt][4 * q + 1] * f, c[dt][4 * q + 2] * f, c[dt][4 * q + 3] * f);
+        }
+}
+
+// Sums of the splits' parts, in their order, eight elements a thread; zeros in rows of no sequence. One launch for all three.
+struct Parts {
+    const float* part;
+    void* out;
+    const int* starts;        // packed: B + 1
+    long rows, width;         // of all sequences; elements of a row
+    int splits;               // 1: nothing to do
+};
+struct PartsArgs {
+    Parts of[3];
+    int B;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void k_parts(const PartsArgs a) {
+    const Parts& p = a.of[blockIdx.y];
+    if (p.splits == 1) return;
+    const long n = p.rows * p.width;
+    const long begin = p.starts != nullptr ? clip_start(p.starts[0], p.rows) : 0, end = p.starts != nullptr ? clip_start(p.starts[a.B], p.rows) : p.rows;
+    for (long i = 8 * (blockIdx.x * 256l + threadIdx.x); i < n; i += 8l * 256 * gridDim.x) {
+        const long row = i / p.width;
+        const bool in = row >= begin && row < end;
+        float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int k = 0; k < p.splits; ++k) {
+            const float4 x = *(const float4*)(p.part + k * n + i), y = *(const float4*)(p.part + k * n + i + 4);
+            sum[0] += x.x, sum[1] += x.y, sum[2] += x.z, sum[3] += x.w, sum[4] += y.x, sum[5] += y.y, sum[6] += y.z, sum[7] += y.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] = in ? sum[j] : 0.0f;
+        store8((T*)p.out + i, 8, sum);
+    }
+}
 
 // |V_j|^2's maxima over a workgroup's rows: 16 lanes a row, eight elements a lane
 template <typename T>
@@ -616,10 +672,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const bool packed = s.q_starts != nullptr;
     const int many = (s.B + (packed ? 1 : 0)) * s.Hk;
-    const int which = blockIdx.x % many, first = a.q_tiles - 1 - blockIdx.x / many;
+    const int which = blockIdx.x % many, turn = blockIdx.x / many, split = turn / a.q_tiles, first = a.q_tiles - 1 - turn % a.q_tiles;
     const int b = which / s.Hk, hk = which % s.Hk;
     if (b == s.B) {
-        if (a.dq != nullptr)
+        if (a.dq != nullptr && a.q_splits == 1)
             outside((T*)a.dq, nullptr, clip_start(s.q_starts[0], s.Tq), clip_start(s.q_starts[s.B], s.Tq), s.Tq, (long)s.Hk * s.G * s.D, 0,
                     first * s.Hk + hk, a.q_tiles * s.Hk);
         return;
@@ -665,7 +721,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) delta = fmaf((float)fo[ks][e], (float)fd[ks][e], delta);
             delta = both_halves(delta, [](float x, float y) { return x + y; });
-            if (on && h == 0) {
+            if (on && h == 0 && split == 0) {
                 a.stat[at] = lse - raised<T>(false);
                 a.stat[a.rows + at] = -delta;
             }
@@ -684,9 +740,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
         const int any_lo = s.window && i_first + ahead - s.window + 1 > 0 ? i_first + ahead - s.window + 1 : 0;
         const int all_lo = s.window && i_last + ahead - s.window + 1 > 0 ? i_last + ahead - s.window + 1 : 0;
         const int block_last = (m0 + BLOCK < M ? m0 + BLOCK : M) - 1;
-        const int to = s.causal ? (block_last / s.G + ahead + 1 < k_to ? block_last / s.G + ahead + 1 : k_to) : k_to;
+        int to = s.causal ? (block_last / s.G + ahead + 1 < k_to ? block_last / s.G + ahead + 1 : k_to) : k_to;
         int from = s.window && m0 / s.G + ahead - s.window + 1 > 0 ? m0 / s.G + ahead - s.window + 1 : 0;
         from &= ~(TILE - 1);
+        share(split, a.q_splits, TILE, from, to);
 
         f32x16 dq[DP / 32] = {};
         for (int i = 0; i < 2; ++i)
@@ -739,10 +796,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
                 stream<DP / 16>(c, cols, [&](int i, x8 x) { dq[i % (DP / 32)] = mfma(x, ds[i / (DP / 32)], dq[i % (DP / 32)]); }, [](int) {});
             }
         }
-        store_row<T, DP>((T*)a.dq + at * s.D, on, s.D, lane, dq, SMALL ? a.scale * __builtin_amdgcn_exp2f(-up) : a.scale);
+        const float times = SMALL ? a.scale * __builtin_amdgcn_exp2f(-up) : a.scale;
+        if (a.q_splits == 1)
+            store_row<T, DP>((T*)a.dq + at * s.D, on, s.D, lane, dq, times);
+        else
+            store_part<DP>(a.q_part + (split * a.rows + at) * s.D, on, s.D, lane, dq, times);
         arrived();
     }
-    if constexpr (SMALL) {
+    if (SMALL && split == 0) {
         d_most = reduce_threads<64 * WAVES, NanMax>(d_most, (float*)smem);
         if (threadIdx.x == 0) a.d_most[which * a.q_tiles + first] = d_most;
     }
@@ -767,9 +828,11 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const bool packed = s.q_starts != nullptr;
     const int many = (s.B + (packed ? 1 : 0)) * s.Hk;
-    const int which = blockIdx.x % many, first = blockIdx.x / many;   // (the first keys are seen by most)
+    const int which = blockIdx.x % many, turn = blockIdx.x / many;
+    const int split = turn / a.kv_tiles, first = turn % a.kv_tiles;   // (the first keys are seen by most)
     const int b = which / s.Hk, hk = which % s.Hk;
     if (b == s.B) {
+        if (a.kv_splits > 1) return;
         const long from = clip_start(s.k_starts[0], s.Tk), to = clip_start(s.k_starts[s.B], s.Tk), width = (long)s.Hk * s.D;
         outside((T*)a.dk, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, a.kv_tiles * s.Hk);
         outside((T*)a.dv, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, a.kv_tiles * s.Hk);
@@ -788,6 +851,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
     const char* v = head_of<T>(a.v, packed, b, seq.k0, hk);
     constexpr bool SMALL = std::is_same<T, fp16>::value;
     const float d_most = SMALL ? largest(a.d_most + which * a.q_tiles, a.q_tiles, lane) : 0.0f;
+    const long all_keys = (packed ? s.Tk : s.B * s.Tk) * s.Hk;
     const int behind = packed ? seq.lk : (int)s.Tk;   // keys with gradients: those that lie behind k_lens have zeros
     auto load = [&](int m0, int buffer) {
         Q.load(m0, M, lds + buffer * BUFFER, wave, lane);
@@ -830,7 +894,8 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
         const int last = w0 + 31 < seq.lk ? w0 + 31 : seq.lk - 1, block_last = n0 + KEYS < seq.lk ? n0 + KEYS - 1 : seq.lk - 1;
         const int any_lo = first_row(w0), any_hi = w0 < seq.lk ? end_row(last) : 0;
         const int all_lo = first_row(last), all_hi = w0 + 32 <= seq.lk ? end_row(w0) : 0;
-        const int from = first_row(n0) / rows * rows, to = n0 < seq.lk ? end_row(block_last) : 0;
+        int from = first_row(n0) / rows * rows, to = n0 < seq.lk ? end_row(block_last) : 0;
+        share(split, a.kv_splits, rows, from, to);
 
         f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
         if (from < to) load(from, 0);
@@ -930,8 +995,15 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
         }
         const int key = w0 + (thread() & 31);
         const long at = ((seq.k0 + key) * s.Hk + hk) * s.D;
-        store_row<T, DP>((T*)a.dk + at, key < behind, s.D, lane, dk, SMALL ? a.scale * __builtin_amdgcn_exp2f(-up) : a.scale);
-        store_row<T, DP>((T*)a.dv + at, key < behind, s.D, lane, dv, SMALL ? __builtin_amdgcn_exp2f(-raised<T>(false)) : 1.0f);
+        const float k_times = SMALL ? a.scale * __builtin_amdgcn_exp2f(-up) : a.scale, v_times = SMALL ? __builtin_amdgcn_exp2f(-raised<T>(false)) : 1.0f;
+        if (a.kv_splits == 1) {
+            store_row<T, DP>((T*)a.dk + at, key < behind, s.D, lane, dk, k_times);
+            store_row<T, DP>((T*)a.dv + at, key < behind, s.D, lane, dv, v_times);
+        } else {
+            const long in = split * all_keys * s.D + at;
+            store_part<DP>(a.k_part + in, key < behind, s.D, lane, dk, k_times);
+            store_part<DP>(a.v_part + in, key < behind, s.D, lane, dv, v_times);
+        }
         arrived();
     }
 }
@@ -944,8 +1016,7 @@ long blocks(long n) { return (n + BLOCK - 1) / BLOCK; }
 
 // Where there are few workgroups the keys are split among several, so that 512 (two for each compute unit) run, each with
 // 128 keys at least; the sums are joined by a second kernel.
-long splits_of(long B, long Hk, long tiles, long max_k) {
-    const long have = B * Hk * tiles;
+long splits_of(long have, long max_k) {
     if (have == 0 || have >= 256) return 1;
     const long want = (512 + have - 1) / have, most = max_k / 128;
     const long n = want < most ? want : most;
@@ -957,11 +1028,22 @@ long splits_of(long B, long Hk, long tiles, long max_k) {
 // 160 / 139, 16 x 512 x 16 x 64 on 4 116 / 98, packed 24 x 2048 x 8 x 64 on 2 357 / 294; with more of them 16 x 1024 x 12 x 64 190 / 204.
 bool few_keys(long B, long Hk, long k_tiles, long D) { return B * Hk * k_tiles <= 256 * (D <= 64 ? 3 : 2); }
 
+// Workgroups that share a tile of dQ's rows, or of dK's and dV's, each with four tiles of the other side at least: so many that
+// 512 run, where tiles make fewer than 256. Gradient with forward, in us without / with: 1 x 1362 x 8
+// on 1 x 64 284 / 82, 1 x 2048 x 16 on 2 x 128 480 / 199, 1 x 8192 x 2 on 1 x 64 448 / 216, 2 x 2277 x 3 x 128 fp16 194 / 200.
+long grad_splits_of(long tiles, long others) {
+    if (tiles >= 256) return 1;
+    const long want = (512 + tiles - 1) / tiles, most = others / 4;
+    const long n = want < most ? want : most;
+    return n < 1 ? 1 : n;
+}
+
 struct Call {
     Shape s;
-    long rows;                 // of all sequences, times heads
+    long rows, keys;           // of all sequences, times heads
     long q_tiles, k_tiles;     // tiles a head that workgroups are launched for
     long splits;
+    long kv_tiles, q_splits, kv_splits;   // of the gradient
 };
 
 int check_shape(const char* what, int type, long B, long Hk, long G, long D, long Tq, long Tk, const int* q_starts,
@@ -981,17 +1063,30 @@ int check_shape(const char* what, int type, long B, long Hk, long G, long D, lon
     c.s = {(int)B, (int)Hk, (int)G, (int)D, Tq, Tk, q_starts, k_starts, k_lens, causal ? 1 : 0, (int)(window < MAX_ROWS ? window : MAX_ROWS),
            scale * LOG2E};
     c.rows = (packed ? 1 : B) * Tq * Hk * G;
+    c.keys = (packed ? 1 : B) * Tk * Hk;
     c.q_tiles = blocks(max_q * G) < 1 ? 1 : blocks(max_q * G);
     c.k_tiles = blocks(max_k) < 1 ? 1 : blocks(max_k);
-    c.splits = splits_of(B, Hk, c.q_tiles, max_k);
+    // (packed rows that max_q and max_k say nothing of count too: parts are held for all rows)
+    const long q_all = packed && blocks(Tq * G) > B * c.q_tiles ? blocks(Tq * G) : B * c.q_tiles;
+    c.splits = B == 0 ? 1 : splits_of(Hk * q_all, max_k);
+    c.kv_tiles = few_keys(B, Hk, c.k_tiles, D) ? 2 * c.k_tiles : c.k_tiles;
+    const long k_all = packed && blocks(Tk) > B * c.kv_tiles ? blocks(Tk) : B * c.kv_tiles;
+    c.q_splits = B == 0 || c.rows == 0 ? 1 : grad_splits_of(Hk * q_all, (max_k + TILE - 1) / TILE);
+    c.kv_splits = B == 0 || c.keys == 0 ? 1 : grad_splits_of(Hk * k_all, (max_q * G + TILE - 1) / TILE);
     // (a launch takes fewer than 2^32 threads, 2^24 workgroups)
-    if ((B + 1) * Hk > MAX_GRID / (c.q_tiles * c.splits) || (B + 1) * Hk > MAX_GRID / (2 * c.k_tiles))
+    if ((B + 1) * Hk > MAX_GRID / (c.q_tiles * c.splits) || (B + 1) * Hk > MAX_GRID / (c.q_tiles * c.q_splits) ||
+        (B + 1) * Hk > MAX_GRID / (c.kv_tiles * c.kv_splits))
         return error(SPANQR_EINVAL, "%s: too many workgroups", what);
     return SPANQR_OK;
 }
 
-// two numbers a row, and the maxima of fp16
-long backward_bytes(const Call& c) { return 8 * c.rows + 4l * c.s.B * c.s.Hk * (c.q_tiles + c.k_tiles); }
+// two numbers a row, the maxima of fp16, and behind them (on 16 bytes) the parts
+long stat_bytes(const Call& c) { return 8 * c.rows + 4l * c.s.B * c.s.Hk * (c.q_tiles + c.k_tiles); }
+long part_bytes(long rows, long splits, long D) { return splits == 1 ? 0 : 4 * rows * splits * D; }
+long backward_bytes(const Call& c) {
+    const long q = part_bytes(c.rows, c.q_splits, c.s.D), kv = 2 * part_bytes(c.keys, c.kv_splits, c.s.D);
+    return q + kv == 0 ? stat_bytes(c) : (stat_bytes(c) + 15) / 16 * 16 + q + kv;
+}
 
 // strides: {batch, row, head}
 int check_heads(const char* what, const char* name, const void* p, const long* strides, bool empty, Heads& h) {
@@ -1039,20 +1134,32 @@ void launch_backward(const BackwardArgs& a, hipStream_t st) {
     if (std::is_same<T, fp16>::value && s.B > 0 && s.Tk > 0 && a.rows > 0)
         k_v_most<T><<<s.B * s.Hk * a.k_tiles, 64 * WAVES, 0, st>>>(a);
     if (a.rows > 0) {
-#define LAUNCH(DP) k_dq<T, DP><<<heads * a.q_tiles, 64 * WAVES, 0, st>>>(a)
+#define LAUNCH(DP) k_dq<T, DP><<<heads * a.q_tiles * a.q_splits, 64 * WAVES, 0, st>>>(a)
         SPANQR_HEADS(LAUNCH)
 #undef LAUNCH
     }
     if (a.dk != nullptr && heads > 0 && s.Tk > 0) {
         if (a.kv_tiles != a.k_tiles) {
-#define LAUNCH(DP) k_dkv<T, DP, 2><<<heads * a.kv_tiles, 64 * WAVES, 0, st>>>(a)
+#define LAUNCH(DP) k_dkv<T, DP, 2><<<heads * a.kv_tiles * a.kv_splits, 64 * WAVES, 0, st>>>(a)
             SPANQR_HEADS(LAUNCH)
 #undef LAUNCH
         } else {
-#define LAUNCH(DP) k_dkv<T, DP, 1><<<heads * a.kv_tiles, 64 * WAVES, 0, st>>>(a)
+#define LAUNCH(DP) k_dkv<T, DP, 1><<<heads * a.kv_tiles * a.kv_splits, 64 * WAVES, 0, st>>>(a)
             SPANQR_HEADS(LAUNCH)
 #undef LAUNCH
         }
+    }
+    if (a.q_splits > 1 || a.kv_splits > 1) {
+        const bool packed = s.q_starts != nullptr;
+        const long q_rows = packed ? s.Tq : s.B * s.Tq, k_rows = packed ? s.Tk : s.B * s.Tk, k_width = (long)s.Hk * s.D, q_width = k_width * s.G;
+        PartsArgs p = {{{a.k_part, a.dk, s.k_starts, k_rows, k_width, a.kv_splits},
+                        {a.v_part, a.dv, s.k_starts, k_rows, k_width, a.kv_splits},
+                        {a.q_part, a.dq, s.q_starts, q_rows, q_width, a.q_splits}},
+                       s.B};
+        long most = 0;
+        for (const Parts& x : p.of) most = x.splits > 1 && x.rows * x.width > most ? x.rows * x.width : most;
+        const long grid = (most / 8 + 255) / 256;
+        k_parts<T><<<dim3(grid < 2048 ? grid : 2048, 3), 256, 0, st>>>(p);
     }
 }
 
@@ -1141,10 +1248,15 @@ int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq
     a.rows = c.rows;
     a.q_tiles = (int)c.q_tiles;
     a.k_tiles = (int)c.k_tiles;
-    a.kv_tiles = few_keys(B, Hk, c.k_tiles, D) ? 2 * a.k_tiles : a.k_tiles;
+    a.kv_tiles = (int)c.kv_tiles;
     a.scale = scale;
     a.v_most = a.stat + 2 * c.rows;
     a.d_most = a.v_most + B * Hk * c.k_tiles;
+    a.q_splits = dq != nullptr ? (int)c.q_splits : 1;
+    a.kv_splits = dk != nullptr ? (int)c.kv_splits : 1;
+    a.q_part = (float*)((char*)workspace + (stat_bytes(c) + 15) / 16 * 16);
+    a.k_part = a.q_part + part_bytes(c.rows, c.q_splits, D) / 4;
+    a.v_part = a.k_part + part_bytes(c.keys, c.kv_splits, D) / 4;
     if (type == SPANQR_BF16)
         launch_backward<bf16>(a, (hipStream_t)stream);
     else

@@ -64,6 +64,13 @@ def test_workspace():
     # packed: by the longest sequence, where it is known
     assert f(32, 2, 8, 128, 32, 70000, 1, 1, 4096) == 4 * 8 * 32 * 16 * 130
     assert f(4, 1, 1, 64, 4, 400, 1, 1, 100) == 0
+    # hints far below what there is do not multiply what is held for all rows
+    assert f(1, 2, 1, 64, 1 << 20, 1 << 20, 1, 1, 1 << 20) == 0
+    g = _lib.lib().spanqr_attention_backward_workspace
+    assert g(1, 1, 1, 64, 1 << 20, 1 << 20, 1, 1, 1) == 8 * (1 << 20) + 4 * 2
+    # few tiles: 11 of dQ's rows in 5 parts (22 tiles of keys, four each at least), 22 of dK's and dV's in 5 (22 of rows)
+    assert g(1, 1, 8, 64, 171, 1362, 0, 0, 0) == (8 * 1368 + 4 * (11 + 11) + 15) // 16 * 16 + 4 * 64 * (5 * 1368 + 2 * 5 * 1362)
+    assert g(0, 1, 8, 64, 171, 1362, 1, 0, 0) == 8 * 1368 and f(0, 1, 8, 64, 171, 1362, 1, 0, 0) == 0
 
 
 def test_python_refusals_on_the_host():
