@@ -1023,17 +1023,19 @@ long splits_of(long have, long max_k) {
     return n < 1 ? 1 : n;
 }
 
-// Whether the gradient of K and V takes 64 keys a workgroup: where 128 make no more than the device runs at once (three
-// workgroups a compute unit of up to 64 wide heads, two of wider ones). Both ways in us with 128 / 64: 8 x 1024 x 8 x 128 on 4 heads
-// 160 / 139, 16 x 512 x 16 x 64 on 4 116 / 98, packed 24 x 2048 x 8 x 64 on 2 357 / 294; with more of them 16 x 1024 x 12 x 64 190 / 204.
-bool few_keys(long B, long Hk, long k_tiles, long D) { return B * Hk * k_tiles <= 256 * (D <= 64 ? 3 : 2); }
+// The workgroups of the gradient that the device runs at once: three a compute unit of up to 64 wide heads, two of wider ones
+long at_once(long D) { return 256 * (D <= 64 ? 3 : 2); }
 
-// Workgroups that share a tile of dQ's rows, or of dK's and dV's, each with four tiles of the other side at least: so many that
-// 512 run, where tiles make fewer than 256. Gradient with forward, in us without / with: 1 x 1362 x 8
-// on 1 x 64 284 / 82, 1 x 2048 x 16 on 2 x 128 480 / 199, 1 x 8192 x 2 on 1 x 64 448 / 216, 2 x 2277 x 3 x 128 fp16 194 / 200.
-long grad_splits_of(long tiles, long others) {
-    if (tiles >= 256) return 1;
-    const long want = (512 + tiles - 1) / tiles, most = others / 4;
+// Whether the gradient of K and V takes 64 keys a workgroup: where 128 make no more than the device runs at once. Both ways in us with 128 / 64: 8 x 1024 x 8 x 128 on 4 heads
+// 160 / 139, 16 x 512 x 16 x 64 on 4 116 / 98, packed 24 x 2048 x 8 x 64 on 2 357 / 294; with more of them 16 x 1024 x 12 x 64 190 / 204.
+bool few_keys(long B, long Hk, long k_tiles, long D) { return B * Hk * k_tiles <= at_once(D); }
+
+// Workgroups that share a tile of dQ's rows, or of dK's and dV's, each with four tiles of the other side at least: as many as run
+// at once, or, where the mask leaves some tiles little to do, as many as that needs. XXX
+long grad_splits_of(long tiles, long others, long D, int causal) {
+    const long slots = at_once(D);
+    if (tiles >= slots) return 1;
+    const long want = (causal ? slots + tiles - 1 : slots) / tiles, most = others / 4;
     const long n = want < most ? want : most;
     return n < 1 ? 1 : n;
 }
@@ -1071,8 +1073,8 @@ int check_shape(const char* what, int type, long B, long Hk, long G, long D, lon
     c.splits = B == 0 ? 1 : splits_of(Hk * q_all, max_k);
     c.kv_tiles = few_keys(B, Hk, c.k_tiles, D) ? 2 * c.k_tiles : c.k_tiles;
     const long k_all = packed && blocks(Tk) > B * c.kv_tiles ? blocks(Tk) : B * c.kv_tiles;
-    c.q_splits = B == 0 || c.rows == 0 ? 1 : grad_splits_of(Hk * q_all, (max_k + TILE - 1) / TILE);
-    c.kv_splits = B == 0 || c.keys == 0 ? 1 : grad_splits_of(Hk * k_all, (max_q * G + TILE - 1) / TILE);
+    c.q_splits = B == 0 || c.rows == 0 ? 1 : grad_splits_of(Hk * q_all, (max_k + TILE - 1) / TILE, D, causal);
+    c.kv_splits = B == 0 || c.keys == 0 ? 1 : grad_splits_of(Hk * k_all, (max_q * G + TILE - 1) / TILE, D, causal);
     // (a launch takes fewer than 2^32 threads, 2^24 workgroups)
     if ((B + 1) * Hk > MAX_GRID / (c.q_tiles * c.splits) || (B + 1) * Hk > MAX_GRID / (c.q_tiles * c.q_splits) ||
         (B + 1) * Hk > MAX_GRID / (c.kv_tiles * c.kv_splits))
@@ -1211,7 +1213,7 @@ long spanqr_attention_backward_workspace(long B, long Hk, long G, long D, long T
     Call c;
     const int none = 0;
     const int rc = check_shape("attention_backward", SPANQR_BF16, B, Hk, G, D, Tq, Tk, packed ? &none : nullptr, packed ? &none : nullptr,
-                               nullptr, max_q, max_k, 0, 0, 1.0f, c);
+                               nullptr, max_q, max_k, 1, 0, 1.0f, c);   // (causal ones have the most parts)
     return rc != SPANQR_OK ? rc : backward_bytes(c);
 }
 
