@@ -401,7 +401,7 @@ int spanqr_block_norm_backward(int type, int wtype, int act, long rows, long D, 
  * -inf. out [rows][Hk G][D] contiguous, 16-byte aligned; lse [rows][Hk G] fp32, log sum exp of the scores, or null; rows of
  * no sequence are written as those that see no key. P is rounded to the type before the product with v.
  * The elements of a sequence have to be finite, also where a mask hides them; scale is positive. A sequence's Tq G and Tk
- * stay below 2^30, Tq Hk G below 2^31. workspace: spanqr_attention_workspace bytes (0 unless the keys are split). */
+ * stay below 2^30, Tq Hk G below 2^31, (B + 1) Hk below 2^24. workspace: spanqr_attention_workspace bytes (0 unless the keys are split). */
 long spanqr_attention_workspace(long B, long Hk, long G, long D, long Tq, long Tk, int packed, long max_q, long max_k);
 int spanqr_attention(int type, long B, long Hk, long G, long D, long Tq, long Tk, const void* q, const long* q_strides,
                      const void* k, const long* k_strides, const void* v, const long* v_strides, const int* q_starts,

@@ -181,7 +181,8 @@ def attention(q, k, v, causal=False, window=None, scale=None, q_starts=None, k_s
     q_starts[b] to q_starts[b + 1] - 1, and k_starts' for the keys (q_starts again where it is not given), int32 [B + 1] on
     the device, ascending. They are read on the device, when the work runs: rows in front of the first sequence and
     behind the last one are not read and have the result 0. max_q and max_k: the longest sequence's rows, as far as
-    known; they set how much is launched, and so over how many parts sums go, but nothing else of what comes out.
+    known; they set how much is launched, and so over how many parts sums go, but nothing else of what comes out. Without them the
+    launch goes by all rows and the number of sequences.
 
     The probabilities are rounded to 16 bits before the product with v; scores, softmax and sums are float32. Within a
     sequence q, k and v have to be finite, also where a mask hides them.

@@ -345,12 +345,67 @@ __device__ void outside(T* p, float* rest, long from, long to, long rows, long w
 }
 __device__ __forceinline__ long clip_start(int s, long T) { return s < 0 ? 0 : s > T ? T : s; }
 
+// What workgroups are dealt out by: tiles of EACH rows (of `per` a row in memory), a sequence's and key head's `n` each, a
+// workgroup taking every step-th of them where it has more. Or, where `work` is not 0, one list a key head for all sequences of a packed
+// call: slot start_b per / EACH + b + t is tile t of sequence b. A sequence's slots lie behind each other and are as many as its
+// tiles, or one more, so that `work` slots are enough whatever the lengths are, which the host does not know. Behind them come
+// the workgroups for the rows of no sequence.
+struct Tiles {
+    int n, work, step;
+};
+struct Place {
+    int b, hk, split, first;   // b: B for rows of no sequence (first: of how many, see `others`), -1 for a slot without a tile
+};
+template <int EACH>
+__device__ __forceinline__ int slot_of(const int* starts, int b, long T, int per) {
+    return (int)((uint64_t)(clip_start(starts[b], T) * per) / EACH) + b;
+}
+// The last sequence whose slots begin at `slot` or before, or -1: each wavefront's lanes look at 64 of them at a time. (Whatever
+// the starts hold, it ends, and looks at B + 1 of them.)
+template <int EACH>
+__device__ __forceinline__ int sequence_of(const int* starts, int B, long T, int per, int slot) {
+    const int lane = threadIdx.x & 63;
+    int b = 0, n = B + 1;
+    while (true) {
+        const int step = (n + 63) / 64, at = b + lane * step;
+        const int k = __popcll(__ballot(lane * step < n && slot_of<EACH>(starts, at < B ? at : B, T, per) <= slot));
+        if (k == 0) return -1;
+        b += (k - 1) * step;
+        n -= (k - 1) * step;
+        if (step == 1) return b < B ? b : -1;
+        n = n < step ? n : step;
+    }
+}
+// LAST: a sequence's last tiles first. extra: with workgroups for the rows of no sequence
+template <int EACH, bool LAST>
+__device__ __forceinline__ Place place_of(const Shape& s, const Tiles& t, const int* starts, long T, int per, bool extra) {
+    const int many = t.work == 0 ? (s.B + (extra ? 1 : 0)) * s.Hk : s.Hk;
+    const int which = blockIdx.x % many, turn = blockIdx.x / many, split = turn / t.n;
+    const int first = LAST ? t.n - 1 - turn % t.n : turn % t.n;
+    if (t.work == 0) return {which / s.Hk, which % s.Hk, split, first};
+    if (first >= t.work) return {s.B, which, split, first - t.work};
+    const int b = sequence_of<EACH>(starts, s.B, T, per, first), tile = b < 0 ? -1 : first - slot_of<EACH>(starts, b, T, per);
+    return {tile < 0 ? -1 : b, which, split, tile};   // (below 0: starts that do not ascend)
+}
+__device__ __forceinline__ int others(const Tiles& t) { return t.work == 0 ? t.n : t.n - t.work; }
+// the maxima that the workgroups of a sequence and key head leave, one for each slot: the first one's place and how many
+__device__ __forceinline__ int maxima_of(const Shape& s, const Tiles& t, int b, int hk, long row0, int rows, int& n) {
+    if (t.work == 0) {
+        n = t.n;
+        return (b * s.Hk + hk) * t.n;
+    }
+    const int from = (int)((uint64_t)row0 / BLOCK);
+    n = (int)((uint64_t)(row0 + rows) / BLOCK) + 1 - from;
+    return hk * t.work + from + b;
+}
+
 struct ForwardArgs {
     Shape s;
     Heads q, k, v;
     void* out;            // [rows of all][heads][D]
     float* lse;           // [rows of all][heads], or null
-    int tiles, splits;
+    Tiles tiles;
+    int splits;
     float* part;          // splits > 1: [split][rows of all x heads][D] sums, and behind them float2 (base, sum) for each
     long rows;            // rows of all x heads
 };
@@ -372,13 +427,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const bool packed = s.q_starts != nullptr;
     // all heads' longest rows of keys first; neighbouring heads go round the XCDs, so that a head's tiles meet in one L2
-    const int many = (s.B + (packed && a.splits == 1 ? 1 : 0)) * s.Hk;
-    const int which = blockIdx.x % many, turn = blockIdx.x / many;
-    const int split = turn / a.tiles, first = a.tiles - 1 - turn % a.tiles;
-    const int b = which / s.Hk, hk = which % s.Hk;
+    const Place place = place_of<BLOCK, true>(s, a.tiles, s.q_starts, s.Tq, s.G, packed && a.splits == 1);
+    const int b = place.b, hk = place.hk, split = place.split, first = place.first;
+    if (b < 0) return;
     if (b == s.B) {
         outside((T*)a.out, a.lse, clip_start(s.q_starts[0], s.Tq), clip_start(s.q_starts[s.B], s.Tq), s.Tq, (long)s.Hk * s.G * s.D,
-                s.Hk * s.G, first * s.Hk + hk, a.tiles * s.Hk);
+                s.Hk * s.G, first * s.Hk + hk, others(a.tiles) * s.Hk);
         return;
     }
     const Seq seq = seq_of(s, b);
@@ -392,7 +446,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) 
     const int chunk = a.splits == 1 ? seq.lk : ((seq.lk + a.splits - 1) / a.splits + TILE - 1) / TILE * TILE;
     const int k_from = split * chunk < seq.lk ? split * chunk : seq.lk, k_to = k_from + chunk < seq.lk ? k_from + chunk : seq.lk;
 
-    for (int tile = first; (long)tile * BLOCK < M; tile += a.tiles) {
+    for (int tile = first; (long)tile * BLOCK < M; tile += a.tiles.step) {
         const int m0 = tile * BLOCK, w0 = m0 + 32 * wave, m = w0 + (lane & 31);
         const int i = (m < M ? m : M - 1) / s.G, g = m - i * s.G;
         const bool on = m < M;
@@ -574,9 +628,9 @@ struct BackwardArgs {
     void *dq, *dk, *dv;   // contiguous
     float* stat;          // [2][rows of all x heads], from k_dq: lse log2 e (inf where nothing is seen), -D
     long rows;
-    int q_tiles, k_tiles, kv_tiles;
+    Tiles q_tiles, k_tiles, kv_tiles;
     float scale;
-    float *v_most, *d_most;   // fp16: the largest |V_j|^2 and |dO_i|^2 of a sequence, key head and workgroup's rows
+    float *v_most, *d_most;   // fp16: the largest |V_j|^2 and |dO_i|^2 of each workgroup of k_tiles and q_tiles
     int q_splits, kv_splits;  // workgroups that share a tile, each going over a part of the other side
     float *q_part, *k_part, *v_part;   // [split][rows of all x heads][D], where there is more than one
 };
@@ -640,12 +694,14 @@ template <typename T>
 __global__ __launch_bounds__(64 * WAVES) void k_v_most(const BackwardArgs a) {
     __shared__ float slot[WAVES];
     const Shape& s = a.s;
-    const int many = s.B * s.Hk, which = blockIdx.x % many, first = blockIdx.x / many, b = which / s.Hk, hk = which % s.Hk;
+    const Place place = place_of<BLOCK, false>(s, a.k_tiles, s.k_starts, s.Tk, 1, false);
+    const int b = place.b, hk = place.hk, first = place.first;
+    if (b < 0) return;
     const Seq seq = seq_of(s, b);
     const T* v = (const T*)head_of<T>(a.v, s.q_starts != nullptr, b, seq.k0, hk);
     const int d = 8 * (threadIdx.x & 15), here = s.D - d >= 8 ? 8 : 0;
     float most = 0.0f;
-    for (int tile = first; (long)tile * BLOCK < seq.lk; tile += a.k_tiles)
+    for (int tile = first; (long)tile * BLOCK < seq.lk; tile += a.k_tiles.step)
         for (int j = tile * BLOCK + (threadIdx.x >> 4); j < (tile + 1) * BLOCK && j < seq.lk; j += 16) {
             float x[8], sum = 0.0f;
             load8(v + j * a.v.row + d, here, x);
@@ -654,7 +710,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_v_most(const BackwardArgs a) {
             most = fmaxf(most, finite(reduce_lanes<16, Sum>(sum)));
         }
     most = reduce_threads<64 * WAVES, NanMax>(most, slot);
-    if (threadIdx.x == 0) a.v_most[which * a.k_tiles + first] = most;
+    int n;
+    if (threadIdx.x == 0) a.v_most[maxima_of(s, a.k_tiles, b, hk, seq.k0, seq.lk, n) + first] = most;
 }
 
 // dQ: as the forward pass, 128 rows a workgroup; a lane has one query. It has dO in registers, so it forms D first, and leaves it
@@ -671,13 +728,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
     const Shape& s = a.s;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const bool packed = s.q_starts != nullptr;
-    const int many = (s.B + (packed ? 1 : 0)) * s.Hk;
-    const int which = blockIdx.x % many, turn = blockIdx.x / many, split = turn / a.q_tiles, first = a.q_tiles - 1 - turn % a.q_tiles;
-    const int b = which / s.Hk, hk = which % s.Hk;
+    const Place place = place_of<BLOCK, true>(s, a.q_tiles, s.q_starts, s.Tq, s.G, packed);
+    const int b = place.b, hk = place.hk, split = place.split, first = place.first;
+    if (b < 0) return;
     if (b == s.B) {
         if (a.dq != nullptr && a.q_splits == 1)
             outside((T*)a.dq, nullptr, clip_start(s.q_starts[0], s.Tq), clip_start(s.q_starts[s.B], s.Tq), s.Tq, (long)s.Hk * s.G * s.D, 0,
-                    first * s.Hk + hk, a.q_tiles * s.Hk);
+                    first * s.Hk + hk, others(a.q_tiles) * s.Hk);
         return;
     }
     const Seq seq = seq_of(s, b);
@@ -690,10 +747,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
     const char* d_out = head_of<T>(a.dout, packed, b, seq.q0, hk * s.G);
     const char* out = head_of<T>(a.out, packed, b, seq.q0, hk * s.G);
     constexpr bool SMALL = std::is_same<T, fp16>::value;
-    const float v_most = SMALL ? largest(a.v_most + which * a.k_tiles, a.k_tiles, lane) : 0.0f;
-    float d_most = 0.0f;
+    float v_most = 0.0f, d_most = 0.0f;
+    if constexpr (SMALL) {
+        int n;
+        const int from = maxima_of(s, a.k_tiles, b, hk, seq.k0, seq.lk, n);
+        v_most = largest(a.v_most + from, n, lane);
+    }
 
-    for (int tile = first; (long)tile * BLOCK < M; tile += a.q_tiles) {
+    for (int tile = first; (long)tile * BLOCK < M; tile += a.q_tiles.step) {
         const int m0 = tile * BLOCK, w0 = m0 + 32 * wave, m = w0 + (lane & 31);
         const int i = (m < M ? m : M - 1) / s.G, g = m - i * s.G;
         const bool on = m < M;
@@ -805,7 +866,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
     }
     if (SMALL && split == 0) {
         d_most = reduce_threads<64 * WAVES, NanMax>(d_most, (float*)smem);
-        if (threadIdx.x == 0) a.d_most[which * a.q_tiles + first] = d_most;
+        int n;
+        if (threadIdx.x == 0) a.d_most[maxima_of(s, a.q_tiles, b, hk, seq.q0 * s.G, M, n) + first] = d_most;
     }
 }
 
@@ -827,15 +889,14 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
     const Shape& s = a.s;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const bool packed = s.q_starts != nullptr;
-    const int many = (s.B + (packed ? 1 : 0)) * s.Hk;
-    const int which = blockIdx.x % many, turn = blockIdx.x / many;
-    const int split = turn / a.kv_tiles, first = turn % a.kv_tiles;   // (the first keys are seen by most)
-    const int b = which / s.Hk, hk = which % s.Hk;
+    const Place place = place_of<KEYS, false>(s, a.kv_tiles, s.k_starts, s.Tk, 1, packed);   // (the first keys are seen by most)
+    const int b = place.b, hk = place.hk, split = place.split, first = place.first;
+    if (b < 0) return;
     if (b == s.B) {
         if (a.kv_splits > 1) return;
         const long from = clip_start(s.k_starts[0], s.Tk), to = clip_start(s.k_starts[s.B], s.Tk), width = (long)s.Hk * s.D;
-        outside((T*)a.dk, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, a.kv_tiles * s.Hk);
-        outside((T*)a.dv, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, a.kv_tiles * s.Hk);
+        outside((T*)a.dk, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, others(a.kv_tiles) * s.Hk);
+        outside((T*)a.dv, nullptr, from, to, s.Tk, width, 0, first * s.Hk + hk, others(a.kv_tiles) * s.Hk);
         return;
     }
     const Seq seq = seq_of(s, b);
@@ -850,7 +911,12 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
     const char* k = head_of<T>(a.k, packed, b, seq.k0, hk);
     const char* v = head_of<T>(a.v, packed, b, seq.k0, hk);
     constexpr bool SMALL = std::is_same<T, fp16>::value;
-    const float d_most = SMALL ? largest(a.d_most + which * a.q_tiles, a.q_tiles, lane) : 0.0f;
+    float d_most = 0.0f;
+    if constexpr (SMALL) {
+        int n;
+        const int from = maxima_of(s, a.q_tiles, b, hk, seq.q0 * s.G, M, n);
+        d_most = largest(a.d_most + from, n, lane);
+    }
     const long all_keys = (packed ? s.Tk : s.B * s.Tk) * s.Hk;
     const int behind = packed ? seq.lk : (int)s.Tk;   // keys with gradients: those that lie behind k_lens have zeros
     auto load = [&](int m0, int buffer) {
@@ -866,7 +932,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
         }
     };
 
-    for (int tile = first; (long)tile * KEYS < behind; tile += a.kv_tiles) {
+    for (int tile = first; (long)tile * KEYS < behind; tile += a.kv_tiles.step) {
         const int n0 = tile * KEYS, w0 = n0 + 32 * (wave % (WAVES / SPLIT)), j = w0 + (lane & 31);
         const bool on = j < seq.lk;
         x8 fk[DP / 16], fv[DP / 16];
@@ -1012,7 +1078,31 @@ constexpr long MAX_ROWS = 1l << 30;      // queries x group, or keys, of a seque
 constexpr long MAX_GRID = (1l << 24) - 1;
 constexpr long MAX_STRIDE = 1l << 24;    // of rows and heads: a tile's offsets stay within 32 bits
 
-long blocks(long n) { return (n + BLOCK - 1) / BLOCK; }
+long tiles_in(long n, long each) { return n < 1 ? 1 : (n + each - 1) / each; }
+
+// Whether the tiles of packed sequences are one list: where those of B sequences, each as long as the longest one (or as all rows, if
+// that is not known), would be more than twice as many. Forward / gradient in us with a list / without: 256 texts of up to 973 in
+// 131072 rows x 40 on 8 x 128 without max_q 1620 / 4742 against 15831 / 27229, 24 of 1024 x 8 on 2 x 128 90 / 345 against 132 / 431. A
+// sequence's tiles lie behind each other there, where else all sequences' longest ones go first: at 24 unlike ones whose longest is
+// known, with 1.5 times the workgroups, 106 / 415 against 101 / 369.
+bool as_list(bool packed, long B, long all, long longest, long each) { return packed && 2 * (all / each + B) < B * tiles_in(longest, each); }
+
+// Tiles of `each` rows, with hints about as many as there are. (Rows that a hint too small says nothing of count too: parts are
+// held for all rows.)
+long count_of(bool packed, long B, long all, long longest, long each) {
+    const long n = as_list(packed, B, all, longest, each) ? all / each + B : B * tiles_in(longest, each);
+    return packed && n < tiles_in(all, each) ? tiles_in(all, each) : n;
+}
+
+// The tiles that workgroups are launched for. Behind a list, for `extra`, 256 workgroups for rows of no sequence. A launch takes fewer than
+// 2^32 threads, 2^24 workgroups: where there are more tiles, each goes over several. n = 0: too many even so.
+Tiles tiles_of(bool packed, long B, long Hk, long all, long longest, long each, long splits, bool extra) {
+    const long slots = all / each + B, tail = !extra ? 0 : slots * Hk < 256 ? slots : (255 + Hk) / Hk, most = MAX_GRID / ((B + 1) * Hk * splits);
+    long n = tiles_in(longest, each);
+    if (as_list(packed, B, all, longest, each) && (slots + tail) * Hk * splits <= MAX_GRID) return {(int)(slots + tail), (int)slots, 1 << 24};
+    n = n < most ? n : most;
+    return {(int)n, 0, (int)n};
+}
 
 // Where there are few workgroups the keys are split among several, so that 512 (two for each compute unit) run, each with
 // 128 keys at least; the sums are joined by a second kernel.
@@ -1028,7 +1118,7 @@ long at_once(long D) { return 256 * (D <= 64 ? 3 : 2); }
 
 // Whether the gradient of K and V takes 64 keys a workgroup: where 128 make no more than the device runs at once. Both ways in us with 128 / 64: 8 x 1024 x 8 x 128 on 4 heads
 // 160 / 139, 16 x 512 x 16 x 64 on 4 116 / 98, packed 24 x 2048 x 8 x 64 on 2 357 / 294; with more of them 16 x 1024 x 12 x 64 190 / 204.
-bool few_keys(long B, long Hk, long k_tiles, long D) { return B * Hk * k_tiles <= at_once(D); }
+bool few_keys(long tiles, long D) { return tiles <= at_once(D); }
 
 // Workgroups that share a tile of dQ's rows, or of dK's and dV's, each with four tiles of the other side at least: as many as run
 // at once, or one more where a mask makes tiles uneven. Both ways in us without / with: 1 x 1362 x 8 on 1 x 64 284 / 81, causal
@@ -1046,9 +1136,10 @@ long grad_splits_of(long tiles, long others, long D, int causal) {
 struct Call {
     Shape s;
     long rows, keys;           // of all sequences, times heads
-    long q_tiles, k_tiles;     // tiles a head that workgroups are launched for
     long splits;
-    long kv_tiles, q_splits, kv_splits;   // of the gradient
+    bool few_keys;             // the gradient of K and V takes 64 keys a workgroup
+    long q_splits, kv_splits;  // of the gradient
+    Tiles tiles, q_tiles, k_tiles, kv_tiles;   // of the forward pass and the gradient
 };
 
 int check_shape(const char* what, int type, long B, long Hk, long G, long D, long Tq, long Tk, const int* q_starts,
@@ -1069,24 +1160,24 @@ int check_shape(const char* what, int type, long B, long Hk, long G, long D, lon
            scale * LOG2E};
     c.rows = (packed ? 1 : B) * Tq * Hk * G;
     c.keys = (packed ? 1 : B) * Tk * Hk;
-    c.q_tiles = blocks(max_q * G) < 1 ? 1 : blocks(max_q * G);
-    c.k_tiles = blocks(max_k) < 1 ? 1 : blocks(max_k);
-    // (packed rows that max_q and max_k say nothing of count too: parts are held for all rows)
-    const long q_all = packed && blocks(Tq * G) > B * c.q_tiles ? blocks(Tq * G) : B * c.q_tiles;
-    c.splits = B == 0 ? 1 : splits_of(Hk * q_all, max_k);
-    c.kv_tiles = few_keys(B, Hk, c.k_tiles, D) ? 2 * c.k_tiles : c.k_tiles;
-    const long k_all = packed && blocks(Tk) > B * c.kv_tiles ? blocks(Tk) : B * c.kv_tiles;
-    c.q_splits = B == 0 || c.rows == 0 ? 1 : grad_splits_of(Hk * q_all, (max_k + TILE - 1) / TILE, D, causal);
-    c.kv_splits = B == 0 || c.keys == 0 ? 1 : grad_splits_of(Hk * k_all, (max_q * G + TILE - 1) / TILE, D, causal);
-    // (a launch takes fewer than 2^32 threads, 2^24 workgroups)
-    if ((B + 1) * Hk > MAX_GRID / (c.q_tiles * c.splits) || (B + 1) * Hk > MAX_GRID / (c.q_tiles * c.q_splits) ||
-        (B + 1) * Hk > MAX_GRID / (c.kv_tiles * c.kv_splits))
-        return error(SPANQR_EINVAL, "%s: too many workgroups", what);
+    const long q_all = Hk * count_of(packed, B, Tq * G, max_q * G, BLOCK), max_m = max_q * G;
+    c.splits = B == 0 ? 1 : splits_of(q_all, max_k);
+    c.few_keys = few_keys(Hk * count_of(packed, B, Tk, max_k, BLOCK), D);
+    const long keys = c.few_keys ? BLOCK / 2 : BLOCK;
+    c.q_splits = B == 0 || c.rows == 0 ? 1 : grad_splits_of(q_all, (max_k + TILE - 1) / TILE, D, causal);
+    c.kv_splits = B == 0 || c.keys == 0 ? 1 : grad_splits_of(Hk * count_of(packed, B, Tk, max_k, keys), (max_m + TILE - 1) / TILE, D, causal);
+    c.tiles = tiles_of(packed, B, Hk, Tq * G, max_m, BLOCK, c.splits, c.splits == 1);
+    c.q_tiles = tiles_of(packed, B, Hk, Tq * G, max_m, BLOCK, c.q_splits, c.q_splits == 1);
+    c.k_tiles = tiles_of(packed, B, Hk, Tk, max_k, BLOCK, 1, false);
+    c.kv_tiles = tiles_of(packed, B, Hk, Tk, max_k, keys, c.kv_splits, c.kv_splits == 1);
+    if (c.tiles.n < 1 || c.q_tiles.n < 1 || c.k_tiles.n < 1 || c.kv_tiles.n < 1)
+        return error(SPANQR_EINVAL, "%s: B = %ld sequences of %ld key heads are too many workgroups", what, B, Hk);
     return SPANQR_OK;
 }
 
 // two numbers a row, the maxima of fp16, and behind them (on 16 bytes) the parts
-long stat_bytes(const Call& c) { return 8 * c.rows + 4l * c.s.B * c.s.Hk * (c.q_tiles + c.k_tiles); }
+long maxima(const Call& c, const Tiles& t) { return (t.work == 0 ? (long)c.s.B * t.n : t.work) * c.s.Hk; }
+long stat_bytes(const Call& c) { return 8 * c.rows + 4 * (maxima(c, c.q_tiles) + maxima(c, c.k_tiles)); }
 long part_bytes(long rows, long splits, long D) { return splits == 1 ? 0 : 4 * rows * splits * D; }
 long backward_bytes(const Call& c) {
     const long q = part_bytes(c.rows, c.q_splits, c.s.D), kv = 2 * part_bytes(c.keys, c.kv_splits, c.s.D);
@@ -1115,11 +1206,13 @@ bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
     else if (s.D <= 96) LAUNCH(96);     \
     else LAUNCH(128);
 
+// extra: as in place_of
+int grid_of(const Shape& s, const Tiles& t, bool extra, int splits) { return (t.work == 0 ? s.B + (extra ? 1 : 0) : 1) * s.Hk * t.n * splits; }
+
 template <typename T>
 void launch_forward(const ForwardArgs& a, hipStream_t st) {
     const Shape& s = a.s;
-    const bool tail = s.q_starts != nullptr && a.splits == 1;
-    const int grid = (s.B + (tail ? 1 : 0)) * s.Hk * a.tiles * a.splits;
+    const int grid = grid_of(s, a.tiles, s.q_starts != nullptr && a.splits == 1, a.splits);
 #define LAUNCH(DP) k_forward<T, DP><<<grid, 64 * WAVES, 0, st>>>(a)
     SPANQR_HEADS(LAUNCH)
 #undef LAUNCH
@@ -1133,29 +1226,28 @@ void launch_forward(const ForwardArgs& a, hipStream_t st) {
 }
 
 template <typename T>
-void launch_backward(const BackwardArgs& a, hipStream_t st) {
+void launch_backward(const BackwardArgs& a, bool few_keys, hipStream_t st) {
     const Shape& s = a.s;
-    const int heads = (s.B + (s.q_starts != nullptr ? 1 : 0)) * s.Hk;
+    const bool packed = s.q_starts != nullptr;
     if (std::is_same<T, fp16>::value && s.B > 0 && s.Tk > 0 && a.rows > 0)
-        k_v_most<T><<<s.B * s.Hk * a.k_tiles, 64 * WAVES, 0, st>>>(a);
+        k_v_most<T><<<grid_of(s, a.k_tiles, false, 1), 64 * WAVES, 0, st>>>(a);
     if (a.rows > 0) {
-#define LAUNCH(DP) k_dq<T, DP><<<heads * a.q_tiles * a.q_splits, 64 * WAVES, 0, st>>>(a)
+#define LAUNCH(DP) k_dq<T, DP><<<grid_of(s, a.q_tiles, packed, a.q_splits), 64 * WAVES, 0, st>>>(a)
         SPANQR_HEADS(LAUNCH)
 #undef LAUNCH
     }
-    if (a.dk != nullptr && heads > 0 && s.Tk > 0) {
-        if (a.kv_tiles != a.k_tiles) {
-#define LAUNCH(DP) k_dkv<T, DP, 2><<<heads * a.kv_tiles * a.kv_splits, 64 * WAVES, 0, st>>>(a)
+    if (a.dk != nullptr && (packed || s.B > 0) && s.Tk > 0) {
+        if (few_keys) {
+#define LAUNCH(DP) k_dkv<T, DP, 2><<<grid_of(s, a.kv_tiles, packed, a.kv_splits), 64 * WAVES, 0, st>>>(a)
             SPANQR_HEADS(LAUNCH)
 #undef LAUNCH
         } else {
-#define LAUNCH(DP) k_dkv<T, DP, 1><<<heads * a.kv_tiles * a.kv_splits, 64 * WAVES, 0, st>>>(a)
+#define LAUNCH(DP) k_dkv<T, DP, 1><<<grid_of(s, a.kv_tiles, packed, a.kv_splits), 64 * WAVES, 0, st>>>(a)
             SPANQR_HEADS(LAUNCH)
 #undef LAUNCH
         }
     }
     if (a.q_splits > 1 || a.kv_splits > 1) {
-        const bool packed = s.q_starts != nullptr;
         const long q_rows = packed ? s.Tq : s.B * s.Tq, k_rows = packed ? s.Tk : s.B * s.Tk, k_width = (long)s.Hk * s.D, q_width = k_width * s.G;
         PartsArgs p = {{{a.k_part, a.dk, s.k_starts, k_rows, k_width, a.kv_splits},
                         {a.v_part, a.dv, s.k_starts, k_rows, k_width, a.kv_splits},
@@ -1201,7 +1293,7 @@ int spanqr_attention(int type, long B, long Hk, long G, long D, long Tq, long Tk
     a.s = c.s;
     a.out = out;
     a.lse = lse;
-    a.tiles = (int)c.q_tiles;
+    a.tiles = c.tiles;
     a.splits = (int)c.splits;
     a.part = (float*)workspace;
     a.rows = c.rows;
@@ -1251,21 +1343,21 @@ int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq
     a.dv = dv;
     a.stat = (float*)workspace;
     a.rows = c.rows;
-    a.q_tiles = (int)c.q_tiles;
-    a.k_tiles = (int)c.k_tiles;
-    a.kv_tiles = (int)c.kv_tiles;
+    a.q_tiles = c.q_tiles;
+    a.k_tiles = c.k_tiles;
+    a.kv_tiles = c.kv_tiles;
     a.scale = scale;
     a.v_most = a.stat + 2 * c.rows;
-    a.d_most = a.v_most + B * Hk * c.k_tiles;
+    a.d_most = a.v_most + maxima(c, c.k_tiles);
     a.q_splits = dq != nullptr ? (int)c.q_splits : 1;
     a.kv_splits = dk != nullptr ? (int)c.kv_splits : 1;
     a.q_part = (float*)((char*)workspace + (stat_bytes(c) + 15) / 16 * 16);
     a.k_part = a.q_part + part_bytes(c.rows, c.q_splits, D) / 4;
     a.v_part = a.k_part + part_bytes(c.keys, c.kv_splits, D) / 4;
     if (type == SPANQR_BF16)
-        launch_backward<bf16>(a, (hipStream_t)stream);
+        launch_backward<bf16>(a, c.few_keys, (hipStream_t)stream);
     else
-        launch_backward<fp16>(a, (hipStream_t)stream);
+        launch_backward<fp16>(a, c.few_keys, (hipStream_t)stream);
     return launched(what);
 }
 

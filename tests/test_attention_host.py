@@ -78,3 +78,16 @@ def test_python_refusals_on_the_host():
     for f in (lambda: sp.attention(q, q, q), lambda: sp.attention_backward(q, q, q, q, q, q[..., 0].float())):
         with pytest.raises(TypeError, match="GPU"):
             f()
+
+
+def test_packed_calls_without_hints():
+    """many sequences whose longest one nobody names: what is launched goes by the rows there are"""
+    f, g = _lib.lib().spanqr_attention_workspace, _lib.lib().spanqr_attention_backward_workspace
+    for B, Hk, G, T in ((512, 8, 1, 1 << 19), (1000, 8, 1, 1 << 20), (1024, 8, 1, 1 << 18), (256, 8, 5, 1 << 17), (1 << 15, 4, 2, 1 << 20)):
+        assert f(B, Hk, G, 128, T, T, 1, 0, 0) == 0, (B, Hk, G, T)
+        # two numbers a row, and a maximum for each slot of the list
+        assert g(B, Hk, G, 128, T, T, 1, 0, 0) == 8 * T * Hk * G + 4 * Hk * (T * G // 128 + B + T // 128 + B), (B, Hk, G, T)
+    assert f(1 << 24, 1, 1, 128, 1 << 24, 1 << 24, 1, 0, 0) == EINVAL   # a workgroup for each is too many
+    assert b"too many workgroups" in _lib.lib().spanqr_last_error()
+    # more tiles than a launch takes workgroups: each goes over several
+    assert f((1 << 23) - 1, 1, 129, 8, 1, 4, 0, 0, 0) == 0

@@ -465,3 +465,47 @@ def test_graph_and_streams(cuda):
         assert all(torch.equal(a, b) for a, b in zip(got, eager))
         if at[1] == 100:
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def lengths(n, most, seed, every=3):
+    """n lengths up to `most`, some of them 0"""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(0, most + 1, (n,), generator=g)
+    x[torch.randint(0, every, (n,), generator=g) == 0] = 0
+    return x.tolist()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,most,long,H,Hk,D,window,front,behind", [
+    (70, 200, 700, 2, 1, 64, None, 5, 900), (130, 40, 1500, 3, 1, 128, 50, 0, 3), (20, 300, 0, 10, 2, 40, None, 400, 0),
+    (4200, 3, 260, 1, 1, 16, None, 1, 2)])
+def test_many_packed_without_hints(cuda, n, most, long, H, Hk, D, window, front, behind, dtype):
+    """sequences of unlike lengths in one list of tiles, one long one among them, with hints and without"""
+    lq = lengths(n, most, seed=1)
+    lk = lengths(n, most, seed=2)
+    lq[n // 2], lk[n // 2] = lq[n // 2] + long, lk[n // 2] + long
+    q, k, v, dout, packed = packed_case(lq, lk, H, Hk, D, dtype, front, behind)
+    got, lse = check(q, k, v, dout, True, window, **packed)
+    sequences = packed.pop("sequences")
+    hints = dict(max_q=max(lq), max_k=max(lk))
+    out, lse2 = sp.attention(q, k, v, causal=True, window=window, return_lse=True, **packed, **hints)
+    if not (torch.equal(out, got["out"]) and torch.equal(lse, lse2)):   # (another number of parts)
+        check(q, k, v, dout, True, window, sequences=sequences, **packed, **hints)
+
+
+def test_more_tiles_than_workgroups(cuda):
+    """a launch takes fewer than 2^24 workgroups; 2^24 tiles are gone over by 2^23"""
+    B = (1 << 23) - 1
+    q, k, v = normal(1, 1, 129, 8, seed=1), normal(1, 4, 1, 8, seed=2), normal(1, 4, 1, 8, seed=3)
+    dout = normal(1, 1, 129, 8, seed=4)
+
+    def all_of(t):
+        return t.expand(B, *t.shape[1:])
+
+    want, lse = sp.attention(q, k, v, return_lse=True)
+    out = sp.attention(all_of(q), all_of(k), all_of(v))
+    assert torch.equal(out[0], want[0]) and not (out != want).any()
+    del out
+    dq, _, _ = sp.attention_backward(all_of(dout), all_of(q), all_of(k), all_of(v), all_of(want), all_of(lse), need_dkv=False)
+    want, _, _ = sp.attention_backward(dout, q, k, v, want, lse)
+    assert torch.equal(dq[0], want[0]) and not (dq != want).any()
