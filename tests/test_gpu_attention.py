@@ -509,3 +509,22 @@ def test_more_tiles_than_workgroups(cuda):
     dq, _, _ = sp.attention_backward(all_of(dout), all_of(q), all_of(k), all_of(v), all_of(want), all_of(lse), need_dkv=False)
     want, _, _ = sp.attention_backward(dout, q, k, v, want, lse)
     assert torch.equal(dq[0], want[0]) and not (dq != want).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_sum_of_many_alike(cuda, dtype):
+    """65536 keys that are not split, all but the first 64 with one score (a head's own), on either side of the sum's base. Sums
+    over a tile's 32 keys a lane, then over 1024 tiles, of half a step of fp32 (2^-24) each; a score's, its exponential's and lse's own
+    roundings 2^-20 of their sizes."""
+    Lk, H = 65536, 256
+    scores = torch.linspace(-4.0, 5.4, H, device=cuda).to(dtype)
+    k = torch.zeros(1, Lk, H, 8, dtype=dtype, device=cuda)
+    k[0, 64:, :, 0] = scores
+    q = torch.zeros(1, 1, H, 8, dtype=dtype, device=cuda)
+    q[..., 0] = 1.0
+    v = torch.ones(1, 1, H, 8, dtype=dtype, device=cuda).expand(1, Lk, H, 8)
+    out, lse = sp.attention(q, k, v, scale=1.0, return_lse=True)
+    want = torch.log(64.0 + (Lk - 64) * scores.double().exp())
+    bound = (Lk // 64 + 33) * 2.0 ** -24 + 2.0 ** -20 * (1.0 + scores.double().abs())
+    assert ((lse[0, 0].double() - want).abs() <= bound).all()
+    assert (out.double() - 1.0).abs().max() <= 4 * HALF[dtype]
