@@ -389,8 +389,8 @@ int spanqr_block_norm_backward(int type, int wtype, int act, long rows, long D, 
                                long workspace_bytes, void* stream);
 
 /* Softmax attention of bf16 or fp16, G heads to each of Hk key heads: out = softmax(scale q k^T) v. q, k and v are [.., Hk G or
- * Hk, D] by their strides {batch, row, head} in elements (host arrays, read at the call): multiples of 8, those of rows and
- * heads below 2^24, neighbouring elements of a head, 16-byte alignment. D: a multiple of 8 up to 128.
+ * Hk, D] by their strides {batch, row, head} in elements (host arrays, read at the call): multiples of 8, those of rows, and
+ * of heads but for k and v, below 2^24, neighbouring elements of a head, 16-byte alignment. D: a multiple of 8 up to 128.
  * q_starts null: B sequences of Tq queries and Tk keys, of which with k_lens (device, B; read when the kernels run, taken as
  * from 0 to Tk; or null) the first k_lens[b] are there, and the others are not read. Else packed: Tq and Tk rows in all,
  * sequence b having the rows q_starts[b] to q_starts[b + 1] - 1 and k_starts' (device, B + 1 each, ascending; read when the

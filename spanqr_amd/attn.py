@@ -10,18 +10,19 @@ import torch
 from . import _lib
 from .tensors import TYPES, check_like, check_same, check_tensor, like, no_tangents, on, once, workspace
 
-MAX_STRIDE = 1 << 24   # of rows and heads, in elements
+MAX_STRIDE = 1 << 24   # of rows, and of q's, the result's and its gradient's heads, in elements
 MAX_HEAD = 128
 MOST = 1 << 40         # more keys or rows than there are say the same, and this fits into the C ABI's numbers
 
 
-def _heads(t):
+def _heads(t, keys=False):
     """(t, its strides {batch, row, head}): neighbouring elements of a head, every head's row on 16 bytes, and strides that the
-    library's offsets reach; as it lies, or copied"""
+    library's offsets reach (keys: k's and v's heads may lie any way apart); as it lies, or copied"""
     s = t.stride()
-    if s[-1] != 1 or (s[0] | s[-2] | s[-3]) & 7 or s[-2] >= MAX_STRIDE or s[-3] >= MAX_STRIDE:
+    if s[-1] != 1 or (s[0] | s[-2] | s[-3]) & 7 or (s[-2] >= MAX_STRIDE and not keys) or s[-3] >= MAX_STRIDE:
+        far = t.dim() - 4, t.dim() - 2 if keys else None
         if not ((s[-1] == 1 or t.shape[-1] == 1) and all(
-                n == 1 or (v % 8 == 0 and (v < MAX_STRIDE or i == t.dim() - 4)) for i, (n, v) in enumerate(zip(t.shape[:-1], s)))):
+                n == 1 or (v % 8 == 0 and (v < MAX_STRIDE or i in far)) for i, (n, v) in enumerate(zip(t.shape[:-1], s)))):
             t = t.contiguous()
             s = t.stride()
         s = tuple(0 if n == 1 else v for n, v in zip(t.shape, s))   # (axes of one element have any)
@@ -109,7 +110,7 @@ def _forward(q, k, v, causal, how, need_lse):
     shape, window, scale, (q_starts, k_starts, k_lens), max_q, max_k = how
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if need_lse else None
-    (q, qs), (k, ks), (v, vs) = _heads(q), _heads(k), _heads(v)
+    (q, qs), (k, ks), (v, vs) = _heads(q), _heads(k, True), _heads(v, True)
     strides = array("q", qs + ks + vs)
     at = strides.buffer_info()[0]
     dev = q.device
@@ -128,7 +129,8 @@ def _backward(dout, q, k, v, out, lse, causal, how, need_dq, need_dkv):
     dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_dq else None
     dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_dkv else None
     dv = torch.empty_like(dk) if need_dkv else None
-    (dout, ds), (q, qs), (k, ks), (v, vs), (out, os) = map(_heads, (dout, q, k, v, out))
+    (dout, ds), (q, qs), (out, os) = map(_heads, (dout, q, out))
+    (k, ks), (v, vs) = _heads(k, True), _heads(v, True)
     strides = array("q", ds + qs + ks + vs + os)
     at = strides.buffer_info()[0]
     lse = lse.contiguous()
@@ -170,7 +172,8 @@ def attention(q, k, v, causal=False, window=None, scale=None, q_starts=None, k_s
     """softmax(scale q k^T) v for each head: q [B, Sq, heads, D], k and v [B, Sk, key heads, D], bfloat16 or float16 on a ROCm
     device, heads a multiple of the key heads (head h reads key head h // (heads / key heads)), D a multiple of 8 up to
     128; scale (positive) is D^-1/2 unless given. Strided tensors, such as the columns of one product, are read as they lie
-    where every head's row starts on 16 bytes. The result has q's shape and is contiguous.
+    where every head's row starts on 16 bytes and rows (of q, heads too) are less than 2^24 elements apart, and copied
+    elsewhere. The result has q's shape and is contiguous.
 
     Query i stands at p = i + Sk - Sq, so that one token's query reads all that is cached. causal: it sees the keys j <= p;
     window: only the last `window` of those. A query that sees no key has the result 0. k_lens: int32 [B] on the device, the

@@ -1080,7 +1080,7 @@ __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const Back
 
 constexpr long MAX_ROWS = 1l << 30;      // queries x group, or keys, of a sequence
 constexpr long MAX_GRID = (1l << 24) - 1;
-constexpr long MAX_STRIDE = 1l << 24;    // of rows and heads: a tile's offsets stay within 32 bits
+constexpr long MAX_STRIDE = 1l << 24;    // of rows, and of heads that share keys: a tile's offsets stay within 32 bits
 
 long tiles_in(long n, long each) { return n < 1 ? 1 : (n + each - 1) / each; }
 
@@ -1188,8 +1188,8 @@ long backward_bytes(const Call& c) {
     return q + kv == 0 ? stat_bytes(c) : (stat_bytes(c) + 15) / 16 * 16 + q + kv;
 }
 
-// strides: {batch, row, head}
-int check_heads(const char* what, const char* name, const void* p, const long* strides, bool empty, Heads& h) {
+// strides: {batch, row, head}; keys: of k and v, whose tiles are of one head
+int check_heads(const char* what, const char* name, const void* p, const long* strides, bool empty, bool keys, Heads& h) {
     if (empty) {
         h = {p, 0, 0, 0};
         return SPANQR_OK;
@@ -1197,9 +1197,9 @@ int check_heads(const char* what, const char* name, const void* p, const long* s
     if (p == nullptr || strides == nullptr) return error(SPANQR_EINVAL, "%s: %s is missing", what, name);
     h = {p, strides[0], strides[1], strides[2]};
     if ((uintptr_t)p % 16 != 0 || h.batch % 8 != 0 || h.row % 8 != 0 || h.head % 8 != 0 || h.batch < 0 || h.row < 0 || h.head < 0 ||
-        h.row >= MAX_STRIDE || h.head >= MAX_STRIDE)
-        return error(SPANQR_EINVAL, "%s: %s needs 16-byte alignment and strides that are multiples of 8, of rows and heads below %ld", what,
-                     name, MAX_STRIDE);
+        h.row >= MAX_STRIDE || (!keys && h.head >= MAX_STRIDE))
+        return error(SPANQR_EINVAL, "%s: %s needs 16-byte alignment and strides that are multiples of 8, of rows%s below %ld", what, name,
+                     keys ? "" : " and heads", MAX_STRIDE);
     return SPANQR_OK;
 }
 bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
@@ -1286,9 +1286,9 @@ int spanqr_attention(int type, long B, long Hk, long G, long D, long Tq, long Tk
     if (rc != SPANQR_OK || c.rows == 0) return rc;
     ForwardArgs a = {};
     const bool none = Tk == 0 || (B == 0 && q_starts == nullptr);
-    if ((rc = check_heads("attention", "q", q, q_strides, false, a.q)) != SPANQR_OK ||
-        (rc = check_heads("attention", "k", k, k_strides, none, a.k)) != SPANQR_OK ||
-        (rc = check_heads("attention", "v", v, v_strides, none, a.v)) != SPANQR_OK)
+    if ((rc = check_heads("attention", "q", q, q_strides, false, false, a.q)) != SPANQR_OK ||
+        (rc = check_heads("attention", "k", k, k_strides, none, true, a.k)) != SPANQR_OK ||
+        (rc = check_heads("attention", "v", v, v_strides, none, true, a.v)) != SPANQR_OK)
         return rc;
     if (out == nullptr || !aligned(out)) return error(SPANQR_EINVAL, "attention: out is missing or not on 16 bytes");
     const long need = c.splits > 1 ? 4 * c.splits * c.rows * (D + 2) : 0;
@@ -1327,11 +1327,11 @@ int spanqr_attention_backward(int type, long B, long Hk, long G, long D, long Tq
     if (rc != SPANQR_OK) return rc;
     const bool packed = q_starts != nullptr, no_q = c.rows == 0, no_k = Tk == 0 || (B == 0 && !packed);
     BackwardArgs a = {};
-    if ((rc = check_heads(what, "q", q, q_strides, no_q, a.q)) != SPANQR_OK ||
-        (rc = check_heads(what, "k", k, k_strides, no_k, a.k)) != SPANQR_OK ||
-        (rc = check_heads(what, "v", v, v_strides, no_k, a.v)) != SPANQR_OK ||
-        (rc = check_heads(what, "out", out, out_strides, no_q, a.out)) != SPANQR_OK ||
-        (rc = check_heads(what, "dout", dout, dout_strides, no_q, a.dout)) != SPANQR_OK)
+    if ((rc = check_heads(what, "q", q, q_strides, no_q, false, a.q)) != SPANQR_OK ||
+        (rc = check_heads(what, "k", k, k_strides, no_k, true, a.k)) != SPANQR_OK ||
+        (rc = check_heads(what, "v", v, v_strides, no_k, true, a.v)) != SPANQR_OK ||
+        (rc = check_heads(what, "out", out, out_strides, no_q, false, a.out)) != SPANQR_OK ||
+        (rc = check_heads(what, "dout", dout, dout_strides, no_q, false, a.dout)) != SPANQR_OK)
         return rc;
     if ((dk != nullptr) != (dv != nullptr) || !aligned(dq) || !aligned(dk) || !aligned(dv))
         return error(SPANQR_EINVAL, "%s: dk and dv belong together, and gradients lie on 16 bytes", what);

@@ -528,3 +528,24 @@ def test_sum_of_many_alike(cuda, dtype):
     bound = (Lk // 64 + 33) * 2.0 ** -24 + 2.0 ** -20 * (1.0 + scores.double().abs())
     assert ((lse[0, 0].double() - want).abs() <= bound).all()
     assert (out.double() - 1.0).abs().max() <= 4 * HALF[dtype]
+
+
+def test_long_cache_with_heads_in_front(cuda):
+    """keys and values as [heads, rows, D] caches whose heads are 2^24 elements and more apart are read as they lie"""
+    S = (1 << 24) // 64 + 1
+    keys, values = normal(2, S, 64, seed=1), normal(2, S, 64, seed=2)
+    k, v = keys.transpose(0, 1)[None], values.transpose(0, 1)[None]
+    assert k.stride(2) > 1 << 24
+    q = normal(1, 1, 8, 64, seed=3)
+    want = sp.attention(q, k.contiguous(), v.contiguous())
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = sp.attention(q, k, v)
+    assert torch.cuda.max_memory_allocated() - before < 16 << 20   # (a copy of the keys is 64 MB)
+    assert torch.equal(got, want)
+    k, v, q, dout = k[:, -200:], v[:, -200:], normal(1, 100, 4, 64, seed=4), normal(1, 100, 4, 64, seed=5)
+    got, lse = sp.attention(q, k, v, causal=True, return_lse=True)
+    want = sp.attention_backward(dout, q, k.contiguous(), v.contiguous(), got, lse, causal=True)
+    assert torch.equal(got, sp.attention(q, k.contiguous(), v.contiguous(), causal=True))
+    assert all(torch.equal(a, b) for a, b in zip(sp.attention_backward(dout, q, k, v, got, lse, causal=True), want))
