@@ -388,3 +388,19 @@ def test_graph_and_streams(cuda):
         assert all(torch.equal(u, v) for u, v in zip(got, eager))
         if i == 0:
             assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_slope_of_large_gates(cuda, dtype):
+    """the slopes where sigmoid is next to 1, to the type's rounding and, of themselves, exp(-g)'s: -g log2 e is rounded to half a step of
+    up to 128, 2^-18, which times ln 2 and with the other roundings stays below 2^-17 (bf16); in fp32 and fp16, which take
+    that out, below 2^-20"""
+    g = torch.linspace(0.0, 80.0, 8001, device=cuda).to(dtype)[:, None]
+    x = torch.ones_like(g)
+    y, h = sp.block_norm(x, torch.zeros_like(x), gate=g, gate_act="sigmoid", eps=0.0)
+    s = torch.sigmoid(g.double())
+    rest = torch.sigmoid(-g.double())
+    more = 2.0 ** (-17 if dtype == torch.bfloat16 else -20)
+    for kind, want in (("sigmoid", s * rest), ("silu", s * (1.0 + g.double() * rest))):
+        got = sp.block_norm_backward(None, x, x, h, gate=g, gate_act=kind, eps=0.0).gate
+        assert ((got.double() - want).abs() <= (HALF[dtype] + more) * want + TINY[dtype]).all(), kind
