@@ -1117,20 +1117,23 @@ long splits_of(long have, long max_k) {
     return n < 1 ? 1 : n;
 }
 
-// The workgroups of the gradient that the device runs at once: three a compute unit of up to 64 wide heads, two of wider ones
-long at_once(long D) { return 256 * (D <= 64 ? 3 : 2); }
+// The workgroups of k_dq and k_dkv that the device runs at once, by the registers that the compiler reports: three a compute unit of
+// up to 64 wide heads (k_dq in bf16 takes 166, k_dkv 168), but two of k_dq in fp16 above 32 (178); two of wider heads. Both ways in us
+// with three for fp16's too / two: causal 5 x 2048 x 8 x 64 192 / 170, 8 x 1024 x 10 x 64 136 / 116. Up to 32 wide in bf16 four would run
+// (123): with four 5 x 2048 x 10 x 32 161 instead of 139, 1 x 1362 x 8 on 1 x 32 65 instead of 70.
+long dq_at_once(int type, long D) { return 256 * (D > 64 || (type == SPANQR_FP16 && D > 32) ? 2 : 3); }
+long dkv_at_once(long D) { return 256 * (D > 64 ? 2 : 3); }
 
 // Whether the gradient of K and V takes 64 keys a workgroup: where 128 make no more than the device runs at once. Both ways in us with 128 / 64: 8 x 1024 x 8 x 128 on 4 heads
 // 160 / 139, 16 x 512 x 16 x 64 on 4 116 / 98, packed 24 x 2048 x 8 x 64 on 2 357 / 294; with more of them 16 x 1024 x 12 x 64 190 / 204.
-bool few_keys(long tiles, long D) { return tiles <= at_once(D); }
+bool few_keys(long tiles, long slots) { return tiles <= slots; }
 
 // Workgroups that share a tile of dQ's rows, or of dK's and dV's, each with four tiles of the other side at least: as many as run
 // at once, or one more where a mask makes tiles uneven. Both ways in us without / with: 1 x 1362 x 8 on 1 x 64 284 / 81, causal
 // 1 x 2048 x 16 on 2 x 128 480 / 199, 1 x 8192 x 2 on 1 x 64 448 / 203, 3 x 4685 x 15 on 3 x 40 814 / 676. Only where tiles make less than half
 // of what runs at once 304 instead of 257 (causal 8 x 1185 x 10 on 2 x 128 fp16); one more without a mask too 201 instead of
 // 177 (2 x 2277 x 3 x 128 fp16).
-long grad_splits_of(long tiles, long others, long D, int causal) {
-    const long slots = at_once(D);
+long grad_splits_of(long tiles, long others, long slots, int causal) {
     if (tiles >= slots) return 1;
     const long want = (causal ? slots + tiles - 1 : slots) / tiles, most = others / 4;
     const long n = want < most ? want : most;
@@ -1166,10 +1169,10 @@ int check_shape(const char* what, int type, long B, long Hk, long G, long D, lon
     c.keys = (packed ? 1 : B) * Tk * Hk;
     const long q_all = Hk * count_of(packed, B, Tq * G, max_q * G, BLOCK), max_m = max_q * G;
     c.splits = B == 0 ? 1 : splits_of(q_all, max_k);
-    c.few_keys = few_keys(Hk * count_of(packed, B, Tk, max_k, BLOCK), D);
+    c.few_keys = few_keys(Hk * count_of(packed, B, Tk, max_k, BLOCK), dkv_at_once(D));
     const long keys = c.few_keys ? BLOCK / 2 : BLOCK;
-    c.q_splits = B == 0 || c.rows == 0 ? 1 : grad_splits_of(q_all, (max_k + TILE - 1) / TILE, D, causal);
-    c.kv_splits = B == 0 || c.keys == 0 ? 1 : grad_splits_of(Hk * count_of(packed, B, Tk, max_k, keys), (max_m + TILE - 1) / TILE, D, causal);
+    c.q_splits = B == 0 || c.rows == 0 ? 1 : grad_splits_of(q_all, (max_k + TILE - 1) / TILE, dq_at_once(type, D), causal);
+    c.kv_splits = B == 0 || c.keys == 0 ? 1 : grad_splits_of(Hk * count_of(packed, B, Tk, max_k, keys), (max_m + TILE - 1) / TILE, dkv_at_once(D), causal);
     c.tiles = tiles_of(packed, B, Hk, Tq * G, max_m, BLOCK, c.splits, c.splits == 1);
     c.q_tiles = tiles_of(packed, B, Hk, Tq * G, max_m, BLOCK, c.q_splits, c.q_splits == 1);
     c.k_tiles = tiles_of(packed, B, Hk, Tk, max_k, BLOCK, 1, false);
@@ -1312,7 +1315,7 @@ long spanqr_attention_backward_workspace(long B, long Hk, long G, long D, long T
     Call c;
     const int none = 0;
     const int rc = check_shape("attention_backward", SPANQR_BF16, B, Hk, G, D, Tq, Tk, packed ? &none : nullptr, packed ? &none : nullptr,
-                               nullptr, max_q, max_k, 1, 0, 1.0f, c);   // (causal ones have the most parts)
+                               nullptr, max_q, max_k, 1, 0, 1.0f, c);   // (causal ones in bf16 have the most parts)
     return rc != SPANQR_OK ? rc : backward_bytes(c);
 }
 

@@ -91,3 +91,17 @@ def test_packed_calls_without_hints():
     assert b"too many workgroups" in _lib.lib().spanqr_last_error()
     # more tiles than a launch takes workgroups: each goes over several
     assert f((1 << 23) - 1, 1, 129, 8, 1, 4, 0, 0, 0) == 0
+
+
+def test_parts_by_what_runs_at_once():
+    """640 tiles of dQ, 64 wide: fewer than the 768 that run at once in bf16, more than fp16's 512"""
+    L = _lib.lib()
+    shape = 5, 8, 1, 64, 2048, 2048
+    stat = 8 * 5 * 2048 * 8 + 4 * 5 * 8 * (16 + 16)
+    row = 4 * 5 * 2048 * 8 * 64   # bytes of a part
+    for type, parts in ((1, 2), (2, 0)):   # (dK and dV have 1280 tiles of 64 keys)
+        assert L.spanqr_attention_backward(type, *shape, PTR, strides(), PTR, strides(), PTR, strides(), PTR, strides(), PTR, strides(), PTR,
+                                           None, None, None, 0, 0, 1, 0, 1.0, PTR, PTR, PTR, None, 0, None) == EINVAL
+        need = int(L.spanqr_last_error().split(b"needs ")[1].split()[0])
+        assert need == stat + parts * row
+        assert need <= L.spanqr_attention_backward_workspace(*shape, 0, 0, 0)
