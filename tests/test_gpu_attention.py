@@ -549,3 +549,69 @@ def test_long_cache_with_heads_in_front(cuda):
     want = sp.attention_backward(dout, q, k.contiguous(), v.contiguous(), got, lse, causal=True)
     assert torch.equal(got, sp.attention(q, k.contiguous(), v.contiguous(), causal=True))
     assert all(torch.equal(a, b) for a, b in zip(sp.attention_backward(dout, q, k, v, got, lse, causal=True), want))
+
+
+@pytest.mark.parametrize("own_keys", [False, True])
+def test_packed_autograd(cuda, own_keys):
+    """the starts as they are kept for the backward pass: bit by bit what attention_backward gives"""
+    starts = [3, 16, 16, 40, 70]
+    others = [0, 30, 41, 41, 90] if own_keys else starts
+    qs, ks = (torch.tensor(s, dtype=torch.int32, device=cuda) for s in (starts, others))
+    how = dict(causal=True, window=20, q_starts=qs, **(dict(k_starts=ks) if own_keys else {}))
+    q, dout = normal(75, 4, 32, seed=1).requires_grad_(), normal(75, 4, 32, seed=4)
+    k, v = (normal(93 if own_keys else 75, 2, 32, seed=s).requires_grad_() for s in (2, 3))
+    out, lse = sp.attention(q, k, v, return_lse=True, **how)
+    got = torch.autograd.grad(out, (q, k, v), dout)
+    want = sp.attention_backward(dout, q, k, v, out, lse, **how)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert got[0][3:16].any() and not got[0][:3].any() and not got[0][70:].any()
+    # one sequence alone, as a batch of one
+    first = [t.detach() for t in (q[3:16], k[others[0]:others[1]], v[others[0]:others[1]])]
+    alone, lse = sp.attention(*(t[None] for t in first), causal=True, window=20, return_lse=True)
+    assert torch.equal(alone[0], out[3:16])
+    dq, dk, dv = sp.attention_backward(dout[None, 3:16], *(t[None] for t in first), alone, lse, causal=True, window=20)
+    assert torch.equal(dq[0], got[0][3:16]) and torch.equal(dk[0], got[1][others[0]:others[1]]) and torch.equal(dv[0], got[2][others[0]:others[1]])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_parts_in_graphs_and_on_streams(cuda, dtype):
+    """gradients whose tiles several workgroups share, a batch's and those of a list of packed sequences: captured, with inputs and
+    starts changed between replays and eager calls between them; and two streams at once, each with a workspace of its own"""
+    L = 2000
+    x = [normal(L, h, 64, seed=s, dtype=dtype) for s, h in ((1, 2), (2, 1), (3, 1), (4, 2))]
+    starts = torch.arange(0, L + 1, 50, dtype=torch.int32, device=cuda)
+
+    def batch(q, k, v, dout):
+        q, k, v, dout = (t[None, :900] for t in (q, k, v, dout))
+        out, lse = sp.attention(q, k, v, causal=True, return_lse=True)
+        return (out, lse, *sp.attention_backward(dout, q, k, v, out, lse, causal=True))
+
+    def packed(q, k, v, dout):
+        out, lse = sp.attention(q, k, v, causal=True, q_starts=starts, return_lse=True)
+        return (out, lse, *sp.attention_backward(dout, q, k, v, out, lse, causal=True, q_starts=starts))
+
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    first = batch(*x) + packed(*x)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(s):
+            a = batch(*x)
+        with torch.cuda.stream(t):
+            b = packed(*x)
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, w) for u, w in zip(a + b, first))
+    graphs = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graphs[0]):
+        a = batch(*x)
+    with torch.cuda.graph(graphs[1]):
+        b = packed(*x)
+    for i, at in enumerate((None, [0] * 20 + [L] * 21, [7] * 3 + list(range(10, 1910, 50)), None)):
+        starts.copy_(torch.arange(0, L + 1, 50) if at is None else torch.tensor(at))
+        for u in x:
+            u.neg_()
+        for graph in graphs:
+            graph.replay()
+        eager = batch(*x) + packed(*x)
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, w) for u, w in zip(a + b, eager)), i
+    assert all(torch.equal(u, w) for u, w in zip(eager, first))
