@@ -8,9 +8,13 @@
 //             dw1 = a sum over rows of v act(g) n1,  dw2 = sum over rows of dy n2,  da = sum of q n1
 //   act(g) = g, 1 / (1 + exp(-g)), or g / (1 + exp(-g)); 1 without a gate
 //
-// Bound by memory: each input is read once and each output written once, the row stays in registers between the two sums
-// (threads and pieces as in norm.hip). Between them would be h, t, n1, dt and the mask in memory if these were operators of
-// their own. Sums are fp32: per thread over at most 16 elements, then a tree in a fixed order. 16384 x 2048 bf16 with gate and
+// Bound by memory: rows of up to 8192 elements are read once and each output written once, the row stays in registers between the
+// two sums (threads and pieces as in norm.hip). Between them would be h, t, n1, dt and the mask in memory if these were operators of
+// their own. Longer rows are read two or three times, from the caches behind the first one (k_block_long, k_block_grad_long).
+// Sums are fp32 in a fixed order. Within a row: per thread over at most 16 elements, or the D / 8192 pieces of eight (up to 2048) of a
+// long one, then a tree. Over rows, for the weights and the scale: a thread's rows one after the other (rows / 256 at
+// most), up to 16 groups, then at most 24 of up to 1536 parts in each of 64 sums, and a tree: rows / 256 + 50 steps of 2^-24 of what is
+// added up, at most. 16384 x 2048 bf16 with gate and
 // dropout: forward 61 us for 0.34 GB, gradient 91 for 0.54 GB and k_block_sums 7, with the 256 MB cache's help above a large
 // copy's 5.2 TB/s; without dropout's ten rounds of multiplications 161 us in all instead of 169.
 #include "host.h"

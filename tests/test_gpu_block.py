@@ -404,3 +404,31 @@ def test_slope_of_large_gates(cuda, dtype):
     for kind, want in (("sigmoid", s * rest), ("silu", s * (1.0 + g.double() * rest))):
         got = sp.block_norm_backward(None, x, x, h, gate=g, gate_act=kind, eps=0.0).gate
         assert ((got.double() - want).abs() <= (HALF[dtype] + more) * want + TINY[dtype]).all(), kind
+
+
+@pytest.mark.parametrize("rows,D,dtype", [(65536, 64, torch.bfloat16), (1 << 20, 40, torch.float32), (30000, 500, torch.float32),
+                                          (20000, 2048, torch.float16), (4096, 9000, torch.float32), (16384, 8200, torch.bfloat16),
+                                          (3, 1 << 20, torch.float32), (300, 100000, torch.bfloat16)])
+def test_long_sums(cuda, rows, D, dtype):
+    """many rows a workgroup, and rows of many pieces a thread. Half a step of fp32 for each addition in a row: within a row a
+    thread's pieces (of 8, 8192 elements apart beyond 8192, 2 of them below), eight elements and a tree of 10 and 16 wavefronts; over
+    rows those of a workgroup's thread, its 16 groups, and 64 parts at a time with a tree of 6; with 40 such steps for the rest"""
+    from spanqr_amd import _lib
+    x, r, dy, dh, z, w1, w2 = inputs(rows, D, dtype, torch.float32, True, 8)
+    dy.abs_()   # (sums that grow with the rows)
+    h = sp.block_norm(x, r, w1, w2, gate=z, scale=0.5)[1]
+    at = torch.tensor([0.5], device=cuda)
+    g = sp.block_norm_backward(dy, dh, x, h, w1, w2, gate=z, scale=at)
+    parts = _lib.lib().spanqr_block_norm_backward_workspace(rows, D) // (4 * (2 * D + 1))
+    in_row = max(2, -(-D // 8192)) + 8 + 10 + 16
+    over_rows = -(-rows // parts) + 16 + -(-parts // 64) + 6
+    y = sp.block_norm(x, r, w1, w2, gate=z, scale=0.5)[0]
+    keep = torch.ones((), device=cuda, dtype=torch.float64)
+    want = plain(x, r, w1, w2, z, "silu", 0.5, keep, 1.0, 1e-6, h, dy, dh)
+    # a row's norms have in_row steps in their sums (half of that of themselves), the gradient's means again: 3 of them at most
+    for name, got, steps in (("y", y, in_row), ("x", g.x, 3 * in_row), ("residual", g.residual, 3 * in_row),
+                             ("post_weight", g.post_weight, 3 * in_row + over_rows), ("weight", g.weight, in_row + over_rows),
+                             ("scale", g.scale, 3 * in_row + over_rows)):
+        value, added = want[name]
+        err, bound = (got.double() - value).abs(), HALF[got.dtype] * value.abs() + (steps + 40) * 2.0 ** -24 * added + TINY[got.dtype]
+        assert (err <= bound).all(), (name, float((err / bound).max()))
