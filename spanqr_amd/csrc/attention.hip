@@ -413,9 +413,9 @@ struct ForwardArgs {
 // A workgroup has 128 rows, a wavefront 32 of them in registers (a lane one query), and goes over the keys in tiles of 64 in
 // two LDS buffers. The softmax's base moves only where a tile's maximum is more than 2^8 above it: sums and products are
 // relative to it anyway, and 64 multiplications a tile and lane are left out. Bound by the matrix pipe and the softmax's vector
-// instructions (5 for each product of 32 cycles), at a clock that falls with what both draw: 16384 x 40 x 128 on 8 heads, causal,
-// bf16 2.7 ms, 1.0 PFLOP/s; 16 x 1024 x 12 x 64 47 us; 4 x 1999 x 16 x 80 with every key seen 118. A token of 40 heads against 8191 keys
-// of 8 is bound by latency, 10.4 us for 34 MB, and 3.6 for k_join.
+// instructions (5 for each product of 32 cycles at 128 wide heads, 13 at 64), at a clock that falls with what both draw: 16384 x 40 x 128 on 8 heads, causal,
+// bf16 2.7 ms, 1.0 PFLOP/s; 16 x 1024 x 12 x 64 46 us; 4 x 1999 x 16 x 80 with every key seen 113. A token of 40 heads against 8191 keys
+// of 8 is bound by latency, 10.1 us for 34 MB, and 3.5 for k_join.
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_forward(const ForwardArgs a) {
     typedef typename Vec<T>::x8 x8;
@@ -721,7 +721,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_v_most(const BackwardArgs a) {
 // dQ: as the forward pass, 128 rows a workgroup; a lane has one query. It has dO in registers, so it forms D first, and leaves it
 // and lse as the gradients take it for the keys' kernel (a pass of its own over O and dO took 15 us of 200 at 16 x 1024 x 12 x 64).
 // Without dq that is all it does. 16384 x 40 x 128 on 8 heads, causal, bf16: 3.3 ms, 1.24 PFLOP/s, the matrix pipe busy for 73 % of
-// the cycles at 1.6 GHz; 16 x 1024 x 12 x 64 57 us.
+// the cycles at 1.6 GHz; 16 x 1024 x 12 x 64 58 us.
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
     typedef typename Vec<T>::x8 x8;
@@ -879,7 +879,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_dq(const BackwardArgs a) {
 // queries that see them; or (SPLIT 2, where 128 keys would leave too few workgroups) 64 keys, two wavefronts sharing 32 and each
 // taking half of every tile's rows. The rows come in tiles of 64, or as many whole queries' rows as that holds. Each product's
 // first operand comes from LDS, which at 128 bytes a cycle feeds no more than the four pipes take. 16384 x 40 x 128 on 8 heads,
-// causal, bf16: 5.5 ms, 0.99 PFLOP/s; 16 x 1024 x 12 x 64 71 us. Sums of dQ by the same kernel would save two of seven products, but need
+// causal, bf16: 5.5 ms, 0.99 PFLOP/s; 16 x 1024 x 12 x 64 72 us. Sums of dQ by the same kernel would save two of seven products, but need
 // atomics, or 4 bytes of partial sums for each 128 keys and element of dQ.
 template <typename T, int DP, int SPLIT>
 __global__ __launch_bounds__(64 * WAVES, DP <= 64 ? 3 : 2) void k_dkv(const BackwardArgs a) {
